@@ -246,6 +246,98 @@ int cs1_gdn_prefill_gated_varlen(const void* q, const void* k, const void* v, co
                                  const int32_t* cu_seqlens, int nseq, int H, int HK, float scale, const void* s_in,
                                  size_t s_in_stride, void* s_out, size_t s_out_stride, void* stream);
 
+/* ---- additions: decoding one token at a time (no counterpart in the reference) ----
+ *
+ * A serving program keeps, for up to nseq sequences, the keys and values of every attention
+ * layer in pages and the state of every Gated DeltaNet layer in one slot a sequence.  Each call
+ * below works on a list of sequences: seqs is a DEVICE array of sequence numbers (null: row i is
+ * sequence i), so a captured graph serves whatever sequences the array names when it is
+ * replayed.  A number outside [0, nseq) is a padding row.  Where a call changes a sequence, the
+ * first row that names it has it and later rows that name it again are padding rows. */
+
+/* The page table, on the device; the struct itself is read during the call.  Sequence s holds
+ * lens[s] tokens, token j in slot j % page of page table[s * max_pages + j / page]; refs[p] counts
+ * the sequences that hold page p (0: free).  A program starts with table filled with -1 and
+ * lens and refs with 0.  Limits: nseq <= 8192, page a multiple of 16, max_pages * page < 2^31.
+ * One layer's K pages and V pages are two buffers ("pools") of [npages, page, Hk, Dh], all layers
+ * under the one table.  A page number outside [0, npages) in a row of the table is never
+ * followed: its tokens are neither read nor written. */
+typedef struct Cs1PageTable {
+    int32_t* table; /* [nseq, max_pages] */
+    int32_t* lens;  /* [nseq] */
+    int32_t* refs;  /* [npages] */
+    int nseq, max_pages, npages, page;
+} Cs1PageTable;
+
+/* Make room for new tokens: lens[s] grows by one for each of the n listed sequences (cu_seqlens
+ * null), or by cu_seqlens[i + 1] - cu_seqlens[i] (a HOST array as in cs1_attention_varlen, n <= 64),
+ * and the pages that this needs are the lowest-numbered free ones, in the order of the list.
+ * All or nothing: *status (device) receives 0, or the number of pages that are missing, or -1
+ * where a sequence would need more than max_pages; if it is not 0 nothing else has changed, and
+ * the step that the room was for must not run.  n <= 8192. */
+int cs1_kv_reserve(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n, int32_t* status,
+                   void* stream);
+
+/* Store the last tokens' keys and values of one layer: row r of k (rows of ldk) and of v (rows of
+ * ldv), Hk * Dh values each, goes to the pages kp and vp.  cu_seqlens null: row i is the last
+ * token (lens[s] - 1) of listed sequence i; else (HOST, any n) rows [cu_seqlens[i], cu_seqlens[i + 1])
+ * are its last tokens in order.  Rows of padding or before position 0 are left out. */
+int cs1_kv_write(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n, const void* k,
+                 int ldk, const void* v, int ldv, void* kp, void* vp, int Hk, int Dh, void* stream);
+
+/* Continue sequences src[i] (device, n <= 8192) as the empty sequences dst[i] (device): dst[i]
+ * shares the whole pages and gets a page of its own, the lowest free ones in list order, for what
+ * the last page holds if it is not full; those tokens' rows (row_bytes a token) are copied in all
+ * npools pools (a HOST array of device pointers to [npages, page * row_bytes bytes]).  Left out are
+ * pairs with a number out of range, whose dst holds tokens or an earlier pair names as dst, or whose src
+ * any pair names as dst.  status as in cs1_kv_reserve (0, or the missing pages, and then nothing has
+ * changed).  workspace: cs1_kv_workspace_bytes(npages, n) bytes, free for other use after the call. */
+size_t cs1_kv_workspace_bytes(int npages, int n);
+int cs1_kv_fork(const Cs1PageTable* pages, const int32_t* src, const int32_t* dst, int n, void* const* pools, int npools,
+                size_t row_bytes, void* workspace, int32_t* status, void* stream);
+
+/* End the listed sequences: each page's count falls by one, the rows of the table become -1 and the lengths 0. */
+int cs1_kv_free(const Cs1PageTable* pages, const int32_t* seqs, int n, void* stream);
+
+/* Move the pages that are held to the start of every pool: with L of them, the i-th held page
+ * from L on moves to the i-th free page before L; table and refs follow.  *status receives L.
+ * workspace: cs1_kv_workspace_bytes(npages, 0) bytes. */
+int cs1_kv_compact(const Cs1PageTable* pages, void* const* pools, int npools, size_t row_bytes, void* workspace,
+                   int32_t* status, void* stream);
+
+/* Copy entry src[i] to entry dst[i] (device, n <= 8192) in each of npools buffers of `entries`
+ * entries of entry_bytes (a multiple of 16): pages, or with a sequence's GDN state or conv ring as
+ * the entry, what cs1_kv_fork does for the Gated DeltaNet layers.  Left out are pairs with a number out of range,
+ * whose dst an earlier pair names as dst, or whose src any pair names as dst. */
+int cs1_kv_copy(void* const* pools, int npools, size_t entry_bytes, int entries, const int32_t* src, const int32_t* dst,
+                int n, void* stream);
+
+/* Attention of one new token per row over the pages (after cs1_kv_write): q, gate (null: none) and
+ * out [B, Hq, Dh], Dh 128 or 256; row r's q head h sees the lens[s] keys of sequence s = seqs[r] through kv
+ * head h / (Hq / Hk).  lse [Hq, B] float32 (null: not written) as in cs1_attention_ex.  Unlike there the
+ * output is rounded once, after the gate.  A padding row, or one of an empty sequence, gets zeros and an
+ * lse of -inf.  The handle holds the partial results of sequences that are split over the chip: it belongs to the
+ * device that is current when it is created and, as a GEMM handle, serves one thread and one
+ * stream at a time (graphs captured with one handle must not run at the same time). */
+void* cs1_attention_paged_create(void);
+void cs1_attention_paged_destroy(void* paged);
+int cs1_attention_paged(void* paged, const void* q, const void* kp, const void* vp, const Cs1PageTable* pages,
+                        const int32_t* seqs, const void* gate, void* out, float* lse, int B, int Hq, int Hk, int Dh,
+                        float scale, void* stream);
+
+/* One token per row through a Gated DeltaNet layer, from the projections to the normed output: conv1d + SiLU
+ * (as cs1_gdn_conv), gates, one step of the delta rule (as cs1_gdn_prefill_gated_x) and, unless z and
+ * norm_w are null, the gated RMSNorm.  Row r of qkv, z, b and a (all in rows of ld) is the token at
+ * position p = lens[s] - 1 of sequence s = seqs[r]; state is float32 [nseq, H, 128, 128] (K-major, as s_out) and
+ * ring bf16 [nseq, 4, (2 HK + H) * 128], the pre-conv row of position i in ring row i % 4; both are
+ * updated in place.  At p = 0 the state and at p < 3 the rows before position 0 count as zero, whatever
+ * is stored.  All in float32, rounded once in out [B, H, 128].  Padding rows (also lens[s] < 1) get
+ * zeros.  lens is a page table's, or any device array of nseq lengths; B <= 8192, state on 16 bytes. */
+int cs1_gdn_decode(const void* qkv, int ld, const void* w, const void* z, const void* b, const void* a,
+                   const void* A_log, const void* dt_bias, const void* norm_w, float eps, void* ring, float* state,
+                   const int32_t* seqs, const int32_t* lens, int nseq, void* out, int B, int H, int HK, float scale,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,32 @@
+// The page table of the decode operations: its checks on the host and the lists of sequences on the device.
+#pragma once
+
+#include "common.h"
+
+namespace q35 {
+
+constexpr int MAX_LISTED = 8192;  // sequences of a table, rows of a list (kv_pages.hip keeps one int each in LDS)
+
+inline bool table_ok(const Cs1PageTable* t) {
+    return t && all_set({t->table, t->lens, t->refs}) && t->nseq > 0 && t->nseq <= MAX_LISTED && t->max_pages > 0 &&
+           t->npages > 0 && t->page >= 16 && t->page % 16 == 0 && (int64_t)t->max_pages * t->page < (int64_t{1} << 31);
+}
+
+inline bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// The sequence of list entry i, or -1 for a padding row.
+__device__ __forceinline__ int listed_seq(const int32_t* __restrict__ seqs, int i, int nseq) {
+    const int s = seqs ? seqs[i] : i;
+    return s >= 0 && s < nseq ? s : -1;
+}
+
+// Whether an entry before i names the same sequence (this thread's share of the entries; the
+// block's threads together see all of them).
+__device__ __forceinline__ bool named_before(const int32_t* __restrict__ seqs, int i, int s) {
+    bool hit = false;
+    if (seqs)
+        for (int j = threadIdx.x; j < i; j += blockDim.x) hit |= seqs[j] == s;
+    return hit;
+}
+
+}  // namespace q35

@@ -85,6 +85,17 @@ ADDITIONS = {
     "cs1_gdn_prefill_gated_x": (_I, [P, P, P, P, P, _I, P, P, P, P, _I, _I, _I, c_float, P, P, P]),
     "cs1_gdn_prefill_gated_varlen": (_I, [P, P, P, P, P, _I, P, P, P, P, P, _I, _I, _I, c_float, P, _SZ, P, _SZ,
                                           P]),
+    "cs1_kv_reserve": (_I, [P, P, P, _I, P, P]),
+    "cs1_kv_write": (_I, [P, P, P, _I, P, _I, P, _I, P, P, _I, _I, P]),
+    "cs1_kv_workspace_bytes": (_SZ, [_I, _I]),
+    "cs1_kv_fork": (_I, [P, P, P, _I, P, _I, _SZ, P, P, P]),
+    "cs1_kv_free": (_I, [P, P, _I, P]),
+    "cs1_kv_compact": (_I, [P, P, _I, _SZ, P, P, P]),
+    "cs1_kv_copy": (_I, [P, _I, _SZ, _I, P, P, _I, P]),
+    "cs1_attention_paged_create": (P, []),
+    "cs1_attention_paged_destroy": (None, [P]),
+    "cs1_attention_paged": (_I, [P, P, P, P, P, P, P, P, P, _I, _I, _I, _I, c_float, P]),
+    "cs1_gdn_decode": (_I, [P, _I, P, P, P, P, P, P, P, c_float, P, P, P, P, _I, P, _I, _I, _I, c_float, P]),
 }
 # ... and test hooks outside the op ABI: one forces the GDN prep / scan kernel forms that the
 # bit-identity tests compare (-1: the shape-based choice), the others give the scan's form and the
@@ -100,6 +111,14 @@ TEST_HOOKS = {
     "q35_gemm_plan_of": (_I, [P, _I, _I, _I, _I, _PI, _PI]),
     "q35_gemm_force": (_I, [P, _I, _I]),
 }
+
+
+class PageTable(ctypes.Structure):
+    """Cs1PageTable: device addresses of table, lens and refs, and the sizes."""
+
+    _fields_ = [("table", c_void_p), ("lens", c_void_p), ("refs", c_void_p), ("nseq", _I), ("max_pages", _I),
+                ("npages", _I), ("page", _I)]
+
 
 HIP_ERROR_INVALID_VALUE = 1
 HIP_ERROR_NOT_SUPPORTED = 801

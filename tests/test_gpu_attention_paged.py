@@ -1,0 +1,265 @@
+"""cs1_attention_paged against attention in float64 (decode_ref.attention), within bounds that follow from
+the roundings of float32 sums and one bfloat16 output."""
+import numpy as np
+import pytest
+
+import decode_ref as R
+from decode_ref import DeviceTable, ints
+from gpu_helpers import dev, empty, get, get_bf16, say, stream
+from qwen3_5_native import hip
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def handle():
+    stream()
+    h = hip.api().cs1_attention_paged_create()
+    assert h
+    yield h
+    hip.api().cs1_attention_paged_destroy(h)
+
+
+class Call:
+    def __init__(self, handle, rng, t, seqs, hq, hk, dh, gate=True, lse=True, std=1.0):
+        self.handle, self.t, self.seqs, self.hq, self.hk, self.dh = handle, t, np.asarray(seqs, np.int32), hq, hk, dh
+        B = len(seqs)
+        self.q, self.gate = R.bf16(rng, B, hq, dh, std=std), R.bf16(rng, B, hq, dh) if gate else None
+        self.kp, self.vp = R.bf16(rng, t.npages, t.page, hk, dh, std=std), R.bf16(rng, t.npages, t.page, hk, dh)
+        self.lse = lse
+
+    def upload(self):
+        self.d = DeviceTable(self.t)
+        self.bufs = [dev(x) for x in (self.q, self.kp, self.vp, self.seqs)]
+        self.g = dev(self.gate) if self.gate is not None else None
+        B = len(self.seqs)
+        self.out, self.l = dev(np.full(B * self.hq * self.dh + 8, 0x7fc1, np.uint16)), dev(np.full(B * self.hq + 1, 5.0, np.float32))
+
+    def launch(self, st=None, null=False):
+        q, kp, vp, seqs = self.bufs
+        hip.check(hip.api().cs1_attention_paged(
+            self.handle, q.at(0), kp.at(0), vp.at(0), self.d.ref, None if null else seqs.at(0), self.g.at(0) if self.g else None,
+            self.out.at(0), self.l.at(0) if self.lse else None, len(self.seqs), self.hq, self.hk, self.dh, self.dh ** -0.5,
+            st or stream().handle), "attention_paged")
+
+    def results(self):
+        B = len(self.seqs)
+        n = B * self.hq * self.dh
+        out, l = get_bf16(self.out, n + 8), get(self.l, np.float32, B * self.hq + 1)
+        assert (out[n:] == 0x7fc1).all() and l[-1] == 5.0, "written behind the last row"
+        return out[:n].reshape(B, self.hq, self.dh), l[:-1].reshape(self.hq, B)
+
+    def check(self, seqs=None):
+        out, l = self.results()
+        want, wl, tol, ltol = R.attention(self.t, self.seqs if seqs is None else seqs, self.q, self.kp, self.vp, self.gate,
+                                          self.hk, self.dh ** -0.5)
+        R.close(R.f64(out), want, tol, "out")
+        if self.lse:
+            R.close(l.astype(np.float64), wl, ltol, "lse")
+
+
+@pytest.mark.parametrize("hq,hk,dh", [(16, 4, 128), (16, 4, 256), (24, 4, 256), (4, 4, 128), (16, 1, 256), (6, 2, 128), (32, 1, 128),
+                                      (17, 1, 256), (40, 2, 128), (1, 1, 256)])
+@pytest.mark.parametrize("page", [16, 48, 64])
+def test_head_layouts(handle, hq, hk, dh, page):
+    say(f"paged attention heads {hq}/{hk} Dh={dh} page={page}")
+    rng = np.random.default_rng(hq * hk + page)
+    lens = [1, 0, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 130, 257, 300]
+    t = R.scattered(rng, len(lens) + 2, lens, page)
+    c = Call(handle, rng, t, rng.permutation(len(lens) + 2), hq, hk, dh, gate=page != 64, lse=page != 16)
+    c.upload()
+    c.launch()
+    c.check()
+
+
+@pytest.mark.parametrize("lens", [[5000], [1, 4000], [700, 700, 700], [8191, 3, 0, 900], [127] * 70, [12000, 1, 1, 1, 1],
+                                  list(range(1, 400, 7)), [2049], [40000]], ids=lambda l: f"{len(l)}x{max(l)}")
+@pytest.mark.parametrize("hq,hk,dh,page", [(16, 4, 128, 16), (24, 4, 256, 208), (20, 1, 256, 32)])
+def test_lengths(handle, lens, hq, hk, dh, page):
+    """Sequences that fill the chip alone and together, split and whole."""
+    say(f"paged attention {len(lens)} sequences up to {max(lens)}, heads {hq}/{hk} Dh={dh} page={page}")
+    rng = np.random.default_rng(sum(lens) + dh)
+    t = R.scattered(rng, len(lens), lens, page)
+    c = Call(handle, rng, t, rng.permutation(len(lens)), hq, hk, dh)
+    c.upload()
+    c.launch()
+    c.check()
+
+
+def test_padding_repeats_and_no_list(handle):
+    say("paged attention: padding rows, a sequence twice, no list")
+    rng = np.random.default_rng(3)
+    t = R.scattered(rng, 5, [70, 0, 33, 500, 16], 16)
+    c = Call(handle, rng, t, [3, -1, 0, 5, 0, 2 ** 31 - 1, 1, -2 ** 31, 4, 3], 8, 2, 128)
+    c.upload()
+    c.launch()
+    c.check()
+    out, l = c.results()
+    for r in (1, 3, 5, 6, 7):
+        assert (out[r] == 0).all() and (l[:, r] == -np.inf).all()
+    c.launch(null=True)  # row i is sequence i; rows from nseq on are padding
+    c.check(seqs=list(range(5)) + [-1] * 5)
+
+
+def test_what_is_not_held_is_not_read(handle):
+    """NaN and infinities in every slot that no token of the sequence has, and in pages of others."""
+    say("paged attention: NaN around")
+    rng = np.random.default_rng(4)
+    lens = [1, 17, 40, 129, 1000, 0]
+    t = R.scattered(rng, 6, lens, 48)
+    c = Call(handle, rng, t, range(6), 16, 4, 256)
+    held = np.zeros((t.npages, t.page), bool)
+    for s, n in enumerate(lens):
+        for j in range(n):
+            held[t.table[s, j // 48], j % 48] = True
+    for pool, bits in ((c.kp, 0x7fc0), (c.vp, 0x7f80)):
+        pool[~held] = bits
+    c.vp[~held, :, ::2] = 0xffc0
+    c.upload()
+    c.launch()
+    c.check()
+    assert np.isfinite(R.f64(c.results()[0])).all()
+
+
+def test_a_token_of_infinities_is_its_own_rows_matter(handle):
+    say("paged attention: infinite values in one sequence")
+    rng = np.random.default_rng(5)
+    t = R.scattered(rng, 3, [40, 50, 300], 16)
+    c = Call(handle, rng, t, range(3), 8, 4, 128)
+    c.vp[t.table[1, 0], 5, 2, 7] = 0x7f80  # +inf in kv head 2, dim 7
+    c.kp[t.table[2, 3], 0, 1] = 0x7fc0     # NaN keys in kv head 1
+    c.upload()
+    c.launch()
+    out = R.f64(c.results()[0])
+    assert np.isfinite(out[0]).all()
+    hit = np.zeros((8, 128), bool)
+    hit[4:6, 7] = True
+    assert (out[1][hit] == np.inf).all() and np.isfinite(out[1][~hit]).all()
+    assert np.isnan(out[2, 2:4]).all() and np.isfinite(out[2, :2]).all() and np.isfinite(out[2, 4:]).all()
+
+
+@pytest.mark.parametrize("std", [8.0, 40.0])
+def test_large_scores(handle, std):
+    """Scores of hundreds to tens of thousands: the maximum moves by far more than a float's exponent holds."""
+    say(f"paged attention: large scores, std {std}")
+    rng = np.random.default_rng(6)
+    t = R.scattered(rng, 4, [3000, 100, 1, 650], 32)
+    c = Call(handle, rng, t, range(4), 16, 4, 128, std=std)
+    c.upload()
+    c.launch()
+    c.check()
+
+
+def test_bad_page_numbers_are_masked(handle):
+    say("paged attention: page numbers out of range")
+    rng = np.random.default_rng(7)
+    t = R.scattered(rng, 4, [100, 700, 30, 64], 16)
+    t.table[0, 2], t.table[1, 0], t.table[1, 43], t.table[2] = t.npages, -1, 2 ** 31 - 1, -2 ** 31
+    c = Call(handle, rng, t, range(4), 16, 4, 256)
+    c.upload()
+    c.launch()
+    c.check()
+
+
+def test_more_tokens_than_the_table_has_room_for(handle):
+    say("paged attention: a length past the table's row")
+    rng = np.random.default_rng(8)
+    t = R.scattered(rng, 2, [64, 20], 16, max_pages=4)
+    c = Call(handle, rng, t, range(2), 8, 4, 128)
+    c.upload()
+    lens = dev(np.array([2 ** 31 - 1, 20], np.int32))
+    c.d.struct.lens = lens.at(0)
+    c.launch()
+    c.check()
+
+
+def test_the_same_bits_every_time_and_in_a_graph(handle):
+    """Repeated, captured and replayed calls; the graph serves other lengths when it is replayed."""
+    say("paged attention: repeats and graphs")
+    rng = np.random.default_rng(9)
+    t = R.scattered(rng, 6, [9000, 5, 700, 64, 0, 2000], 64, spare=8)
+    c = Call(handle, rng, t, [0, 5, 2, 3, 4, 1, -1], 16, 4, 256)
+    c.upload()
+    c.launch()
+    c.check()
+    first = c.results()
+    for _ in range(3):
+        c.launch()
+        for a, b in zip(c.results(), first):
+            np.testing.assert_array_equal(a, b)
+    g = hip.Graph(stream(), c.launch)
+    for lens in ([9000, 5, 700, 64, 0, 2000], [1, 0, 650, 33, 0, 1999], [8999, 5, 1, 64, 0, 2000]):
+        t.lens[:] = lens
+        hip.upload(c.d.lens, t.lens, stream())
+        g.launch(stream())
+        stream().sync()
+        c.check()
+        again = c.results()
+        g.launch(stream())
+        for a, b in zip(c.results(), again):
+            np.testing.assert_array_equal(a, b)
+
+
+def test_two_streams_with_a_handle_each(handle):
+    say("paged attention: two streams, a handle each")
+    rng = np.random.default_rng(10)
+    other = hip.Stream()
+    h2 = hip.api().cs1_attention_paged_create()
+    t = R.scattered(rng, 4, [6000, 800, 3, 2500], 16)
+    a, b = Call(handle, rng, t, range(4), 16, 4, 128), Call(h2, rng, t, range(4), 24, 4, 256)
+    a.upload()
+    b.upload()
+    stream().sync()
+    for _ in range(5):
+        a.launch()
+        b.launch(other.handle)
+    other.sync()
+    a.check()
+    b.check()
+    other.destroy()
+    hip.api().cs1_attention_paged_destroy(h2)
+
+
+def test_sizes_one_after_another_with_one_handle(handle):
+    """A large call, a small one, a split one: nothing of the call before is left in the handle."""
+    say("paged attention: sizes in turn")
+    rng = np.random.default_rng(11)
+    for lens, hq, hk, dh in (([3000] * 20, 24, 4, 256), ([5], 16, 4, 128), ([20000], 16, 1, 256), ([100, 4000], 32, 1, 128)):
+        t = R.scattered(rng, len(lens), lens, 32)
+        c = Call(handle, rng, t, range(len(lens)), hq, hk, dh)
+        c.upload()
+        c.launch()
+        c.check()
+
+
+def test_many_rows(handle):
+    say("paged attention: 3000 rows")
+    rng = np.random.default_rng(12)
+    lens = rng.integers(0, 40, 100)
+    t = R.scattered(rng, 100, lens.tolist(), 16)
+    c = Call(handle, rng, t, rng.integers(-1, 101, 3000), 4, 2, 128)
+    c.upload()
+    c.launch()
+    c.check()
+
+
+def test_refusals_with_a_handle(handle):
+    say("paged attention: refusals")
+    rng = np.random.default_rng(13)
+    t = R.scattered(rng, 1, [5], 16)
+    c = Call(handle, rng, t, [0], 4, 2, 128)
+    c.upload()
+    api, st = hip.api(), stream().handle
+    q, kp, vp, seqs = (b.at(0) for b in c.bufs)
+    out = c.out.at(0)
+
+    def call(q=q, kp=kp, vp=vp, gate=None, out=out, B=1, hq=4, hk=2, dh=128):
+        return api.cs1_attention_paged(handle, q, kp, vp, c.d.ref, seqs, gate, out, None, B, hq, hk, dh, 1.0, st)
+
+    assert call(dh=64) == call(hq=5) == call(hk=0) == call(B=-1) == call(hq=0) == hip.HIP_ERROR_INVALID_VALUE
+    assert call(q=None) == call(kp=None) == call(vp=None) == call(out=None) == hip.HIP_ERROR_INVALID_VALUE
+    assert call(q=q + 8) == call(kp=kp + 2) == call(vp=vp + 4) == call(out=out + 8) == call(gate=q + 2) == hip.HIP_ERROR_INVALID_VALUE
+    assert call(B=1 << 23) == hip.HIP_ERROR_INVALID_VALUE
+    assert call(B=0, q=None) == 0
+    (out_before, _) = c.results()
+    assert (out_before == 0x7fc1).all()

@@ -1,0 +1,238 @@
+"""The page operations (cs1_kv_*) against the bookkeeping step by step (decode_ref.Table): table, lengths,
+counts and every byte of the pools are equal after each call."""
+import numpy as np
+import pytest
+
+import decode_ref as R
+from decode_ref import DeviceTable, Table, ints, pointers, pool_buffers, read_pool
+from gpu_helpers import dev, empty, get, say, stream
+from qwen3_5_native import hip
+
+pytestmark = pytest.mark.gpu
+
+
+class Cache:
+    """A device table with pools, and the same on the host."""
+
+    def __init__(self, t, rng, npools, width):
+        self.t, self.d, self.width = t, DeviceTable(t), width
+        self.pools = [R.bf16(rng, t.npages, t.page, width) for _ in range(npools)]
+        self.bufs = pool_buffers(self.pools)
+        self.ptrs = pointers(self.bufs)
+        self.status = ints([77])
+        self.ws = empty(hip.api().cs1_kv_workspace_bytes(t.npages, 8192))
+
+    def check(self, what):
+        self.d.check()
+        for i, (b, p) in enumerate(zip(self.bufs, self.pools)):
+            np.testing.assert_array_equal(read_pool(b, p), p, err_msg=f"{what}: pool {i}")
+
+    def status_is(self, want):
+        assert int(get(self.status, np.int32, 1)[0]) == want
+
+    def reserve(self, seqs, cu=None, null=False):
+        say(f"  reserve {len(seqs)} cu={cu is not None}")
+        want = self.t.reserve(seqs, cu)
+        b = ints(seqs) if len(seqs) else None
+        hip.check(hip.api().cs1_kv_reserve(self.d.ref, None if null or b is None else b.at(0),
+                                           cu.ctypes.data if cu is not None else None, len(seqs), self.status.at(0),
+                                           stream().handle), "reserve")
+        self.status_is(want)
+        self.check("reserve")
+        return want
+
+    def write(self, seqs, cu, rng, layer=0, pad=(0, 8)):
+        rows = len(seqs) if cu is None else int(cu[-1])
+        say(f"  write {rows} rows of {len(seqs)} sequences")
+        k, v = R.bf16(rng, rows, self.width + pad[0]), R.bf16(rng, rows, self.width + pad[1])
+        kp, vp = 2 * layer, 2 * layer + 1
+        self.t.write(seqs, cu, k[:, :self.width], v[:, :self.width], self.pools[kp], self.pools[vp])
+        b, kb, vb = ints(seqs), dev(k), dev(v)
+        hip.check(hip.api().cs1_kv_write(self.d.ref, b.at(0), cu.ctypes.data if cu is not None else None, len(seqs),
+                                         kb.at(0), self.width + pad[0], vb.at(0), self.width + pad[1], self.bufs[kp].at(0),
+                                         self.bufs[vp].at(0), self.width // 8, 8, stream().handle), "write")
+        self.check("write")
+
+    def fork(self, src, dst):
+        say(f"  fork {len(src)}")
+        want = self.t.fork(src, dst, self.pools)
+        a, b = ints(src), ints(dst)
+        hip.check(hip.api().cs1_kv_fork(self.d.ref, a.at(0), b.at(0), len(src), self.ptrs, len(self.bufs),
+                                        2 * self.width, self.ws.at(0), self.status.at(0), stream().handle), "fork")
+        self.status_is(want)
+        self.check("fork")
+        return want
+
+    def free(self, seqs):
+        say(f"  free {len(seqs)}")
+        self.t.free(seqs)
+        b = ints(seqs)
+        hip.check(hip.api().cs1_kv_free(self.d.ref, b.at(0), len(seqs), stream().handle), "free")
+        self.check("free")
+
+    def compact(self):
+        say("  compact")
+        want = self.t.compact(self.pools)
+        hip.check(hip.api().cs1_kv_compact(self.d.ref, self.ptrs, len(self.bufs), 2 * self.width, self.ws.at(0),
+                                           self.status.at(0), stream().handle), "compact")
+        self.status_is(want)
+        self.check("compact")
+
+
+@pytest.mark.parametrize("nseq,page,npages,max_pages,npools,width", [
+    (1, 16, 5, 4, 2, 8), (6, 16, 40, 9, 2, 512), (13, 48, 61, 7, 4, 72), (40, 64, 150, 5, 6, 128), (9, 208, 30, 3, 2, 1024)])
+def test_a_server_at_work(nseq, page, npages, max_pages, npools, width):
+    """Random calls: ragged prompts and single tokens, forks, ends, compactions; pools that run out."""
+    say(f"server nseq={nseq} page={page} npages={npages}")
+    rng = np.random.default_rng(nseq * page)
+    c = Cache(Table(nseq, max_pages, npages, page), rng, npools, width)
+    seen = set()
+    for step in range(30):
+        kind = rng.choice(["prompt", "token", "token", "fork", "free", "compact"])
+        pick = rng.permutation(nseq)[:rng.integers(1, nseq + 1)]
+        # padding and a sequence named twice among them
+        pick = np.concatenate([pick, [-1, nseq, pick[0]]])[rng.permutation(len(pick) + 3)]
+        if kind == "prompt" and len(pick) <= 64:
+            lens = rng.integers(0, 2 * page + 3, len(pick))
+            cu = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+            got = c.reserve(pick, cu)
+            if got == 0:
+                c.write(pick, cu, rng, layer=int(rng.integers(npools // 2)))
+            seen.add(("prompt", np.sign(got)))
+        elif kind == "token":
+            got = c.reserve(pick)
+            if got == 0:
+                c.write(pick, None, rng, layer=int(rng.integers(npools // 2)), pad=(16, 0))
+            seen.add(("token", np.sign(got)))
+        elif kind == "fork":
+            src, dst = rng.integers(-1, nseq + 1, len(pick)), pick
+            got = c.fork(src, dst)
+            seen.add(("fork", np.sign(got)))
+        elif kind == "free":
+            c.free(pick[:max(1, len(pick) // 2)])
+        else:
+            c.compact()
+    say(f"  seen {sorted((k, int(v)) for k, v in seen)}")
+
+
+def test_what_reserve_says_when_room_is_short():
+    say("reserve: short of pages, of a table's width, empty lists, null list")
+    rng = np.random.default_rng(0)
+    c = Cache(Table(4, 3, 6, 16), rng, 2, 8)
+    assert c.reserve([0, 1], np.array([0, 48, 90], np.int32)) == 0  # three pages each: all six
+    assert c.reserve([2, 3]) == 2
+    assert c.reserve([0]) == -1
+    assert c.reserve([1, 2, 0]) == -1
+    assert c.reserve([1], np.array([0, 6], np.int32)) == 0  # fills its last page
+    c.free([0])
+    # 16 and 33 tokens need one page and three, of three that are free; 49 are more than a row's three pages hold
+    assert c.reserve([2, 3, 2], np.array([0, 16, 49, 60], np.int32)) == 1
+    assert c.reserve([2, 3, 2], np.array([0, 16, 65, 70], np.int32)) == -1
+    assert c.reserve([2, 3], np.array([0, 16, 64], np.int32)) == 1
+    assert c.reserve([2, 3], np.array([0, 16, 48], np.int32)) == 0
+    assert c.reserve([]) == 0
+    assert c.reserve([-1, 9, -5]) == 0
+    c.free([0, 1, 2, 3])
+    assert c.reserve([0, 1, 2, 3, 4, 5], null=True) == 0  # no list: row i is sequence i, rows from nseq on are padding
+
+
+def test_long_lists_and_many_pages():
+    """Lists of more entries than the planning block has threads, pages over several scans."""
+    say("8192 sequences, 9001 pages")
+    rng = np.random.default_rng(1)
+    c = Cache(Table(8192, 3, 9001, 16), rng, 2, 8)
+    every = rng.permutation(8192).astype(np.int32)
+    assert c.reserve(every) == 0
+    assert c.reserve(every[:1000]) == 0
+    c.free(every[rng.permutation(8192)[:4000]])
+    c.compact()
+    src = every[rng.integers(0, 8192, 5000)]
+    empties = np.flatnonzero(c.t.lens == 0)
+    assert c.fork(src, np.resize(empties, 5000)) == 0
+    for _ in range(17):
+        c.reserve(every[:3000])
+    c.compact()
+
+
+@pytest.mark.parametrize("page,part", [(16, 0), (16, 1), (16, 15), (64, 33), (1024, 1000)])
+def test_forks_share_whole_pages_and_copy_the_filled_rows(page, part):
+    say(f"fork page={page} part={part}")
+    rng = np.random.default_rng(part)
+    c = Cache(Table(12, 4, 40, page), rng, 66, 24)  # more pools than one launch takes
+    assert c.reserve([3, 5], np.array([0, 2 * page + part, 2 * page + part + 7], np.int32)) == 0
+    assert c.fork([3, 3, 3, 5, 3, 0, 3, 8], [4, 6, 5, 7, 4, 9, 3, 10]) == 0
+    # a source that is a destination, a destination twice, out of range
+    assert c.fork([3, 0, 3, 3, -1, 3], [0, 1, 2, 2, 11, 12]) == 0
+    c.free([3, 6, 4])
+    c.compact()
+
+
+def test_fork_without_room_changes_nothing():
+    say("fork without room")
+    rng = np.random.default_rng(5)
+    c = Cache(Table(6, 4, 5, 16), rng, 2, 8)
+    assert c.reserve([0], np.array([0, 40], np.int32)) == 0
+    assert c.fork([0, 0, 0, 0], [1, 2, 3, 4]) == 2
+    assert c.fork([0, 0], [1, 2]) == 0
+
+
+def test_numbers_that_no_table_should_hold_are_not_followed():
+    """Page numbers out of range in a table's row: no row is written there, no count changes."""
+    say("bad page numbers")
+    rng = np.random.default_rng(6)
+    t = R.scattered(rng, 3, [40, 20, 17], 16)
+    t.table[0, 1], t.table[1, 1], t.table[2, 1] = t.npages, -7, 2 ** 31 - 1
+    c = Cache(t, rng, 2, 64)
+    c.write([0, 1, 2], np.array([0, 40, 60, 77], np.int32), rng)
+    c.write([0, 1, 2], np.array([0, 50, 90, 110], np.int32), rng)  # more rows than tokens: those before position 0 are left out
+
+
+@pytest.mark.parametrize("bytes_,entries,npools", [(16, 9, 1), (48, 5, 3), (16384 + 16, 7, 70), (2 * 128 * 128 * 4, 6, 2)])
+def test_copies_of_entries(bytes_, entries, npools):
+    say(f"copy {bytes_} bytes, {entries} entries, {npools} pools")
+    rng = np.random.default_rng(entries)
+    pools = [R.bf16(rng, entries, bytes_ // 2) for _ in range(npools)]
+    bufs = pool_buffers(pools)
+    src = np.array([0, 1, 3, -1, 0, entries, 2, 4], np.int32)
+    dst = np.array([2, 2, 1, 0, entries, 1, 3, 4], np.int32)
+    want = [p.copy() for p in pools]
+    for s, d in R.Table(entries, 1, 1, 16).pairs(src, dst, entries):
+        for w, p in zip(want, pools):
+            w[d] = p[s]
+    a, b, ptrs = ints(src), ints(dst), pointers(bufs)
+    hip.check(hip.api().cs1_kv_copy(ptrs, npools, bytes_, entries, a.at(0), b.at(0), len(src),
+                                    stream().handle), "copy")
+    for b, w in zip(bufs, want):
+        np.testing.assert_array_equal(read_pool(b, w), w)
+
+
+def test_offsets_past_32_bits():
+    """The last page of a pool of 5 GiB receives rows, is forked and moves to the front."""
+    say("a pool of 5 GiB")
+    page, width = 64, 1024
+    npages = (5 << 30) // (page * width * 2)
+    t = Table(3, 4, npages, page)
+    t.table[0, 0], t.refs[npages - 1], t.lens[0] = npages - 1, 1, 37
+    t.refs[npages - 2], t.table[1, 0], t.lens[1] = 1, npages - 2, 1
+    t.refs[1:npages - 2] = 1  # held by nobody here: only pages 0 and 1 are of interest
+    t.refs[1] = 0
+    d = DeviceTable(t)
+    pool_k, pool_v = empty(npages * page * width * 2), empty(npages * page * width * 2)
+    rng = np.random.default_rng(2)
+    k, v = R.bf16(rng, 37, width), R.bf16(rng, 37, width)
+    kb, vb = dev(k), dev(v)
+    cu = np.array([0, 37], np.int32)
+    api, st, first, third = hip.api(), stream().handle, ints([0]), ints([2])
+    hip.check(api.cs1_kv_write(d.ref, first.at(0), cu.ctypes.data, 1, kb.at(0), width, vb.at(0), width, pool_k.at(0),
+                               pool_v.at(0), 8, 128, st), "write")
+    last = (npages - 1) * page * width * 2
+    np.testing.assert_array_equal(get(pool_k, np.uint16, 37 * width, last).reshape(37, width), k)
+    ws, status, ptrs = empty(api.cs1_kv_workspace_bytes(npages, 1)), ints([1]), pointers([pool_k, pool_v])
+    hip.check(api.cs1_kv_fork(d.ref, first.at(0), third.at(0), 1, ptrs, 2, width * 2, ws.at(0), status.at(0), st), "fork")
+    assert get(status, np.int32, 1)[0] == 0
+    np.testing.assert_array_equal(get(pool_v, np.uint16, 37 * width, 0).reshape(37, width), v)  # page 0 was the lowest free
+    hip.check(api.cs1_kv_compact(d.ref, ptrs, 2, width * 2, ws.at(0), status.at(0), st), "compact")
+    assert get(status, np.int32, 1)[0] == npages - 1
+    table, _, refs = d.state()
+    assert table[0, 0] == 1 and refs[npages - 1] == 0 and refs[1] == 1
+    np.testing.assert_array_equal(get(pool_v, np.uint16, 37 * width, page * width * 2).reshape(37, width), v)
