@@ -181,7 +181,7 @@ def attention(t, seqs, q, kp, vp, gate, hk, scale):
     A score is a sum of Dh products of bfloat16 values, each exact in float32, so a float32 sum in any order is
     off by at most Dh E32 sum |q k|; it is scaled (E32) and taken to an exponential of base 2, whose argument
     carries two more roundings of |S| and whose value one of a step (2 E32).  The probability's weight goes to the product in two
-    bfloat16 parts, the second rounded: E16^2 of the weight.  The sums over n keys add n E32 each at most."""
+    bfloat16 parts: eight bits cut off, which leaves less than 2 E16 of it, and that rest rounded: 2 E16^2 of the weight.  The sums over n keys add n E32 each at most."""
     B, hq, dh = q.shape
     out, lse = np.zeros((B, hq, dh)), np.full((hq, B), -np.inf)
     tol, ltol = np.zeros((B, hq, dh)), np.zeros((hq, B))
@@ -202,7 +202,7 @@ def attention(t, seqs, q, kp, vp, gate, hk, scale):
             z = w.sum()
             p = w / z
             o = p @ v
-            rel = 2 * (off + off.max()) + 4 * E32 + E16 * E16 + 2 * n * E32  # of each weight, and of their sum
+            rel = 2 * (off + off.max()) + 4 * E32 + 2 * E16 * E16 + 2 * n * E32  # of each weight, and of their sum
             f = 1.0
             if gate is not None:
                 f = 1 / (1 + np.exp(-f64(gate[r, h])))
