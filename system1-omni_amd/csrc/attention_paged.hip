@@ -9,7 +9,7 @@
 // Work: a row and kv head's keys in units of 32, shares of consecutive units to blocks (plan_share below); the q
 // heads of a kv head are the rows of one matrix tile, up to 16 of them (more take several tiles, which read
 // the keys again).  A block's four waves take every fourth unit, each with a running maximum and sum of its own, and join
-// through LDS; the shares of a sequence that has several join in a second, small kernel.
+// through LDS; the shares of a sequence that has several are joined by the last of them to end.
 //
 // A unit in registers, without LDS: S^T = K Q^T takes K rows as they lie (lane l: key l % 16, 8 dims a load) and leaves
 // lane l with q head l % 16 and keys 4 (l / 16) .. + 3 of each 16; that is the layout in which O^T = V^T P^T wants P^T,
@@ -23,6 +23,7 @@
 // P goes to the product in two bfloat16 parts (hi cut off, lo the rounded rest: p to 2^-15): the matrix cores wait for
 // memory here, and the second product leaves the rounding of out the only one that counts.  lo is never zero (LEAST), so
 // that an infinite v gives the infinity that it should and not inf + 0 inf.
+#include <algorithm>
 #include <new>
 #include <type_traits>
 
@@ -34,19 +35,23 @@ namespace {
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int UNIT = 32, ROWS = 16;
+constexpr int LEAST_SHARE = 4;               // units
+constexpr int GROUP = 16, GROUPS_MAX = 64;   // shares that one block joins, groups of a sequence
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float LEAST = 0x1p-126f;  // bfloat16's smallest normal value
 constexpr float RISE = 6.f;  // in powers of two: P stays under 2^6, far from where float32 sums lose anything
 
 struct Paged {
     int device, cus, target;
-    float* part;  // [2 target, ROWS, 256] partial sums, then [2 target, ROWS, 2] maximum and sum
+    float* part;  // [2 target, ROWS, 256] partial sums, [2 target, ROWS, 2] maximum and sum
+    int* count;   // [2 target] shares of a group, [2 target] groups of a sequence that are done
 };
 
 struct Args {
     const bf16 *q, *kp, *vp, *gate;
     bf16* out;
     float *lse, *part, *ml;
+    int* count;
     const int32_t *table, *lens, *seqs;
     int nseq, max_pages, npages, page, B, Hq, Hk, G, tiles, target;
     float scale_log2;
@@ -76,17 +81,17 @@ __device__ __forceinline__ T wave_scan(T x) {  // inclusive
 __device__ __forceinline__ int scalar(int x, int i) { return __builtin_amdgcn_readlane(x, i); }
 
 // The units of a share: all sequences' units over the number of shares that fill the chip, at least one
-// for each wave.  Each wave works it out from the lengths, which only the device knows.
-__device__ __forceinline__ int units_per_share(const Args& a) {
+// for each wave.  Each wave works it out from the lengths, which only the device knows (n0: row lane's).
+__device__ __forceinline__ int units_per_share(const Args& a, int n0) {
     int64_t total = 0;
     for (int r0 = 0; r0 < a.B; r0 += 64) {
-        int64_t u = units_of(keys_of(a, r0 + (threadIdx.x & 63)));
+        int64_t u = units_of(r0 == 0 ? n0 : keys_of(a, r0 + (threadIdx.x & 63)));
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) u += __shfl_xor(u, o, 64);
         total += (int64_t)((uint64_t)(uint32_t)scalar((int)(u >> 32), 0) << 32 | (uint32_t)scalar((int)u, 0));
     }
     total *= a.Hk * a.tiles;
-    return (int)max((int64_t)WAVES, (total + a.target - 1) / a.target);
+    return (int)max((int64_t)LEAST_SHARE, (total + a.target - 1) / a.target);
 }
 
 struct Share {
@@ -96,12 +101,13 @@ struct Share {
 // Share number idx: rows in order, a row's splits, and in each the kv heads and tiles.  Rows without keys
 // have one share (it writes their zeros).  Slots count the shares of rows that have several: with u units and
 // p units a share that is ceil(u / p) < 2 u / p of them, so all slots are fewer than twice the target.
-__device__ __forceinline__ bool find_share(const Args& a, int idx, int per, Share& sh) {
+__device__ __forceinline__ bool find_share(const Args& a, int idx, int n0, Share& sh) {
+    const int per = units_per_share(a, n0);
     const int lane = threadIdx.x & 63, each = a.Hk * a.tiles;
     int64_t before = 0;
     int slots = 0;
     for (int r0 = 0; r0 < a.B; r0 += 64) {
-        const int r = r0 + lane, n = keys_of(a, r), splits = r < a.B ? max(1, (units_of(n) + per - 1) / per) : 0;
+        const int r = r0 + lane, n = r0 == 0 ? n0 : keys_of(a, r), splits = r < a.B ? max(1, (units_of(n) + per - 1) / per) : 0;
         const int mine = splits * each, in = wave_scan(mine), sl = splits > 1 ? mine : 0, in_sl = wave_scan(sl);
         const uint64_t hit = __ballot(idx >= before + in - mine && idx < before + in);
         if (hit) {
@@ -136,14 +142,29 @@ __device__ __forceinline__ void store_out(const Args& a, size_t at, const f32x4&
     *reinterpret_cast<u32x2*>(a.out + at) = u32x2{pack2(y[0], y[1]), pack2(y[2], y[3])};
 }
 
+__device__ __forceinline__ float log_sum(float top, float sum) {
+    return sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
+}
+
+// Values that another block reads in the same launch.  Each XCD has an L2 of its own, so they are written through
+// it and read past it (the accesses of an agent-scope atomic); a fence would instead write back all that the L2 holds,
+// for every wave that executes it: 240 us in place of 25 for 32768 keys in 1024 shares.
+__device__ __forceinline__ void put_shared(float* p, f32x2 v) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x2 get_shared(const float* p) {
+    return __builtin_bit_cast(f32x2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                                       __HIP_MEMORY_SCOPE_AGENT));
+}
+
 template <int DH>
 __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args a) {
     constexpr int C = DH / 32, H = DH / 128, PITCH = DH + 8;
     extern __shared__ __attribute__((aligned(16))) float lds[];  // Q as operands, [C][64 lanes] x 16 bytes; later [WAVES][rows][PITCH]
     __shared__ float wm[WAVES][ROWS], wl[WAVES][ROWS];
     Share sh;
-    const int per = units_per_share(a);
-    if (!find_share(a, blockIdx.x, per, sh)) return;
+    if (!find_share(a, blockIdx.x, keys_of(a, threadIdx.x & 63), sh)) return;
     const int lane = threadIdx.x & 63, wave = scalar(threadIdx.x >> 6, 0), col = lane & 15, grp = lane >> 4;
     const int rows = min(ROWS, a.G - sh.tile * ROWS), head0 = sh.head * a.G + sh.tile * ROWS;
     const int s = scalar(sh.n > 0 ? (a.seqs ? a.seqs[sh.row] : sh.row) : 0, 0);
@@ -308,6 +329,19 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
                 *reinterpret_cast<f32x4*>(to + 4) = f32x4{acc[h][4][r], acc[h][5][r], acc[h][6][r], acc[h][7][r]};
             }
     __syncthreads();
+    // four dims of a row's result: to the output, or to a slot
+    auto store = [&](int slot, int row, int d, float top, float sum, const f32x4& o, bool out) {
+        const int head = head0 + row;
+        if (out) {
+            store_out(a, ((size_t)sh.row * a.Hq + head) * DH + d, o, sum);
+            if (a.lse && d == 0) a.lse[(size_t)head * a.B + sh.row] = log_sum(top, sum);
+            return;
+        }
+        const size_t at = (size_t)slot * ROWS + row;
+        put_shared(a.part + at * DH + d, f32x2{o[0], o[1]});
+        put_shared(a.part + at * DH + d + 2, f32x2{o[2], o[3]});
+        if (d == 0) put_shared(a.ml + at * 2, f32x2{top, sum});
+    };
     for (int e = threadIdx.x; e < rows * (DH / 4); e += THREADS) {
         const int row = e / (DH / 4), d = e % (DH / 4) * 4;
         float top = -INFINITY, sum = 0.f;
@@ -320,49 +354,59 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
             sum += wl[w][row] * f;
             o += *reinterpret_cast<const f32x4*>(lds + ((size_t)w * rows + row) * PITCH + d) * f;
         }
-        const int head = head0 + row;
-        if (sh.splits == 1) {
-            store_out(a, ((size_t)sh.row * a.Hq + head) * DH + d, o, sum);
-            if (a.lse && d == 0) a.lse[(size_t)head * a.B + sh.row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
-        } else {
-            const size_t at = (size_t)(sh.slot + sh.split) * ROWS + row;
-            *reinterpret_cast<f32x4*>(a.part + at * DH + d) = o;
-            if (d == 0) *reinterpret_cast<f32x2*>(a.ml + at * 2) = f32x2{top, sum};
-        }
+        store(sh.slot + sh.split, row, d, top, sum, o, sh.splits == 1);
     }
-}
+    if (sh.splits == 1) return;
 
-// Joins the shares of a row's q head where there are several: one block of DH / 4 threads (four dims each).
-template <int DH>
-__global__ void __launch_bounds__(64) attention_paged_join_kernel(const Args a) {
-    const int row = blockIdx.x / a.Hq, head = blockIdx.x % a.Hq, kv = head / a.G, tile = head % a.G / ROWS;
-    const int lane = threadIdx.x, per = units_per_share(a), each = a.Hk * a.tiles;
-    const int n = keys_of(a, row), splits = max(1, (units_of(n) + per - 1) / per);
-    if (splits == 1) return;
-    int slot = 0;
-    for (int r0 = 0; r0 <= row; r0 += 64) {
-        const int r = r0 + lane, k = r < row ? (units_of(keys_of(a, r)) + per - 1) / per : 0;
-        slot += __shfl(wave_scan(k > 1 ? k * each : 0), 63, 64);
-    }
-    slot += (kv * a.tiles + tile) * splits;
-    const int in_tile = head % a.G % ROWS;
-    float top = -INFINITY, sum = 0.f;
-    for (int k = 0; k < splits; k++) top = fmaxf(top, a.ml[((size_t)(slot + k) * ROWS + in_tile) * 2]);
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < splits; k++) {
-        const size_t at = (size_t)(slot + k) * ROWS + in_tile;
-        const float m = a.ml[at * 2], f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
-        sum += a.ml[at * 2 + 1] * f;
-        if (lane < DH / 4) o += *reinterpret_cast<const f32x4*>(a.part + at * DH + lane * 4) * f;
-    }
-    if (lane < DH / 4) store_out(a, ((size_t)row * a.Hq + head) * DH + lane * 4, o, sum);
-    if (a.lse && lane == 0) a.lse[(size_t)head * a.B + row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
+    // Groups of `group` shares: the last of a group to end joins it, the last group joins the groups; always in order, so the
+    // result does not depend on which ends last.  The counters are zero again afterwards.
+    const int group = max(GROUP, (sh.splits + GROUPS_MAX - 1) / GROUPS_MAX), groups = (sh.splits + group - 1) / group;
+    const int g0 = sh.split / group * group;
+    auto last_of = [&](int* count, int n) {
+        __shared__ int last;
+        wait_vm_all();  // what this wave has put is where the others look
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+            if (last) *count = 0;
+        }
+        __syncthreads();
+        return last != 0;
+    };
+    // n results from slot on, `step` slots apart: out, or back to the first slot
+    auto join = [&](int slot, int step, int n, bool out) {
+        f32x2* const ml = reinterpret_cast<f32x2*>(lds);
+        for (int e = threadIdx.x; e < n * rows; e += THREADS)
+            ml[e] = get_shared(a.ml + ((size_t)(slot + e / rows * step) * ROWS + e % rows) * 2);
+        __syncthreads();
+        for (int e = threadIdx.x; e < rows * (DH / 4); e += THREADS) {
+            const int row = e / (DH / 4), d = e % (DH / 4) * 4;
+            float top = -INFINITY, sum = 0.f;
+            for (int k = 0; k < n; k++) top = fmaxf(top, ml[k * rows + row][0]);
+            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+            float* const from = a.part + ((size_t)slot * ROWS + row) * DH + d;
+#pragma unroll 16
+            for (int k = 0; k < n; k++) {
+                const float* const p = from + (size_t)k * step * ROWS * DH;
+                const f32x2 m = ml[k * rows + row], lo = get_shared(p), hi = get_shared(p + 2);
+                const float f = m[0] == top ? 1.f : __builtin_amdgcn_exp2f(m[0] - top);
+                sum += m[1] * f;
+                o += f32x4{lo[0], lo[1], hi[0], hi[1]} * f;
+            }
+            store(slot, row, d, top, sum, o, out);
+        }
+    };
+    if (!last_of(a.count + sh.slot + g0 / group, min(group, sh.splits - g0))) return;
+    join(sh.slot + g0, 1, min(group, sh.splits - g0), groups == 1);
+    if (groups == 1 || !last_of(a.count + 2 * a.target + sh.slot, groups)) return;
+    join(sh.slot, group, groups, true);
 }
 
 template <int DH>
 size_t lds_bytes(int rows) {
     const size_t q = 16 * 64 * (DH / 32), join = sizeof(float) * WAVES * rows * (DH + 8);
-    return q > join ? q : join;
+    const size_t group = sizeof(f32x2) * GROUPS_MAX * rows;
+    return std::max(q, std::max(join, group));
 }
 
 template <int DH>
@@ -375,9 +419,6 @@ template <int DH>
 int launch(const Args& a, hipStream_t st) {
     const int64_t shares = (int64_t)a.target + (int64_t)a.B * a.Hk * a.tiles;
     attention_paged_kernel<DH><<<(unsigned)shares, THREADS, lds_bytes<DH>(a.G < ROWS ? a.G : ROWS), st>>>(a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    if ((int64_t)a.max_pages * a.page > WAVES * UNIT) attention_paged_join_kernel<DH><<<a.B * a.Hq, 64, 0, st>>>(a);
     return hipGetLastError();
 }
 
@@ -397,12 +438,17 @@ extern "C" void* cs1_attention_paged_create(void) {
     if (!p) return nullptr;
     p->device = device;
     p->cus = cus;
-    p->target = 4 * cus;
-    if (hipMalloc(reinterpret_cast<void**>(&p->part), sizeof(float) * 2 * p->target * ROWS * (256 + 2)) != hipSuccess) {
+    p->target = std::min(4 * cus, GROUPS_MAX * GROUPS_MAX);
+    const size_t floats = (size_t)2 * p->target * ROWS * (256 + 2), counts = (size_t)4 * p->target;
+    p->part = nullptr;
+    if (hipMalloc(reinterpret_cast<void**>(&p->part), 4 * (floats + counts)) != hipSuccess ||
+        hipMemset(p->part + floats, 0, 4 * counts) != hipSuccess || hipStreamSynchronize(nullptr) != hipSuccess) {
         (void)hipGetLastError();
+        if (p->part) (void)hipFree(p->part);
         delete p;
         return nullptr;
     }
+    p->count = reinterpret_cast<int*>(p->part + floats);
     return p;
 }
 
@@ -434,6 +480,7 @@ extern "C" int cs1_attention_paged(void* paged, const void* q, const void* kp, c
     a.lse = lse;
     a.part = p->part;
     a.ml = p->part + (size_t)2 * p->target * ROWS * 256;
+    a.count = p->count;
     a.table = pages->table;
     a.lens = pages->lens;
     a.seqs = seqs;
