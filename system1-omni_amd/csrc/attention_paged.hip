@@ -6,10 +6,12 @@
 //
 // The keys and values are read once and nothing else is of size, so the rate of that stream is the bound.
 //
-// Work: a row and kv head's keys in units of 32, shares of consecutive units to blocks (plan_share below); the q
-// heads of a kv head are the rows of one matrix tile, up to 16 of them (more take several tiles, which read
-// the keys again).  A block's four waves take every fourth unit, each with a running maximum and sum of its own, and join
-// through LDS; the shares of a sequence that has several are joined by the last of them to end.
+// Work: the q heads of a kv head are the rows of one matrix tile, up to 16 of them (more take several tiles, which read
+// the keys again).  The keys of all rows, kv heads and tiles, in chunks of 128, are one line of work that is cut into equal
+// stretches, one for each block that the chip holds at once: whatever the lengths, every block streams the same amount and all end
+// together.  A stretch may begin and end inside a sequence; what it has of one (a segment) is joined with the other
+// blocks' parts by the last of them to end.  Within a block four waves take every fourth unit of 32 keys, each with a
+// running maximum and sum of its own, and join through LDS.
 //
 // A unit in registers, without LDS: S^T = K Q^T takes K rows as they lie (lane l: key l % 16, 8 dims a load) and leaves
 // lane l with q head l % 16 and keys 4 (l / 16) .. + 3 of each 16; that is the layout in which O^T = V^T P^T wants P^T,
@@ -35,36 +37,39 @@ namespace {
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int UNIT = 32, ROWS = 16;
-constexpr int LEAST_SHARE = 4;               // units
-constexpr int GROUP = 16, GROUPS_MAX = 64;   // shares that one block joins, groups of a sequence
+constexpr int CHUNK_UNITS = 4, CHUNK = CHUNK_UNITS * UNIT;
+constexpr int GROUP = 64, BATCH = 16;  // parts that one block joins, and how many of them are on their way at once
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float LEAST = 0x1p-126f;  // bfloat16's smallest normal value
 constexpr float RISE = 6.f;  // in powers of two: P stays under 2^6, far from where float32 sums lose anything
 
 struct Paged {
-    int device, cus, target;
-    float* part;  // [2 target, ROWS, 256] partial sums, [2 target, ROWS, 2] maximum and sum
-    int* count;   // [2 target] shares of a group, [2 target] groups of a sequence that are done
+    int device, cus, blocks;
+    float* part;  // [2 blocks, ROWS, 256] partial sums, [2 blocks, ROWS, 2] maximum and sum
+    int* count;   // [2 blocks] parts of a group, [2 blocks] groups of a sequence that are done
 };
 
 struct Args {
     const bf16 *q, *kp, *vp, *gate;
     bf16* out;
     float *lse, *part, *ml;
-    int* count;
+    int *count, *count2;
     const int32_t *table, *lens, *seqs;
-    int nseq, max_pages, npages, page, B, Hq, Hk, G, tiles, target;
+    int nseq, max_pages, npages, page, B, Hq, Hk, G, tiles, blocks;
     float scale_log2;
 };
 
-// Keys of row r (0 for padding).
-__device__ __forceinline__ int keys_of(const Args& a, int r) {
-    if (r >= a.B) return 0;
-    const int s = listed_seq(a.seqs, r, a.nseq);
-    return s < 0 ? 0 : (int)min((int64_t)max(a.lens[s], 0), (int64_t)a.max_pages * a.page);
+// Row r's sequence (of its keys: none for padding).
+struct Row {
+    int s, n;
+};
+__device__ __forceinline__ Row row_of(const Args& a, int r) {
+    const int s = r < a.B ? listed_seq(a.seqs, r, a.nseq) : -1;
+    return s < 0 ? Row{0, 0} : Row{s, (int)min((int64_t)max(a.lens[s], 0), (int64_t)a.max_pages * a.page)};
 }
 
-__device__ __forceinline__ int units_of(int n) { return n / UNIT + (n % UNIT != 0); }
+// Chunks of a row's work for one kv head and tile (a row without keys has one: its zeros are written).
+__device__ __forceinline__ int chunks_of(int n) { return max(1, n / CHUNK + (n % CHUNK != 0)); }
 
 template <typename T>
 __device__ __forceinline__ T wave_scan(T x) {  // inclusive
@@ -80,55 +85,65 @@ __device__ __forceinline__ T wave_scan(T x) {  // inclusive
 // Lane i's value, one for the wave.
 __device__ __forceinline__ int scalar(int x, int i) { return __builtin_amdgcn_readlane(x, i); }
 
-// The units of a share: all sequences' units over the number of shares that fill the chip, at least one
-// for each wave.  Each wave works it out from the lengths, which only the device knows (n0: row lane's).
-__device__ __forceinline__ int units_per_share(const Args& a, int n0) {
-    int64_t total = 0;
-    for (int r0 = 0; r0 < a.B; r0 += 64) {
-        int64_t u = units_of(r0 == 0 ? n0 : keys_of(a, r0 + (threadIdx.x & 63)));
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) u += __shfl_xor(u, o, 64);
-        total += (int64_t)((uint64_t)(uint32_t)scalar((int)(u >> 32), 0) << 32 | (uint32_t)scalar((int)u, 0));
-    }
-    total *= a.Hk * a.tiles;
-    return (int)max((int64_t)LEAST_SHARE, (total + a.target - 1) / a.target);
-}
+// Rows in the work's order, looked at 64 at a time by each wave for itself: only the device knows the lengths.
+struct Rows {
+    Row first;  // row `lane`
 
-struct Share {
-    int row, split, splits, head, tile, n, slot;  // slot: of the first split's partial results
+    __device__ __forceinline__ explicit Rows(const Args& a) : first(row_of(a, threadIdx.x & 63)) {}
+    __device__ __forceinline__ Row at(const Args& a, int r0) const {
+        return r0 == 0 ? first : row_of(a, r0 + (threadIdx.x & 63));
+    }
+    __device__ __forceinline__ int total(const Args& a) const {
+        int sum = 0;
+        for (int r0 = 0; r0 < a.B; r0 += 64) {
+            const int c = r0 + (int)(threadIdx.x & 63) < a.B ? chunks_of(at(a, r0).n) : 0;
+            sum += scalar(wave_scan(c), 63);
+        }
+        return sum * a.Hk * a.tiles;
+    }
 };
 
-// Share number idx: rows in order, a row's splits, and in each the kv heads and tiles.  Rows without keys
-// have one share (it writes their zeros).  Slots count the shares of rows that have several: with u units and
-// p units a share that is ceil(u / p) < 2 u / p of them, so all slots are fewer than twice the target.
-__device__ __forceinline__ bool find_share(const Args& a, int idx, int n0, Share& sh) {
-    const int per = units_per_share(a, n0);
-    const int lane = threadIdx.x & 63, each = a.Hk * a.tiles;
-    int64_t before = 0;
-    int slots = 0;
+struct Segment {
+    int row, s, n, head, tile;  // the n keys of row `row`'s sequence s for kv head `head` and a tile of q heads
+    int from, to;            // chunks of it
+    int first, parts, part;  // the first block that has some of it, how many have, and which of them this is
+    int slot0;               // where the first one's results go; the others' go to 2 x their block
+
+    __device__ __forceinline__ int slot(int k) const { return k == 0 ? slot0 : 2 * (first + k); }
+};
+
+// The segment that begins at chunk `pos` of a stretch that ends at `end`, stretches being `each` chunks long.
+__device__ __forceinline__ Segment segment_at(const Args& a, const Rows& rows, int pos, int end, int each) {
+    const int lane = threadIdx.x & 63, heads = a.Hk * a.tiles;
+    Segment s = {};
+    int before = 0;
     for (int r0 = 0; r0 < a.B; r0 += 64) {
-        const int r = r0 + lane, n = r0 == 0 ? n0 : keys_of(a, r), splits = r < a.B ? max(1, (units_of(n) + per - 1) / per) : 0;
-        const int mine = splits * each, in = wave_scan(mine), sl = splits > 1 ? mine : 0, in_sl = wave_scan(sl);
-        const uint64_t hit = __ballot(idx >= before + in - mine && idx < before + in);
+        const Row row = rows.at(a, r0);
+        const int c = r0 + lane < a.B ? chunks_of(row.n) : 0;
+        const int in = before + wave_scan(c) * heads;
+        const uint64_t hit = __ballot(pos < in);
         if (hit) {
-            const int w = __ffsll((unsigned long long)hit) - 1;
-            const int k = (int)(idx - before) - scalar(in - mine, w);
-            sh.row = r0 + w;
-            sh.splits = scalar(splits, w);
-            sh.n = scalar(n, w);
-            sh.split = k / each;
-            sh.head = k % each / a.tiles;
-            sh.tile = k % a.tiles;
-            sh.slot = slots + scalar(in_sl - sl, w) + (sh.head * a.tiles + sh.tile) * sh.splits;
-            return true;
+            const int w = __ffsll((unsigned long long)hit) - 1, chunks = scalar(c, w);
+            const int start = scalar(in, w) - chunks * heads, k = (pos - start) / chunks, whole = start + k * chunks;
+            s.row = r0 + w;
+            s.s = scalar(row.s, w);
+            s.n = scalar(row.n, w);
+            s.head = k / a.tiles;
+            s.tile = k % a.tiles;
+            s.from = pos - whole;
+            s.to = min(chunks, end - whole);
+            s.first = whole / each;
+            s.parts = (whole + chunks - 1) / each - s.first + 1;
+            s.part = pos / each - s.first;
+            s.slot0 = 2 * s.first + (whole > s.first * each);
+            break;
         }
-        before += scalar(in, 63);
-        slots += scalar(in_sl, 63);
+        before = scalar(in, 63);
     }
-    return false;
+    return s;
 }
 
-// The output of q heads [first, first + count) from sums o over l (zero: no key).
+// Four dims of an output from sums o over l (zero: no key).
 __device__ __forceinline__ void store_out(const Args& a, size_t at, const f32x4& o, float l) {
     const float inv = l != 0.f ? 1.f / l : 0.f;
     float y[4];
@@ -146,36 +161,55 @@ __device__ __forceinline__ float log_sum(float top, float sum) {
     return sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
 }
 
-// Values that another block reads in the same launch.  Each XCD has an L2 of its own, so they are written through
-// it and read past it (the accesses of an agent-scope atomic); a fence would instead write back all that the L2 holds,
-// for every wave that executes it: 240 us in place of 25 for 32768 keys in 1024 shares.
-__device__ __forceinline__ void put_shared(float* p, f32x2 v) {
-    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
-                       __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ f32x2 get_shared(const float* p) {
-    return __builtin_bit_cast(f32x2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
-                                                       __HIP_MEMORY_SCOPE_AGENT));
-}
+// Results that another block reads in the same launch.  Each XCD has an L2 of its own, so they are written through
+// it and read past it (device scope, the SC1 bit).  A fence instead would write back all that the L2 holds, for every
+// wave that executes it: 240 us in place of 25 for 32768 keys in 1024 parts.
+struct Shared {
+    static constexpr int SC1 = 0x10;
+    __amdgpu_buffer_rsrc_t part, ml;
+
+    __device__ __forceinline__ explicit Shared(const Args& a)
+        : part(__builtin_amdgcn_make_buffer_rsrc(a.part, (short)0, 0x7fffffff, 0x00020000)),
+          ml(__builtin_amdgcn_make_buffer_rsrc(a.ml, (short)0, 0x7fffffff, 0x00020000)) {}
+    // byte offsets: under 2^31 for the handle's 2 x blocks slots of at most 16 x 256 floats
+    __device__ __forceinline__ f32x4 get(int at) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, at, 0, SC1));
+    }
+    __device__ __forceinline__ void put(int at, const f32x4& v) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), part, at, 0, SC1);
+    }
+    __device__ __forceinline__ f32x2 get_ml(int at) const {
+        return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(ml, at, 0, SC1));
+    }
+    __device__ __forceinline__ void put_ml(int at, const f32x2& v) const {
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), ml, at, 0, SC1);
+    }
+};
 
 template <int DH>
 __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args a) {
     constexpr int C = DH / 32, H = DH / 128, PITCH = DH + 8;
     extern __shared__ __attribute__((aligned(16))) float lds[];  // Q as operands, [C][64 lanes] x 16 bytes; later [WAVES][rows][PITCH]
     __shared__ float wm[WAVES][ROWS], wl[WAVES][ROWS];
-    Share sh;
-    if (!find_share(a, blockIdx.x, keys_of(a, threadIdx.x & 63), sh)) return;
-    const int lane = threadIdx.x & 63, wave = scalar(threadIdx.x >> 6, 0), col = lane & 15, grp = lane >> 4;
+    const Rows lengths(a);
+    const int total = lengths.total(a), each = (total + a.blocks - 1) / a.blocks;
+    const int begin = (int)blockIdx.x * each, end = min(total, begin + each);
+    for (int pos = begin; pos < end;) {
+    const Segment sh = segment_at(a, lengths, pos, end, each);
+    // what follows from the lane is worked out again for each segment: kept over the loop it would take a fifth of the registers
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, wave = scalar(tid >> 6, 0), col = lane & 15, grp = lane >> 4;
+    pos += sh.to - sh.from;
     const int rows = min(ROWS, a.G - sh.tile * ROWS), head0 = sh.head * a.G + sh.tile * ROWS;
-    const int s = scalar(sh.n > 0 ? (a.seqs ? a.seqs[sh.row] : sh.row) : 0, 0);
-    // the row's units in equal parts
-    const int units = units_of(sh.n), part = (units + sh.splits - 1) / sh.splits;
-    const int u_end = min(units, (sh.split + 1) * part);
-    int u = sh.split * part + wave;
+    const int u_end = min(sh.to * CHUNK_UNITS, sh.n / UNIT + (sh.n % UNIT != 0));
+    int u = sh.from * CHUNK_UNITS + wave;
 
+    __syncthreads();  // the segment before is done with LDS
     u32x4* const qf = reinterpret_cast<u32x4*>(lds);
 #pragma unroll
-    for (int c = wave; c < C; c += WAVES) {
+    for (int i = 0; i < C / WAVES; i++) {
+        const int c = wave + i * WAVES;
         u32x4 q = {0, 0, 0, 0};
         if (col < rows) q = *reinterpret_cast<const u32x4*>(a.q + ((size_t)sh.row * a.Hq + head0 + col) * DH + c * 32 + grp * 8);
         qf[c * 64 + lane] = q;
@@ -196,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
         where = 0;
         valid = 0;
         if (key < (uint32_t)sh.n) {
-            const int pg = a.table[(size_t)s * a.max_pages + slot];
+            const int pg = a.table[(size_t)sh.s * a.max_pages + slot];
             if (pg >= 0 && pg < a.npages) {
                 where = ((int64_t)pg * a.page + (key - slot * a.page)) * token;
                 valid = min(16, (int)(sh.n - key));
@@ -312,6 +346,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
     if (u < u_end) unit(std::false_type{});
 
     // the waves join
+    asm volatile("" : "+v"(tid));
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     if (grp == 0) {
@@ -329,6 +364,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
                 *reinterpret_cast<f32x4*>(to + 4) = f32x4{acc[h][4][r], acc[h][5][r], acc[h][6][r], acc[h][7][r]};
             }
     __syncthreads();
+    const Shared shared(a);
     // four dims of a row's result: to the output, or to a slot
     auto store = [&](int slot, int row, int d, float top, float sum, const f32x4& o, bool out) {
         const int head = head0 + row;
@@ -337,12 +373,11 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
             if (a.lse && d == 0) a.lse[(size_t)head * a.B + sh.row] = log_sum(top, sum);
             return;
         }
-        const size_t at = (size_t)slot * ROWS + row;
-        put_shared(a.part + at * DH + d, f32x2{o[0], o[1]});
-        put_shared(a.part + at * DH + d + 2, f32x2{o[2], o[3]});
-        if (d == 0) put_shared(a.ml + at * 2, f32x2{top, sum});
+        const int at = slot * ROWS + row;
+        shared.put((at * DH + d) * 4, o);
+        if (d == 0) shared.put_ml(at * 8, f32x2{top, sum});
     };
-    for (int e = threadIdx.x; e < rows * (DH / 4); e += THREADS) {
+    for (int e = tid; e < rows * (DH / 4); e += THREADS) {
         const int row = e / (DH / 4), d = e % (DH / 4) * 4;
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -354,58 +389,73 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
             sum += wl[w][row] * f;
             o += *reinterpret_cast<const f32x4*>(lds + ((size_t)w * rows + row) * PITCH + d) * f;
         }
-        store(sh.slot + sh.split, row, d, top, sum, o, sh.splits == 1);
+        store(sh.slot(sh.part), row, d, top, sum, o, sh.parts == 1);
     }
-    if (sh.splits == 1) return;
+    if (sh.parts == 1) continue;
 
-    // Groups of `group` shares: the last of a group to end joins it, the last group joins the groups; always in order, so the
+    // Groups of `group` parts: the last of a group to end joins it, the last group joins the groups; always in order, so the
     // result does not depend on which ends last.  The counters are zero again afterwards.
-    const int group = max(GROUP, (sh.splits + GROUPS_MAX - 1) / GROUPS_MAX), groups = (sh.splits + group - 1) / group;
-    const int g0 = sh.split / group * group;
+    const int least = (sh.parts + GROUP - 1) / GROUP, group = (sh.parts + least - 1) / least;
+    const int groups = (sh.parts + group - 1) / group;
+    const int g0 = sh.part / group * group, members = min(group, sh.parts - g0);
     auto last_of = [&](int* count, int n) {
         __shared__ int last;
         wait_vm_all();  // what this wave has put is where the others look
         __syncthreads();
-        if (threadIdx.x == 0) {
+        if (tid == 0) {
             last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
             if (last) *count = 0;
         }
         __syncthreads();
         return last != 0;
     };
-    // n results from slot on, `step` slots apart: out, or back to the first slot
-    auto join = [&](int slot, int step, int n, bool out) {
+    // the results of n parts from number k0 on, every `step`-th: out, or to the first one's place
+    auto join = [&](int k0, int step, int n, bool out) {
         f32x2* const ml = reinterpret_cast<f32x2*>(lds);
-        for (int e = threadIdx.x; e < n * rows; e += THREADS)
-            ml[e] = get_shared(a.ml + ((size_t)(slot + e / rows * step) * ROWS + e % rows) * 2);
-        __syncthreads();
-        for (int e = threadIdx.x; e < rows * (DH / 4); e += THREADS) {
-            const int row = e / (DH / 4), d = e % (DH / 4) * 4;
+        for (int e0 = 0; e0 < rows * (DH / 4); e0 += THREADS) {
+            const int e = e0 + tid, row = min(e / (DH / 4), rows - 1), d = e % (DH / 4) * 4;
+            // the first batch is on its way while the maxima and sums are looked at
+            f32x4 v[BATCH];
+            auto load = [&](int k1) {
+#pragma unroll
+                for (int i = 0; i < BATCH; i++)
+                    v[i] = shared.get(((sh.slot(k0 + min(k1 + i, n - 1) * step) * ROWS + row) * DH + d) * 4);
+            };
+            load(0);
+            if (e0 == 0) {
+                for (int i = tid; i < n * rows; i += THREADS)
+                    ml[i] = shared.get_ml((sh.slot(k0 + i / rows * step) * ROWS + i % rows) * 8);
+                __syncthreads();
+            }
             float top = -INFINITY, sum = 0.f;
             for (int k = 0; k < n; k++) top = fmaxf(top, ml[k * rows + row][0]);
             f32x4 o = {0.f, 0.f, 0.f, 0.f};
-            float* const from = a.part + ((size_t)slot * ROWS + row) * DH + d;
-#pragma unroll 16
-            for (int k = 0; k < n; k++) {
-                const float* const p = from + (size_t)k * step * ROWS * DH;
-                const f32x2 m = ml[k * rows + row], lo = get_shared(p), hi = get_shared(p + 2);
-                const float f = m[0] == top ? 1.f : __builtin_amdgcn_exp2f(m[0] - top);
-                sum += m[1] * f;
-                o += f32x4{lo[0], lo[1], hi[0], hi[1]} * f;
+            for (int k1 = 0; k1 < n; k1 += BATCH) {
+                if (k1 > 0) load(k1);
+#pragma unroll
+                for (int i = 0; i < BATCH; i++)
+                    if (k1 + i < n) {
+                        const f32x2 m = ml[(k1 + i) * rows + row];
+                        const float f = m[0] == top ? 1.f : __builtin_amdgcn_exp2f(m[0] - top);
+                        sum += m[1] * f;
+                        o += v[i] * f;
+                    }
             }
-            store(slot, row, d, top, sum, o, out);
+            if (e < rows * (DH / 4)) store(sh.slot(k0), row, d, top, sum, o, out);
         }
+        __syncthreads();
     };
-    if (!last_of(a.count + sh.slot + g0 / group, min(group, sh.splits - g0))) return;
-    join(sh.slot + g0, 1, min(group, sh.splits - g0), groups == 1);
-    if (groups == 1 || !last_of(a.count + 2 * a.target + sh.slot, groups)) return;
-    join(sh.slot, group, groups, true);
+    if (!last_of(a.count + sh.slot(g0), members)) continue;
+    join(g0, 1, members, groups == 1);
+    if (groups == 1 || !last_of(a.count2 + sh.slot0, groups)) continue;
+    join(0, group, groups, true);
+    }
 }
 
 template <int DH>
 size_t lds_bytes(int rows) {
     const size_t q = 16 * 64 * (DH / 32), join = sizeof(float) * WAVES * rows * (DH + 8);
-    const size_t group = sizeof(f32x2) * GROUPS_MAX * rows;
+    const size_t group = sizeof(f32x2) * GROUP * rows;
     return std::max(q, std::max(join, group));
 }
 
@@ -417,8 +467,7 @@ bool configure() {
 
 template <int DH>
 int launch(const Args& a, hipStream_t st) {
-    const int64_t shares = (int64_t)a.target + (int64_t)a.B * a.Hk * a.tiles;
-    attention_paged_kernel<DH><<<(unsigned)shares, THREADS, lds_bytes<DH>(a.G < ROWS ? a.G : ROWS), st>>>(a);
+    attention_paged_kernel<DH><<<a.blocks, THREADS, lds_bytes<DH>(a.G < ROWS ? a.G : ROWS), st>>>(a);
     return hipGetLastError();
 }
 
@@ -437,9 +486,9 @@ extern "C" void* cs1_attention_paged_create(void) {
     Paged* const p = new (std::nothrow) Paged;
     if (!p) return nullptr;
     p->device = device;
-    p->cus = cus;
-    p->target = std::min(4 * cus, GROUPS_MAX * GROUPS_MAX);
-    const size_t floats = (size_t)2 * p->target * ROWS * (256 + 2), counts = (size_t)4 * p->target;
+    p->cus = std::min(cus, GROUP * GROUP / 3);
+    p->blocks = 3 * p->cus;
+    const size_t floats = (size_t)2 * p->blocks * ROWS * (256 + 2), counts = (size_t)4 * p->blocks;
     p->part = nullptr;
     if (hipMalloc(reinterpret_cast<void**>(&p->part), 4 * (floats + counts)) != hipSuccess ||
         hipMemset(p->part + floats, 0, 4 * counts) != hipSuccess || hipStreamSynchronize(nullptr) != hipSuccess) {
@@ -479,8 +528,9 @@ extern "C" int cs1_attention_paged(void* paged, const void* q, const void* kp, c
     a.out = static_cast<bf16*>(out);
     a.lse = lse;
     a.part = p->part;
-    a.ml = p->part + (size_t)2 * p->target * ROWS * 256;
+    a.ml = p->part + (size_t)2 * p->blocks * ROWS * 256;
     a.count = p->count;
+    a.count2 = p->count + 2 * p->blocks;
     a.table = pages->table;
     a.lens = pages->lens;
     a.seqs = seqs;
@@ -493,7 +543,7 @@ extern "C" int cs1_attention_paged(void* paged, const void* q, const void* kp, c
     a.Hk = Hk;
     a.G = Hq / Hk;
     a.tiles = (a.G + ROWS - 1) / ROWS;
-    a.target = p->target;
+    a.blocks = p->cus;
     a.scale_log2 = scale * LOG2E;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     return Dh == 128 ? launch<128>(a, st) : launch<256>(a, st);
