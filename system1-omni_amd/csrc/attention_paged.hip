@@ -71,14 +71,17 @@ __device__ __forceinline__ Row row_of(const Args& a, int r) {
 // Chunks of a row's work for one kv head and tile (a row without keys has one: its zeros are written).
 __device__ __forceinline__ int chunks_of(int n) { return max(1, n / CHUNK + (n % CHUNK != 0)); }
 
-template <typename T>
-__device__ __forceinline__ T wave_scan(T x) {  // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const T below = __shfl_up(x, o, 64);
-        if (lane >= o) x += below;
-    }
+// Sum over this lane and those below: within rows of 16 lanes, then each row's last lane to the next row (into rows
+// 1 and 3), then lane 31 to the upper half.
+__device__ __forceinline__ int wave_scan(int x) {
+#define Q35_ADD(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false)
+    Q35_ADD(0x111, 0xf);
+    Q35_ADD(0x112, 0xf);
+    Q35_ADD(0x114, 0xf);
+    Q35_ADD(0x118, 0xf);
+    Q35_ADD(0x142, 0xa);
+    Q35_ADD(0x143, 0xc);
+#undef Q35_ADD
     return x;
 }
 
@@ -86,20 +89,31 @@ __device__ __forceinline__ T wave_scan(T x) {  // inclusive
 __device__ __forceinline__ int scalar(int x, int i) { return __builtin_amdgcn_readlane(x, i); }
 
 // Rows in the work's order, looked at 64 at a time by each wave for itself: only the device knows the lengths.
-struct Rows {
-    Row first;  // row `lane`
+// The lane's number, found again where it is asked for: what follows from it would otherwise be kept in registers
+// over the loop over the keys, which has none to spare.
+__device__ __forceinline__ int lane_here() {
+    int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
 
-    __device__ __forceinline__ explicit Rows(const Args& a) : first(row_of(a, threadIdx.x & 63)) {}
-    __device__ __forceinline__ Row at(const Args& a, int r0) const {
-        return r0 == 0 ? first : row_of(a, r0 + (threadIdx.x & 63));
-    }
-    __device__ __forceinline__ int total(const Args& a) const {
-        int sum = 0;
-        for (int r0 = 0; r0 < a.B; r0 += 64) {
-            const int c = r0 + (int)(threadIdx.x & 63) < a.B ? chunks_of(at(a, r0).n) : 0;
-            sum += scalar(wave_scan(c), 63);
-        }
-        return sum * a.Hk * a.tiles;
+// One value from the four of a lane's column (lanes 16 apart), in each of them: rows of 16 lanes are swapped, then halves.
+template <typename F>
+__device__ __forceinline__ float over_groups(float x, F f) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+struct Rows {
+    Row row;      // row `lane`
+    int chunks, upto;  // its chunks, and those of the rows up to it
+
+    __device__ __forceinline__ Rows() {}
+    __device__ __forceinline__ Rows(const Args& a, int r0) : row(row_of(a, r0 + (threadIdx.x & 63))) {
+        chunks = r0 + (int)(threadIdx.x & 63) < a.B ? chunks_of(row.n) : 0;
+        upto = wave_scan(chunks);
     }
 };
 
@@ -113,42 +127,45 @@ struct Segment {
 };
 
 // The segment that begins at chunk `pos` of a stretch that ends at `end`, stretches being `each` chunks long.
-__device__ __forceinline__ Segment segment_at(const Args& a, const Rows& rows, int pos, int end, int each) {
-    const int lane = threadIdx.x & 63, heads = a.Hk * a.tiles;
+__device__ __forceinline__ Segment segment_at(const Args& a, const Rows& first, int pos, int end, int each) {
+    const int heads = a.Hk * a.tiles;
     Segment s = {};
-    int before = 0;
-    for (int r0 = 0; r0 < a.B; r0 += 64) {
-        const Row row = rows.at(a, r0);
-        const int c = r0 + lane < a.B ? chunks_of(row.n) : 0;
-        const int in = before + wave_scan(c) * heads;
-        const uint64_t hit = __ballot(pos < in);
-        if (hit) {
-            const int w = __ffsll((unsigned long long)hit) - 1, chunks = scalar(c, w);
-            const int start = scalar(in, w) - chunks * heads, k = (pos - start) / chunks, whole = start + k * chunks;
-            s.row = r0 + w;
-            s.s = scalar(row.s, w);
-            s.n = scalar(row.n, w);
-            s.head = k / a.tiles;
-            s.tile = k % a.tiles;
-            s.from = pos - whole;
-            s.to = min(chunks, end - whole);
-            s.first = whole / each;
-            s.parts = (whole + chunks - 1) / each - s.first + 1;
-            s.part = pos / each - s.first;
-            s.slot0 = 2 * s.first + (whole > s.first * each);
-            break;
-        }
-        before = scalar(in, 63);
+    auto find = [&](const Rows& rows, int r0, int before) {
+        const uint64_t hit = __ballot(pos < before + rows.upto * heads);
+        if (!hit) return false;
+        const int w = __ffsll((unsigned long long)hit) - 1, chunks = scalar(rows.chunks, w);
+        const int start = before + (scalar(rows.upto, w) - chunks) * heads, k = (pos - start) / chunks;
+        const int whole = start + k * chunks;
+        s.row = r0 + w;
+        s.s = scalar(rows.row.s, w);
+        s.n = scalar(rows.row.n, w);
+        s.head = k / a.tiles;
+        s.tile = k % a.tiles;
+        s.from = pos - whole;
+        s.to = min(chunks, end - whole);
+        s.first = whole / each;
+        s.parts = (whole + chunks - 1) / each - s.first + 1;
+        s.part = pos / each - s.first;
+        s.slot0 = 2 * s.first + (whole > s.first * each);
+        return true;
+    };
+    if (find(first, 0, 0)) return s;
+    int before = scalar(first.upto, 63) * heads;
+    for (int r0 = 64; r0 < a.B; r0 += 64) {
+        const Rows rows(a, r0);
+        if (find(rows, r0, before)) break;
+        before += scalar(rows.upto, 63) * heads;
     }
     return s;
 }
 
-// Four dims of an output from sums o over l (zero: no key).
-__device__ __forceinline__ void store_out(const Args& a, size_t at, const f32x4& o, float l) {
+// Four dims of an output from sums o over l (zero: no key); g: their gates, if there are any.
+__device__ __forceinline__ u32x2 load_gate(const Args& a, size_t at) {
+    return a.gate ? *reinterpret_cast<const u32x2*>(a.gate + at) : u32x2{0, 0};
+}
+__device__ __forceinline__ void store_out(const Args& a, size_t at, const f32x4& o, float l, const u32x2& g) {
     const float inv = l != 0.f ? 1.f / l : 0.f;
     float y[4];
-    u32x2 g = {0, 0};
-    if (a.gate) g = *reinterpret_cast<const u32x2*>(a.gate + at);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         y[e] = l != 0.f ? o[e] * inv : 0.f;
@@ -187,19 +204,26 @@ struct Shared {
 };
 
 template <int DH>
-__global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, DH == 256 ? 1 : 2) attention_paged_kernel(const Args a) {
     constexpr int C = DH / 32, H = DH / 128, PITCH = DH + 8;
     extern __shared__ __attribute__((aligned(16))) float lds[];  // Q as operands, [C][64 lanes] x 16 bytes; later [WAVES][rows][PITCH]
     __shared__ float wm[WAVES][ROWS], wl[WAVES][ROWS];
-    const Rows lengths(a);
-    const int total = lengths.total(a), each = (total + a.blocks - 1) / a.blocks;
+    const int wave = scalar(threadIdx.x >> 6, 0);
+    __shared__ Rows first[64];  // (the loop over the keys has no registers for it)
+    int total;
+    {
+        const Rows rows(a, 0);
+        if (threadIdx.x < 64) first[threadIdx.x] = rows;
+        total = scalar(rows.upto, 63);
+    }
+    for (int r0 = 64; r0 < a.B; r0 += 64) total += scalar(Rows(a, r0).upto, 63);
+    total *= a.Hk * a.tiles;
+    const int each = (total + a.blocks - 1) / a.blocks;
     const int begin = (int)blockIdx.x * each, end = min(total, begin + each);
+    __syncthreads();
     for (int pos = begin; pos < end;) {
-    const Segment sh = segment_at(a, lengths, pos, end, each);
-    // what follows from the lane is worked out again for each segment: kept over the loop it would take a fifth of the registers
-    int tid = threadIdx.x;
-    asm volatile("" : "+v"(tid));
-    const int lane = tid & 63, wave = scalar(tid >> 6, 0), col = lane & 15, grp = lane >> 4;
+    const Segment sh = segment_at(a, first[lane_here()], pos, end, each);
+    const int lane = lane_here(), col = lane & 15, grp = lane >> 4;
     pos += sh.to - sh.from;
     const int rows = min(ROWS, a.G - sh.tile * ROWS), head0 = sh.head * a.G + sh.tile * ROWS;
     const int u_end = min(sh.to * CHUNK_UNITS, sh.n / UNIT + (sh.n % UNIT != 0));
@@ -207,9 +231,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
 
     __syncthreads();  // the segment before is done with LDS
     u32x4* const qf = reinterpret_cast<u32x4*>(lds);
-#pragma unroll
-    for (int i = 0; i < C / WAVES; i++) {
-        const int c = wave + i * WAVES;
+    for (int c = wave; c < C; c += WAVES) {
         u32x4 q = {0, 0, 0, 0};
         if (col < rows) q = *reinterpret_cast<const u32x4*>(a.q + ((size_t)sh.row * a.Hq + head0 + col) * DH + c * 32 + grp * 8);
         qf[c * 64 + lane] = q;
@@ -221,29 +243,22 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
         for (int j = 0; j < 8; j++) acc[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
 
-    // where the next units' halves lie: lane i has half i % 2 of unit i / 2 from here (element offset, valid keys)
+    // where the next units' halves lie: lane i has half i % 2 of unit i / 2 from here, the pool's row / 16 and 5 bits of valid keys
     const size_t token = (size_t)a.Hk * DH;
-    int64_t where = 0;
-    int valid = 0, next = 64;
+    uint32_t where = 0;
+    int next = 64;
     auto look_up = [&](int from) {
-        const uint32_t key = (uint32_t)(from + (lane >> 1) * WAVES) * UNIT + (lane & 1) * 16, slot = key / (uint32_t)a.page;
+        const int i = lane_here();
+        const uint32_t key = (uint32_t)(from + (i >> 1) * WAVES) * UNIT + (i & 1) * 16, slot = key / (uint32_t)a.page;
         where = 0;
-        valid = 0;
         if (key < (uint32_t)sh.n) {
             const int pg = a.table[(size_t)sh.s * a.max_pages + slot];
-            if (pg >= 0 && pg < a.npages) {
-                where = ((int64_t)pg * a.page + (key - slot * a.page)) * token;
-                valid = min(16, (int)(sh.n - key));
-            }
+            if (pg >= 0 && pg < a.npages)
+                where = ((uint32_t)pg * a.page + (key - slot * a.page)) / 16 << 5 | min(16, (int)(sh.n - key));
         }
-        where += sh.head * DH;
-    };
-    auto lane_of = [&](int64_t x, int i) {
-        const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, i), hi = __builtin_amdgcn_readlane((uint32_t)(x >> 32), i);
-        return (int64_t)((uint64_t)hi << 32 | lo);
     };
     u32x4 kf[2][C], vf[H][8];
-    int64_t v_at[2];
+    size_t v_at[2];
     int have[2], v_have[2];
     // byte offsets of this lane in a half: 32 bits next to a base that the wave shares
     const uint32_t row_b = 2 * (uint32_t)token, k_lane = col * row_b + grp * 16, v_lane = grp * 4 * row_b + col * 16;
@@ -254,11 +269,12 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
         }
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            v_at[t] = lane_of(where, next + t);
-            have[t] = __builtin_amdgcn_readlane(valid, next + t);
-            const char* const p = reinterpret_cast<const char*>(a.kp + v_at[t]);
+            const uint32_t w = __builtin_amdgcn_readlane(where, next + t);
+            v_at[t] = (size_t)(w >> 5) * (16 * token) + sh.head * DH;
+            have[t] = w & 31;
+            const char* const p = reinterpret_cast<const char*>(a.kp + v_at[t]) + k_lane;
 #pragma unroll
-            for (int c = 0; c < C; c++) kf[t][c] = *reinterpret_cast<const u32x4*>(p + (k_lane + c * 64));
+            for (int c = 0; c < C; c++) kf[t][c] = *reinterpret_cast<const u32x4*>(p + c * 64);
         }
         next += 2;
     };
@@ -266,12 +282,12 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             v_have[t] = have[t];
-            const char* const p = reinterpret_cast<const char*>(a.vp + v_at[t]);
 #pragma unroll
-            for (int h = 0; h < H; h++)
+            for (int i = 0; i < 4; i++) {
+                const char* const p = reinterpret_cast<const char*>(a.vp + v_at[t]) + (size_t)i * row_b + v_lane;
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    vf[h][t * 4 + i] = *reinterpret_cast<const u32x4*>(p + (v_lane + i * row_b + h * 256));
+                for (int h = 0; h < H; h++) vf[h][t * 4 + i] = *reinterpret_cast<const u32x4*>(p + h * 256);
+            }
         }
     };
     if (u < u_end) {
@@ -281,12 +297,12 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
     __syncthreads();
     // one unit; more: the wave has another after it
     auto unit = [&](auto more) {
-        f32x4 st[2];
+        f32x4 st[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < C; c++) {
+            const u32x4 q = qf[c * 64 + lane];
 #pragma unroll
-            for (int c = 0; c < C; c++) st[t] = mfma16(kf[t][c], qf[c * 64 + lane], st[t]);
+            for (int t = 0; t < 2; t++) st[t] = mfma16(kf[t][c], q, st[t]);
         }
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (decltype(more)::value) load_k(u + WAVES);
@@ -302,8 +318,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
 #pragma unroll
         for (int i = 0; i < 8; i++) top = fmaxf(top, sc[i]);
         if (__any(top > m + RISE)) {
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+            top = fmaxf(m, over_groups(top, [](float x, float y) { return fmaxf(x, y); }));
             const float keep = top == m ? 1.f : __builtin_amdgcn_exp2f(m - top);
             m = top;
             l *= keep;
@@ -346,39 +361,42 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
     if (u < u_end) unit(std::false_type{});
 
     // the waves join
-    asm volatile("" : "+v"(tid));
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    if (grp == 0) {
-        wm[wave][col] = m;
-        wl[wave][col] = l;
+    const int tid = wave * 64 + lane_here();
+    l = over_groups(l, [](float x, float y) { return x + y; });
+    const int row_c = tid & 15, row_g = tid >> 4 & 3;
+    if (row_g == 0) {
+        wm[wave][row_c] = m;
+        wl[wave][row_c] = l;
     }
     __syncthreads();  // Q is no longer read
-    if (col < rows)
+    if (row_c < rows)
 #pragma unroll
         for (int h = 0; h < H; h++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                float* const to = lds + ((size_t)wave * rows + col) * PITCH + h * 128 + (grp * 4 + r) * 8;
+                float* const to = lds + (wave * rows + row_c) * PITCH + h * 128 + (row_g * 4 + r) * 8;
                 *reinterpret_cast<f32x4*>(to) = f32x4{acc[h][0][r], acc[h][1][r], acc[h][2][r], acc[h][3][r]};
                 *reinterpret_cast<f32x4*>(to + 4) = f32x4{acc[h][4][r], acc[h][5][r], acc[h][6][r], acc[h][7][r]};
             }
     __syncthreads();
     const Shared shared(a);
+    constexpr int QUADS = DH / 4;  // of a row's dims
+    const size_t out0 = ((size_t)sh.row * a.Hq + head0) * DH;
     // four dims of a row's result: to the output, or to a slot
-    auto store = [&](int slot, int row, int d, float top, float sum, const f32x4& o, bool out) {
-        const int head = head0 + row;
+    auto store = [&](int slot, int e, float top, float sum, const f32x4& o, const u32x2& g, bool out) {
+        const int row = e / QUADS, d = e % QUADS * 4;
         if (out) {
-            store_out(a, ((size_t)sh.row * a.Hq + head) * DH + d, o, sum);
-            if (a.lse && d == 0) a.lse[(size_t)head * a.B + sh.row] = log_sum(top, sum);
+            store_out(a, out0 + row * DH + d, o, sum, g);
+            if (a.lse && d == 0) a.lse[(size_t)(head0 + row) * a.B + sh.row] = log_sum(top, sum);
             return;
         }
         const int at = slot * ROWS + row;
         shared.put((at * DH + d) * 4, o);
         if (d == 0) shared.put_ml(at * 8, f32x2{top, sum});
     };
-    for (int e = tid; e < rows * (DH / 4); e += THREADS) {
-        const int row = e / (DH / 4), d = e % (DH / 4) * 4;
+    for (int e = tid; e < rows * QUADS; e += THREADS) {
+        const int row = e / QUADS, d = e % QUADS * 4;
+        const u32x2 g = load_gate(a, out0 + row * DH + d);
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int w = 0; w < WAVES; w++) top = fmaxf(top, wm[w][row]);
@@ -389,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
             sum += wl[w][row] * f;
             o += *reinterpret_cast<const f32x4*>(lds + ((size_t)w * rows + row) * PITCH + d) * f;
         }
-        store(sh.slot(sh.part), row, d, top, sum, o, sh.parts == 1);
+        store(sh.slot(sh.part), e, top, sum, o, g, sh.parts == 1);
     }
     if (sh.parts == 1) continue;
 
@@ -409,54 +427,72 @@ __global__ void __launch_bounds__(THREADS, 2) attention_paged_kernel(const Args 
         __syncthreads();
         return last != 0;
     };
-    // the results of n parts from number k0 on, every `step`-th: out, or to the first one's place
+    // The results of n parts from number k0 on, every `step`-th: out, or to the first one's place.  The time is that of
+    // getting at them, so many are asked for at once: a row's four dims are summed by as many threads as there are for them, each
+    // with every `ways`-th part, BATCH of them on their way together, the first while a wave per row finds the parts' weights.
     auto join = [&](int k0, int step, int n, bool out) {
-        f32x2* const ml = reinterpret_cast<f32x2*>(lds);
-        for (int e0 = 0; e0 < rows * (DH / 4); e0 += THREADS) {
-            const int e = e0 + tid, row = min(e / (DH / 4), rows - 1), d = e % (DH / 4) * 4;
-            // the first batch is on its way while the maxima and sums are looked at
+        const int items = rows * QUADS, ways = max(1, THREADS / items);
+        float* const weight = lds;                        // [GROUP, ROWS]
+        float* const other = lds + GROUP * ROWS;          // [THREADS, 4]
+        for (int e0 = 0; e0 < items; e0 += THREADS) {
+            const int way = ways > 1 ? tid / items : 0, e = ways > 1 ? tid % items : e0 + tid;
+            const bool works = way < ways && e < items;
+            const int row = works ? e / QUADS : 0, d = e % QUADS * 4;
             f32x4 v[BATCH];
             auto load = [&](int k1) {
 #pragma unroll
-                for (int i = 0; i < BATCH; i++)
-                    v[i] = shared.get(((sh.slot(k0 + min(k1 + i, n - 1) * step) * ROWS + row) * DH + d) * 4);
+                for (int i = 0; i < BATCH; i++)  // (behind the last: the last again)
+                    v[i] = shared.get(((sh.slot(k0 + min(k1 + i * ways, n - 1) * step) * ROWS + row) * DH + d) * 4);
             };
-            load(0);
+            load(way);
+            const u32x2 g = load_gate(a, out0 + row * DH + d);
             if (e0 == 0) {
-                for (int i = tid; i < n * rows; i += THREADS)
-                    ml[i] = shared.get_ml((sh.slot(k0 + i / rows * step) * ROWS + i % rows) * 8);
+                const int k = tid & 63;
+                for (int r = wave; r < rows; r += WAVES) {
+                    const f32x2 m = shared.get_ml((sh.slot(k0 + min(k, n - 1) * step) * ROWS + r) * 8);
+                    const float top = lane_max<64>(m[0]), f = m[0] == top ? 1.f : __builtin_amdgcn_exp2f(m[0] - top);
+                    weight[k * ROWS + r] = f;
+                    const float sum = lane_sum<64>(k < n ? m[1] * f : 0.f);
+                    if (k == 0) {
+                        wm[0][r] = top;
+                        wl[0][r] = sum;
+                    }
+                }
                 __syncthreads();
             }
-            float top = -INFINITY, sum = 0.f;
-            for (int k = 0; k < n; k++) top = fmaxf(top, ml[k * rows + row][0]);
             f32x4 o = {0.f, 0.f, 0.f, 0.f};
-            for (int k1 = 0; k1 < n; k1 += BATCH) {
-                if (k1 > 0) load(k1);
+            for (int k1 = way; k1 < n; k1 += BATCH * ways) {
+                if (k1 > way) load(k1);
 #pragma unroll
-                for (int i = 0; i < BATCH; i++)
-                    if (k1 + i < n) {
-                        const f32x2 m = ml[(k1 + i) * rows + row];
-                        const float f = m[0] == top ? 1.f : __builtin_amdgcn_exp2f(m[0] - top);
-                        sum += m[1] * f;
-                        o += v[i] * f;
-                    }
+                for (int i = 0; i < BATCH; i++) {
+                    const int k = k1 + i * ways;
+                    const f32x4 more = o + v[i] * weight[min(k, n - 1) * ROWS + row];
+                    if (k < n) o = more;
+                }
             }
-            if (e < rows * (DH / 4)) store(sh.slot(k0), row, d, top, sum, o, out);
+            if (ways > 1) {
+                if (works && way > 0) *reinterpret_cast<f32x4*>(other + (way * items + e) * 4) = o;
+                __syncthreads();
+                if (way == 0)
+                    for (int w = 1; w < ways; w++) o += *reinterpret_cast<const f32x4*>(other + (w * items + e) * 4);
+            }
+            if (works && way == 0) store(sh.slot(k0), e, wm[0][row], wl[0][row], o, g, out);
         }
         __syncthreads();
     };
     if (!last_of(a.count + sh.slot(g0), members)) continue;
-    join(g0, 1, members, groups == 1);
-    if (groups == 1 || !last_of(a.count2 + sh.slot0, groups)) continue;
-    join(0, group, groups, true);
+    for (bool whole = groups == 1;; whole = true) {
+        join(whole ? 0 : g0, whole && groups > 1 ? group : 1, whole ? groups > 1 ? groups : members : members, whole);
+        if (whole || !last_of(a.count2 + sh.slot0, groups)) break;
+    }
     }
 }
 
 template <int DH>
 size_t lds_bytes(int rows) {
     const size_t q = 16 * 64 * (DH / 32), join = sizeof(float) * WAVES * rows * (DH + 8);
-    const size_t group = sizeof(f32x2) * GROUP * rows;
-    return std::max(q, std::max(join, group));
+    const size_t parts = sizeof(float) * (GROUP * ROWS + THREADS * 4);
+    return std::max(q, std::max(join, parts));
 }
 
 template <int DH>
@@ -513,7 +549,8 @@ extern "C" int cs1_attention_paged(void* paged, const void* q, const void* kp, c
                                    int Dh, float scale, void* stream) {
     const Paged* const p = static_cast<const Paged*>(paged);
     if (!p || !table_ok(pages) || (Dh != 128 && Dh != 256) || Hk <= 0 || Hq <= 0 || Hq % Hk != 0 || B < 0 ||
-        (int64_t)B * Hq > (1 << 22) || (int64_t)Hk * Dh > (1 << 24))
+        (int64_t)B * Hq > (1 << 22) || (int64_t)Hk * Dh > (1 << 24) ||
+        (int64_t)pages->npages * pages->page >= (int64_t{1} << 31))
         return hipErrorInvalidValue;
     if (B == 0) return hipSuccess;
     if (!all_set({q, kp, vp, out}) || !on16(q) || !on16(kp) || !on16(vp) || !on16(out) || !on16(gate))
