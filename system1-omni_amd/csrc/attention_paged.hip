@@ -37,7 +37,8 @@ namespace {
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int UNIT = 32, ROWS = 16;
-constexpr int CHUNK_UNITS = 4, CHUNK = CHUNK_UNITS * UNIT;
+constexpr int FINE = 4, COARSE = 16;  // units of a chunk
+constexpr int ALONE = 8;              // units of a sequence that is one chunk whatever the chunks' size
 constexpr int GROUP = 64, BATCH = 16;  // parts that one block joins, and how many of them are on their way at once
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float LEAST = 0x1p-126f;  // bfloat16's smallest normal value
@@ -55,7 +56,8 @@ struct Args {
     float *lse, *part, *ml;
     int *count, *count2;
     const int32_t *table, *lens, *seqs;
-    int nseq, max_pages, npages, page, B, Hq, Hk, G, tiles, blocks;
+    int nseq, max_pages, npages, page, B, Hq, Hk, G, tiles, blocks, unit;
+    uint32_t page_inverse, blocks_inverse;  // 2^32 over page / 16, rounded down, and over blocks, rounded up
     float scale_log2;
 };
 
@@ -68,8 +70,12 @@ __device__ __forceinline__ Row row_of(const Args& a, int r) {
     return s < 0 ? Row{0, 0} : Row{s, (int)min((int64_t)max(a.lens[s], 0), (int64_t)a.max_pages * a.page)};
 }
 
-// Chunks of a row's work for one kv head and tile (a row without keys has one: its zeros are written).
-__device__ __forceinline__ int chunks_of(int n) { return max(1, n / CHUNK + (n % CHUNK != 0)); }
+__device__ __forceinline__ int units_of(int n) { return n / UNIT + (n % UNIT != 0); }
+
+// Chunks of a row's work for one kv head and tile.  A row without keys has one: its zeros are written.
+__device__ __forceinline__ int chunks_of(const Args& a, int n) {
+    return n <= ALONE * UNIT ? 1 : (units_of(n) + a.unit - 1) / (uint32_t)a.unit;
+}
 
 // Sum over this lane and those below: within rows of 16 lanes, then each row's last lane to the next row (into rows
 // 1 and 3), then lane 31 to the upper half.
@@ -88,7 +94,6 @@ __device__ __forceinline__ int wave_scan(int x) {
 // Lane i's value, one for the wave.
 __device__ __forceinline__ int scalar(int x, int i) { return __builtin_amdgcn_readlane(x, i); }
 
-// Rows in the work's order, looked at 64 at a time by each wave for itself: only the device knows the lengths.
 // The lane's number, found again where it is asked for: what follows from it would otherwise be kept in registers
 // over the loop over the keys, which has none to spare.
 __device__ __forceinline__ int lane_here() {
@@ -106,27 +111,29 @@ __device__ __forceinline__ float over_groups(float x, F f) {
     return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// Rows in the work's order, looked at 64 at a time by each wave for itself: only the device knows the lengths.
 struct Rows {
     Row row;      // row `lane`
     int chunks, upto;  // its chunks, and those of the rows up to it
 
     __device__ __forceinline__ Rows() {}
     __device__ __forceinline__ Rows(const Args& a, int r0) : row(row_of(a, r0 + (threadIdx.x & 63))) {
-        chunks = r0 + (int)(threadIdx.x & 63) < a.B ? chunks_of(row.n) : 0;
+        chunks = r0 + (int)(threadIdx.x & 63) < a.B ? chunks_of(a, row.n) : 0;
         upto = wave_scan(chunks);
     }
 };
 
 struct Segment {
     int row, s, n, head, tile;  // the n keys of row `row`'s sequence s for kv head `head` and a tile of q heads
-    int from, to;            // chunks of it
-    int first, parts, part;  // the first block that has some of it, how many have, and which of them this is
-    int slot0;               // where the first one's results go; the others' go to 2 x their block
+    int from, to, chunks;       // units of it, and how many chunks they are
+    int first, parts, part;     // the first block that has some of it, how many have, and which of them this is
+    int slot0;                  // where the first one's results go; the others' go to 2 x their block
 
     __device__ __forceinline__ int slot(int k) const { return k == 0 ? slot0 : 2 * (first + k); }
 };
 
-// The segment that begins at chunk `pos` of a stretch that ends at `end`, stretches being `each` chunks long.
+// The segment that begins at chunk `pos` of this block's stretch, which ends at `end`; stretches are `each` chunks long.
+// (What runs once a launch is kept short: its instructions come from memory, and divisions are long.)
 __device__ __forceinline__ Segment segment_at(const Args& a, const Rows& first, int pos, int end, int each) {
     const int heads = a.Hk * a.tiles;
     Segment s = {};
@@ -134,18 +141,21 @@ __device__ __forceinline__ Segment segment_at(const Args& a, const Rows& first, 
         const uint64_t hit = __ballot(pos < before + rows.upto * heads);
         if (!hit) return false;
         const int w = __ffsll((unsigned long long)hit) - 1, chunks = scalar(rows.chunks, w);
-        const int start = before + (scalar(rows.upto, w) - chunks) * heads, k = (pos - start) / chunks;
-        const int whole = start + k * chunks;
+        int whole = before + (scalar(rows.upto, w) - chunks) * heads;
         s.row = r0 + w;
         s.s = scalar(rows.row.s, w);
         s.n = scalar(rows.row.n, w);
-        s.head = k / a.tiles;
-        s.tile = k % a.tiles;
-        s.from = pos - whole;
-        s.to = min(chunks, end - whole);
-        s.first = whole / each;
-        s.parts = (whole + chunks - 1) / each - s.first + 1;
-        s.part = pos / each - s.first;
+        for (; whole + chunks <= pos; whole += chunks)
+            if (++s.tile == a.tiles) {
+                s.tile = 0;
+                s.head++;
+            }
+        s.from = (pos - whole) * a.unit;
+        s.chunks = min(whole + chunks, end) - pos;
+        s.to = whole + chunks <= end ? units_of(s.n) : s.from + s.chunks * a.unit;
+        s.first = whole >= (int)blockIdx.x * each ? blockIdx.x : whole / (uint32_t)each;
+        s.part = blockIdx.x - s.first;
+        s.parts = (whole + chunks <= end ? blockIdx.x : (whole + chunks - 1) / (uint32_t)each) - s.first + 1;
         s.slot0 = 2 * s.first + (whole > s.first * each);
         return true;
     };
@@ -204,7 +214,7 @@ struct Shared {
 };
 
 template <int DH>
-__global__ void __launch_bounds__(THREADS, DH == 256 ? 1 : 2) attention_paged_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args a) {
     constexpr int C = DH / 32, H = DH / 128, PITCH = DH + 8;
     extern __shared__ __attribute__((aligned(16))) float lds[];  // Q as operands, [C][64 lanes] x 16 bytes; later [WAVES][rows][PITCH]
     __shared__ float wm[WAVES][ROWS], wl[WAVES][ROWS];
@@ -218,16 +228,16 @@ __global__ void __launch_bounds__(THREADS, DH == 256 ? 1 : 2) attention_paged_ke
     }
     for (int r0 = 64; r0 < a.B; r0 += 64) total += scalar(Rows(a, r0).upto, 63);
     total *= a.Hk * a.tiles;
-    const int each = (total + a.blocks - 1) / a.blocks;
+    const int each = __umulhi(total - 1, a.blocks_inverse) + 1;  // (one more than need be where the inverse's rounding shows)
     const int begin = (int)blockIdx.x * each, end = min(total, begin + each);
     __syncthreads();
     for (int pos = begin; pos < end;) {
     const Segment sh = segment_at(a, first[lane_here()], pos, end, each);
     const int lane = lane_here(), col = lane & 15, grp = lane >> 4;
-    pos += sh.to - sh.from;
+    pos += sh.chunks;
     const int rows = min(ROWS, a.G - sh.tile * ROWS), head0 = sh.head * a.G + sh.tile * ROWS;
-    const int u_end = min(sh.to * CHUNK_UNITS, sh.n / UNIT + (sh.n % UNIT != 0));
-    int u = sh.from * CHUNK_UNITS + wave;
+    const int u_end = sh.to;
+    int u = sh.from + wave;
 
     __syncthreads();  // the segment before is done with LDS
     u32x4* const qf = reinterpret_cast<u32x4*>(lds);
@@ -249,19 +259,28 @@ __global__ void __launch_bounds__(THREADS, DH == 256 ? 1 : 2) attention_paged_ke
     int next = 64;
     auto look_up = [&](int from) {
         const int i = lane_here();
-        const uint32_t key = (uint32_t)(from + (i >> 1) * WAVES) * UNIT + (i & 1) * 16, slot = key / (uint32_t)a.page;
+        const uint32_t half = 2 * (from + (i >> 1) * WAVES) + (i & 1), page = (uint32_t)a.page / 16;
+        uint32_t slot = __umulhi(half, a.page_inverse);
+        slot += (slot + 1) * page <= half;
         where = 0;
-        if (key < (uint32_t)sh.n) {
+        if (16 * half < (uint32_t)sh.n) {
             const int pg = a.table[(size_t)sh.s * a.max_pages + slot];
-            if (pg >= 0 && pg < a.npages)
-                where = ((uint32_t)pg * a.page + (key - slot * a.page)) / 16 << 5 | min(16, (int)(sh.n - key));
+            if (pg >= 0 && pg < a.npages) where = (pg * page + half - slot * page) << 5 | min(16, (int)(sh.n - 16 * half));
         }
     };
+    // The next unit is on its way while one is worked on.  A half's rows are read through a buffer descriptor that ends with
+    // the last valid one: rows behind it, and whole units behind the wave's last, come as zeros and cost no access.
     u32x4 kf[2][C], vf[H][8];
-    size_t v_at[2];
-    int have[2], v_have[2];
-    // byte offsets of this lane in a half: 32 bits next to a base that the wave shares
+    size_t at[2];
+    int have[2];
     const uint32_t row_b = 2 * (uint32_t)token, k_lane = col * row_b + grp * 16, v_lane = grp * 4 * row_b + col * 16;
+    auto half_rows = [&](const bf16* pool, size_t from, int rows) {
+        const uint64_t p = reinterpret_cast<uint64_t>(pool + from);
+        const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p), hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
+        return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((uint64_t)hi << 32 | lo), (short)0,
+                                                 __builtin_amdgcn_readfirstlane(rows > 0 ? (rows - 1) * row_b + 2 * DH : 0),
+                                                 0x00020000);
+    };
     auto load_k = [&](int from) {
         if (next == 64) {
             look_up(from);
@@ -269,25 +288,26 @@ __global__ void __launch_bounds__(THREADS, DH == 256 ? 1 : 2) attention_paged_ke
         }
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const uint32_t w = __builtin_amdgcn_readlane(where, next + t);
-            v_at[t] = (size_t)(w >> 5) * (16 * token) + sh.head * DH;
+            const uint32_t w = from < u_end ? __builtin_amdgcn_readlane(where, next + t) : 0;
+            at[t] = (size_t)(w >> 5) * (16 * token) + sh.head * DH;
             have[t] = w & 31;
-            const char* const p = reinterpret_cast<const char*>(a.kp + v_at[t]) + k_lane;
+            const auto r = half_rows(a.kp, at[t], have[t]);
 #pragma unroll
-            for (int c = 0; c < C; c++) kf[t][c] = *reinterpret_cast<const u32x4*>(p + c * 64);
+            for (int c = 0; c < C; c++)
+                kf[t][c] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, k_lane + c * 64, 0, 0));
         }
         next += 2;
     };
     auto load_v = [&]() {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            v_have[t] = have[t];
+            const auto r = half_rows(a.vp, at[t], have[t]);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const char* const p = reinterpret_cast<const char*>(a.vp + v_at[t]) + (size_t)i * row_b + v_lane;
+            for (int h = 0; h < H; h++)
 #pragma unroll
-                for (int h = 0; h < H; h++) vf[h][t * 4 + i] = *reinterpret_cast<const u32x4*>(p + h * 256);
-            }
+                for (int i = 0; i < 4; i++)
+                    vf[h][t * 4 + i] = __builtin_bit_cast(
+                        u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, v_lane + h * 256, i * row_b, 0));
         }
     };
     if (u < u_end) {
@@ -295,26 +315,25 @@ __global__ void __launch_bounds__(THREADS, DH == 256 ? 1 : 2) attention_paged_ke
         load_v();
     }
     __syncthreads();
-    // one unit; more: the wave has another after it
-    auto unit = [&](auto more) {
-        f32x4 st[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (; u < u_end; u += WAVES) {
+        const int valid[2] = {have[0], have[1]};
+        f32x4 st[2][2] = {};  // two sums a half: a product does not wait for the one before
 #pragma unroll
         for (int c = 0; c < C; c++) {
             const u32x4 q = qf[c * 64 + lane];
 #pragma unroll
-            for (int t = 0; t < 2; t++) st[t] = mfma16(kf[t][c], q, st[t]);
+            for (int t = 0; t < 2; t++) st[t][c & 1] = mfma16(kf[t][c], q, st[t][c & 1]);
         }
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (decltype(more)::value) load_k(u + WAVES);
+        load_k(u + WAVES);
         __builtin_amdgcn_sched_barrier(0);
         float sc[8], top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; i++) sc[i] = st[i >> 2][i & 3] * a.scale_log2;
-        const bool whole = v_have[0] + v_have[1] == UNIT;
-        if (!whole)
+        for (int i = 0; i < 8; i++) sc[i] = (st[i >> 2][0][i & 3] + st[i >> 2][1][i & 3]) * a.scale_log2;
+        if (valid[0] + valid[1] < UNIT)
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (grp * 4 + (i & 3) >= v_have[i >> 2]) sc[i] = -INFINITY;
+                if (grp * 4 + (i & 3) >= valid[i >> 2]) sc[i] = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; i++) top = fmaxf(top, sc[i]);
         if (__any(top > m + RISE)) {
@@ -336,29 +355,24 @@ __global__ void __launch_bounds__(THREADS, DH == 256 ? 1 : 2) attention_paged_ke
             ph[i] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302);
             pl[i] = pack2(fmaxf(p0 - lo_f32(ph[i]), LEAST), fmaxf(p1 - hi_f32(ph[i]), LEAST));
         }
-        if (!whole)  // what lies where no key is may be anything; zero times it would not be zero
 #pragma unroll
-            for (int h = 0; h < H; h++)
+        for (int h = 0; h < H; h++) {
+            u32x4 vt[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (grp * 4 + (i & 3) >= v_have[i >> 2]) vf[h][i] = u32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int h = 0; h < H; h++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                u32x4 vt;
+            for (int j = 0; j < 8; j++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    vt[i] = __builtin_amdgcn_perm(vf[h][2 * i + 1][j >> 1], vf[h][2 * i][j >> 1], j & 1 ? 0x07060302 : 0x05040100);
-                acc[h][j] = mfma16(vt, ph, acc[h][j]);
-                acc[h][j] = mfma16(vt, pl, acc[h][j]);
-            }
+                    vt[j][i] = __builtin_amdgcn_perm(vf[h][2 * i + 1][j >> 1], vf[h][2 * i][j >> 1],
+                                                     j & 1 ? 0x07060302 : 0x05040100);
+#pragma unroll
+            for (int j = 0; j < 8; j++) acc[h][j] = mfma16(vt[j], ph, acc[h][j]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) acc[h][j] = mfma16(vt[j], pl, acc[h][j]);
+        }
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (decltype(more)::value) load_v();
+        load_v();
         __builtin_amdgcn_sched_barrier(0);
-    };
-    for (; u + WAVES < u_end; u += WAVES) unit(std::true_type{});
-    if (u < u_end) unit(std::false_type{});
+    }
 
     // the waves join
     const int tid = wave * 64 + lane_here();
@@ -394,28 +408,16 @@ __global__ void __launch_bounds__(THREADS, DH == 256 ? 1 : 2) attention_paged_ke
         shared.put((at * DH + d) * 4, o);
         if (d == 0) shared.put_ml(at * 8, f32x2{top, sum});
     };
-    for (int e = tid; e < rows * QUADS; e += THREADS) {
-        const int row = e / QUADS, d = e % QUADS * 4;
-        const u32x2 g = load_gate(a, out0 + row * DH + d);
-        float top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) top = fmaxf(top, wm[w][row]);
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            const float f = wm[w][row] == top ? 1.f : __builtin_amdgcn_exp2f(wm[w][row] - top);
-            sum += wl[w][row] * f;
-            o += *reinterpret_cast<const f32x4*>(lds + ((size_t)w * rows + row) * PITCH + d) * f;
-        }
-        store(sh.slot(sh.part), e, top, sum, o, g, sh.parts == 1);
-    }
-    if (sh.parts == 1) continue;
-
     // Groups of `group` parts: the last of a group to end joins it, the last group joins the groups; always in order, so the
     // result does not depend on which ends last.  The counters are zero again afterwards.
-    const int least = (sh.parts + GROUP - 1) / GROUP, group = (sh.parts + least - 1) / least;
-    const int groups = (sh.parts + group - 1) / group;
-    const int g0 = sh.part / group * group, members = min(group, sh.parts - g0);
+    int group = 1, groups = 1, g0 = 0, members = 1;
+    if (sh.parts > 1) {
+        groups = (sh.parts + GROUP - 1) / GROUP;
+        group = (sh.parts + groups - 1) / (uint32_t)groups;
+        groups = (sh.parts + group - 1) / (uint32_t)group;
+        g0 = sh.part / (uint32_t)group * group;
+        members = min(group, sh.parts - g0);
+    }
     auto last_of = [&](int* count, int n) {
         __shared__ int last;
         wait_vm_all();  // what this wave has put is where the others look
@@ -427,63 +429,71 @@ __global__ void __launch_bounds__(THREADS, DH == 256 ? 1 : 2) attention_paged_ke
         __syncthreads();
         return last != 0;
     };
-    // The results of n parts from number k0 on, every `step`-th: out, or to the first one's place.  The time is that of
-    // getting at them, so many are asked for at once: a row's four dims are summed by as many threads as there are for them, each
-    // with every `ways`-th part, BATCH of them on their way together, the first while a wave per row finds the parts' weights.
-    auto join = [&](int k0, int step, int n, bool out) {
-        const int items = rows * QUADS, ways = max(1, THREADS / items);
-        float* const weight = lds;                        // [GROUP, ROWS]
-        float* const other = lds + GROUP * ROWS;          // [THREADS, 4]
+    // Stage 0: this block's waves.  1: a group's parts, 2: the groups.  A row's four dims are summed by as many threads as there
+    // are for them.  The time of 1 and 2 is that of getting at the parts, so many are asked for at once: a thread has every
+    // `ways`-th, BATCH of them on their way together, the first while a wave per row finds the parts' weights.
+    float* const weight = lds;               // [GROUP, ROWS]
+    float* const other = lds + GROUP * ROWS;  // [THREADS, 4]
+    const int items = rows * QUADS, rows_log = rows > 1 ? 32 - __builtin_clz(rows - 1) : 0;
+    for (int stage = 0;; stage++) {
+        const bool out = stage == 0 ? sh.parts == 1 : stage == 2 || groups == 1;
+        const int k0 = stage == 1 ? g0 : 0, step = stage == 2 ? group : 1, n = stage == 1 ? members : groups;
+        const int ways = stage == 0 ? 1 : max(1, THREADS / QUADS >> rows_log);
         for (int e0 = 0; e0 < items; e0 += THREADS) {
-            const int way = ways > 1 ? tid / items : 0, e = ways > 1 ? tid % items : e0 + tid;
-            const bool works = way < ways && e < items;
+            const int way = ways > 1 ? tid / QUADS >> rows_log : 0;
+            const int e = e0 + (ways > 1 ? tid & ((QUADS << rows_log) - 1) : tid);
+            const bool works = e < items;
             const int row = works ? e / QUADS : 0, d = e % QUADS * 4;
-            f32x4 v[BATCH];
-            auto load = [&](int k1) {
-#pragma unroll
-                for (int i = 0; i < BATCH; i++)  // (behind the last: the last again)
-                    v[i] = shared.get(((sh.slot(k0 + min(k1 + i * ways, n - 1) * step) * ROWS + row) * DH + d) * 4);
-            };
-            load(way);
-            const u32x2 g = load_gate(a, out0 + row * DH + d);
-            if (e0 == 0) {
-                const int k = tid & 63;
-                for (int r = wave; r < rows; r += WAVES) {
-                    const f32x2 m = shared.get_ml((sh.slot(k0 + min(k, n - 1) * step) * ROWS + r) * 8);
-                    const float top = lane_max<64>(m[0]), f = m[0] == top ? 1.f : __builtin_amdgcn_exp2f(m[0] - top);
-                    weight[k * ROWS + r] = f;
-                    const float sum = lane_sum<64>(k < n ? m[1] * f : 0.f);
-                    if (k == 0) {
-                        wm[0][r] = top;
-                        wl[0][r] = sum;
-                    }
-                }
-                __syncthreads();
-            }
+            u32x2 g = {0, 0};
             f32x4 o = {0.f, 0.f, 0.f, 0.f};
-            for (int k1 = way; k1 < n; k1 += BATCH * ways) {
-                if (k1 > way) load(k1);
+            float top, sum = 0.f;
+            if (out) g = load_gate(a, out0 + row * DH + d);
+            if (stage == 0) {
+                top = fmaxf(fmaxf(wm[0][row], wm[1][row]), fmaxf(wm[2][row], wm[3][row]));
 #pragma unroll
-                for (int i = 0; i < BATCH; i++) {
-                    const int k = k1 + i * ways;
-                    const f32x4 more = o + v[i] * weight[min(k, n - 1) * ROWS + row];
-                    if (k < n) o = more;
+                for (int w = 0; w < WAVES; w++) {
+                    const float f = wm[w][row] == top ? 1.f : __builtin_amdgcn_exp2f(wm[w][row] - top);
+                    sum += wl[w][row] * f;
+                    o += *reinterpret_cast<const f32x4*>(lds + (w * rows + row) * PITCH + d) * f;
                 }
+            } else {
+                for (int k1 = way; k1 - way < n; k1 += BATCH * ways) {
+                    f32x4 v[BATCH];
+#pragma unroll
+                    for (int i = 0; i < BATCH; i++) {  // behind the last part: past the buffer's end, which is no access
+                        const int k = k1 + i * ways;
+                        v[i] = shared.get(k < n ? ((sh.slot(k0 + k * step) * ROWS + row) * DH + d) * 4 : -1);
+                    }
+                    if (e0 == 0 && k1 == way) {
+                        const int k = tid & 63;
+                        for (int r = wave; r < rows; r += WAVES) {
+                            const f32x2 m = shared.get_ml((sh.slot(k0 + min(k, n - 1) * step) * ROWS + r) * 8);
+                            const float most = lane_max<64>(m[0]);
+                            const float f = k >= n ? 0.f : m[0] == most ? 1.f : __builtin_amdgcn_exp2f(m[0] - most);
+                            weight[k * ROWS + r] = f;
+                            const float all = lane_sum<64>(k < n ? m[1] * f : 0.f);
+                            if (k == 0) {
+                                wm[0][r] = most;
+                                wl[0][r] = all;
+                            }
+                        }
+                        __syncthreads();
+                    }
+#pragma unroll
+                    for (int i = 0; i < BATCH; i++) o += v[i] * weight[min(k1 + i * ways, GROUP - 1) * ROWS + row];
+                }
+                if (ways > 1) {
+                    if (works && way > 0) *reinterpret_cast<f32x4*>(other + (way * items + e) * 4) = o;
+                    __syncthreads();
+                    if (way == 0)
+                        for (int w = 1; w < ways; w++) o += *reinterpret_cast<const f32x4*>(other + (w * items + (works ? e : 0)) * 4);
+                }
+                top = wm[0][row];
+                sum = wl[0][row];
             }
-            if (ways > 1) {
-                if (works && way > 0) *reinterpret_cast<f32x4*>(other + (way * items + e) * 4) = o;
-                __syncthreads();
-                if (way == 0)
-                    for (int w = 1; w < ways; w++) o += *reinterpret_cast<const f32x4*>(other + (w * items + e) * 4);
-            }
-            if (works && way == 0) store(sh.slot(k0), e, wm[0][row], wl[0][row], o, g, out);
+            if (works && way == 0) store(out ? 0 : sh.slot(stage == 0 ? sh.part : k0), e, top, sum, o, g, out);
         }
-        __syncthreads();
-    };
-    if (!last_of(a.count + sh.slot(g0), members)) continue;
-    for (bool whole = groups == 1;; whole = true) {
-        join(whole ? 0 : g0, whole && groups > 1 ? group : 1, whole ? groups > 1 ? groups : members : members, whole);
-        if (whole || !last_of(a.count2 + sh.slot0, groups)) break;
+        if (out || !last_of(stage == 0 ? a.count + sh.slot(g0) : a.count2 + sh.slot0, stage == 0 ? members : groups)) break;
     }
     }
 }
@@ -515,7 +525,7 @@ using namespace q35;
 extern "C" void* cs1_attention_paged_create(void) {
     int device;
     const int cus = device_cus();
-    if (cus == 0 || hipGetDevice(&device) != hipSuccess || !configure<128>() || !configure<256>()) {
+    if (cus < 2 || hipGetDevice(&device) != hipSuccess || !configure<128>() || !configure<256>()) {
         (void)hipGetLastError();
         return nullptr;
     }
@@ -523,7 +533,7 @@ extern "C" void* cs1_attention_paged_create(void) {
     if (!p) return nullptr;
     p->device = device;
     p->cus = std::min(cus, GROUP * GROUP / 3);
-    p->blocks = 3 * p->cus;
+    p->blocks = p->cus;
     const size_t floats = (size_t)2 * p->blocks * ROWS * (256 + 2), counts = (size_t)4 * p->blocks;
     p->part = nullptr;
     if (hipMalloc(reinterpret_cast<void**>(&p->part), 4 * (floats + counts)) != hipSuccess ||
@@ -550,7 +560,8 @@ extern "C" int cs1_attention_paged(void* paged, const void* q, const void* kp, c
     const Paged* const p = static_cast<const Paged*>(paged);
     if (!p || !table_ok(pages) || (Dh != 128 && Dh != 256) || Hk <= 0 || Hq <= 0 || Hq % Hk != 0 || B < 0 ||
         (int64_t)B * Hq > (1 << 22) || (int64_t)Hk * Dh > (1 << 24) ||
-        (int64_t)pages->npages * pages->page >= (int64_t{1} << 31))
+        (int64_t)pages->npages * pages->page >= (int64_t{1} << 31) ||
+        (int64_t)B * Hk * ((Hq / Hk + ROWS - 1) / ROWS) * ((int64_t)pages->max_pages * pages->page / UNIT + 1) >= (int64_t{1} << 31))
         return hipErrorInvalidValue;
     if (B == 0) return hipSuccess;
     if (!all_set({q, kp, vp, out}) || !on16(q) || !on16(kp) || !on16(vp) || !on16(out) || !on16(gate))
@@ -581,6 +592,11 @@ extern "C" int cs1_attention_paged(void* paged, const void* q, const void* kp, c
     a.G = Hq / Hk;
     a.tiles = (a.G + ROWS - 1) / ROWS;
     a.blocks = p->cus;
+    // Chunks of 128 keys for few sequences, of 512 for many, so that no block has a sequence's last few keys to itself (43
+    // of up to 4096, 16/4 heads of 128: 46.9 us with 128, 41.3 with 512; one of 12000: 14.9 and 15.4)
+    a.unit = (int64_t)B * Hk * a.tiles * 4 < a.blocks ? FINE : COARSE;
+    a.page_inverse = (uint32_t)std::min<uint64_t>(0xffffffffu, (uint64_t{1} << 32) / (a.page / 16));
+    a.blocks_inverse = (uint32_t)(((uint64_t{1} << 32) + a.blocks - 1) / a.blocks);
     a.scale_log2 = scale * LOG2E;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     return Dh == 128 ? launch<128>(a, st) : launch<256>(a, st);
