@@ -20,8 +20,15 @@ __device__ __forceinline__ int listed_seq(const int32_t* __restrict__ seqs, int 
     return s >= 0 && s < nseq ? s : -1;
 }
 
-// Whether an entry before i names the same sequence (this thread's share of the entries; the
-// block's threads together see all of them).
+// Whether an entry before i names the same sequence, asked by a whole wave for itself.
+__device__ __forceinline__ bool wave_named_before(const int32_t* __restrict__ seqs, int i, int s) {
+    bool hit = false;
+    if (seqs)
+        for (int j = threadIdx.x & 63; j < i; j += 64) hit |= seqs[j] == s;
+    return __any(hit);
+}
+
+// The same with this thread's share of the entries; the block's threads together see all of them.
 __device__ __forceinline__ bool named_before(const int32_t* __restrict__ seqs, int i, int s) {
     bool hit = false;
     if (seqs)
