@@ -6,8 +6,8 @@
 // With need_i new pages for entry i and off_i the sum of the needs before it, the free page with k
 // free pages below it goes to the entry with off_i <= k < off_i + need_i.  One block of 1024 threads does
 // that: a scan over the needs, then scans over 4096 counts at a time until enough pages are found.
-// What moves keys and values is a kernel of its own that fills the chip: 16-byte accesses, a page's
-// filled rows being one run of bytes in each pool.
+// What moves keys and values is a kernel of its own that fills the chip: a page's filled rows are one run of bytes in
+// each pool.
 #include "common.h"
 #include "paged.h"
 
@@ -15,7 +15,7 @@ namespace q35 {
 namespace {
 
 constexpr int PLAN_THREADS = 1024, PLAN_WAVES = PLAN_THREADS / 64;
-constexpr int PER = MAX_LISTED / PLAN_THREADS;  // list entries a thread has at most
+constexpr int PER_MAX = MAX_LISTED / PLAN_THREADS;  // list entries a thread has at most
 constexpr int SEQS_MAX = 64, POOLS_MAX = 64;    // offsets and pools that travel with a launch
 constexpr int MOVE_THREADS = 256;
 
@@ -67,62 +67,65 @@ __device__ __forceinline__ int entry_of(const int* off, int n, int k) {
     return lo;
 }
 
-// Calls take(k, page) for the `total` lowest free pages, k = 0 .., or for all there are; returns their number.
+// Whether pages p .. p + 3 are free, as four bits.
+__device__ __forceinline__ uint32_t free_pages(const int32_t* __restrict__ refs, int npages, int p) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (p + e < npages && refs[p + e] == 0) bits |= 1u << e;
+    return bits;
+}
+
+// Calls take(k, page) for the `total` lowest free pages, k = 0 .., or for all there are; returns their number. bits: of
+// pages 4 threadIdx.x .. + 3, asked for early by the caller.
 template <typename Take>
-__device__ __forceinline__ int take_free(const int32_t* refs, int npages, int total, int* red, Take take) {
+__device__ __forceinline__ int take_free(const int32_t* refs, int npages, int total, uint32_t bits, int* red, Take take) {
     int found = 0;
     for (int base = 0; base < npages && found < total; base += 4 * PLAN_THREADS) {
         const int p = base + 4 * threadIdx.x;
-        bool free[4];
-        int mine = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            free[e] = p + e < npages && refs[p + e] == 0;
-            mine += free[e];
-        }
-        int all, k = found + block_scan(mine, red, all);
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (free[e]) {
-                if (k < total) take(k, p + e);
-                k++;
-            }
+        if (base > 0) bits = free_pages(refs, npages, p);
+        int all, k = found + block_scan(__popc(bits), red, all);
+        for (; bits && k < total; bits &= bits - 1, k++) take(k, p + __ffs(bits) - 1);
         found = min(total, found + all);
     }
     return found;
 }
 
+// PER: list entries a thread has at most. Lists of up to 1024 have one each, which leaves a third of the code: what runs once
+// takes its time to arrive (6.4 us with eight, 4.9 with one).
+template <int PER>
 __global__ void __launch_bounds__(PLAN_THREADS)
     kv_reserve_kernel(const Cs1PageTable t, const int32_t* __restrict__ seqs, const Offsets cu, int n, int32_t* status) {
     __shared__ int work[MAX_LISTED];  // first entry that names a sequence, then the offsets off_i
     __shared__ int red[PLAN_WAVES];
     const int tid = threadIdx.x;
+    const uint32_t bits = free_pages(t.refs, t.npages, 4 * tid);
+    const int per = PER == 1 ? 1 : (n + PLAN_THREADS - 1) / PLAN_THREADS, i0 = tid * per;
+    int seq[PER], len[PER];
+#pragma unroll
+    for (int e = 0; e < PER; e++) {
+        seq[e] = e < per && i0 + e < n ? listed_seq(seqs, i0 + e, t.nseq) : -1;
+        len[e] = seq[e] >= 0 ? max(t.lens[seq[e]], 0) : 0;
+    }
     for (int s = tid; s < t.nseq; s += PLAN_THREADS) work[s] = n;
     __syncthreads();
-    for (int i = tid; i < n; i += PLAN_THREADS) {
-        const int s = listed_seq(seqs, i, t.nseq);
-        if (s >= 0) atomicMin(&work[s], i);
-    }
+#pragma unroll
+    for (int e = 0; e < PER; e++)
+        if (seq[e] >= 0) atomicMin(&work[seq[e]], i0 + e);
     __syncthreads();
-    const int per = (n + PLAN_THREADS - 1) / PLAN_THREADS, i0 = tid * per;
     int need[PER], mine = 0;
-    uint32_t has = 0;  // the entries that have their sequence
     bool wide = false;
 #pragma unroll
     for (int e = 0; e < PER; e++) {
         const int i = i0 + e;
         need[e] = 0;
-        if (e >= per || i >= n) continue;
-        const int s = listed_seq(seqs, i, t.nseq);
-        if (s < 0 || work[s] != i) continue;
-        has |= 1u << e;
-        const int64_t len = max(t.lens[s], 0), to = len + (cu.n ? cu.at[i + 1] - cu.at[i] : 1);
-        if (to > (int64_t)t.max_pages * t.page) {
+        if (seq[e] >= 0 && work[seq[e]] != i) seq[e] = -1;
+        if (seq[e] < 0) continue;
+        const int64_t to = (int64_t)len[e] + (cu.n ? cu.at[i + 1] - cu.at[i] : 1);
+        if (to > (int64_t)t.max_pages * t.page)
             wide = true;
-            continue;
-        }
-        need[e] = pages_of(to, t.page) - pages_of(len, t.page);
-        mine += need[e];
+        else
+            mine += need[e] = pages_of(to, t.page) - pages_of(len[e], t.page);
     }
     if (__syncthreads_or(wide)) {
         if (tid == 0) *status = -1;
@@ -139,7 +142,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
         const int i = entry_of(work, n, k), s = listed_seq(seqs, i, t.nseq);
         return t.table + (size_t)s * t.max_pages + pages_of(max(t.lens[s], 0), t.page) + (k - work[i]);
     };
-    const int found = take_free(t.refs, t.npages, total, red, [&](int k, int p) {
+    const int found = take_free(t.refs, t.npages, total, bits, red, [&](int k, int p) {
         *slot(k) = p;
         t.refs[p] = 1;
     });
@@ -154,42 +157,57 @@ __global__ void __launch_bounds__(PLAN_THREADS)
         __syncthreads();  // slot() has read the lengths
 #pragma unroll
         for (int e = 0; e < PER; e++)
-            if (has >> e & 1) {
-                const int i = i0 + e;
-                int32_t* const len = t.lens + listed_seq(seqs, i, t.nseq);
-                *len = max(*len, 0) + (cu.n ? cu.at[i + 1] - cu.at[i] : 1);
-            }
+            if (seq[e] >= 0) t.lens[seq[e]] = len[e] + (cu.n ? cu.at[i0 + e + 1] - cu.at[i0 + e] : 1);
     }
     if (tid == 0) *status = total - found;
 }
 
-// One block a row: its keys by the first half of the threads, its values by the second.
+// One wave a row.  The first of its keys and values are asked for before it is known where they go.
+constexpr int ROWS_BLOCK = MOVE_THREADS / 64;
+
 __global__ void __launch_bounds__(MOVE_THREADS)
-    kv_write_kernel(const Cs1PageTable t, const int32_t* __restrict__ seqs, const Offsets cu, int first,
+    kv_write_kernel(const Cs1PageTable t, const int32_t* __restrict__ seqs, const Offsets cu, int first, int rows,
                     const bf16* __restrict__ k, int ldk, const bf16* __restrict__ v, int ldv, char* kp, char* vp,
                     int width) {
-    const int r = blockIdx.x;
+    const int lane = threadIdx.x & 63, r = __builtin_amdgcn_readfirstlane(blockIdx.x * ROWS_BLOCK + (threadIdx.x >> 6));
+    if (r >= rows) return;
+    const size_t row = cu.n ? (size_t)cu.at[0] + r : (size_t)r;
+    const int packs = width / 8;
+    const u32x4* const kr = reinterpret_cast<const u32x4*>(k + row * ldk);
+    const u32x4* const vr = reinterpret_cast<const u32x4*>(v + row * ldv);
+    u32x4 a[2], b[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        if (lane + 64 * i < packs) {
+            a[i] = kr[lane + 64 * i];
+            b[i] = vr[lane + 64 * i];
+        }
     int i = r, back = 1;  // list entry, and how far from the end of its sequence the row is
     if (cu.n) {
-        i = 0;
-        while (i + 1 < cu.n && r >= cu.at[i + 1] - cu.at[0]) i++;
+        // (the last offset is behind every row)
+        i = __popcll(__ballot(lane < cu.n && r >= cu.at[min(lane, cu.n - 1) + 1] - cu.at[0]));
         back = cu.at[i + 1] - cu.at[0] - r;
         i += first;
     }
-    const int s = listed_seq(seqs, i, t.nseq);
+    const int s = __builtin_amdgcn_readfirstlane(listed_seq(seqs, i, t.nseq));
     if (s < 0) return;
-    const bool again = named_before(seqs, i, s);
-    const int pos = t.lens[s] - back;
-    if (__syncthreads_or(again) || pos < 0 || pos / t.page >= t.max_pages) return;
-    const int pg = t.table[(size_t)s * t.max_pages + pos / t.page];
+    const int pos = __builtin_amdgcn_readfirstlane(t.lens[s]) - back;
+    if (pos < 0 || pos / t.page >= t.max_pages || wave_named_before(seqs, i, s)) return;
+    const int pg = __builtin_amdgcn_readfirstlane(t.table[(size_t)s * t.max_pages + pos / t.page]);
     if (pg < 0 || pg >= t.npages) return;
-    const size_t row = cu.n ? (size_t)cu.at[0] + r : (size_t)r;
-    const size_t to = ((size_t)pg * t.page + pos % t.page) * width * 2;
-    const bool value = threadIdx.x >= MOVE_THREADS / 2;
-    const char* const from = reinterpret_cast<const char*>(value ? v + row * ldv : k + row * ldk);
-    char* const at = (value ? vp : kp) + to;
-    for (int e = (threadIdx.x % (MOVE_THREADS / 2)) * 16; e < width * 2; e += MOVE_THREADS / 2 * 16)
-        *reinterpret_cast<u32x4*>(at + e) = *reinterpret_cast<const u32x4*>(from + e);
+    const size_t to = ((size_t)pg * t.page + pos % t.page) * packs;
+    u32x4* const kt = reinterpret_cast<u32x4*>(kp) + to;
+    u32x4* const vt = reinterpret_cast<u32x4*>(vp) + to;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        if (lane + 64 * i < packs) {
+            kt[lane + 64 * i] = a[i];
+            vt[lane + 64 * i] = b[i];
+        }
+    for (int e = lane + 128; e < packs; e += 64) {
+        kt[e] = kr[e];
+        vt[e] = vr[e];
+    }
 }
 
 // What a fork does for one pair: the last page that is not full (rows of it, 0: none), copied from `from` to `to`.
@@ -197,34 +215,40 @@ struct Pair {
     int32_t on, from, to, rows;
 };
 
+template <int PER>
 __global__ void __launch_bounds__(PLAN_THREADS)
     kv_fork_plan_kernel(const Cs1PageTable t, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int n,
                         Pair* __restrict__ plan, int32_t* status) {
     __shared__ int work[MAX_LISTED];
     __shared__ int red[PLAN_WAVES];
     const int tid = threadIdx.x;
-    for (int s = tid; s < t.nseq; s += PLAN_THREADS) work[s] = n;
-    __syncthreads();
-    for (int i = tid; i < n; i += PLAN_THREADS) {
-        const int d = listed_seq(dst, i, t.nseq);
-        if (d >= 0) atomicMin(&work[d], i);
-    }
-    __syncthreads();
-    const int per = (n + PLAN_THREADS - 1) / PLAN_THREADS, i0 = tid * per;
+    const uint32_t bits = free_pages(t.refs, t.npages, 4 * tid);
+    const int per = PER == 1 ? 1 : (n + PLAN_THREADS - 1) / PLAN_THREADS, i0 = tid * per;
+    int from[PER], to[PER];
     Pair mine[PER];
-    int need = 0;
 #pragma unroll
     for (int e = 0; e < PER; e++) {
-        const int i = i0 + e;
+        const bool in = e < per && i0 + e < n;
+        from[e] = in ? listed_seq(src, i0 + e, t.nseq) : -1;
+        to[e] = in ? listed_seq(dst, i0 + e, t.nseq) : -1;
         mine[e] = Pair{0, -1, -1, 0};
-        if (e >= per || i >= n) continue;
-        const int s = listed_seq(src, i, t.nseq), d = listed_seq(dst, i, t.nseq);
-        if (s < 0 || d < 0 || work[d] != i || work[s] != n || t.lens[d] > 0) continue;
-        const int len = t.lens[s];
+        if (from[e] < 0 || to[e] < 0 || t.lens[to[e]] > 0) continue;
+        const int len = t.lens[from[e]];
         if (len <= 0 || pages_of(len, t.page) > t.max_pages) continue;
         mine[e].on = 1;
         mine[e].rows = len % t.page;
-        if (mine[e].rows) mine[e].from = t.table[(size_t)s * t.max_pages + len / t.page];
+        if (mine[e].rows) mine[e].from = t.table[(size_t)from[e] * t.max_pages + len / t.page];
+    }
+    for (int s = tid; s < t.nseq; s += PLAN_THREADS) work[s] = n;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; e++)
+        if (to[e] >= 0) atomicMin(&work[to[e]], i0 + e);
+    __syncthreads();
+    int need = 0;
+#pragma unroll
+    for (int e = 0; e < PER; e++) {
+        if (mine[e].on && (work[to[e]] != i0 + e || work[from[e]] != n)) mine[e] = Pair{0, -1, -1, 0};
         need += mine[e].rows > 0;
     }
     int total, off = block_scan(need, red, total);
@@ -238,7 +262,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
         off += mine[e].rows > 0;
     }
     __syncthreads();
-    const int found = take_free(t.refs, t.npages, total, red, [&](int k, int p) {
+    const int found = take_free(t.refs, t.npages, total, bits, red, [&](int k, int p) {
         plan[entry_of(work, n, k)].to = p;
         t.refs[p] = 1;
     });
@@ -252,37 +276,70 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     if (tid == 0) *status = total - found;
 }
 
-// Blocks y = 0 of the first launch: the pair's row of the table, the shared pages' counts, the length. The others: the
-// filled rows of the unfinished page, in pool y - 1, CHUNK bytes a block.
-constexpr int FORK_CHUNK = MOVE_THREADS * 16 * 4;
+// How entries are copied: a block has a chunk of one pool for `run` pairs in a row and reads it once for all that have
+// the same source, so that copies of one entry cost their writing alone (8 copies of 50 MiB: 73 us, and 140 with a
+// block for each).  What is written goes past the caches; so does what is read, where it is read once.
+constexpr int QUADS = 4, CHUNK = MOVE_THREADS * 16 * QUADS;
 
+__device__ __forceinline__ void load_chunk(u32x4 (&r)[QUADS], const char* from, size_t chunk, size_t bytes, bool once) {
+#pragma unroll
+    for (int q = 0; q < QUADS; q++) {
+        const size_t e = chunk * CHUNK + (q * MOVE_THREADS + threadIdx.x) * 16;
+        const u32x4* const p = reinterpret_cast<const u32x4*>(from + e);
+        if (e < bytes) r[q] = once ? __builtin_nontemporal_load(p) : *p;
+    }
+}
+__device__ __forceinline__ void store_chunk(const u32x4 (&r)[QUADS], char* to, size_t chunk, size_t bytes) {
+#pragma unroll
+    for (int q = 0; q < QUADS; q++) {
+        const size_t e = chunk * CHUNK + (q * MOVE_THREADS + threadIdx.x) * 16;
+        if (e < bytes) __builtin_nontemporal_store(r[q], reinterpret_cast<u32x4*>(to + e));
+    }
+}
+
+constexpr int RUN_MAX = 8;
+
+// Runs where there are blocks enough without the pairs apart (4096: sixteen a CU).
+int run_of(size_t chunks, int pools, int n) {
+    const size_t blocks = chunks * pools * n;
+    return blocks >= 4096 * RUN_MAX ? RUN_MAX : blocks <= 4096 ? 1 : (int)(blocks / 4096);
+}
+
+// Blocks y = 0 of the first launch: the pairs' rows of the table, the shared pages' counts, the lengths. The others: a
+// chunk of the filled rows of the unfinished pages, in pool y - 1.
 __global__ void __launch_bounds__(MOVE_THREADS)
     kv_fork_kernel(const Cs1PageTable t, const int32_t* __restrict__ src, const int32_t* __restrict__ dst,
-                   const Pair* __restrict__ plan, const Pools pools, size_t row_bytes, int tables) {
-    const Pair pr = plan[blockIdx.z];
-    if (!pr.on) return;
-    const int pool = (int)blockIdx.y - tables;
+                   const Pair* __restrict__ plan, const Pools pools, size_t row_bytes, int tables, int n, int run) {
+    const int pool = (int)blockIdx.y - tables, i0 = blockIdx.z * run, i1 = min(n, i0 + run);
     if (pool < 0) {
-        if (blockIdx.x > 0) return;
-        const int s = src[blockIdx.z], d = dst[blockIdx.z], len = t.lens[s], full = len / t.page;
-        for (int j = threadIdx.x; j < full; j += MOVE_THREADS) {
-            const int p = t.table[(size_t)s * t.max_pages + j];
-            t.table[(size_t)d * t.max_pages + j] = p;
-            if (p >= 0 && p < t.npages) atomicAdd(&t.refs[p], 1);
-        }
-        if (threadIdx.x == 0) {
-            if (pr.rows) t.table[(size_t)d * t.max_pages + full] = pr.to;
-            t.lens[d] = len;
+        for (int i = i0 + blockIdx.x; i < i1; i += gridDim.x) {
+            const Pair pr = plan[i];
+            if (!pr.on) continue;
+            const int s = src[i], d = dst[i], len = t.lens[s], full = len / t.page;
+            for (int j = threadIdx.x; j < full; j += MOVE_THREADS) {
+                const int p = t.table[(size_t)s * t.max_pages + j];
+                t.table[(size_t)d * t.max_pages + j] = p;
+                if (p >= 0 && p < t.npages) atomicAdd(&t.refs[p], 1);
+            }
+            if (threadIdx.x == 0) {
+                if (pr.rows) t.table[(size_t)d * t.max_pages + full] = pr.to;
+                t.lens[d] = len;
+            }
         }
         return;
     }
-    if (pr.from < 0 || pr.from >= t.npages) return;
-    const size_t bytes = pr.rows * row_bytes, page_bytes = t.page * row_bytes;
-    const size_t end = min(bytes, ((size_t)blockIdx.x + 1) * FORK_CHUNK);
-    const char* const from = pools.p[pool] + pr.from * page_bytes;
-    char* const to = pools.p[pool] + pr.to * page_bytes;
-    for (size_t e = (size_t)blockIdx.x * FORK_CHUNK + threadIdx.x * 16; e < end; e += MOVE_THREADS * 16)
-        *reinterpret_cast<u32x4*>(to + e) = *reinterpret_cast<const u32x4*>(from + e);
+    const size_t page_bytes = t.page * row_bytes;
+    u32x4 r[QUADS];
+    int held = -1, rows = 0;
+    for (int i = i0; i < i1; i++) {
+        const Pair pr = plan[i];
+        if (!pr.on || pr.from < 0 || pr.from >= t.npages || blockIdx.x * (size_t)CHUNK >= pr.rows * row_bytes) continue;
+        if (pr.from != held || pr.rows != rows)
+            load_chunk(r, pools.p[pool] + pr.from * page_bytes, blockIdx.x, pr.rows * row_bytes, false);
+        held = pr.from;
+        rows = pr.rows;
+        store_chunk(r, pools.p[pool] + pr.to * page_bytes, blockIdx.x, pr.rows * row_bytes);
+    }
 }
 
 __global__ void __launch_bounds__(MOVE_THREADS)
@@ -344,8 +401,6 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     }
 }
 
-constexpr int COMPACT_CHUNK = MOVE_THREADS * 16 * 4;
-
 // Blocks before `tables`: a sequence's row of the table each. The others move pages, a chunk at a time.
 __global__ void __launch_bounds__(MOVE_THREADS)
     kv_compact_kernel(const Cs1PageTable t, const int32_t* __restrict__ ws, const Pools pools, int npools,
@@ -371,37 +426,52 @@ __global__ void __launch_bounds__(MOVE_THREADS)
             t.refs[to[k]] = t.refs[from[k]];
             t.refs[from[k]] = 0;
         }
-    const int chunks = (int)((page_bytes + COMPACT_CHUNK - 1) / COMPACT_CHUNK);
-    const int64_t items = (int64_t)moves * npools * chunks;
-    for (int64_t it = block; it < items; it += blocks) {
-        const int chunk = (int)(it % chunks), pool = (int)(it / chunks % npools), k = (int)(it / chunks / npools);
-        const char* const a = pools.p[pool] + from[k] * page_bytes;
-        char* const b = pools.p[pool] + to[k] * page_bytes;
-        const size_t end = min(page_bytes, ((size_t)chunk + 1) * COMPACT_CHUNK);
-        for (size_t e = (size_t)chunk * COMPACT_CHUNK + threadIdx.x * 16; e < end; e += MOVE_THREADS * 16)
-            *reinterpret_cast<u32x4*>(b + e) = *reinterpret_cast<const u32x4*>(a + e);
+    // the next chunk is on its way while one is stored
+    const uint32_t chunks = (uint32_t)((page_bytes + CHUNK - 1) / CHUNK), items = (uint32_t)moves * npools * chunks;
+    u32x4 r[QUADS], next[QUADS];
+    auto place = [&](uint32_t it, const int32_t* pages, uint32_t& chunk) {
+        const uint32_t page = it / chunks, k = page / (uint32_t)npools;
+        chunk = it - page * chunks;
+        return pools.p[page - k * npools] + pages[k] * page_bytes;
+    };
+    uint32_t it = block, chunk;
+    if (it < items) {
+        const char* const a = place(it, from, chunk);
+        load_chunk(next, a, chunk, page_bytes, true);
+    }
+    for (; it < items; it += blocks) {
+#pragma unroll
+        for (int q = 0; q < QUADS; q++) r[q] = next[q];
+        if (it + blocks < items) {
+            const char* const a = place(it + blocks, from, chunk);
+            load_chunk(next, a, chunk, page_bytes, true);
+        }
+        char* const b = place(it, to, chunk);
+        store_chunk(r, b, chunk, page_bytes);
     }
 }
 
-constexpr int COPY_CHUNK = MOVE_THREADS * 16 * 4;
-
-// Block: a chunk (x) of pair z's entry in pool y.
+// Block: a chunk (x) of a run of pairs (z) in pool y.
 __global__ void __launch_bounds__(MOVE_THREADS)
     kv_copy_kernel(const Pools pools, size_t bytes, int entries, const int32_t* __restrict__ src,
-                   const int32_t* __restrict__ dst, int n) {
-    const int i = blockIdx.z, s = src[i], d = dst[i];
-    if (s < 0 || s >= entries || d < 0 || d >= entries) return;
-    bool out = false;
-    for (int j = threadIdx.x; j < n; j += MOVE_THREADS) {
-        const int other = dst[j];
-        out |= other == s || (j < i && other == d);
+                   const int32_t* __restrict__ dst, int n, int run) {
+    const int i0 = blockIdx.z * run, i1 = min(n, i0 + run), lane = threadIdx.x & 63;
+    char* const pool = pools.p[blockIdx.y];
+    u32x4 r[QUADS];
+    int held = -1;
+    for (int i = i0; i < i1; i++) {
+        const int s = src[i], d = dst[i];
+        if (s < 0 || s >= entries || d < 0 || d >= entries) continue;
+        bool out = false;  // each wave for itself
+        for (int j = lane; j < n; j += 64) {
+            const int other = dst[j];
+            out |= other == s || (j < i && other == d);
+        }
+        if (__any(out)) continue;
+        if (s != held) load_chunk(r, pool + s * bytes, blockIdx.x, bytes, i + 1 == i1 || src[i + 1] != s);
+        held = s;
+        store_chunk(r, pool + d * bytes, blockIdx.x, bytes);
     }
-    if (__syncthreads_or(out)) return;
-    const char* const a = pools.p[blockIdx.y] + s * bytes;
-    char* const b = pools.p[blockIdx.y] + d * bytes;
-    const size_t end = min(bytes, ((size_t)blockIdx.x + 1) * COPY_CHUNK);
-    for (size_t e = (size_t)blockIdx.x * COPY_CHUNK + threadIdx.x * 16; e < end; e += MOVE_THREADS * 16)
-        *reinterpret_cast<u32x4*>(b + e) = *reinterpret_cast<const u32x4*>(a + e);
 }
 
 // Nondecreasing HOST offsets from 0.
@@ -443,7 +513,8 @@ extern "C" int cs1_kv_reserve(const Cs1PageTable* pages, const int32_t* seqs, co
     cu.n = cu_seqlens ? n : 0;
     if (cu_seqlens)
         for (int i = 0; i <= n; i++) cu.at[i] = cu_seqlens[i];
-    kv_reserve_kernel<<<1, PLAN_THREADS, 0, static_cast<hipStream_t>(stream)>>>(*pages, seqs, cu, n, status);
+    const auto kernel = n <= PLAN_THREADS ? kv_reserve_kernel<1> : kv_reserve_kernel<PER_MAX>;
+    kernel<<<1, PLAN_THREADS, 0, static_cast<hipStream_t>(stream)>>>(*pages, seqs, cu, n, status);
     return hipGetLastError();
 }
 
@@ -460,7 +531,7 @@ extern "C" int cs1_kv_write(const Cs1PageTable* pages, const int32_t* seqs, cons
     if (!all_set({k, v, kp, vp}) || !on16(k) || !on16(v) || !on16(kp) || !on16(vp)) return hipErrorInvalidValue;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     auto launch = [&](const Offsets& cu, int first, int rows) {
-        kv_write_kernel<<<rows, MOVE_THREADS, 0, st>>>(*pages, seqs, cu, first, static_cast<const bf16*>(k), ldk,
+        kv_write_kernel<<<cdiv(rows, ROWS_BLOCK), MOVE_THREADS, 0, st>>>(*pages, seqs, cu, first, rows, static_cast<const bf16*>(k), ldk,
                                                        static_cast<const bf16*>(v), ldv, static_cast<char*>(kp),
                                                        static_cast<char*>(vp), (int)width);
         return hipGetLastError();
@@ -488,20 +559,22 @@ extern "C" int cs1_kv_fork(const Cs1PageTable* pages, const int32_t* src, const 
                            int npools, size_t row_bytes, void* workspace, int32_t* status, void* stream) {
     if (!table_ok(pages) || n < 0 || n > MAX_LISTED || !pools_ok(pools, npools) || !status) return hipErrorInvalidValue;
     if (npools > 0 && (row_bytes == 0 || row_bytes % 16 != 0 || row_bytes > ((size_t)1 << 32))) return hipErrorInvalidValue;
-    const size_t chunks = npools > 0 ? ((pages->page - 1) * row_bytes + FORK_CHUNK - 1) / FORK_CHUNK : 1;
+    const size_t chunks = npools > 0 ? ((pages->page - 1) * row_bytes + CHUNK - 1) / CHUNK : 1;
     if (chunks > CHUNKS_MAX) return hipErrorInvalidValue;
     if (n > 0 && (!all_set({src, dst, workspace}) || !on16(workspace))) return hipErrorInvalidValue;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     Pair* const plan = static_cast<Pair*>(workspace);
-    kv_fork_plan_kernel<<<1, PLAN_THREADS, 0, st>>>(*pages, src, dst, n, plan, status);
+    const auto kernel = n <= PLAN_THREADS ? kv_fork_plan_kernel<1> : kv_fork_plan_kernel<PER_MAX>;
+    kernel<<<1, PLAN_THREADS, 0, st>>>(*pages, src, dst, n, plan, status);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || n == 0) return e;
     int first = 0;
     do {
         Pools some = {};
         const int k = some_pools(pools, npools, first, some), tables = first == 0;
-        kv_fork_kernel<<<dim3((unsigned)chunks, k + tables, n), MOVE_THREADS, 0, st>>>(*pages, src, dst, plan, some,
-                                                                                      row_bytes, tables);
+        const int run = run_of(chunks, k, n);
+        kv_fork_kernel<<<dim3((unsigned)chunks, k + tables, cdiv(n, run)), MOVE_THREADS, 0, st>>>(
+            *pages, src, dst, plan, some, row_bytes, tables, n, run);
         e = hipGetLastError();
         first += k;
     } while (first < npools && e == hipSuccess);
@@ -521,7 +594,9 @@ extern "C" int cs1_kv_compact(const Cs1PageTable* pages, void* const* pools, int
         return hipErrorInvalidValue;
     if (npools > 0 && (row_bytes == 0 || row_bytes % 16 != 0 || row_bytes > ((size_t)1 << 32))) return hipErrorInvalidValue;
     const size_t page_bytes = pages->page * row_bytes;
-    if (npools > 0 && page_bytes / COMPACT_CHUNK > CHUNKS_MAX) return hipErrorInvalidValue;
+    if (npools > 0 && (page_bytes / CHUNK > CHUNKS_MAX ||
+                       (uint64_t)(pages->npages / 2 + 1) * POOLS_MAX * (page_bytes / CHUNK + 1) >= uint64_t{1} << 31))
+        return hipErrorInvalidValue;
     const int cus = device_cus();
     if (cus == 0) return hipErrorInvalidDevice;
     const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -545,15 +620,16 @@ extern "C" int cs1_kv_copy(void* const* pools, int npools, size_t entry_bytes, i
                            const int32_t* dst, int n, void* stream) {
     if (!pools_ok(pools, npools) || n < 0 || n > MAX_LISTED || entries < 0 || entry_bytes % 16 != 0)
         return hipErrorInvalidValue;
-    const size_t chunks = (entry_bytes + COPY_CHUNK - 1) / COPY_CHUNK;
+    const size_t chunks = (entry_bytes + CHUNK - 1) / CHUNK;
     if (chunks > CHUNKS_MAX) return hipErrorInvalidValue;
     if (npools == 0 || n == 0 || entries == 0 || entry_bytes == 0) return hipSuccess;
     if (!all_set({src, dst})) return hipErrorInvalidValue;
     for (int first = 0; first < npools; first += POOLS_MAX) {
         Pools some = {};
         const int k = some_pools(pools, npools, first, some);
-        kv_copy_kernel<<<dim3((unsigned)chunks, k, n), MOVE_THREADS, 0, static_cast<hipStream_t>(stream)>>>(
-            some, entry_bytes, entries, src, dst, n);
+        const int run = run_of(chunks, k, n);
+        kv_copy_kernel<<<dim3((unsigned)chunks, k, cdiv(n, run)), MOVE_THREADS, 0, static_cast<hipStream_t>(stream)>>>(
+            some, entry_bytes, entries, src, dst, n, run);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
