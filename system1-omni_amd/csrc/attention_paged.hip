@@ -37,7 +37,6 @@ namespace {
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int UNIT = 32, ROWS = 16;
-constexpr int FINE = 4, COARSE = 16;  // units of a chunk
 constexpr int ALONE = 8;              // units of a sequence that is one chunk whatever the chunks' size
 constexpr int GROUP = 64, BATCH = 16;  // parts that one block joins, and how many of them are on their way at once
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -56,7 +55,7 @@ struct Args {
     float *lse, *part, *ml;
     int *count, *count2;
     const int32_t *table, *lens, *seqs;
-    int nseq, max_pages, npages, page, B, Hq, Hk, G, tiles, blocks, unit;
+    int nseq, max_pages, npages, page, B, Hq, Hk, G, tiles, blocks, unit, pad;
     uint32_t page_inverse, blocks_inverse;  // 2^32 over page / 16, rounded down, and over blocks, rounded up
     float scale_log2;
 };
@@ -72,9 +71,10 @@ __device__ __forceinline__ Row row_of(const Args& a, int r) {
 
 __device__ __forceinline__ int units_of(int n) { return n / UNIT + (n % UNIT != 0); }
 
-// Chunks of a row's work for one kv head and tile.  A row without keys has one: its zeros are written.
+// Chunks of a row's work for one kv head and tile, of a.unit units each.  A row without keys has one: its zeros are written.
+// The first a.pad chunks stand for the time that a block needs to begin with it, and have no keys.
 __device__ __forceinline__ int chunks_of(const Args& a, int n) {
-    return n <= ALONE * UNIT ? 1 : (units_of(n) + a.unit - 1) / (uint32_t)a.unit;
+    return a.pad + (n <= ALONE * UNIT ? 1 : (units_of(n) + a.unit - 1) / (uint32_t)a.unit);
 }
 
 // Sum over this lane and those below: within rows of 16 lanes, then each row's last lane to the next row (into rows
@@ -125,7 +125,7 @@ struct Rows {
 
 struct Segment {
     int row, s, n, head, tile;  // the n keys of row `row`'s sequence s for kv head `head` and a tile of q heads
-    int from, to, chunks;       // units of it, and how many chunks they are
+    int from, to, next;         // units of it (none: the stretch ends before its keys), and the chunk behind them
     int first, parts, part;     // the first block that has some of it, how many have, and which of them this is
     int slot0;                  // where the first one's results go; the others' go to 2 x their block
 
@@ -150,13 +150,15 @@ __device__ __forceinline__ Segment segment_at(const Args& a, const Rows& first, 
                 s.tile = 0;
                 s.head++;
             }
-        s.from = (pos - whole) * a.unit;
-        s.chunks = min(whole + chunks, end) - pos;
-        s.to = whole + chunks <= end ? units_of(s.n) : s.from + s.chunks * a.unit;
-        s.first = whole >= (int)blockIdx.x * each ? blockIdx.x : whole / (uint32_t)each;
+        s.next = min(whole + chunks, end);
+        const int keys = whole + a.pad, begin = max(pos, keys);
+        if (begin >= end) return true;
+        s.from = (begin - keys) * a.unit;
+        s.to = whole + chunks <= end ? units_of(s.n) : (end - keys) * a.unit;
+        s.first = keys >= (int)blockIdx.x * each ? blockIdx.x : keys / (uint32_t)each;
         s.part = blockIdx.x - s.first;
         s.parts = (whole + chunks <= end ? blockIdx.x : (whole + chunks - 1) / (uint32_t)each) - s.first + 1;
-        s.slot0 = 2 * s.first + (whole > s.first * each);
+        s.slot0 = 2 * s.first + (keys > s.first * each);
         return true;
     };
     if (find(first, 0, 0)) return s;
@@ -234,7 +236,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
     for (int pos = begin; pos < end;) {
     const Segment sh = segment_at(a, first[lane_here()], pos, end, each);
     const int lane = lane_here(), col = lane & 15, grp = lane >> 4;
-    pos += sh.chunks;
+    pos = sh.next;
+    if (sh.parts == 0) break;
     const int rows = min(ROWS, a.G - sh.tile * ROWS), head0 = sh.head * a.G + sh.tile * ROWS;
     const int u_end = sh.to;
     int u = sh.from + wave;
@@ -592,9 +595,9 @@ extern "C" int cs1_attention_paged(void* paged, const void* q, const void* kp, c
     a.G = Hq / Hk;
     a.tiles = (a.G + ROWS - 1) / ROWS;
     a.blocks = p->cus;
-    // Chunks of 128 keys for few sequences, of 512 for many, so that no block has a sequence's last few keys to itself (43
-    // of up to 4096, 16/4 heads of 128: 46.9 us with 128, 41.3 with 512; one of 12000: 14.9 and 15.4)
-    a.unit = (int64_t)B * Hk * a.tiles * 4 < a.blocks ? FINE : COARSE;
+    const bool many = (int64_t)B * Hk * a.tiles * 16 >= a.blocks;
+    a.unit = many ? 2 : 4;
+    a.pad = many ? 4 : 0;
     a.page_inverse = (uint32_t)std::min<uint64_t>(0xffffffffu, (uint64_t{1} << 32) / (a.page / 16));
     a.blocks_inverse = (uint32_t)(((uint64_t{1} << 32) + a.blocks - 1) / a.blocks);
     a.scale_log2 = scale * LOG2E;
