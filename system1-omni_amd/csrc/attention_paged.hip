@@ -111,16 +111,10 @@ __device__ __forceinline__ float over_groups(float x, F f) {
     return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// Rows in the work's order, looked at 64 at a time by each wave for itself: only the device knows the lengths.
+// Rows in the work's order, a wave's 64 at a time: only the device knows the lengths.
 struct Rows {
-    Row row;      // row `lane`
-    int chunks, upto;  // its chunks, and those of the rows up to it
-
-    __device__ __forceinline__ Rows() {}
-    __device__ __forceinline__ Rows(const Args& a, int r0) : row(row_of(a, r0 + (threadIdx.x & 63))) {
-        chunks = r0 + (int)(threadIdx.x & 63) < a.B ? chunks_of(a, row.n) : 0;
-        upto = wave_scan(chunks);
-    }
+    Row row;           // one row,
+    int chunks, upto;  // its chunks, and those of the wave's rows up to it
 };
 
 struct Segment {
@@ -132,43 +126,35 @@ struct Segment {
     __device__ __forceinline__ int slot(int k) const { return k == 0 ? slot0 : 2 * (first + k); }
 };
 
-// The segment that begins at chunk `pos` of this block's stretch, which ends at `end`; stretches are `each` chunks long.
+// Looks for the segment that begins at chunk `pos` of this block's stretch, which ends at `end`, among 64 rows from r0 on,
+// which begin at chunk `before`; stretches are `each` chunks long.
 // (What runs once a launch is kept short: its instructions come from memory, and divisions are long.)
-__device__ __forceinline__ Segment segment_at(const Args& a, const Rows& first, int pos, int end, int each) {
+__device__ __forceinline__ bool segment_at(const Args& a, const Rows& rows, int r0, int before, int pos, int end, int each,
+                                           Segment& s) {
     const int heads = a.Hk * a.tiles;
-    Segment s = {};
-    auto find = [&](const Rows& rows, int r0, int before) {
-        const uint64_t hit = __ballot(pos < before + rows.upto * heads);
-        if (!hit) return false;
-        const int w = __ffsll((unsigned long long)hit) - 1, chunks = scalar(rows.chunks, w);
-        int whole = before + (scalar(rows.upto, w) - chunks) * heads;
-        s.row = r0 + w;
-        s.s = scalar(rows.row.s, w);
-        s.n = scalar(rows.row.n, w);
-        for (; whole + chunks <= pos; whole += chunks)
-            if (++s.tile == a.tiles) {
-                s.tile = 0;
-                s.head++;
-            }
-        s.next = min(whole + chunks, end);
-        const int keys = whole + a.pad, begin = max(pos, keys);
-        if (begin >= end) return true;
-        s.from = (begin - keys) * a.unit;
-        s.to = whole + chunks <= end ? units_of(s.n) : (end - keys) * a.unit;
-        s.first = keys >= (int)blockIdx.x * each ? blockIdx.x : keys / (uint32_t)each;
-        s.part = blockIdx.x - s.first;
-        s.parts = (whole + chunks <= end ? blockIdx.x : (whole + chunks - 1) / (uint32_t)each) - s.first + 1;
-        s.slot0 = 2 * s.first + (keys > s.first * each);
-        return true;
-    };
-    if (find(first, 0, 0)) return s;
-    int before = scalar(first.upto, 63) * heads;
-    for (int r0 = 64; r0 < a.B; r0 += 64) {
-        const Rows rows(a, r0);
-        if (find(rows, r0, before)) break;
-        before += scalar(rows.upto, 63) * heads;
-    }
-    return s;
+    const uint64_t hit = __ballot(pos < before + rows.upto * heads);
+    if (!hit) return false;
+    const int w = __ffsll((unsigned long long)hit) - 1, chunks = scalar(rows.chunks, w);
+    int whole = before + (scalar(rows.upto, w) - chunks) * heads;
+    s = {};
+    s.row = r0 + w;
+    s.s = scalar(rows.row.s, w);
+    s.n = scalar(rows.row.n, w);
+    for (; whole + chunks <= pos; whole += chunks)
+        if (++s.tile == a.tiles) {
+            s.tile = 0;
+            s.head++;
+        }
+    s.next = min(whole + chunks, end);
+    const int keys = whole + a.pad, begin = max(pos, keys);
+    if (begin >= end) return true;
+    s.from = (begin - keys) * a.unit;
+    s.to = whole + chunks <= end ? units_of(s.n) : (end - keys) * a.unit;
+    s.first = keys >= (int)blockIdx.x * each ? blockIdx.x : keys / (uint32_t)each;
+    s.part = blockIdx.x - s.first;
+    s.parts = (whole + chunks <= end ? blockIdx.x : (whole + chunks - 1) / (uint32_t)each) - s.first + 1;
+    s.slot0 = 2 * s.first + (keys > s.first * each);
+    return true;
 }
 
 // Four dims of an output from sums o over l (zero: no key); g: their gates, if there are any.
@@ -221,20 +207,35 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
     extern __shared__ __attribute__((aligned(16))) float lds[];  // Q as operands, [C][64 lanes] x 16 bytes; later [WAVES][rows][PITCH]
     __shared__ float wm[WAVES][ROWS], wl[WAVES][ROWS];
     const int wave = scalar(threadIdx.x >> 6, 0);
-    __shared__ Rows first[64];  // (the loop over the keys has no registers for it)
-    int total;
-    {
-        const Rows rows(a, 0);
-        if (threadIdx.x < 64) first[threadIdx.x] = rows;
-        total = scalar(rows.upto, 63);
-    }
-    for (int r0 = 64; r0 < a.B; r0 += 64) total += scalar(Rows(a, r0).upto, 63);
-    total *= a.Hk * a.tiles;
+    // THREADS rows at a time, a thread each, in LDS; of more than that, those last looked at
+    __shared__ Rows table[THREADS];
+    __shared__ int sums[WAVES];
+    auto look_at = [&](int r0) {
+        const int i = wave * 64 + lane_here(), r = r0 + i;
+        Rows x;
+        x.row = row_of(a, r);
+        x.chunks = r < a.B ? chunks_of(a, x.row.n) : 0;
+        x.upto = wave_scan(x.chunks);
+        __syncthreads();
+        table[i] = x;
+        if ((i & 63) == 63) sums[wave] = x.upto;
+        __syncthreads();
+        return sums[0] + sums[1] + sums[2] + sums[3];
+    };
+    const int heads = a.Hk * a.tiles;
+    int total = look_at(0);
+    for (int r0 = THREADS; r0 < a.B; r0 += THREADS) total += look_at(r0);
+    total = __builtin_amdgcn_readfirstlane(total * heads);
     const int each = __umulhi(total - 1, a.blocks_inverse) + 1;  // (one more than need be where the inverse's rounding shows)
     const int begin = (int)blockIdx.x * each, end = min(total, begin + each);
-    __syncthreads();
     for (int pos = begin; pos < end;) {
-    const Segment sh = segment_at(a, first[lane_here()], pos, end, each);
+    Segment sh = {};
+    for (int r0 = 0, before = 0; r0 < a.B; r0 += 64) {
+        const int w = r0 / 64 % WAVES;
+        if (w == 0 && a.B > THREADS) (void)look_at(r0);
+        if (segment_at(a, table[w * 64 + lane_here()], r0, before, pos, end, each, sh)) break;
+        before += __builtin_amdgcn_readfirstlane(sums[w]) * heads;
+    }
     const int lane = lane_here(), col = lane & 15, grp = lane >> 4;
     pos = sh.next;
     if (sh.parts == 0) break;
