@@ -1,5 +1,7 @@
 """cs1_attention_paged against attention in float64 (decode_ref.attention), within bounds that follow from
 the roundings of float32 sums and one bfloat16 output."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -243,6 +245,52 @@ def test_many_rows(handle):
     c.check()
 
 
+@pytest.mark.parametrize("lens,hq,hk,dh,page", [
+    ([3] * 299 + [7000], 4, 2, 128, 16),                                   # more rows than a block looks at together, one split
+    ([900, 0, 31] * 86, 4, 1, 256, 64),                                     # 258 of them, several a block
+    ([9000] + [1] * 256 + [5000, 0, 4097], 2, 2, 128, 48),
+    ([40] * 513, 16, 16, 128, 16),                                          # thousands of kv heads, several a block
+    ([2048, 2048], 48, 1, 256, 256),                                        # three tiles of a kv head
+    ([5000, 4096, 4095, 4097], 16, 4, 256, 4096),                           # a page larger than a sequence
+    ([70000], 2, 1, 128, 1024), ([1], 16, 4, 128, 65536),
+], ids=lambda v: f"{len(v)}x{max(v)}" if isinstance(v, list) else str(v))
+def test_many_rows_and_large_pages(handle, lens, hq, hk, dh, page):
+    say(f"paged attention {len(lens)} sequences up to {max(lens)}, heads {hq}/{hk} Dh={dh} page={page}")
+    rng = np.random.default_rng(len(lens))
+    t = R.scattered(rng, len(lens), lens, page, spare=1)
+    c = Call(handle, rng, t, rng.permutation(len(lens)), hq, hk, dh)
+    c.upload()
+    c.launch()
+    c.check()
+
+
+def test_offsets_past_32_bits(handle):
+    """Keys and values behind 4 GiB of a pool."""
+    say("paged attention: pools of 5 GiB")
+    page, hk, dh, hq = 64, 8, 128, 16
+    rng = np.random.default_rng(14)
+    npages = (5 << 30) // (page * hk * dh * 2)
+    t = R.Table(2, 3, npages, page)
+    t.table[0], t.table[1, 0], t.lens[:] = [npages - 1, 3, npages - 2], npages - 5, [150, 9]
+    small = R.Table(2, 3, 6, page)  # the same pages, numbered from 0
+    order = [npages - 1, 3, npages - 2, npages - 5]
+    small.table[0], small.table[1, 0], small.lens[:] = [0, 1, 2], 3, [150, 9]
+    c = Call(handle, rng, small, [1, 0], hq, hk, dh)
+    want, wl, tol, ltol = R.attention(small, c.seqs, c.q, c.kp, c.vp, c.gate, hk, dh ** -0.5)
+    c.upload()
+    c.t, c.d = t, DeviceTable(t)
+    size = page * hk * dh * 2
+    pools = [empty(npages * size), empty(npages * size)]
+    for pool, arr in zip(pools, (c.kp, c.vp)):
+        for i, p in enumerate(order):
+            hip.upload(pool, arr[i], stream(), offset=p * size)
+    c.bufs[1:3] = pools
+    c.launch()
+    out, l = c.results()
+    R.close(R.f64(out), want, tol, "out")
+    R.close(l.astype(np.float64), wl, ltol, "lse")
+
+
 def test_refusals_with_a_handle(handle):
     say("paged attention: refusals")
     rng = np.random.default_rng(13)
@@ -261,5 +309,11 @@ def test_refusals_with_a_handle(handle):
     assert call(q=q + 8) == call(kp=kp + 2) == call(vp=vp + 4) == call(out=out + 8) == call(gate=q + 2) == hip.HIP_ERROR_INVALID_VALUE
     assert call(B=1 << 23) == hip.HIP_ERROR_INVALID_VALUE
     assert call(B=0, q=None) == 0
+    big = hip.PageTable(c.d.table.at(0), c.d.lens.at(0), c.d.refs.at(0), 1, 1, 1 << 27, 16)  # 2^31 tokens in the pool
+    c.d.ref = ctypes.byref(big)
+    assert call() == hip.HIP_ERROR_INVALID_VALUE
+    long = hip.PageTable(c.d.table.at(0), c.d.lens.at(0), c.d.refs.at(0), 1, 1 << 26, 4, 16)  # 2^25 units a row
+    c.d.ref = ctypes.byref(long)
+    assert call(B=64) == hip.HIP_ERROR_INVALID_VALUE
     (out_before, _) = c.results()
     assert (out_before == 0x7fc1).all()
