@@ -55,7 +55,7 @@ struct Args {
     float *lse, *part, *ml;
     int *count, *count2;
     const int32_t *table, *lens, *seqs;
-    int nseq, max_pages, npages, page, B, Hq, Hk, G, tiles, blocks, unit, pad;
+    int nseq, max_pages, npages, page, B, Hq, Hk, G, tiles, blocks, halve, unit, pad;
     uint32_t page_inverse, blocks_inverse;  // 2^32 over page / 16, rounded down, and over blocks, rounded up
     float scale_log2;
 };
@@ -226,7 +226,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
     int total = look_at(0);
     for (int r0 = THREADS; r0 < a.B; r0 += THREADS) total += look_at(r0);
     total = __builtin_amdgcn_readfirstlane(total * heads);
-    const int each = __umulhi(total - 1, a.blocks_inverse) + 1;  // (one more than need be where the inverse's rounding shows)
+    // With heads of 128 two blocks fit on a CU (and are launched for many sequences): where these are short, on average under
+    // 256 keys, a block's time is that of beginning and ending each, and two at once hide it.  300 sequences of up to 40 keys
+    // take 23.4 us so and 32.1 with one, 128 of up to 1000 52.6 and 45.5 (16/4 heads).
+    const uint32_t inverse = a.halve && total >= 8 * a.B * heads ? 2 * a.blocks_inverse : a.blocks_inverse;
+    const int each = __umulhi(total - 1, inverse) + 1;  // (one more than need be where the inverse's rounding shows)
     const int begin = (int)blockIdx.x * each, end = min(total, begin + each);
     for (int pos = begin; pos < end;) {
     Segment sh = {};
@@ -536,8 +540,8 @@ extern "C" void* cs1_attention_paged_create(void) {
     Paged* const p = new (std::nothrow) Paged;
     if (!p) return nullptr;
     p->device = device;
-    p->cus = std::min(cus, GROUP * GROUP / 3);
-    p->blocks = p->cus;
+    p->cus = std::min(cus, GROUP * GROUP / 2);
+    p->blocks = 2 * p->cus;
     const size_t floats = (size_t)2 * p->blocks * ROWS * (256 + 2), counts = (size_t)4 * p->blocks;
     p->part = nullptr;
     if (hipMalloc(reinterpret_cast<void**>(&p->part), 4 * (floats + counts)) != hipSuccess ||
@@ -595,7 +599,8 @@ extern "C" int cs1_attention_paged(void* paged, const void* q, const void* kp, c
     a.Hk = Hk;
     a.G = Hq / Hk;
     a.tiles = (a.G + ROWS - 1) / ROWS;
-    a.blocks = p->cus;
+    a.halve = Dh == 128 && (int64_t)B * Hk * a.tiles >= p->blocks;  // the blocks, if the sequences are long
+    a.blocks = a.halve ? p->blocks : p->cus;
     const bool many = (int64_t)B * Hk * a.tiles * 16 >= a.blocks;
     a.unit = many ? 2 : 4;
     a.pad = many ? 4 : 0;
