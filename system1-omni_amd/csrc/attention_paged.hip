@@ -6,25 +6,26 @@
 //
 // The keys and values are read once and nothing else is of size, so the rate of that stream is the bound.
 //
-// Work: the q heads of a kv head are the rows of one matrix tile, up to 16 of them (more take several tiles, which read
-// the keys again).  The keys of all rows, kv heads and tiles, in chunks of 128, are one line of work that is cut into equal
-// stretches, one for each block that the chip holds at once: whatever the lengths, every block streams the same amount and all end
-// together.  A stretch may begin and end inside a sequence; what it has of one (a segment) is joined with the other
-// blocks' parts by the last of them to end.  Within a block four waves take every fourth unit of 32 keys, each with a
-// running maximum and sum of its own, and join through LDS.
+// Work: the q heads of a kv head are the rows of one matrix tile, up to 16 of them (more take several tiles, which
+// read the keys again).  The keys of all rows, kv heads and tiles, in chunks of 64 or 128, are one line of work that
+// is cut into equal stretches, one for each CU: whatever the lengths, every block streams the same amount and all end
+// about together (9 sequences of 9000 to 32768 keys, 24/4 heads of 256: 176 us, 5.5 TB/s; with a block for each share
+// of a sequence, two and four to a CU, 185 and 203 us).  A stretch may begin and end inside a sequence; what it has
+// of one (a segment) is joined with the other blocks' parts by the last of them to end.  Within a block four waves
+// take every fourth unit of 32 keys, each with a running maximum and sum of its own, and join through LDS.
 //
-// A unit in registers, without LDS: S^T = K Q^T takes K rows as they lie (lane l: key l % 16, 8 dims a load) and leaves
-// lane l with q head l % 16 and keys 4 (l / 16) .. + 3 of each 16; that is the layout in which O^T = V^T P^T wants P^T,
-// with the unit's keys in the order (i < 4: 4 g + i, else 16 + 4 g + i - 4) for lane group g.  V rows are loaded 16
-// lanes x 16 bytes at a time (256 bytes in a row), lane l holding dims 8 (l % 16) .. + 7 of its group's eight
-// keys, and two-byte permutes make columns of eight keys of them: the tile's row m is dim 8 m + j.  Each q head stays
-// in its lanes from the scores to the output, so maximum and sum need no exchange but between lane groups,
-// and that only when the maximum rises by more than RISE or at the end.  The next unit's K is on its way while this one's
+// A unit in registers, without LDS: S^T = K Q^T takes K rows as they lie (lane l: key l % 16, 8 dims a load) and
+// leaves lane l with q head l % 16 and keys 4 (l / 16) .. + 3 of each 16; that is the layout in which O^T = V^T P^T
+// wants P^T, with the unit's keys in the order (i < 4: 4 g + i, else 16 + 4 g + i - 4) for lane group g.  V rows are
+// loaded 16 lanes x 16 bytes at a time (256 bytes in a row), lane l holding dims 8 (l % 16) .. + 7 of its group's
+// eight keys, and two-byte permutes make columns of eight keys of them: the tile's row m is dim 8 m + j.  Each q head
+// stays in its lanes from the scores to the output, so maximum and sum need no exchange but between lane groups, and
+// that only when the maximum rises by more than RISE or at the end.  The next unit's K is on its way while this one's
 // probabilities are formed, its V while the next scores are.
 //
-// P goes to the product in two bfloat16 parts (hi cut off, lo the rounded rest: p to 2^-15): the matrix cores wait for
-// memory here, and the second product leaves the rounding of out the only one that counts.  lo is never zero (LEAST), so
-// that an infinite v gives the infinity that it should and not inf + 0 inf.
+// P goes to the product in two bfloat16 parts (hi cut off, lo the rounded rest: p to 2^-15): the matrix cores wait
+// for memory here, and the second product leaves the rounding of out the only one that counts.  lo is never zero
+// (LEAST), so that an infinite v gives the infinity that it should and not inf + 0 inf.
 #include <algorithm>
 #include <new>
 #include <type_traits>
@@ -36,6 +37,7 @@ namespace q35 {
 namespace {
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
+static_assert(WAVES == 4, "the waves' maxima and the rows' sums are joined by name");
 constexpr int UNIT = 32, ROWS = 16;
 constexpr int ALONE = 8;              // units of a sequence that is one chunk whatever the chunks' size
 constexpr int GROUP = 64, BATCH = 16;  // parts that one block joins, and how many of them are on their way at once
@@ -71,8 +73,8 @@ __device__ __forceinline__ Row row_of(const Args& a, int r) {
 
 __device__ __forceinline__ int units_of(int n) { return n / UNIT + (n % UNIT != 0); }
 
-// Chunks of a row's work for one kv head and tile, of a.unit units each.  A row without keys has one: its zeros are written.
-// The first a.pad chunks stand for the time that a block needs to begin with it, and have no keys.
+// Chunks of a row's work for one kv head and tile, of a.unit units each.  A row without keys has one: its zeros are
+// written. The first a.pad chunks stand for the time that a block needs to begin with it, and have no keys.
 __device__ __forceinline__ int chunks_of(const Args& a, int n) {
     return a.pad + (n <= ALONE * UNIT ? 1 : (units_of(n) + a.unit - 1) / (uint32_t)a.unit);
 }
@@ -102,7 +104,8 @@ __device__ __forceinline__ int lane_here() {
     return lane;
 }
 
-// One value from the four of a lane's column (lanes 16 apart), in each of them: rows of 16 lanes are swapped, then halves.
+// One value from the four of a lane's column (lanes 16 apart), in each of them: rows of 16 lanes are swapped, then
+// halves.
 template <typename F>
 __device__ __forceinline__ float over_groups(float x, F f) {
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -126,11 +129,11 @@ struct Segment {
     __device__ __forceinline__ int slot(int k) const { return k == 0 ? slot0 : 2 * (first + k); }
 };
 
-// Looks for the segment that begins at chunk `pos` of this block's stretch, which ends at `end`, among 64 rows from r0 on,
-// which begin at chunk `before`; stretches are `each` chunks long.
-// (What runs once a launch is kept short: its instructions come from memory, and divisions are long.)
-__device__ __forceinline__ bool segment_at(const Args& a, const Rows& rows, int r0, int before, int pos, int end, int each,
-                                           Segment& s) {
+// Looks for the segment that begins at chunk `pos` of this block's stretch, which ends at `end`, among 64 rows from
+// r0 on, which begin at chunk `before`; stretches are `each` chunks long. (What runs once a launch is kept short: its
+// instructions come from memory, and divisions are long.)
+__device__ __forceinline__ bool segment_at(const Args& a, const Rows& rows, int r0, int before, int pos, int end,
+                                           int each, Segment& s) {
     const int heads = a.Hk * a.tiles;
     const uint64_t hit = __ballot(pos < before + rows.upto * heads);
     if (!hit) return false;
@@ -204,7 +207,8 @@ struct Shared {
 template <int DH>
 __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args a) {
     constexpr int C = DH / 32, H = DH / 128, PITCH = DH + 8;
-    extern __shared__ __attribute__((aligned(16))) float lds[];  // Q as operands, [C][64 lanes] x 16 bytes; later [WAVES][rows][PITCH]
+    // Q as operands, [C][64 lanes] x 16 bytes; then the waves' results, [WAVES][rows][PITCH]; then what joins parts
+    extern __shared__ __attribute__((aligned(16))) float lds[];
     __shared__ float wm[WAVES][ROWS], wl[WAVES][ROWS];
     const int wave = scalar(threadIdx.x >> 6, 0);
     // THREADS rows at a time, a thread each, in LDS; of more than that, those last looked at
@@ -226,283 +230,294 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
     int total = look_at(0);
     for (int r0 = THREADS; r0 < a.B; r0 += THREADS) total += look_at(r0);
     total = __builtin_amdgcn_readfirstlane(total * heads);
-    // With heads of 128 two blocks fit on a CU (and are launched for many sequences): where these are short, on average under
-    // 256 keys, a block's time is that of beginning and ending each, and two at once hide it.  300 sequences of up to 40 keys
-    // take 23.4 us so and 32.1 with one, 128 of up to 1000 52.6 and 45.5 (16/4 heads).
+    // With heads of 128 two blocks fit on a CU (and are launched for many sequences): where these are short, on
+    // average under 256 keys, a block's time is that of beginning and ending each, and two at once hide it.  300
+    // sequences of up to 40 keys take 23.4 us so and 32.1 with one, 128 of up to 1000 52.6 and 45.5 (16/4 heads).
     const uint32_t inverse = a.halve && total >= 8 * a.B * heads ? 2 * a.blocks_inverse : a.blocks_inverse;
     const int each = __umulhi(total - 1, inverse) + 1;  // (one more than need be where the inverse's rounding shows)
     const int begin = (int)blockIdx.x * each, end = min(total, begin + each);
     for (int pos = begin; pos < end;) {
-    Segment sh = {};
-    for (int r0 = 0, before = 0; r0 < a.B; r0 += 64) {
-        const int w = r0 / 64 % WAVES;
-        if (w == 0 && a.B > THREADS) (void)look_at(r0);
-        if (segment_at(a, table[w * 64 + lane_here()], r0, before, pos, end, each, sh)) break;
-        before += __builtin_amdgcn_readfirstlane(sums[w]) * heads;
-    }
-    const int lane = lane_here(), col = lane & 15, grp = lane >> 4;
-    pos = sh.next;
-    if (sh.parts == 0) break;
-    const int rows = min(ROWS, a.G - sh.tile * ROWS), head0 = sh.head * a.G + sh.tile * ROWS;
-    const int u_end = sh.to;
-    int u = sh.from + wave;
+        Segment sh = {};
+        for (int r0 = 0, before = 0; r0 < a.B; r0 += 64) {
+            const int w = r0 / 64 % WAVES;
+            if (w == 0 && a.B > THREADS) (void)look_at(r0);
+            if (segment_at(a, table[w * 64 + lane_here()], r0, before, pos, end, each, sh)) break;
+            before += __builtin_amdgcn_readfirstlane(sums[w]) * heads;
+        }
+        const int lane = lane_here(), col = lane & 15, grp = lane >> 4;
+        pos = sh.next;
+        if (sh.parts == 0) break;
+        const int rows = min(ROWS, a.G - sh.tile * ROWS), head0 = sh.head * a.G + sh.tile * ROWS;
+        const size_t out0 = ((size_t)sh.row * a.Hq + head0) * DH;  // of q, gate and out
+        const int u_end = sh.to;
+        int u = sh.from + wave;
 
-    __syncthreads();  // the segment before is done with LDS
-    u32x4* const qf = reinterpret_cast<u32x4*>(lds);
-    for (int c = wave; c < C; c += WAVES) {
-        u32x4 q = {0, 0, 0, 0};
-        if (col < rows) q = *reinterpret_cast<const u32x4*>(a.q + ((size_t)sh.row * a.Hq + head0 + col) * DH + c * 32 + grp * 8);
-        qf[c * 64 + lane] = q;
-    }
-    f32x4 acc[H][8];
-#pragma unroll
-    for (int h = 0; h < H; h++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) acc[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-
-    // where the next units' halves lie: lane i has half i % 2 of unit i / 2 from here, the pool's row / 16 and 5 bits of valid keys
-    const size_t token = (size_t)a.Hk * DH;
-    uint32_t where = 0;
-    int next = 64;
-    auto look_up = [&](int from) {
-        const int i = lane_here();
-        const uint32_t half = 2 * (from + (i >> 1) * WAVES) + (i & 1), page = (uint32_t)a.page / 16;
-        uint32_t slot = __umulhi(half, a.page_inverse);
-        slot += (slot + 1) * page <= half;
-        where = 0;
-        if (16 * half < (uint32_t)sh.n) {
-            const int pg = a.table[(size_t)sh.s * a.max_pages + slot];
-            if (pg >= 0 && pg < a.npages) where = (pg * page + half - slot * page) << 5 | min(16, (int)(sh.n - 16 * half));
+        __syncthreads();  // the segment before is done with LDS
+        u32x4* const qf = reinterpret_cast<u32x4*>(lds);
+        for (int c = wave; c < C; c += WAVES) {
+            u32x4 q = {0, 0, 0, 0};
+            if (col < rows) q = *reinterpret_cast<const u32x4*>(a.q + out0 + col * DH + c * 32 + grp * 8);
+            qf[c * 64 + lane] = q;
         }
-    };
-    // The next unit is on its way while one is worked on.  A half's rows are read through a buffer descriptor that ends with
-    // the last valid one: rows behind it, and whole units behind the wave's last, come as zeros and cost no access.
-    u32x4 kf[2][C], vf[H][8];
-    size_t at[2];
-    int have[2];
-    const uint32_t row_b = 2 * (uint32_t)token, k_lane = col * row_b + grp * 16, v_lane = grp * 4 * row_b + col * 16;
-    auto half_rows = [&](const bf16* pool, size_t from, int rows) {
-        const uint64_t p = reinterpret_cast<uint64_t>(pool + from);
-        const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p), hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
-        return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((uint64_t)hi << 32 | lo), (short)0,
-                                                 __builtin_amdgcn_readfirstlane(rows > 0 ? (rows - 1) * row_b + 2 * DH : 0),
-                                                 0x00020000);
-    };
-    auto load_k = [&](int from) {
-        if (next == 64) {
-            look_up(from);
-            next = 0;
-        }
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const uint32_t w = from < u_end ? __builtin_amdgcn_readlane(where, next + t) : 0;
-            at[t] = (size_t)(w >> 5) * (16 * token) + sh.head * DH;
-            have[t] = w & 31;
-            const auto r = half_rows(a.kp, at[t], have[t]);
-#pragma unroll
-            for (int c = 0; c < C; c++)
-                kf[t][c] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, k_lane + c * 64, 0, 0));
-        }
-        next += 2;
-    };
-    auto load_v = [&]() {
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const auto r = half_rows(a.vp, at[t], have[t]);
-#pragma unroll
-            for (int h = 0; h < H; h++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    vf[h][t * 4 + i] = __builtin_bit_cast(
-                        u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, v_lane + h * 256, i * row_b, 0));
-        }
-    };
-    if (u < u_end) {
-        load_k(u);
-        load_v();
-    }
-    __syncthreads();
-    for (; u < u_end; u += WAVES) {
-        const int valid[2] = {have[0], have[1]};
-        f32x4 st[2][2] = {};  // two sums a half: a product does not wait for the one before
-#pragma unroll
-        for (int c = 0; c < C; c++) {
-            const u32x4 q = qf[c * 64 + lane];
-#pragma unroll
-            for (int t = 0; t < 2; t++) st[t][c & 1] = mfma16(kf[t][c], q, st[t][c & 1]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        load_k(u + WAVES);
-        __builtin_amdgcn_sched_barrier(0);
-        float sc[8], top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; i++) sc[i] = (st[i >> 2][0][i & 3] + st[i >> 2][1][i & 3]) * a.scale_log2;
-        if (valid[0] + valid[1] < UNIT)
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (grp * 4 + (i & 3) >= valid[i >> 2]) sc[i] = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; i++) top = fmaxf(top, sc[i]);
-        if (__any(top > m + RISE)) {
-            top = fmaxf(m, over_groups(top, [](float x, float y) { return fmaxf(x, y); }));
-            const float keep = top == m ? 1.f : __builtin_amdgcn_exp2f(m - top);
-            m = top;
-            l *= keep;
-#pragma unroll
-            for (int h = 0; h < H; h++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) acc[h][j] *= keep;
-        }
-        const float base = m == -INFINITY ? 0.f : m;  // no key yet: exp2(-inf) = 0
-        u32x4 ph, pl;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float p0 = __builtin_amdgcn_exp2f(sc[2 * i] - base), p1 = __builtin_amdgcn_exp2f(sc[2 * i + 1] - base);
-            l += p0 + p1;
-            ph[i] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302);
-            pl[i] = pack2(fmaxf(p0 - lo_f32(ph[i]), LEAST), fmaxf(p1 - hi_f32(ph[i]), LEAST));
-        }
-#pragma unroll
-        for (int h = 0; h < H; h++) {
-            u32x4 vt[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    vt[j][i] = __builtin_amdgcn_perm(vf[h][2 * i + 1][j >> 1], vf[h][2 * i][j >> 1],
-                                                     j & 1 ? 0x07060302 : 0x05040100);
-#pragma unroll
-            for (int j = 0; j < 8; j++) acc[h][j] = mfma16(vt[j], ph, acc[h][j]);
-#pragma unroll
-            for (int j = 0; j < 8; j++) acc[h][j] = mfma16(vt[j], pl, acc[h][j]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        load_v();
-        __builtin_amdgcn_sched_barrier(0);
-    }
-
-    // the waves join
-    const int tid = wave * 64 + lane_here();
-    l = over_groups(l, [](float x, float y) { return x + y; });
-    const int row_c = tid & 15, row_g = tid >> 4 & 3;
-    if (row_g == 0) {
-        wm[wave][row_c] = m;
-        wl[wave][row_c] = l;
-    }
-    __syncthreads();  // Q is no longer read
-    if (row_c < rows)
+        f32x4 acc[H][8];
 #pragma unroll
         for (int h = 0; h < H; h++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                float* const to = lds + (wave * rows + row_c) * PITCH + h * 128 + (row_g * 4 + r) * 8;
-                *reinterpret_cast<f32x4*>(to) = f32x4{acc[h][0][r], acc[h][1][r], acc[h][2][r], acc[h][3][r]};
-                *reinterpret_cast<f32x4*>(to + 4) = f32x4{acc[h][4][r], acc[h][5][r], acc[h][6][r], acc[h][7][r]};
+            for (int j = 0; j < 8; j++) acc[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+
+        // where the next units' halves lie: lane i has half i % 2 of unit i / 2 from here, the pool's row / 16 and 5
+        // bits of valid keys
+        const size_t token = (size_t)a.Hk * DH;
+        uint32_t where = 0;
+        int next = 64;
+        auto look_up = [&](int from) {
+            const int i = lane_here();
+            const uint32_t half = 2 * (from + (i >> 1) * WAVES) + (i & 1), page = (uint32_t)a.page / 16;
+            uint32_t slot = __umulhi(half, a.page_inverse);
+            slot += (slot + 1) * page <= half;
+            where = 0;
+            if (16 * half < (uint32_t)sh.n) {
+                const int pg = a.table[(size_t)sh.s * a.max_pages + slot];
+                if (pg >= 0 && pg < a.npages)
+                    where = (pg * page + half - slot * page) << 5 | min(16, (int)(sh.n - 16 * half));
             }
-    __syncthreads();
-    const Shared shared(a);
-    constexpr int QUADS = DH / 4;  // of a row's dims
-    const size_t out0 = ((size_t)sh.row * a.Hq + head0) * DH;
-    // four dims of a row's result: to the output, or to a slot
-    auto store = [&](int slot, int e, float top, float sum, const f32x4& o, const u32x2& g, bool out) {
-        const int row = e / QUADS, d = e % QUADS * 4;
-        if (out) {
-            store_out(a, out0 + row * DH + d, o, sum, g);
-            if (a.lse && d == 0) a.lse[(size_t)(head0 + row) * a.B + sh.row] = log_sum(top, sum);
-            return;
-        }
-        const int at = slot * ROWS + row;
-        shared.put((at * DH + d) * 4, o);
-        if (d == 0) shared.put_ml(at * 8, f32x2{top, sum});
-    };
-    // Groups of `group` parts: the last of a group to end joins it, the last group joins the groups; always in order, so the
-    // result does not depend on which ends last.  The counters are zero again afterwards.
-    int group = 1, groups = 1, g0 = 0, members = 1;
-    if (sh.parts > 1) {
-        groups = (sh.parts + GROUP - 1) / GROUP;
-        group = (sh.parts + groups - 1) / (uint32_t)groups;
-        groups = (sh.parts + group - 1) / (uint32_t)group;
-        g0 = sh.part / (uint32_t)group * group;
-        members = min(group, sh.parts - g0);
-    }
-    auto last_of = [&](int* count, int n) {
-        __shared__ int last;
-        wait_vm_all();  // what this wave has put is where the others look
-        __syncthreads();
-        if (tid == 0) {
-            last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
-            if (last) *count = 0;
-        }
-        __syncthreads();
-        return last != 0;
-    };
-    // Stage 0: this block's waves.  1: a group's parts, 2: the groups.  A row's four dims are summed by as many threads as there
-    // are for them.  The time of 1 and 2 is that of getting at the parts, so many are asked for at once: a thread has every
-    // `ways`-th, BATCH of them on their way together, the first while a wave per row finds the parts' weights.
-    float* const weight = lds;               // [GROUP, ROWS]
-    float* const other = lds + GROUP * ROWS;  // [THREADS, 4]
-    const int items = rows * QUADS, rows_log = rows > 1 ? 32 - __builtin_clz(rows - 1) : 0;
-    for (int stage = 0;; stage++) {
-        const bool out = stage == 0 ? sh.parts == 1 : stage == 2 || groups == 1;
-        const int k0 = stage == 1 ? g0 : 0, step = stage == 2 ? group : 1, n = stage == 1 ? members : groups;
-        const int ways = stage == 0 ? 1 : max(1, THREADS / QUADS >> rows_log);
-        for (int e0 = 0; e0 < items; e0 += THREADS) {
-            const int way = ways > 1 ? tid / QUADS >> rows_log : 0;
-            const int e = e0 + (ways > 1 ? tid & ((QUADS << rows_log) - 1) : tid);
-            const bool works = e < items;
-            const int row = works ? e / QUADS : 0, d = e % QUADS * 4;
-            u32x2 g = {0, 0};
-            f32x4 o = {0.f, 0.f, 0.f, 0.f};
-            float top, sum = 0.f;
-            if (out) g = load_gate(a, out0 + row * DH + d);
-            if (stage == 0) {
-                top = fmaxf(fmaxf(wm[0][row], wm[1][row]), fmaxf(wm[2][row], wm[3][row]));
+        };
+        // The next unit is on its way while one is worked on.  A half's rows are read through a buffer descriptor
+        // that ends with the last valid one: rows behind it, and whole units behind the wave's last, come as zeros
+        // and cost no access.
+        u32x4 kf[2][C], vf[H][8];
+        size_t at[2];
+        int have[2];
+        const uint32_t row_b = 2 * (uint32_t)token;  // bytes of a token's row
+        const uint32_t k_lane = col * row_b + grp * 16, v_lane = grp * 4 * row_b + col * 16;
+        auto half_rows = [&](const bf16* pool, size_t from, int rows) {
+            const uint64_t p = reinterpret_cast<uint64_t>(pool + from);
+            const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p);
+            const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
+            const int bytes = __builtin_amdgcn_readfirstlane(rows > 0 ? (rows - 1) * row_b + 2 * DH : 0);
+            return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((uint64_t)hi << 32 | lo), (short)0, bytes,
+                                                     0x00020000);
+        };
+        auto load_k = [&](int from) {
+            if (next == 64) {
+                look_up(from);
+                next = 0;
+            }
 #pragma unroll
-                for (int w = 0; w < WAVES; w++) {
-                    const float f = wm[w][row] == top ? 1.f : __builtin_amdgcn_exp2f(wm[w][row] - top);
-                    sum += wl[w][row] * f;
-                    o += *reinterpret_cast<const f32x4*>(lds + (w * rows + row) * PITCH + d) * f;
+            for (int t = 0; t < 2; t++) {
+                const uint32_t w = from < u_end ? __builtin_amdgcn_readlane(where, next + t) : 0;
+                at[t] = (size_t)(w >> 5) * (16 * token) + sh.head * DH;
+                have[t] = w & 31;
+                const auto r = half_rows(a.kp, at[t], have[t]);
+#pragma unroll
+                for (int c = 0; c < C; c++)
+                    kf[t][c] =
+                        __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, k_lane + c * 64, 0, 0));
+            }
+            next += 2;
+        };
+        auto load_v = [&]() {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const auto r = half_rows(a.vp, at[t], have[t]);
+#pragma unroll
+                for (int h = 0; h < H; h++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        vf[h][t * 4 + i] = __builtin_bit_cast(
+                            u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, v_lane + h * 256, i * row_b, 0));
+            }
+        };
+        if (u < u_end) {
+            load_k(u);
+            load_v();
+        }
+        __syncthreads();
+        for (; u < u_end; u += WAVES) {
+            const int valid[2] = {have[0], have[1]};
+            f32x4 st[2][2] = {};  // two sums a half: a product does not wait for the one before
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                const u32x4 q = qf[c * 64 + lane];
+#pragma unroll
+                for (int t = 0; t < 2; t++) st[t][c & 1] = mfma16(kf[t][c], q, st[t][c & 1]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load_k(u + WAVES);
+            __builtin_amdgcn_sched_barrier(0);
+            float sc[8], top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; i++) sc[i] = (st[i >> 2][0][i & 3] + st[i >> 2][1][i & 3]) * a.scale_log2;
+            if (valid[0] + valid[1] < UNIT)
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (grp * 4 + (i & 3) >= valid[i >> 2]) sc[i] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fmaxf(top, sc[i]);
+            if (__any(top > m + RISE)) {
+                top = fmaxf(m, over_groups(top, [](float x, float y) { return fmaxf(x, y); }));
+                const float keep = top == m ? 1.f : __builtin_amdgcn_exp2f(m - top);
+                m = top;
+                l *= keep;
+#pragma unroll
+                for (int h = 0; h < H; h++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) acc[h][j] *= keep;
+            }
+            const float base = m == -INFINITY ? 0.f : m;  // no key yet: exp2(-inf) = 0
+            u32x4 ph, pl;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float p0 = __builtin_amdgcn_exp2f(sc[2 * i] - base);
+                const float p1 = __builtin_amdgcn_exp2f(sc[2 * i + 1] - base);
+                l += p0 + p1;
+                ph[i] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302);
+                pl[i] = pack2(fmaxf(p0 - lo_f32(ph[i]), LEAST), fmaxf(p1 - hi_f32(ph[i]), LEAST));
+            }
+#pragma unroll
+            for (int h = 0; h < H; h++) {
+                u32x4 vt[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        vt[j][i] = __builtin_amdgcn_perm(vf[h][2 * i + 1][j >> 1], vf[h][2 * i][j >> 1],
+                                                         j & 1 ? 0x07060302 : 0x05040100);
+#pragma unroll
+                for (int j = 0; j < 8; j++) acc[h][j] = mfma16(vt[j], ph, acc[h][j]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) acc[h][j] = mfma16(vt[j], pl, acc[h][j]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load_v();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+
+        // the waves join
+        const int tid = wave * 64 + lane_here();
+        l = over_groups(l, [](float x, float y) { return x + y; });
+        const int row_c = tid & 15, row_g = tid >> 4 & 3;
+        if (row_g == 0) {
+            wm[wave][row_c] = m;
+            wl[wave][row_c] = l;
+        }
+        __syncthreads();  // Q is no longer read
+        if (row_c < rows)
+#pragma unroll
+            for (int h = 0; h < H; h++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float* const to = lds + (wave * rows + row_c) * PITCH + h * 128 + (row_g * 4 + r) * 8;
+                    *reinterpret_cast<f32x4*>(to) = f32x4{acc[h][0][r], acc[h][1][r], acc[h][2][r], acc[h][3][r]};
+                    *reinterpret_cast<f32x4*>(to + 4) = f32x4{acc[h][4][r], acc[h][5][r], acc[h][6][r], acc[h][7][r]};
                 }
-            } else {
-                for (int k1 = way; k1 - way < n; k1 += BATCH * ways) {
-                    f32x4 v[BATCH];
+        __syncthreads();
+        const Shared shared(a);
+        constexpr int QUADS = DH / 4;  // of a row's dims
+        // four dims of a row's result: to the output, or to a slot
+        auto store = [&](int slot, int e, float top, float sum, const f32x4& o, const u32x2& g, bool out) {
+            const int row = e / QUADS, d = e % QUADS * 4;
+            if (out) {
+                store_out(a, out0 + row * DH + d, o, sum, g);
+                if (a.lse && d == 0) a.lse[(size_t)(head0 + row) * a.B + sh.row] = log_sum(top, sum);
+                return;
+            }
+            const int at = slot * ROWS + row;
+            shared.put((at * DH + d) * 4, o);
+            if (d == 0) shared.put_ml(at * 8, f32x2{top, sum});
+        };
+        // Groups of `group` parts: the last of a group to end joins it, the last group joins the groups; always in
+        // order, so the result does not depend on which ends last.  The counters are zero again afterwards.
+        int group = 1, groups = 1, g0 = 0, members = 1;
+        if (sh.parts > 1) {
+            groups = (sh.parts + GROUP - 1) / GROUP;
+            group = (sh.parts + groups - 1) / (uint32_t)groups;
+            groups = (sh.parts + group - 1) / (uint32_t)group;
+            g0 = sh.part / (uint32_t)group * group;
+            members = min(group, sh.parts - g0);
+        }
+        auto last_of = [&](int* count, int n) {
+            __shared__ int last;
+            wait_vm_all();  // what this wave has put is where the others look
+            __syncthreads();
+            if (tid == 0) {
+                last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+                if (last) *count = 0;
+            }
+            __syncthreads();
+            return last != 0;
+        };
+        // Stage 0: this block's waves.  1: a group's parts, 2: the groups.  A row's four dims are summed by as many
+        // threads as there are for them.  The time of 1 and 2 is that of getting at the parts, so many are asked for
+        // at once: a thread has every `ways`-th, BATCH of them on their way together, the first while a wave per row
+        // finds the parts' weights.
+        float* const weight = lds;               // [GROUP, ROWS]
+        float* const other = lds + GROUP * ROWS;  // [THREADS, 4]
+        const int items = rows * QUADS, rows_log = rows > 1 ? 32 - __builtin_clz(rows - 1) : 0;
+        for (int stage = 0;; stage++) {
+            const bool out = stage == 0 ? sh.parts == 1 : stage == 2 || groups == 1;
+            const int k0 = stage == 1 ? g0 : 0, step = stage == 2 ? group : 1, n = stage == 1 ? members : groups;
+            const int ways = stage == 0 ? 1 : max(1, THREADS / QUADS >> rows_log);
+            for (int e0 = 0; e0 < items; e0 += THREADS) {
+                const int way = ways > 1 ? tid / QUADS >> rows_log : 0;
+                const int e = e0 + (ways > 1 ? tid & ((QUADS << rows_log) - 1) : tid);
+                const bool works = e < items;
+                const int row = works ? e / QUADS : 0, d = e % QUADS * 4;
+                u32x2 g = {0, 0};
+                f32x4 o = {0.f, 0.f, 0.f, 0.f};
+                float top, sum = 0.f;
+                if (out) g = load_gate(a, out0 + row * DH + d);
+                if (stage == 0) {
+                    top = fmaxf(fmaxf(wm[0][row], wm[1][row]), fmaxf(wm[2][row], wm[3][row]));
 #pragma unroll
-                    for (int i = 0; i < BATCH; i++) {  // behind the last part: past the buffer's end, which is no access
-                        const int k = k1 + i * ways;
-                        v[i] = shared.get(k < n ? ((sh.slot(k0 + k * step) * ROWS + row) * DH + d) * 4 : -1);
+                    for (int w = 0; w < WAVES; w++) {
+                        const float f = wm[w][row] == top ? 1.f : __builtin_amdgcn_exp2f(wm[w][row] - top);
+                        sum += wl[w][row] * f;
+                        o += *reinterpret_cast<const f32x4*>(lds + (w * rows + row) * PITCH + d) * f;
                     }
-                    if (e0 == 0 && k1 == way) {
-                        const int k = tid & 63;
-                        for (int r = wave; r < rows; r += WAVES) {
-                            const f32x2 m = shared.get_ml((sh.slot(k0 + min(k, n - 1) * step) * ROWS + r) * 8);
-                            const float most = lane_max<64>(m[0]);
-                            const float f = k >= n ? 0.f : m[0] == most ? 1.f : __builtin_amdgcn_exp2f(m[0] - most);
-                            weight[k * ROWS + r] = f;
-                            const float all = lane_sum<64>(k < n ? m[1] * f : 0.f);
-                            if (k == 0) {
-                                wm[0][r] = most;
-                                wl[0][r] = all;
-                            }
+                } else {
+                    for (int k1 = way; k1 - way < n; k1 += BATCH * ways) {
+                        f32x4 v[BATCH];
+#pragma unroll
+                        for (int i = 0; i < BATCH; i++) {  // behind the last part: past the buffer's end, no access
+                            const int k = k1 + i * ways;
+                            v[i] = shared.get(k < n ? ((sh.slot(k0 + k * step) * ROWS + row) * DH + d) * 4 : -1);
                         }
-                        __syncthreads();
-                    }
+                        if (e0 == 0 && k1 == way) {
+                            const int k = tid & 63;
+                            for (int r = wave; r < rows; r += WAVES) {
+                                const f32x2 m = shared.get_ml((sh.slot(k0 + min(k, n - 1) * step) * ROWS + r) * 8);
+                                const float most = lane_max<64>(m[0]);
+                                const float f = k >= n ? 0.f : m[0] == most ? 1.f : __builtin_amdgcn_exp2f(m[0] - most);
+                                weight[k * ROWS + r] = f;
+                                const float all = lane_sum<64>(k < n ? m[1] * f : 0.f);
+                                if (k == 0) {
+                                    wm[0][r] = most;
+                                    wl[0][r] = all;
+                                }
+                            }
+                            __syncthreads();
+                        }
 #pragma unroll
-                    for (int i = 0; i < BATCH; i++) o += v[i] * weight[min(k1 + i * ways, GROUP - 1) * ROWS + row];
+                        for (int i = 0; i < BATCH; i++) o += v[i] * weight[min(k1 + i * ways, GROUP - 1) * ROWS + row];
+                    }
+                    if (ways > 1) {
+                        if (works && way > 0) *reinterpret_cast<f32x4*>(other + (way * items + e) * 4) = o;
+                        __syncthreads();
+                        if (way == 0)
+                            for (int w = 1; w < ways; w++)
+                                o += *reinterpret_cast<const f32x4*>(other + (w * items + (works ? e : 0)) * 4);
+                    }
+                    top = wm[0][row];
+                    sum = wl[0][row];
                 }
-                if (ways > 1) {
-                    if (works && way > 0) *reinterpret_cast<f32x4*>(other + (way * items + e) * 4) = o;
-                    __syncthreads();
-                    if (way == 0)
-                        for (int w = 1; w < ways; w++) o += *reinterpret_cast<const f32x4*>(other + (w * items + (works ? e : 0)) * 4);
-                }
-                top = wm[0][row];
-                sum = wl[0][row];
+                if (works && way == 0) store(out ? 0 : sh.slot(stage == 0 ? sh.part : k0), e, top, sum, o, g, out);
             }
-            if (works && way == 0) store(out ? 0 : sh.slot(stage == 0 ? sh.part : k0), e, top, sum, o, g, out);
+            if (out) break;
+            int* const count = stage == 0 ? a.count + sh.slot(g0) : a.count2 + sh.slot0;
+            if (!last_of(count, stage == 0 ? members : groups)) break;
         }
-        if (out || !last_of(stage == 0 ? a.count + sh.slot(g0) : a.count2 + sh.slot0, stage == 0 ? members : groups)) break;
-    }
     }
 }
 
@@ -562,14 +577,17 @@ extern "C" void cs1_attention_paged_destroy(void* paged) {
     delete p;
 }
 
-extern "C" int cs1_attention_paged(void* paged, const void* q, const void* kp, const void* vp, const Cs1PageTable* pages,
-                                   const int32_t* seqs, const void* gate, void* out, float* lse, int B, int Hq, int Hk,
-                                   int Dh, float scale, void* stream) {
+extern "C" int cs1_attention_paged(void* paged, const void* q, const void* kp, const void* vp,
+                                   const Cs1PageTable* pages, const int32_t* seqs, const void* gate, void* out,
+                                   float* lse, int B, int Hq, int Hk, int Dh, float scale, void* stream) {
     const Paged* const p = static_cast<const Paged*>(paged);
-    if (!p || !table_ok(pages) || (Dh != 128 && Dh != 256) || Hk <= 0 || Hq <= 0 || Hq % Hk != 0 || B < 0 ||
-        (int64_t)B * Hq > (1 << 22) || (int64_t)Hk * Dh > (1 << 24) ||
-        (int64_t)pages->npages * pages->page >= (int64_t{1} << 31) ||
-        (int64_t)B * Hk * ((Hq / Hk + ROWS - 1) / ROWS) * ((int64_t)pages->max_pages * pages->page / UNIT + 1) >= (int64_t{1} << 31))
+    if (!p || !table_ok(pages) || (Dh != 128 && Dh != 256) || Hk <= 0 || Hq <= 0 || Hq % Hk != 0 || B < 0)
+        return hipErrorInvalidValue;
+    // what the kernel counts in 32 bits: heads, bytes of a half, the pool's rows, all rows' units
+    constexpr int64_t LIMIT = int64_t{1} << 31;
+    const int64_t pairs = (int64_t)B * Hk * ((Hq / Hk + ROWS - 1) / ROWS);
+    if ((int64_t)B * Hq > (1 << 22) || (int64_t)Hk * Dh > (1 << 24) || (int64_t)pages->npages * pages->page >= LIMIT ||
+        pairs * ((int64_t)pages->max_pages * pages->page / UNIT + 1) >= LIMIT)
         return hipErrorInvalidValue;
     if (B == 0) return hipSuccess;
     if (!all_set({q, kp, vp, out}) || !on16(q) || !on16(kp) || !on16(vp) || !on16(out) || !on16(gate))
@@ -599,9 +617,12 @@ extern "C" int cs1_attention_paged(void* paged, const void* q, const void* kp, c
     a.Hk = Hk;
     a.G = Hq / Hk;
     a.tiles = (a.G + ROWS - 1) / ROWS;
-    a.halve = Dh == 128 && (int64_t)B * Hk * a.tiles >= p->blocks;  // the blocks, if the sequences are long
+    a.halve = Dh == 128 && pairs >= p->blocks;  // the blocks, if the sequences are long
     a.blocks = a.halve ? p->blocks : p->cus;
-    const bool many = (int64_t)B * Hk * a.tiles * 16 >= a.blocks;
+    // Where blocks have several sequences, the chunks are small and beginning one counts as much as 8 units of its
+    // keys (about 7 us): 43 sequences of up to 4096, 16/4 heads of 256, take 71 us so, 91 if it counts as nothing.
+    // One sequence alone is better cut into whole chunks of 4.
+    const bool many = pairs * 16 >= a.blocks;
     a.unit = many ? 2 : 4;
     a.pad = many ? 4 : 0;
     a.page_inverse = (uint32_t)std::min<uint64_t>(0xffffffffu, (uint64_t{1} << 32) / (a.page / 16));

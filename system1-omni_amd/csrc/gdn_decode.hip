@@ -58,17 +58,18 @@ __global__ void __launch_bounds__(THREADS, 8) gdn_decode_kernel(const Step t) {
     bf16* const out = t.out + ((size_t)row * t.H + h) * DK;
     const int s = __builtin_amdgcn_readfirstlane(listed_seq(t.seqs, row, t.nseq));
     const int p = __builtin_amdgcn_readfirstlane(s < 0 ? -1 : max(t.lens[s], 0) - 1);
-    if (p < 0 || wave_named_before(t.seqs, row, s)) {  // a padding row
+    if (p < 0 || named_before(t.seqs, row, s)) {  // a padding row
         if (tid < DK) out[tid] = 0;
         return;
     }
 
-    // Everything is asked for before anything is waited for.  The state goes past the caches (this layer's is not read
-    // again before the other layers' have gone through them): 61 rows of 48 heads take 74 us so and 86 with ordinary accesses.
-    // Columns 4 c .. 4 c + 3 of rows r0 + 16 i:
+    // Everything is asked for before anything is waited for.  The state goes past the caches (this layer's is not
+    // read again before the other layers' have gone through them): 61 rows of 48 heads take 74 us so and 86 with
+    // ordinary accesses. Columns 4 c .. 4 c + 3 of rows r0 + 16 i:
     const int c = tid & 31, r0 = tid >> 5;
     constexpr int NT = 2;  // the accesses' cache policy
-    const auto st = __builtin_amdgcn_make_buffer_rsrc(t.state + ((size_t)s * t.H + h) * DK * DK, (short)0, DK * DK * 4, 0x00020000);
+    const auto st = __builtin_amdgcn_make_buffer_rsrc(t.state + ((size_t)s * t.H + h) * DK * DK, (short)0, DK * DK * 4,
+                                                      0x00020000);
     const int at = (r0 * DK + 4 * c) * 4;
     f32x4 S[ROWS];
     if (p > 0) {
@@ -106,7 +107,9 @@ __global__ void __launch_bounds__(THREADS, 8) gdn_decode_kernel(const Step t) {
     }
     __syncthreads();
 
-    auto dot = [&](const float* a, const float* b) { return wave_sum(a[lane] * b[lane] + a[64 + lane] * b[64 + lane]); };
+    auto dot = [&](const float* a, const float* b) {
+        return wave_sum(a[lane] * b[lane] + a[64 + lane] * b[64 + lane]);
+    };
     const float qi = rsqrtf(dot(y, y) + 1e-6f) * t.scale, ki = rsqrtf(dot(y + DK, y + DK) + 1e-6f);
     const float d = gates[0], beta = gates[1];
     f32x4 sk = {0.f, 0.f, 0.f, 0.f}, sq = {0.f, 0.f, 0.f, 0.f};
@@ -138,8 +141,8 @@ __global__ void __launch_bounds__(THREADS, 8) gdn_decode_kernel(const Step t) {
     for (int i = 0; i < ROWS; i++) {
 #pragma unroll
         for (int e = 0; e < 4; e++) S[i][e] = fmaf(y[DK + r0 + i * STEP] * ki, u[e], S[i][e]);
-        // (no scalar offset: with one, the compiler writes the next product over S[i] in the instruction after the store, and gfx950
-        // then stores some lanes' new value)
+        // (no scalar offset: with one, the compiler writes the next product over S[i] in the instruction after the
+        // store, and gfx950 then stores some lanes' new value)
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, S[i]), st, at + i * STEP * DK * 4, 0, NT);
     }
     if (wave > 0) return;
@@ -170,7 +173,8 @@ extern "C" int cs1_gdn_decode(const void* qkv, int ld, const void* w, const void
                               const void* A_log, const void* dt_bias, const void* norm_w, float eps, void* ring,
                               float* state, const int32_t* seqs, const int32_t* lens, int nseq, void* out, int B, int H,
                               int HK, float scale, void* stream) {
-    if (B < 0 || B > MAX_LISTED || H <= 0 || HK <= 0 || H % HK != 0 || (int64_t)B * H > (1 << 22) || nseq <= 0) return hipErrorInvalidValue;
+    if (B < 0 || B > MAX_LISTED || H <= 0 || HK <= 0 || H % HK != 0 || (int64_t)B * H > (1 << 22) || nseq <= 0)
+        return hipErrorInvalidValue;
     const int64_t conv = ((int64_t)2 * HK + H) * DK;
     if (ld < conv || (z == nullptr) != (norm_w == nullptr)) return hipErrorInvalidValue;
     if (B == 0) return hipSuccess;

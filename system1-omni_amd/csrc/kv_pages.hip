@@ -79,7 +79,8 @@ __device__ __forceinline__ uint32_t free_pages(const int32_t* __restrict__ refs,
 // Calls take(k, page) for the `total` lowest free pages, k = 0 .., or for all there are; returns their number. bits: of
 // pages 4 threadIdx.x .. + 3, asked for early by the caller.
 template <typename Take>
-__device__ __forceinline__ int take_free(const int32_t* refs, int npages, int total, uint32_t bits, int* red, Take take) {
+__device__ __forceinline__ int take_free(const int32_t* refs, int npages, int total, uint32_t bits, int* red,
+                                         Take take) {
     int found = 0;
     for (int base = 0; base < npages && found < total; base += 4 * PLAN_THREADS) {
         const int p = base + 4 * threadIdx.x;
@@ -91,11 +92,12 @@ __device__ __forceinline__ int take_free(const int32_t* refs, int npages, int to
     return found;
 }
 
-// PER: list entries a thread has at most. Lists of up to 1024 have one each, which leaves a third of the code: what runs once
-// takes its time to arrive (6.4 us with eight, 4.9 with one).
+// PER: list entries a thread has at most. Lists of up to 1024 have one each, which leaves a third of the code: what
+// runs once takes its time to arrive (6.4 us with eight, 4.9 with one).
 template <int PER>
 __global__ void __launch_bounds__(PLAN_THREADS)
-    kv_reserve_kernel(const Cs1PageTable t, const int32_t* __restrict__ seqs, const Offsets cu, int n, int32_t* status) {
+    kv_reserve_kernel(const Cs1PageTable t, const int32_t* __restrict__ seqs, const Offsets cu, int n,
+                      int32_t* status) {
     __shared__ int work[MAX_LISTED];  // first entry that names a sequence, then the offsets off_i
     __shared__ int red[PLAN_WAVES];
     const int tid = threadIdx.x;
@@ -192,7 +194,7 @@ __global__ void __launch_bounds__(MOVE_THREADS)
     const int s = __builtin_amdgcn_readfirstlane(listed_seq(seqs, i, t.nseq));
     if (s < 0) return;
     const int pos = __builtin_amdgcn_readfirstlane(t.lens[s]) - back;
-    if (pos < 0 || pos / t.page >= t.max_pages || wave_named_before(seqs, i, s)) return;
+    if (pos < 0 || pos / t.page >= t.max_pages || named_before(seqs, i, s)) return;
     const int pg = __builtin_amdgcn_readfirstlane(t.table[(size_t)s * t.max_pages + pos / t.page]);
     if (pg < 0 || pg >= t.npages) return;
     const size_t to = ((size_t)pg * t.page + pos % t.page) * packs;
@@ -346,7 +348,7 @@ __global__ void __launch_bounds__(MOVE_THREADS)
     kv_free_kernel(const Cs1PageTable t, const int32_t* __restrict__ seqs) {
     const int i = blockIdx.x, s = listed_seq(seqs, i, t.nseq);
     if (s < 0) return;
-    if (__syncthreads_or(named_before(seqs, i, s))) return;
+    if (named_before(seqs, i, s)) return;
     int32_t* const row = t.table + (size_t)s * t.max_pages;
     const int held = min(pages_of(max(t.lens[s], 0), t.page), t.max_pages);
     for (int j = threadIdx.x; j < held; j += MOVE_THREADS) {
@@ -428,7 +430,8 @@ __global__ void __launch_bounds__(MOVE_THREADS)
         }
     const uint32_t chunks = (uint32_t)((page_bytes + CHUNK - 1) / CHUNK), pages = (uint32_t)moves * chunks;
     for (uint32_t it = block; it < pages * npools; it += blocks) {
-        const uint32_t pool = it / max(pages, 1u), left = it - pool * pages, k = left / chunks, chunk = left - k * chunks;
+        const uint32_t pool = it / max(pages, 1u), left = it - pool * pages;
+        const uint32_t k = left / chunks, chunk = left - k * chunks;
         u32x4 r[QUADS];
         load_chunk(r, pools.p[pool] + from[k] * page_bytes, chunk, page_bytes, true);
         store_chunk(r, pools.p[pool] + to[k] * page_bytes, chunk, page_bytes);
@@ -474,6 +477,8 @@ bool pools_ok(void* const* pools, int npools) {
     return true;
 }
 
+bool row_ok(size_t row_bytes) { return row_bytes > 0 && row_bytes % 16 == 0 && row_bytes <= ((size_t)1 << 32); }
+
 // Up to POOLS_MAX of them from number `first` on; their count.
 int some_pools(void* const* pools, int npools, int first, Pools& out) {
     const int n = npools - first < POOLS_MAX ? npools - first : POOLS_MAX;
@@ -515,9 +520,9 @@ extern "C" int cs1_kv_write(const Cs1PageTable* pages, const int32_t* seqs, cons
     if (!all_set({k, v, kp, vp}) || !on16(k) || !on16(v) || !on16(kp) || !on16(vp)) return hipErrorInvalidValue;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     auto launch = [&](const Offsets& cu, int first, int rows) {
-        kv_write_kernel<<<cdiv(rows, ROWS_BLOCK), MOVE_THREADS, 0, st>>>(*pages, seqs, cu, first, rows, static_cast<const bf16*>(k), ldk,
-                                                       static_cast<const bf16*>(v), ldv, static_cast<char*>(kp),
-                                                       static_cast<char*>(vp), (int)width);
+        kv_write_kernel<<<cdiv(rows, ROWS_BLOCK), MOVE_THREADS, 0, st>>>(
+            *pages, seqs, cu, first, rows, static_cast<const bf16*>(k), ldk, static_cast<const bf16*>(v), ldv,
+            static_cast<char*>(kp), static_cast<char*>(vp), (int)width);
         return hipGetLastError();
     };
     Offsets cu;
@@ -542,7 +547,7 @@ extern "C" size_t cs1_kv_workspace_bytes(int npages, int n) {
 extern "C" int cs1_kv_fork(const Cs1PageTable* pages, const int32_t* src, const int32_t* dst, int n, void* const* pools,
                            int npools, size_t row_bytes, void* workspace, int32_t* status, void* stream) {
     if (!table_ok(pages) || n < 0 || n > MAX_LISTED || !pools_ok(pools, npools) || !status) return hipErrorInvalidValue;
-    if (npools > 0 && (row_bytes == 0 || row_bytes % 16 != 0 || row_bytes > ((size_t)1 << 32))) return hipErrorInvalidValue;
+    if (npools > 0 && !row_ok(row_bytes)) return hipErrorInvalidValue;
     const size_t chunks = npools > 0 ? ((pages->page - 1) * row_bytes + CHUNK - 1) / CHUNK : 1;
     if (chunks > CHUNKS_MAX) return hipErrorInvalidValue;
     if (n > 0 && (!all_set({src, dst, workspace}) || !on16(workspace))) return hipErrorInvalidValue;
@@ -576,7 +581,7 @@ extern "C" int cs1_kv_compact(const Cs1PageTable* pages, void* const* pools, int
                               void* workspace, int32_t* status, void* stream) {
     if (!table_ok(pages) || !pools_ok(pools, npools) || !status || !workspace || !on16(workspace))
         return hipErrorInvalidValue;
-    if (npools > 0 && (row_bytes == 0 || row_bytes % 16 != 0 || row_bytes > ((size_t)1 << 32))) return hipErrorInvalidValue;
+    if (npools > 0 && !row_ok(row_bytes)) return hipErrorInvalidValue;
     const size_t page_bytes = pages->page * row_bytes;
     if (npools > 0 && (page_bytes / CHUNK > CHUNKS_MAX ||
                        (uint64_t)(pages->npages / 2 + 1) * POOLS_MAX * (page_bytes / CHUNK + 1) >= uint64_t{1} << 31))
@@ -592,11 +597,13 @@ extern "C" int cs1_kv_compact(const Cs1PageTable* pages, void* const* pools, int
     do {
         Pools some = {};
         const int k = some_pools(pools, npools, first, some), tables = first == 0 ? pages->nseq : 0;
-        // a block for each chunk that may move, as far as that is 128 a CU (blocks that go on to a second chunk wait for the
-        // first one's stores to be taken: 326 us with 8 a CU, in a pool of 1400 pages of 128 KiB with 700 held in 16 pools)
+        // a block for each chunk that may move, as far as that is 128 a CU (blocks that go on to a second chunk wait
+        // for the first one's stores to be taken: 326 us with 8 a CU, in a pool of 1400 pages of 128 KiB with 700
+        // held in 16 pools)
         const size_t most = (size_t)(pages->npages / 2) * k * (page_bytes / CHUNK + 1), cap = (size_t)128 * cus;
         const unsigned movers = (unsigned)(most < cap ? most + 1 : cap);
-        kv_compact_kernel<<<tables + movers, MOVE_THREADS, 0, st>>>(*pages, ws, some, k, npools > 0 ? page_bytes : 0, tables);
+        kv_compact_kernel<<<tables + movers, MOVE_THREADS, 0, st>>>(*pages, ws, some, k, npools > 0 ? page_bytes : 0,
+                                                                    tables);
         e = hipGetLastError();
         first += k;
     } while (first < npools && e == hipSuccess);

@@ -21,19 +21,11 @@ __device__ __forceinline__ int listed_seq(const int32_t* __restrict__ seqs, int 
 }
 
 // Whether an entry before i names the same sequence, asked by a whole wave for itself.
-__device__ __forceinline__ bool wave_named_before(const int32_t* __restrict__ seqs, int i, int s) {
+__device__ __forceinline__ bool named_before(const int32_t* __restrict__ seqs, int i, int s) {
     bool hit = false;
     if (seqs)
         for (int j = threadIdx.x & 63; j < i; j += 64) hit |= seqs[j] == s;
     return __any(hit);
-}
-
-// The same with this thread's share of the entries; the block's threads together see all of them.
-__device__ __forceinline__ bool named_before(const int32_t* __restrict__ seqs, int i, int s) {
-    bool hit = false;
-    if (seqs)
-        for (int j = threadIdx.x; j < i; j += blockDim.x) hit |= seqs[j] == s;
-    return hit;
 }
 
 }  // namespace q35
