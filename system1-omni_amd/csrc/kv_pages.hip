@@ -301,10 +301,11 @@ __device__ __forceinline__ void store_chunk(const u32x4 (&r)[QUADS], char* to, s
 
 constexpr int RUN_MAX = 8;
 
-// Runs where there are blocks enough without the pairs apart (4096: sixteen a CU).
+// Runs where there are blocks enough without the pairs apart (2048: eight a CU).
 int run_of(size_t chunks, int pools, int n) {
     const size_t blocks = chunks * pools * n;
-    return blocks >= 4096 * RUN_MAX ? RUN_MAX : blocks <= 4096 ? 1 : (int)(blocks / 4096);
+    const int most = blocks >= 2048 * RUN_MAX ? RUN_MAX : blocks <= 2048 ? 1 : (int)(blocks / 2048);
+    return (int)cdiv(n, (int)cdiv(n, most));  // as even as it goes
 }
 
 // Blocks y = 0 of the first launch: the pairs' rows of the table, the shared pages' counts, the lengths. The others: a
@@ -331,16 +332,20 @@ __global__ void __launch_bounds__(MOVE_THREADS)
         return;
     }
     const size_t page_bytes = t.page * row_bytes;
+    const int lane = threadIdx.x & 63, i = min(i0 + lane, n - 1);
+    const Pair mine = plan[i];  // lane k has pair k of the run
+    const int on = lane < i1 - i0 && mine.on && mine.from >= 0 && mine.from < t.npages ? mine.rows : 0;
     u32x4 r[QUADS];
-    int held = -1, rows = 0;
-    for (int i = i0; i < i1; i++) {
-        const Pair pr = plan[i];
-        if (!pr.on || pr.from < 0 || pr.from >= t.npages || blockIdx.x * (size_t)CHUNK >= pr.rows * row_bytes) continue;
-        if (pr.from != held || pr.rows != rows)
-            load_chunk(r, pools.p[pool] + pr.from * page_bytes, blockIdx.x, pr.rows * row_bytes, false);
-        held = pr.from;
-        rows = pr.rows;
-        store_chunk(r, pools.p[pool] + pr.to * page_bytes, blockIdx.x, pr.rows * row_bytes);
+    int held = -1, held_rows = 0;
+    for (int k = 0; k < i1 - i0; k++) {
+        const int rows = __builtin_amdgcn_readlane(on, k), from = __builtin_amdgcn_readlane(mine.from, k);
+        if (blockIdx.x * (size_t)CHUNK >= rows * row_bytes) continue;
+        if (from != held || rows != held_rows)
+            load_chunk(r, pools.p[pool] + from * page_bytes, blockIdx.x, rows * row_bytes, false);
+        held = from;
+        held_rows = rows;
+        char* const to = pools.p[pool] + __builtin_amdgcn_readlane(mine.to, k) * page_bytes;
+        store_chunk(r, to, blockIdx.x, rows * row_bytes);
     }
 }
 
@@ -442,22 +447,27 @@ __global__ void __launch_bounds__(MOVE_THREADS)
 __global__ void __launch_bounds__(MOVE_THREADS)
     kv_copy_kernel(const Pools pools, size_t bytes, int entries, const int32_t* __restrict__ src,
                    const int32_t* __restrict__ dst, int n, int run) {
-    const int i0 = blockIdx.z * run, i1 = min(n, i0 + run), lane = threadIdx.x & 63;
+    const int i0 = blockIdx.z * run, count = min(n - i0, run), lane = threadIdx.x & 63;
     char* const pool = pools.p[blockIdx.y];
+    // each wave for itself: lane k has pair k of the run, and all of them are held against 64 destinations at a time
+    const int s = lane < count ? src[i0 + lane] : -1, d = lane < count ? dst[i0 + lane] : -1;
+    uint32_t out = 0;
+    for (int j0 = 0; j0 < n; j0 += 64) {
+        const int j = j0 + lane, other = j < n ? dst[j] : -1;
+        for (int k = 0; k < count; k++)
+            if (__any(j < n && (other == __builtin_amdgcn_readlane(s, k) ||
+                                (j < i0 + k && other == __builtin_amdgcn_readlane(d, k)))))
+                out |= 1u << k;
+    }
     u32x4 r[QUADS];
     int held = -1;
-    for (int i = i0; i < i1; i++) {
-        const int s = src[i], d = dst[i];
-        if (s < 0 || s >= entries || d < 0 || d >= entries) continue;
-        bool out = false;  // each wave for itself
-        for (int j = lane; j < n; j += 64) {
-            const int other = dst[j];
-            out |= other == s || (j < i && other == d);
-        }
-        if (__any(out)) continue;
-        if (s != held) load_chunk(r, pool + s * bytes, blockIdx.x, bytes, i + 1 == i1 || src[i + 1] != s);
-        held = s;
-        store_chunk(r, pool + d * bytes, blockIdx.x, bytes);
+    for (int k = 0; k < count; k++) {
+        const int from = __builtin_amdgcn_readlane(s, k), to = __builtin_amdgcn_readlane(d, k);
+        if (out >> k & 1 || from < 0 || from >= entries || to < 0 || to >= entries) continue;
+        const bool again = k + 1 < count && __builtin_amdgcn_readlane(s, k + 1) == from;
+        if (from != held) load_chunk(r, pool + from * bytes, blockIdx.x, bytes, !again);
+        held = from;
+        store_chunk(r, pool + to * bytes, blockIdx.x, bytes);
     }
 }
 
