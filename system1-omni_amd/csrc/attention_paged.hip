@@ -236,11 +236,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
     const uint32_t inverse = a.halve && total >= 8 * a.B * heads ? 2 * a.blocks_inverse : a.blocks_inverse;
     const int each = __umulhi(total - 1, inverse) + 1;  // (one more than need be where the inverse's rounding shows)
     const int begin = (int)blockIdx.x * each, end = min(total, begin + each);
+    // (the rows go on from one segment to the next: r0 the 64 that are searched, which begin at chunk `before`)
+    int r0 = 0, before = 0, seen = (a.B - 1) / THREADS * THREADS;
     for (int pos = begin; pos < end;) {
         Segment sh = {};
-        for (int r0 = 0, before = 0; r0 < a.B; r0 += 64) {
+        for (; r0 < a.B; r0 += 64) {
             const int w = r0 / 64 % WAVES;
-            if (w == 0 && a.B > THREADS) (void)look_at(r0);
+            if (r0 - w * 64 != seen) (void)look_at(seen = r0 - w * 64);
             if (segment_at(a, table[w * 64 + lane_here()], r0, before, pos, end, each, sh)) break;
             before += __builtin_amdgcn_readfirstlane(sums[w]) * heads;
         }

@@ -87,8 +87,8 @@ __global__ void __launch_bounds__(THREADS, 8) gdn_decode_kernel(const Step t) {
         bf16* const ring = t.ring + (size_t)s * 4 * conv + ch;
         const u32x2 w = *reinterpret_cast<const u32x2*>(t.w + (size_t)ch * 4);
         const bf16 now = x[ch];
-        const bf16 x1 = ring[(size_t)((p + 3) & 3) * conv], x2 = ring[(size_t)((p + 2) & 3) * conv];
-        const bf16 x3 = ring[(size_t)((p + 1) & 3) * conv];
+        const bf16 x1 = ring[(size_t)((p - 1) & 3) * conv], x2 = ring[(size_t)((p - 2) & 3) * conv];
+        const bf16 x3 = ring[(size_t)((p - 3) & 3) * conv];
         float acc = p > 2 ? lo_f32(w[0]) * f32(x3) : 0.f;
         acc = p > 1 ? fmaf(hi_f32(w[0]), f32(x2), acc) : acc;
         acc = p > 0 ? fmaf(lo_f32(w[1]), f32(x1), acc) : acc;

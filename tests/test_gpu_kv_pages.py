@@ -206,6 +206,44 @@ def test_copies_of_entries(bytes_, entries, npools):
         np.testing.assert_array_equal(read_pool(b, w), w)
 
 
+@pytest.mark.parametrize("bytes_,entries,npools,n", [(16384 + 16, 40, 64, 90), (16 * 700, 30, 3, 8192), (3 * 16384, 9, 66, 40)])
+def test_copies_in_runs(bytes_, entries, npools, n):
+    """So many blocks that each takes several pairs, in lists that name entries out of range, twice and as source and destination."""
+    say(f"copy {bytes_} bytes, {entries} entries, {npools} pools, {n} pairs")
+    rng = np.random.default_rng(n)
+    pools = [R.bf16(rng, entries, bytes_ // 2) for _ in range(npools)]
+    bufs = pool_buffers(pools)
+    half = entries // 2
+    src = np.repeat(rng.integers(-1, half + 1, n), rng.integers(1, 9, n))[:n].astype(np.int32)
+    dst = rng.integers(half, entries + 2, n).astype(np.int32)
+    src[-1], dst[-2] = entries, -3
+    want = [p.copy() for p in pools]
+    pairs = list(R.Table(entries, 1, 1, 16).pairs(src, dst, entries))
+    assert len(pairs) > 3
+    for s, d in pairs:
+        for w, p in zip(want, pools):
+            w[d] = p[s]
+    a, b, ptrs = ints(src), ints(dst), pointers(bufs)
+    hip.check(hip.api().cs1_kv_copy(ptrs, npools, bytes_, entries, a.at(0), b.at(0), n, stream().handle), "copy")
+    for b, w in zip(bufs, want):
+        np.testing.assert_array_equal(read_pool(b, w), w)
+
+
+def test_forks_in_runs():
+    """A block takes several pairs: of the same source, of others, of one without rows to copy, of one that is left out."""
+    say("fork in runs")
+    rng = np.random.default_rng(11)
+    c = Cache(Table(90, 3, 200, 64), rng, 64, 1024)
+    lens = [100, 64, 127, 65, 1, 129]
+    assert c.reserve(range(6), np.cumsum([0] + lens).astype(np.int32)) == 0
+    src = np.repeat([0, 1, 2, 3, 4, 5, 2, 0, -1, 4, 89], 7)[:74]
+    dst = np.arange(6, 80)
+    dst[[9, 20, 33]] = [6, 90, 2]  # twice, out of range, one that holds tokens (and so sequence 2 is no source)
+    assert c.fork(src, dst) == 0
+    c.free([0, 2, 5, 7, 8])
+    c.compact()
+
+
 def test_offsets_past_32_bits():
     """The last page of a pool of 5 GiB receives rows, is forked and moves to the front."""
     say("a pool of 5 GiB")
