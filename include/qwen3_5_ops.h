@@ -253,15 +253,18 @@ int cs1_gdn_prefill_gated_varlen(const void* q, const void* k, const void* v, co
  * below works on a list of sequences: seqs is a DEVICE array of sequence numbers (null: row i is
  * sequence i), so a captured graph serves whatever sequences the array names when it is
  * replayed.  A number outside [0, nseq) is a padding row.  Where a call changes a sequence, the
- * first row that names it has it and later rows that name it again are padding rows. */
+ * first row that names it has it and later rows that name it again are padding rows.  Calls on one
+ * table run one after another, on one stream or ordered by events.  All take device pointers of the
+ * device that is current, allocate nothing and may be captured. */
 
 /* The page table, on the device; the struct itself is read during the call.  Sequence s holds
  * lens[s] tokens, token j in slot j % page of page table[s * max_pages + j / page]; refs[p] counts
  * the sequences that hold page p (0: free).  A program starts with table filled with -1 and
  * lens and refs with 0.  Limits: nseq <= 8192, page a multiple of 16, max_pages * page < 2^31.
  * One layer's K pages and V pages are two buffers ("pools") of [npages, page, Hk, Dh], all layers
- * under the one table.  A page number outside [0, npages) in a row of the table is never
- * followed: its tokens are neither read nor written. */
+ * under the one table, on 16 bytes.  Only the calls below change the three arrays.  A page number
+ * outside [0, npages) in a row of the table is never followed: its tokens are neither read nor
+ * written. */
 typedef struct Cs1PageTable {
     int32_t* table; /* [nseq, max_pages] */
     int32_t* lens;  /* [nseq] */
@@ -274,14 +277,16 @@ typedef struct Cs1PageTable {
  * and the pages that this needs are the lowest-numbered free ones, in the order of the list.
  * All or nothing: *status (device) receives 0, or the number of pages that are missing, or -1
  * where a sequence would need more than max_pages; if it is not 0 nothing else has changed, and
- * the step that the room was for must not run.  n <= 8192. */
+ * the step that the room was for must not run (it would write over the sequences' last tokens): a
+ * program that cannot tell beforehand keeps this call out of the step's graph.  n <= 8192. */
 int cs1_kv_reserve(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n, int32_t* status,
                    void* stream);
 
 /* Store the last tokens' keys and values of one layer: row r of k (rows of ldk) and of v (rows of
  * ldv), Hk * Dh values each, goes to the pages kp and vp.  cu_seqlens null: row i is the last
- * token (lens[s] - 1) of listed sequence i; else (HOST, any n) rows [cu_seqlens[i], cu_seqlens[i + 1])
- * are its last tokens in order.  Rows of padding or before position 0 are left out. */
+ * token (lens[s] - 1) of listed sequence i; else (HOST, cu_seqlens[n] <= 2^23) rows [cu_seqlens[i],
+ * cu_seqlens[i + 1]) are its last tokens in order.  Rows of padding or before position 0 are left out.
+ * Hk * Dh and both row lengths are multiples of 8, k and v on 16 bytes, n <= 8192; Hk * Dh <= 2^24. */
 int cs1_kv_write(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n, const void* k,
                  int ldk, const void* v, int ldv, void* kp, void* vp, int Hk, int Dh, void* stream);
 
@@ -290,25 +295,29 @@ int cs1_kv_write(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* 
  * the last page holds if it is not full; those tokens' rows (row_bytes a token) are copied in all
  * npools pools (a HOST array of device pointers to [npages, page * row_bytes bytes]).  Left out are
  * pairs with a number out of range, whose dst holds tokens or an earlier pair names as dst, or whose src
- * any pair names as dst.  status as in cs1_kv_reserve (0, or the missing pages, and then nothing has
- * changed).  workspace: cs1_kv_workspace_bytes(npages, n) bytes, free for other use after the call. */
+ * is empty or any pair names as dst.  status as in cs1_kv_reserve (0, or the missing pages, and then
+ * nothing has changed).  row_bytes: a multiple of 16, up to 2^32; page * row_bytes <= 2^36.  workspace:
+ * cs1_kv_workspace_bytes(npages, n) bytes on 16, this call's own until it is done on the device. */
 size_t cs1_kv_workspace_bytes(int npages, int n);
-int cs1_kv_fork(const Cs1PageTable* pages, const int32_t* src, const int32_t* dst, int n, void* const* pools, int npools,
-                size_t row_bytes, void* workspace, int32_t* status, void* stream);
+int cs1_kv_fork(const Cs1PageTable* pages, const int32_t* src, const int32_t* dst, int n, void* const* pools,
+                int npools, size_t row_bytes, void* workspace, int32_t* status, void* stream);
 
-/* End the listed sequences: each page's count falls by one, the rows of the table become -1 and the lengths 0. */
+/* End the listed sequences: each page's count falls by one, the rows of the table become -1 and the
+ * lengths 0.  n <= 8192. */
 int cs1_kv_free(const Cs1PageTable* pages, const int32_t* seqs, int n, void* stream);
 
 /* Move the pages that are held to the start of every pool: with L of them, the i-th held page
  * from L on moves to the i-th free page before L; table and refs follow.  *status receives L.
- * workspace: cs1_kv_workspace_bytes(npages, 0) bytes. */
+ * row_bytes as in cs1_kv_fork; (npages / 2 + 1) * (page * row_bytes / 16384 + 1) < 2^25 (half a TiB a
+ * pool).  workspace: cs1_kv_workspace_bytes(npages, 0) bytes, as there. */
 int cs1_kv_compact(const Cs1PageTable* pages, void* const* pools, int npools, size_t row_bytes, void* workspace,
                    int32_t* status, void* stream);
 
 /* Copy entry src[i] to entry dst[i] (device, n <= 8192) in each of npools buffers of `entries`
- * entries of entry_bytes (a multiple of 16): pages, or with a sequence's GDN state or conv ring as
- * the entry, what cs1_kv_fork does for the Gated DeltaNet layers.  Left out are pairs with a number out of range,
- * whose dst an earlier pair names as dst, or whose src any pair names as dst. */
+ * entries of entry_bytes (a multiple of 16, up to 2^36): pages, or with a sequence's GDN state or conv
+ * ring as the entry, what cs1_kv_fork does for the Gated DeltaNet layers (lengths are not looked at
+ * here).  Left out are pairs with a number out of range, whose dst an earlier pair names as dst, or
+ * whose src any pair names as dst. */
 int cs1_kv_copy(void* const* pools, int npools, size_t entry_bytes, int entries, const int32_t* src, const int32_t* dst,
                 int n, void* stream);
 
@@ -316,9 +325,11 @@ int cs1_kv_copy(void* const* pools, int npools, size_t entry_bytes, int entries,
  * out [B, Hq, Dh], Dh 128 or 256; row r's q head h sees the lens[s] keys of sequence s = seqs[r] through kv
  * head h / (Hq / Hk).  lse [Hq, B] float32 (null: not written) as in cs1_attention_ex.  Unlike there the
  * output is rounded once, after the gate.  A padding row, or one of an empty sequence, gets zeros and an
- * lse of -inf.  The handle holds the partial results of sequences that are split over the chip: it belongs to the
- * device that is current when it is created and, as a GEMM handle, serves one thread and one
- * stream at a time (graphs captured with one handle must not run at the same time). */
+ * lse of -inf.  q, kp, vp, gate and out on 16 bytes; Hk * Dh <= 2^24, B * Hq <= 2^22, npages * page < 2^31 and
+ * B * Hk * ceil(Hq / Hk / 16) * (max_pages * page / 32 + 1) < 2^31.  The handle holds the partial
+ * results of sequences that are split over the chip (16 MiB): it belongs to the device that is current
+ * when it is created (not during a capture; null if that fails) and, as a GEMM handle, serves one
+ * thread and one stream at a time (graphs captured with one handle must not run at the same time). */
 void* cs1_attention_paged_create(void);
 void cs1_attention_paged_destroy(void* paged);
 int cs1_attention_paged(void* paged, const void* q, const void* kp, const void* vp, const Cs1PageTable* pages,
