@@ -296,7 +296,7 @@ int cs1_kv_write(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* 
  * npools pools (a HOST array of device pointers to [npages, page * row_bytes bytes]).  Left out are
  * pairs with a number out of range, whose dst holds tokens or an earlier pair names as dst, or whose src
  * is empty or any pair names as dst.  status as in cs1_kv_reserve (0, or the missing pages, and then
- * nothing has changed).  row_bytes: a multiple of 16, up to 2^32; page * row_bytes <= 2^36.  workspace:
+ * nothing has changed).  row_bytes: a multiple of 16, up to 2^32; page * row_bytes <= 2^34.  workspace:
  * cs1_kv_workspace_bytes(npages, n) bytes on 16, this call's own until it is done on the device. */
 size_t cs1_kv_workspace_bytes(int npages, int n);
 int cs1_kv_fork(const Cs1PageTable* pages, const int32_t* src, const int32_t* dst, int n, void* const* pools,
@@ -308,13 +308,13 @@ int cs1_kv_free(const Cs1PageTable* pages, const int32_t* seqs, int n, void* str
 
 /* Move the pages that are held to the start of every pool: with L of them, the i-th held page
  * from L on moves to the i-th free page before L; table and refs follow.  *status receives L.
- * row_bytes as in cs1_kv_fork; (npages / 2 + 1) * (page * row_bytes / 16384 + 1) < 2^25 (half a TiB a
+ * row_bytes as in cs1_kv_fork; (npages / 2 + 1) * (page * row_bytes / 4096 + 1) < 2^25 (256 GiB a
  * pool).  workspace: cs1_kv_workspace_bytes(npages, 0) bytes, as there. */
 int cs1_kv_compact(const Cs1PageTable* pages, void* const* pools, int npools, size_t row_bytes, void* workspace,
                    int32_t* status, void* stream);
 
 /* Copy entry src[i] to entry dst[i] (device, n <= 8192) in each of npools buffers of `entries`
- * entries of entry_bytes (a multiple of 16, up to 2^36): pages, or with a sequence's GDN state or conv
+ * entries of entry_bytes (a multiple of 16, up to 2^34): pages, or with a sequence's GDN state or conv
  * ring as the entry, what cs1_kv_fork does for the Gated DeltaNet layers (lengths are not looked at
  * here).  Left out are pairs with a number out of range, whose dst an earlier pair names as dst, or
  * whose src any pair names as dst. */

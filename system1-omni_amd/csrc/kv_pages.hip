@@ -193,8 +193,10 @@ __global__ void __launch_bounds__(MOVE_THREADS)
     }
     const int s = __builtin_amdgcn_readfirstlane(listed_seq(seqs, i, t.nseq));
     if (s < 0) return;
-    const int pos = __builtin_amdgcn_readfirstlane(t.lens[s]) - back;
-    if (pos < 0 || pos / t.page >= t.max_pages || named_before(seqs, i, s)) return;
+    const int len = t.lens[s];
+    const bool again = named_before(seqs, i, s);  // (both on their way together)
+    const int pos = __builtin_amdgcn_readfirstlane(len) - back;
+    if (again || pos < 0 || pos / t.page >= t.max_pages) return;
     const int pg = __builtin_amdgcn_readfirstlane(t.table[(size_t)s * t.max_pages + pos / t.page]);
     if (pg < 0 || pg >= t.npages) return;
     const size_t to = ((size_t)pg * t.page + pos % t.page) * packs;
@@ -279,24 +281,19 @@ __global__ void __launch_bounds__(PLAN_THREADS)
 }
 
 // How entries are copied: a block has a chunk of one pool for `run` pairs in a row and reads it once for all that have
-// the same source, so that copies of one entry cost their writing alone (8 copies of 50 MiB: 73 us, and 140 with a
-// block for each).  What is written goes past the caches; so does what is read, where it is read once.
-constexpr int QUADS = 4, CHUNK = MOVE_THREADS * 16 * QUADS;
+// the same source, so that copies of one entry cost their writing alone (8 copies of 50 MiB: 73 us, and 110 with a
+// block for each).  What is written goes past the caches; so does what is read, where it is read once.  One access a
+// thread: with four, and a quarter of the blocks, the 8 copies take 78 us and the compaction below 302 in place of 268.
+constexpr int CHUNK = MOVE_THREADS * 16;
 
-__device__ __forceinline__ void load_chunk(u32x4 (&r)[QUADS], const char* from, size_t chunk, size_t bytes, bool once) {
-#pragma unroll
-    for (int q = 0; q < QUADS; q++) {
-        const size_t e = chunk * CHUNK + (q * MOVE_THREADS + threadIdx.x) * 16;
-        const u32x4* const p = reinterpret_cast<const u32x4*>(from + e);
-        if (e < bytes) r[q] = once ? __builtin_nontemporal_load(p) : *p;
-    }
+__device__ __forceinline__ void load_chunk(u32x4& r, const char* from, size_t chunk, size_t bytes, bool once) {
+    const size_t e = chunk * CHUNK + threadIdx.x * 16;
+    const u32x4* const p = reinterpret_cast<const u32x4*>(from + e);
+    if (e < bytes) r = once ? __builtin_nontemporal_load(p) : *p;
 }
-__device__ __forceinline__ void store_chunk(const u32x4 (&r)[QUADS], char* to, size_t chunk, size_t bytes) {
-#pragma unroll
-    for (int q = 0; q < QUADS; q++) {
-        const size_t e = chunk * CHUNK + (q * MOVE_THREADS + threadIdx.x) * 16;
-        if (e < bytes) __builtin_nontemporal_store(r[q], reinterpret_cast<u32x4*>(to + e));
-    }
+__device__ __forceinline__ void store_chunk(const u32x4& r, char* to, size_t chunk, size_t bytes) {
+    const size_t e = chunk * CHUNK + threadIdx.x * 16;
+    if (e < bytes) __builtin_nontemporal_store(r, reinterpret_cast<u32x4*>(to + e));
 }
 
 constexpr int RUN_MAX = 8;
@@ -335,7 +332,7 @@ __global__ void __launch_bounds__(MOVE_THREADS)
     const int lane = threadIdx.x & 63, i = min(i0 + lane, n - 1);
     const Pair mine = plan[i];  // lane k has pair k of the run
     const int on = lane < i1 - i0 && mine.on && mine.from >= 0 && mine.from < t.npages ? mine.rows : 0;
-    u32x4 r[QUADS];
+    u32x4 r = {};
     int held = -1, held_rows = 0;
     for (int k = 0; k < i1 - i0; k++) {
         const int rows = __builtin_amdgcn_readlane(on, k), from = __builtin_amdgcn_readlane(mine.from, k);
@@ -353,9 +350,10 @@ __global__ void __launch_bounds__(MOVE_THREADS)
     kv_free_kernel(const Cs1PageTable t, const int32_t* __restrict__ seqs) {
     const int i = blockIdx.x, s = listed_seq(seqs, i, t.nseq);
     if (s < 0) return;
+    const int len = t.lens[s];
     if (named_before(seqs, i, s)) return;
     int32_t* const row = t.table + (size_t)s * t.max_pages;
-    const int held = min(pages_of(max(t.lens[s], 0), t.page), t.max_pages);
+    const int held = min(pages_of(max(len, 0), t.page), t.max_pages);
     for (int j = threadIdx.x; j < held; j += MOVE_THREADS) {
         const int p = row[j];
         if (p >= 0 && p < t.npages) atomicSub(&t.refs[p], 1);
@@ -437,7 +435,7 @@ __global__ void __launch_bounds__(MOVE_THREADS)
     for (uint32_t it = block; it < pages * npools; it += blocks) {
         const uint32_t pool = it / max(pages, 1u), left = it - pool * pages;
         const uint32_t k = left / chunks, chunk = left - k * chunks;
-        u32x4 r[QUADS];
+        u32x4 r = {};
         load_chunk(r, pools.p[pool] + from[k] * page_bytes, chunk, page_bytes, true);
         store_chunk(r, pools.p[pool] + to[k] * page_bytes, chunk, page_bytes);
     }
@@ -459,7 +457,7 @@ __global__ void __launch_bounds__(MOVE_THREADS)
                                 (j < i0 + k && other == __builtin_amdgcn_readlane(d, k)))))
                 out |= 1u << k;
     }
-    u32x4 r[QUADS];
+    u32x4 r = {};
     int held = -1;
     for (int k = 0; k < count; k++) {
         const int from = __builtin_amdgcn_readlane(s, k), to = __builtin_amdgcn_readlane(d, k);
@@ -607,10 +605,10 @@ extern "C" int cs1_kv_compact(const Cs1PageTable* pages, void* const* pools, int
     do {
         Pools some = {};
         const int k = some_pools(pools, npools, first, some), tables = first == 0 ? pages->nseq : 0;
-        // a block for each chunk that may move, as far as that is 128 a CU (blocks that go on to a second chunk wait
-        // for the first one's stores to be taken: 326 us with 8 a CU, in a pool of 1400 pages of 128 KiB with 700
-        // held in 16 pools)
-        const size_t most = (size_t)(pages->npages / 2) * k * (page_bytes / CHUNK + 1), cap = (size_t)128 * cus;
+        // a block for each chunk that may move, as far as that is 512 a CU (blocks that go on to a second chunk wait
+        // for the first one's stores to be taken: 268 us so, 284 with 128 and 326 with 8, in a pool of 1400 pages of
+        // 128 KiB with 700 held in 16 pools; 299 with 2048, when half of them find nothing to do)
+        const size_t most = (size_t)(pages->npages / 2) * k * (page_bytes / CHUNK + 1), cap = (size_t)512 * cus;
         const unsigned movers = (unsigned)(most < cap ? most + 1 : cap);
         kv_compact_kernel<<<tables + movers, MOVE_THREADS, 0, st>>>(*pages, ws, some, k, npools > 0 ? page_bytes : 0,
                                                                     tables);
