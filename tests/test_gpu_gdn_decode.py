@@ -207,3 +207,30 @@ def test_the_same_bits_every_time_and_in_a_graph():
     reset()
     g.launch(stream())
     s.check()
+
+
+def test_offsets_past_32_bits():
+    """Sequences whose states lie behind 4 GiB."""
+    say("gdn step: states of 4.4 GB")
+    rng = np.random.default_rng(17)
+    H, HK, many = 48, 16, 1400
+    c = Step(rng, [2, 0, 1], [9, 1, 700], H, HK)
+    want, S, ring2, tol, stol = c.want()
+    c.upload()
+    at = np.array([many - 1, 3, many - 30])  # where sequences 0, 1, 2 are
+    lens = np.zeros(many, np.int32)
+    lens[at] = c.lens
+    size, rsize = H * D * D * 4, 4 * c.conv * 2
+    state, ring = empty(many * size), empty(many * rsize)
+    for i, s in enumerate(at):
+        hip.upload(state, c.state[i], stream(), offset=int(s) * size)
+        hip.upload(ring, c.ring[i], stream(), offset=int(s) * rsize)
+    c.bufs.update(state=state, ring=ring, lens=dev(lens), seqs=ints(at[c.seqs]))
+    c.lens = lens
+    c.launch()
+    out = get_bf16(c.out, c.n_out).reshape(3, H, D)
+    R.close(R.f64(out), want, tol, "out")
+    for i, s in enumerate(at):
+        got = get(state, np.float32, H * D * D, int(s) * size).reshape(H, D, D)
+        R.close(got.astype(np.float64), S[i], stol[i], f"state {i}")
+        np.testing.assert_array_equal(get_bf16(ring, 4 * c.conv, int(s) * rsize).reshape(4, c.conv), ring2[i])

@@ -244,6 +244,49 @@ def test_forks_in_runs():
     c.compact()
 
 
+def test_pages_in_a_graph():
+    """Free, fork, reserve, write, compact and copy recorded once and replayed for other lists, with eager calls between."""
+    say("the page calls in a graph")
+    rng = np.random.default_rng(21)
+    c = Cache(Table(12, 6, 60, 16), rng, 2, 64)
+    assert c.reserve([0, 1, 2], np.array([0, 40, 56, 80], np.int32)) == 0
+    gone, src, dst, new = (ints([-1] * 4) for _ in range(4))
+    k, v = R.bf16(rng, 4, 64), R.bf16(rng, 4, 64)
+    kb, vb, st, api = dev(k), dev(v), stream().handle, hip.api()
+    entries = [R.bf16(rng, 12, 24)]
+    ebufs = pool_buffers(entries)
+    status, eptrs = [ints([77]) for _ in range(3)], pointers(ebufs)
+
+    def record():
+        hip.check(api.cs1_kv_free(c.d.ref, gone.at(0), 4, st), "free")
+        hip.check(api.cs1_kv_fork(c.d.ref, src.at(0), dst.at(0), 4, c.ptrs, 2, 128, c.ws.at(0), status[0].at(0), st), "fork")
+        hip.check(api.cs1_kv_copy(eptrs, 1, 48, 12, src.at(0), dst.at(0), 4, st), "copy")
+        hip.check(api.cs1_kv_reserve(c.d.ref, new.at(0), None, 4, status[1].at(0), st), "reserve")
+        hip.check(api.cs1_kv_write(c.d.ref, new.at(0), None, 4, kb.at(0), 64, vb.at(0), 64, c.bufs[0].at(0), c.bufs[1].at(0), 8, 8, st), "write")
+        hip.check(api.cs1_kv_compact(c.d.ref, c.ptrs, 2, 128, c.ws.at(0), status[2].at(0), st), "compact")
+
+    g = hip.Graph(stream(), record)
+    c.check("recorded")  # and nothing has run
+    lists = [([-1, -1, -1, -1], [0, 0, 2, 1], [3, 4, 5, 6], [0, 3, 4, 5]), ([1, 4, 1, 12], [3, 3, 0, -1], [1, 4, 7, 8], [1, 3, 7, 1]),
+             ([0, 2, 3, 5], [7, 1, 6, 6], [8, 9, 10, 10], [10, 9, 8, -1]), ([9, 9, 9, 9], [8, 8, 8, 8], [0, 2, 3, 5], [5, 0, 2, 3])]
+    for one in lists:
+        for buf, x in zip((gone, src, dst, new), one):
+            hip.upload(buf, np.array(x, np.int32), stream())
+        g.launch(stream())
+        t = c.t
+        t.free(one[0])
+        want = [t.fork(one[1], one[2], c.pools)]
+        for s, d in list(t.pairs(one[1], one[2], 12)):
+            entries[0][d] = entries[0][s]
+        want.append(t.reserve(one[3]))
+        t.write(one[3], None, k, v, c.pools[0], c.pools[1])
+        want.append(t.compact(c.pools))
+        assert [int(get(s, np.int32, 1)[0]) for s in status] == want
+        c.check("replayed")
+        np.testing.assert_array_equal(read_pool(ebufs[0], entries[0]), entries[0])
+        assert c.reserve([6]) == 0  # an eager call between
+
+
 def test_offsets_past_32_bits():
     """The last page of a pool of 5 GiB receives rows, is forked and moves to the front."""
     say("a pool of 5 GiB")
