@@ -254,12 +254,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
         const int u_end = sh.to;
         int u = sh.from + wave;
 
-        __syncthreads();  // the segment before is done with LDS
+        // Q and the table are asked for together, and are there before any key is asked for: a wait for Q alone would
+        // be one for all of them (2000 sequences of up to 100 keys: 218 us so, 250 with one after the other)
         u32x4* const qf = reinterpret_cast<u32x4*>(lds);
-        for (int c = wave; c < C; c += WAVES) {
-            u32x4 q = {0, 0, 0, 0};
-            if (col < rows) q = *reinterpret_cast<const u32x4*>(a.q + out0 + col * DH + c * 32 + grp * 8);
-            qf[c * 64 + lane] = q;
+        u32x4 qs[C / WAVES];
+#pragma unroll
+        for (int i = 0; i < C / WAVES; i++) {
+            qs[i] = u32x4{0, 0, 0, 0};
+            if (col < rows)
+                qs[i] = *reinterpret_cast<const u32x4*>(a.q + out0 + col * DH + (wave + i * WAVES) * 32 + grp * 8);
         }
         f32x4 acc[H][8];
 #pragma unroll
@@ -331,6 +334,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
                             u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, v_lane + h * 256, i * row_b, 0));
             }
         };
+        if (u < u_end) {
+            look_up(u);
+            next = 0;
+        }
+        __syncthreads();  // the segment before is done with LDS
+#pragma unroll
+        for (int i = 0; i < C / WAVES; i++) qf[(wave + i * WAVES) * 64 + lane] = qs[i];
         if (u < u_end) {
             load_k(u);
             load_v();

@@ -56,9 +56,10 @@ __global__ void __launch_bounds__(THREADS, 8) gdn_decode_kernel(const Step t) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int group = t.H / t.HK, hk = h / group;
     bf16* const out = t.out + ((size_t)row * t.H + h) * DK;
+    const int early = early_entry(t.seqs, row);
     const int s = __builtin_amdgcn_readfirstlane(listed_seq(t.seqs, row, t.nseq));
     const int p = __builtin_amdgcn_readfirstlane(s < 0 ? -1 : max(t.lens[s], 0) - 1);
-    if (p < 0 || named_before(t.seqs, row, s)) {  // a padding row
+    if (p < 0 || named_before(t.seqs, row, s, early)) {  // a padding row
         if (tid < DK) out[tid] = 0;
         return;
     }

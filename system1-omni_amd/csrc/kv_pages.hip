@@ -69,10 +69,13 @@ __device__ __forceinline__ int entry_of(const int* off, int n, int k) {
 
 // Whether pages p .. p + 3 are free, as four bits.
 __device__ __forceinline__ uint32_t free_pages(const int32_t* __restrict__ refs, int npages, int p) {
+    int count[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) count[e] = refs[min(p + e, npages - 1)];
     uint32_t bits = 0;
 #pragma unroll
     for (int e = 0; e < 4; e++)
-        if (p + e < npages && refs[p + e] == 0) bits |= 1u << e;
+        bits |= (uint32_t)((p + e < npages) & (count[e] == 0)) << e;
     return bits;
 }
 
@@ -101,6 +104,8 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     __shared__ int work[MAX_LISTED];  // first entry that names a sequence, then the offsets off_i
     __shared__ int red[PLAN_WAVES];
     const int tid = threadIdx.x;
+    asm volatile("" ::"s"(t.table), "s"(t.lens), "s"(t.refs), "s"(t.nseq), "s"(t.max_pages), "s"(t.npages), "s"(t.page),
+                 "s"(seqs), "s"(cu.n), "s"(n), "s"(status));
     const uint32_t bits = free_pages(t.refs, t.npages, 4 * tid);
     const int per = PER == 1 ? 1 : (n + PLAN_THREADS - 1) / PLAN_THREADS, i0 = tid * per;
     int seq[PER], len[PER];
@@ -172,6 +177,11 @@ __global__ void __launch_bounds__(MOVE_THREADS)
                     const bf16* __restrict__ k, int ldk, const bf16* __restrict__ v, int ldv, char* kp, char* vp,
                     int width) {
     const int lane = threadIdx.x & 63, r = __builtin_amdgcn_readfirstlane(blockIdx.x * ROWS_BLOCK + (threadIdx.x >> 6));
+    // all arguments at once, here and in the other kernels: where they are asked for one by one, as they are used, each
+    // is a wait (64 forks and a token each in 16 layers take 104 us so, 93 with this)
+    asm volatile("" ::"s"(t.table), "s"(t.lens), "s"(t.nseq), "s"(t.max_pages), "s"(t.npages), "s"(t.page), "s"(seqs),
+                 "s"(cu.n), "s"(cu.at[0]), "s"(first), "s"(rows), "s"(k), "s"(ldk), "s"(v), "s"(ldv), "s"(kp), "s"(vp),
+                 "s"(width));
     if (r >= rows) return;
     const size_t row = cu.n ? (size_t)cu.at[0] + r : (size_t)r;
     const int packs = width / 8;
@@ -191,12 +201,11 @@ __global__ void __launch_bounds__(MOVE_THREADS)
         back = cu.at[i + 1] - cu.at[0] - r;
         i += first;
     }
+    const int early = early_entry(seqs, i);
     const int s = __builtin_amdgcn_readfirstlane(listed_seq(seqs, i, t.nseq));
     if (s < 0) return;
-    const int len = t.lens[s];
-    const bool again = named_before(seqs, i, s);  // (both on their way together)
-    const int pos = __builtin_amdgcn_readfirstlane(len) - back;
-    if (again || pos < 0 || pos / t.page >= t.max_pages) return;
+    const int pos = __builtin_amdgcn_readfirstlane(t.lens[s]) - back;
+    if (pos < 0 || pos / t.page >= t.max_pages || named_before(seqs, i, s, early)) return;
     const int pg = __builtin_amdgcn_readfirstlane(t.table[(size_t)s * t.max_pages + pos / t.page]);
     if (pg < 0 || pg >= t.npages) return;
     const size_t to = ((size_t)pg * t.page + pos % t.page) * packs;
@@ -226,6 +235,8 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     __shared__ int work[MAX_LISTED];
     __shared__ int red[PLAN_WAVES];
     const int tid = threadIdx.x;
+    asm volatile("" ::"s"(t.table), "s"(t.lens), "s"(t.refs), "s"(t.nseq), "s"(t.max_pages), "s"(t.npages), "s"(t.page),
+                 "s"(src), "s"(dst), "s"(n), "s"(plan), "s"(status));
     const uint32_t bits = free_pages(t.refs, t.npages, 4 * tid);
     const int per = PER == 1 ? 1 : (n + PLAN_THREADS - 1) / PLAN_THREADS, i0 = tid * per;
     int from[PER], to[PER];
@@ -310,6 +321,8 @@ int run_of(size_t chunks, int pools, int n) {
 __global__ void __launch_bounds__(MOVE_THREADS)
     kv_fork_kernel(const Cs1PageTable t, const int32_t* __restrict__ src, const int32_t* __restrict__ dst,
                    const Pair* __restrict__ plan, const Pools pools, size_t row_bytes, int tables, int n, int run) {
+    asm volatile("" ::"s"(t.table), "s"(t.lens), "s"(t.refs), "s"(t.max_pages), "s"(t.npages), "s"(t.page), "s"(src),
+                 "s"(dst), "s"(plan), "s"(row_bytes), "s"(tables), "s"(n), "s"(run));
     const int pool = (int)blockIdx.y - tables, i0 = blockIdx.z * run, i1 = min(n, i0 + run);
     if (pool < 0) {
         for (int i = i0 + blockIdx.x; i < i1; i += gridDim.x) {
@@ -348,10 +361,12 @@ __global__ void __launch_bounds__(MOVE_THREADS)
 
 __global__ void __launch_bounds__(MOVE_THREADS)
     kv_free_kernel(const Cs1PageTable t, const int32_t* __restrict__ seqs) {
-    const int i = blockIdx.x, s = listed_seq(seqs, i, t.nseq);
+    asm volatile("" ::"s"(t.table), "s"(t.lens), "s"(t.refs), "s"(t.nseq), "s"(t.max_pages), "s"(t.npages), "s"(t.page),
+                 "s"(seqs));
+    const int i = blockIdx.x, early = early_entry(seqs, i), s = listed_seq(seqs, i, t.nseq);
     if (s < 0) return;
     const int len = t.lens[s];
-    if (named_before(seqs, i, s)) return;
+    if (named_before(seqs, i, s, early)) return;
     int32_t* const row = t.table + (size_t)s * t.max_pages;
     const int held = min(pages_of(max(len, 0), t.page), t.max_pages);
     for (int j = threadIdx.x; j < held; j += MOVE_THREADS) {
@@ -445,8 +460,9 @@ __global__ void __launch_bounds__(MOVE_THREADS)
 __global__ void __launch_bounds__(MOVE_THREADS)
     kv_copy_kernel(const Pools pools, size_t bytes, int entries, const int32_t* __restrict__ src,
                    const int32_t* __restrict__ dst, int n, int run) {
-    const int i0 = blockIdx.z * run, count = min(n - i0, run), lane = threadIdx.x & 63;
     char* const pool = pools.p[blockIdx.y];
+    asm volatile("" ::"s"(pool), "s"(bytes), "s"(entries), "s"(src), "s"(dst), "s"(n), "s"(run));
+    const int i0 = blockIdx.z * run, count = min(n - i0, run), lane = threadIdx.x & 63;
     // each wave for itself: lane k has pair k of the run, and all of them are held against 64 destinations at a time
     const int s = lane < count ? src[i0 + lane] : -1, d = lane < count ? dst[i0 + lane] : -1;
     uint32_t out = 0;

@@ -20,11 +20,16 @@ __device__ __forceinline__ int listed_seq(const int32_t* __restrict__ seqs, int 
     return s >= 0 && s < nseq ? s : -1;
 }
 
-// Whether an entry before i names the same sequence, asked by a whole wave for itself.
-__device__ __forceinline__ bool named_before(const int32_t* __restrict__ seqs, int i, int s) {
-    bool hit = false;
+// Whether an entry before i names the same sequence, asked by a whole wave for itself; early: the lane's of the first 64
+// entries, asked for when the kernel begins.
+__device__ __forceinline__ int early_entry(const int32_t* __restrict__ seqs, int i) {
+    const int j = threadIdx.x & 63;
+    return seqs && j < i ? seqs[j] : -1;
+}
+__device__ __forceinline__ bool named_before(const int32_t* __restrict__ seqs, int i, int s, int early) {
+    bool hit = early == s;
     if (seqs)
-        for (int j = threadIdx.x & 63; j < i; j += 64) hit |= seqs[j] == s;
+        for (int j = 64 + (threadIdx.x & 63); j < i; j += 64) hit |= seqs[j] == s;
     return __any(hit);
 }
 
