@@ -39,7 +39,6 @@ namespace {
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 static_assert(WAVES == 4, "the waves' maxima and the rows' sums are joined by name");
 constexpr int UNIT = 32, ROWS = 16;
-constexpr int ALONE = 8;              // units of a sequence that is one chunk whatever the chunks' size
 constexpr int GROUP = 64, BATCH = 16;  // parts that one block joins, and how many of them are on their way at once
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float LEAST = 0x1p-126f;  // bfloat16's smallest normal value
@@ -74,9 +73,12 @@ __device__ __forceinline__ Row row_of(const Args& a, int r) {
 __device__ __forceinline__ int units_of(int n) { return n / UNIT + (n % UNIT != 0); }
 
 // Chunks of a row's work for one kv head and tile, of a.unit units each.  A row without keys has one: its zeros are
-// written. The first a.pad chunks stand for the time that a block needs to begin with it, and have no keys.
+// written. The first a.pad chunks stand for the time that a block needs to begin with it, and have no keys.  Up to 4
+// units of 2, and 12 of 4, are one chunk, which is not cut: one sequence of 300 keys (16/4 heads of 128) takes 8.5 us
+// so and 9.8 in parts, one of 500 (of 256) in one 14.9 and in parts 12.2; with 8 of 2, 300 sequences of up to 400 keys
+// take 80 us in place of 66, the work being shared out worse.
 __device__ __forceinline__ int chunks_of(const Args& a, int n) {
-    return a.pad + (n <= ALONE * UNIT ? 1 : (units_of(n) + a.unit - 1) / (uint32_t)a.unit);
+    return a.pad + (n <= 4 * UNIT * (a.unit - 1) ? 1 : (units_of(n) + a.unit - 1) / (uint32_t)a.unit);
 }
 
 // Sum over this lane and those below: within rows of 16 lanes, then each row's last lane to the next row (into rows
@@ -231,9 +233,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
     for (int r0 = THREADS; r0 < a.B; r0 += THREADS) total += look_at(r0);
     total = __builtin_amdgcn_readfirstlane(total * heads);
     // With heads of 128 two blocks fit on a CU (and are launched for many sequences): where these are short, on
-    // average under 256 keys, a block's time is that of beginning and ending each, and two at once hide it.  300
-    // sequences of up to 40 keys take 23.4 us so and 32.1 with one, 128 of up to 1000 52.6 and 45.5 (16/4 heads).
-    const uint32_t inverse = a.halve && total >= 8 * a.B * heads ? 2 * a.blocks_inverse : a.blocks_inverse;
+    // average under 10 chunks (384 keys), a block's time is that of beginning and ending each, and two at once hide it.
+    // 200 sequences of 260 to 384 keys take 35.3 us so and 39.0 with one, of 200 to 800 53.4 and 48.5 (16/4 heads).
+    const uint32_t inverse = a.halve && total >= 10 * a.B * heads ? 2 * a.blocks_inverse : a.blocks_inverse;
     const int each = __umulhi(total - 1, inverse) + 1;  // (one more than need be where the inverse's rounding shows)
     const int begin = (int)blockIdx.x * each, end = min(total, begin + each);
     // (the rows go on from one segment to the next: r0 the 64 that are searched, which begin at chunk `before`)
