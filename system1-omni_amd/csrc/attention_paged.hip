@@ -56,9 +56,12 @@ struct Args {
     float *lse, *part, *ml;
     int *count, *count2;
     const int32_t *table, *lens, *seqs;
-    int nseq, max_pages, npages, page, B, Hq, Hk, G, tiles, blocks, halve, unit, pad;
+    int nseq, max_pages, npages, page, B, Hq, Hk, G, tiles, blocks, halve, unit, pad_alone;
     uint32_t page_inverse, blocks_inverse;  // 2^32 over page / 16, rounded down, and over blocks, rounded up
     float scale_log2;
+
+    __device__ __forceinline__ int pad() const { return pad_alone & 255; }
+    __device__ __forceinline__ int alone() const { return pad_alone >> 8; }
 };
 
 // Row r's sequence (of its keys: none for padding).
@@ -73,12 +76,9 @@ __device__ __forceinline__ Row row_of(const Args& a, int r) {
 __device__ __forceinline__ int units_of(int n) { return n / UNIT + (n % UNIT != 0); }
 
 // Chunks of a row's work for one kv head and tile, of a.unit units each.  A row without keys has one: its zeros are
-// written. The first a.pad chunks stand for the time that a block needs to begin with it, and have no keys.  Up to 4
-// units of 2, and 12 of 4, are one chunk, which is not cut: one sequence of 300 keys (16/4 heads of 128) takes 8.5 us
-// so and 9.8 in parts, one of 500 (of 256) in one 14.9 and in parts 12.2; with 8 of 2, 300 sequences of up to 400 keys
-// take 80 us in place of 66, the work being shared out worse.
+// written. The first a.pad() chunks stand for the time that a block needs to begin with it, and have no keys.
 __device__ __forceinline__ int chunks_of(const Args& a, int n) {
-    return a.pad + (n <= 4 * UNIT * (a.unit - 1) ? 1 : (units_of(n) + a.unit - 1) / (uint32_t)a.unit);
+    return a.pad() + (n <= a.alone() * UNIT ? 1 : (units_of(n) + a.unit - 1) / (uint32_t)a.unit);
 }
 
 // Sum over this lane and those below: within rows of 16 lanes, then each row's last lane to the next row (into rows
@@ -151,7 +151,7 @@ __device__ __forceinline__ bool segment_at(const Args& a, const Rows& rows, int 
             s.head++;
         }
     s.next = min(whole + chunks, end);
-    const int keys = whole + a.pad, begin = max(pos, keys);
+    const int keys = whole + a.pad(), begin = max(pos, keys);
     if (begin >= end) return true;
     s.from = (begin - keys) * a.unit;
     s.to = whole + chunks <= end ? units_of(s.n) : (end - keys) * a.unit;
@@ -635,10 +635,14 @@ extern "C" int cs1_attention_paged(void* paged, const void* q, const void* kp, c
     a.blocks = a.halve ? p->blocks : p->cus;
     // Where blocks have several sequences, the chunks are small and beginning one counts as much as 8 units of its
     // keys (about 7 us): 43 sequences of up to 4096, 16/4 heads of 256, take 71 us so, 91 if it counts as nothing.
-    // One sequence alone is better cut into whole chunks of 4.
-    const bool many = pairs * 16 >= a.blocks;
-    a.unit = many ? 2 : 4;
-    a.pad = many ? 4 : 0;
+    // A few alone are better cut into whole chunks of 4.  Short sequences are one chunk, which is not cut, and joined
+    // by no one; the fewer sequences, the longer they may be without the work being shared out badly: one of 300 keys
+    // (heads of 128) takes 8.4 us with 12 units and 9.8 with 8, 64 of 100 to 200 (256) 12.4 with 8 and 20.0 with 4, 40 of
+    // up to 1000 22.4 and 25.6 with 12, 300 of up to 400 66 with 4 and 80 with 8.
+    const bool several = pairs * 16 >= a.blocks, many = pairs > p->cus;
+    a.unit = several ? 2 : 4;
+    const int pad = many ? 4 : several ? 3 : 0, alone = many ? 4 : several ? 8 : 12;
+    a.pad_alone = alone << 8 | pad;
     a.page_inverse = (uint32_t)std::min<uint64_t>(0xffffffffu, (uint64_t{1} << 32) / (a.page / 16));
     a.blocks_inverse = (uint32_t)(((uint64_t{1} << 32) + a.blocks - 1) / a.blocks);
     a.scale_log2 = scale * LOG2E;
