@@ -24,8 +24,8 @@
 // probabilities are formed, its V while the next scores are.
 //
 // P goes to the product in two bfloat16 parts (hi cut off, lo the rounded rest: p to 2^-15): the matrix cores wait
-// for memory here, and the second product leaves the rounding of out the only one that counts.  lo is never zero
-// (LEAST), so that an infinite v gives the infinity that it should and not inf + 0 inf.
+// for memory here, and the second product leaves the rounding of out the only one that counts.  Where p is not zero
+// lo is not either (LEAST), so that an infinite v gives the infinity that it should and not inf + 0 inf.
 #include <algorithm>
 #include <new>
 #include <type_traits>
@@ -63,6 +63,10 @@ struct Args {
     __device__ __forceinline__ int pad() const { return pad_alone & 255; }
     __device__ __forceinline__ int alone() const { return pad_alone >> 8; }
 };
+
+// What a part of p leaves of it, at least LEAST unless p is zero: the median, since p is zero or no less than LEAST.  (A
+// zero must stay one: LEAST times a value of bfloat16's largest size is 4.)
+__device__ __forceinline__ float rest(float p, float part) { return __builtin_amdgcn_fmed3f(p - part, p, LEAST); }
 
 // Row r's sequence (of its keys: none for padding).
 struct Row {
@@ -387,7 +391,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
                 const float p1 = __builtin_amdgcn_exp2f(sc[2 * i + 1] - base);
                 l += p0 + p1;
                 ph[i] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302);
-                pl[i] = pack2(fmaxf(p0 - lo_f32(ph[i]), LEAST), fmaxf(p1 - hi_f32(ph[i]), LEAST));
+                pl[i] = pack2(rest(p0, lo_f32(ph[i])), rest(p1, hi_f32(ph[i])));
             }
 #pragma unroll
             for (int h = 0; h < H; h++) {

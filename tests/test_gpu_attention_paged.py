@@ -140,6 +140,25 @@ def test_a_token_of_infinities_is_its_own_rows_matter(handle):
     assert np.isnan(out[2, 2:4]).all() and np.isfinite(out[2, :2]).all() and np.isfinite(out[2, 4:]).all()
 
 
+@pytest.mark.parametrize("dh", [128, 256])
+def test_a_key_without_weight_adds_nothing(handle, dh):
+    """Values of bfloat16's largest size under keys whose weight is far below float32's range."""
+    say(f"paged attention: the largest values without weight, Dh={dh}")
+    rng = np.random.default_rng(15)
+    t = R.scattered(rng, 2, [40, 700], 16)
+    c = Call(handle, rng, t, range(2), 8, 4, dh)
+    c.q[:], c.kp[:] = 0, 0
+    c.q[..., 0] = R.O.f32_to_bf16(np.full(c.q[..., 0].size, 128.0, np.float32)).reshape(c.q[..., 0].shape)
+    low = R.O.f32_to_bf16(np.array([-64.0], np.float32))[0]  # scores of 0 but for these: -512 and less
+    for s, j in ((0, 5), (0, 39), (1, 0), (1, 321), (1, 699)):
+        at = t.table[s, j // 16], j % 16
+        c.kp[at][:, 0] = low
+        c.vp[at] = np.where(rng.random((4, dh)) < 0.5, 0x7f7f, 0xff7f)
+    c.upload()
+    c.launch()
+    c.check()
+
+
 @pytest.mark.parametrize("std", [8.0, 40.0])
 def test_large_scores(handle, std):
     """Scores of hundreds to tens of thousands: the maximum moves by far more than a float's exponent holds."""
