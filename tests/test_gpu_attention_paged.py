@@ -159,6 +159,40 @@ def test_a_key_without_weight_adds_nothing(handle, dh):
     c.check()
 
 
+def test_weights_keep_all_their_bits(handle):
+    """Three keys whose values cancel to 2^-18 of their size: what a weight loses below float32's last bits shows.
+
+    Scores 0, S and 0 with one product each, exact up to the exponential's argument (two roundings of |S log2 e| < 1.5)
+    and the exponential (one step): the weight of S is off by 4 E32.  Three products of three parts each are summed: 8
+    sums, a step of the largest term at most, 16 E32.  The terms are of the size of the middle one, below 2."""
+    say("paged attention: weights to the last bit")
+    rng = np.random.default_rng(16)
+    hk, dh = 4, 256
+    t = R.scattered(rng, 1, [3], 16)
+    c = Call(handle, rng, t, [0], hk, hk, dh, gate=False)
+    c.q[:], c.kp[:] = 0, 0
+    c.q[..., 0] = 0x4180  # 16, so that the score is the key's value
+    grid = R.f64(np.arange(0xbe80, 0xbf80, dtype=np.uint16))  # -1/4 to -1
+    w = np.exp(grid).astype(np.float32)
+    rest = w - R.f64((w.view(np.uint32) >> 16).astype(np.uint16))
+    lost = np.abs(rest - R.f64(R.O.f32_to_bf16(rest.astype(np.float32)).reshape(-1))) / w  # in two parts
+    S = grid[np.argsort(lost)[-hk:]]
+    bf = lambda x: R.O.f32_to_bf16(np.asarray(x, np.float32).reshape(-1)).reshape(np.shape(x))  # noqa: E731
+    page = t.table[0, 0]
+    c.kp[page, 1, :, 0] = bf(S)
+    p = np.exp(S)[:, None]
+    v1 = bf(rng.uniform(1, 2, (hk, dh)))
+    v0 = bf(-p * R.f64(v1))
+    v2 = bf(-(p * R.f64(v1) + R.f64(v0)))
+    c.vp[page, 0], c.vp[page, 1], c.vp[page, 2] = v0, v1, v2
+    want = (p * R.f64(v1) + R.f64(v0) + R.f64(v2)) / (p + 2)
+    assert np.abs(want).max() < 2.0 ** -16
+    c.upload()
+    c.launch()
+    out, _ = c.results()
+    R.close(R.f64(out)[0], want, 20 * R.E32 * 2 / (p + 2) + 1.01 * R.E16 * np.abs(want), "out")
+
+
 @pytest.mark.parametrize("std", [8.0, 40.0])
 def test_large_scores(handle, std):
     """Scores of hundreds to tens of thousands: the maximum moves by far more than a float's exponent holds."""
