@@ -260,8 +260,8 @@ int cs1_gdn_prefill_gated_varlen(const void* q, const void* k, const void* v, co
 /* The page table, on the device; the struct itself is read during the call.  Sequence s holds
  * lens[s] tokens, token j in slot j % page of page table[s * max_pages + j / page]; refs[p] counts
  * the sequences that hold page p (0: free).  A program starts with table filled with -1 and
- * lens and refs with 0.  Limits: nseq <= 8192, page a multiple of 16, max_pages * page < 2^31.
- * One layer's K pages and V pages are two buffers ("pools") of [npages, page, Hk, Dh], all layers
+ * lens and refs with 0.  Limits: nseq <= 8192, npages <= 2^30, page a multiple of 16, max_pages *
+ * page < 2^31. One layer's K pages and V pages are two buffers ("pools") of [npages, page, Hk, Dh], all layers
  * under the one table, on 16 bytes.  Only the calls below change the three arrays.  A page number
  * outside [0, npages) in a row of the table is never followed: its tokens are neither read nor
  * written. */

@@ -6,10 +6,13 @@
 namespace q35 {
 
 constexpr int MAX_LISTED = 8192;  // sequences of a table, rows of a list (kv_pages.hip keeps one int each in LDS)
+// A scan's step past the last page is an int, and so is the last of compaction's entries (half as many again).
+constexpr int MAX_PAGES = 1 << 30;
 
 inline bool table_ok(const Cs1PageTable* t) {
     return t && all_set({t->table, t->lens, t->refs}) && t->nseq > 0 && t->nseq <= MAX_LISTED && t->max_pages > 0 &&
-           t->npages > 0 && t->page >= 16 && t->page % 16 == 0 && (int64_t)t->max_pages * t->page < (int64_t{1} << 31);
+           t->npages > 0 && t->npages <= MAX_PAGES && t->page >= 16 && t->page % 16 == 0 &&
+           (int64_t)t->max_pages * t->page < (int64_t{1} << 31);
 }
 
 inline bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -128,3 +128,20 @@ def test_gdn_decode(api):
         assert call(**{name: N}) == INVALID, name
     assert call(state=A + 4) == INVALID and call(w=A + 2) == INVALID and call(out=A + 4) == INVALID
     assert call(B=0, x=N, out=N) == 0
+
+
+@pytest.mark.parametrize("npages", [(1 << 30) + 1, 2 ** 31 - 4096, 2 ** 31 - 1])
+def test_more_pages_than_are_counted_in_32_bits(api, npages):
+    """The scans over the counts step past the last page, and compaction's plan has half as many entries again behind it."""
+    t = table(npages=npages)
+    assert api.cs1_kv_reserve(t, N, N, 0, A, N) == INVALID
+    assert api.cs1_kv_write(t, N, N, 0, N, 512, N, 512, N, N, 4, 128, N) == INVALID
+    assert api.cs1_kv_fork(t, N, N, 0, N, 0, 16, N, A, N) == INVALID
+    assert api.cs1_kv_free(t, N, 0, N) == INVALID
+    assert api.cs1_kv_compact(t, N, 0, 16, A, A, N) == INVALID
+    assert api.cs1_attention_paged(A, N, N, N, t, N, N, N, N, 0, 16, 4, 128, 1.0, N) == INVALID
+
+
+def test_as_many_pages_as_are_counted(api):
+    assert api.cs1_kv_write(table(npages=1 << 30), N, N, 0, N, 512, N, 512, N, N, 4, 128, N) == 0
+    assert api.cs1_kv_free(table(npages=1 << 30), N, 0, N) == 0
