@@ -317,6 +317,32 @@ def test_many_rows_and_large_pages(handle, lens, hq, hk, dh, page):
     c.check()
 
 
+@pytest.mark.parametrize("lens,hq,hk", [
+    ([300 + i * 37 % 601 for i in range(130)], 16, 4),              # 13.8 chunks a sequence, few of them cut
+    ([300 + i * 37 % 601 for i in range(129)] + [30000], 16, 4),     # one over many blocks' stretches, with a join
+    ([384] * 128, 16, 4),                                            # ten chunks each: the first that is halved
+    ([384] * 127 + [320], 16, 4),                                    # one less: the last that is not
+    ([0, 1500, 129, 128, 4096] * 26, 16, 4),                         # empty ones and whole ones among cut ones
+    ([500 + 3 * i for i in range(64)], 32, 8),
+    ([450] * 255 + [9000], 32, 1),                                   # two tiles of a kv head
+    ([1000] * 9 + [8000], 64, 64),                                   # one q head each
+], ids=["130", "129+30000", "at", "below", "mixed", "64x8", "tiles", "64 heads"])
+def test_half_the_blocks_with_twice_the_stretch(handle, lens, hq, hk):
+    """Heads of 128 and at least twice as many (sequence, kv head, tile) as CUs: half of the blocks do the work, if that is ten
+    chunks or more a sequence on average."""
+    say(f"paged attention, stretches for half the blocks: {len(lens)} sequences up to {max(lens)}, heads {hq}/{hk}")
+    rng = np.random.default_rng(len(lens) + hk)
+    t = R.scattered(rng, len(lens), lens, 48)
+    c = Call(handle, rng, t, rng.permutation(len(lens)), hq, hk, 128)
+    c.upload()
+    c.launch()
+    c.check()
+    first = c.results()
+    c.launch()
+    for a, b in zip(c.results(), first):
+        np.testing.assert_array_equal(a, b)
+
+
 def test_offsets_past_32_bits(handle):
     """Keys and values behind 4 GiB of a pool."""
     say("paged attention: pools of 5 GiB")
