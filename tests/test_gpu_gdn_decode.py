@@ -134,6 +134,20 @@ def test_many_rows():
     s.check()
 
 
+def test_repeats_far_into_a_list():
+    """Sequences that rows past the 64th name, named again: zeros there, and one block a head has the state."""
+    say("gdn decode: repeats past the first 64 rows")
+    rng = np.random.default_rng(18)
+    seqs = rng.permutation(320)[:300]
+    again = [130, 192, 260, 296, 297, 298, 299]
+    seqs[again] = seqs[[129, 64, 65, 64, 127, 128, 200]]
+    s = Step(rng, seqs, rng.integers(1, 9, 320), 2, 1)
+    s.upload()
+    s.launch()
+    s.check()
+    assert (s.results()[0][again] == 0).all()
+
+
 def test_steps_follow_the_prefill():
     """Twenty tokens one at a time from what a prefill leaves, against a prefill of all of them."""
     say("gdn decode after a prefill")
