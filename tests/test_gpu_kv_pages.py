@@ -244,6 +244,89 @@ def test_forks_in_runs():
     c.compact()
 
 
+@pytest.mark.parametrize("width", [1024, 1032, 1536, 2048, 8200])
+def test_wide_rows(width):
+    """Rows around and past the 128 packs that a wave holds at once, single tokens and prompts."""
+    say(f"write rows of {width}")
+    rng = np.random.default_rng(width)
+    t = R.scattered(rng, 7, [5, 33, 0, 16, 48, 1, 17], 16)
+    c = Cache(t, rng, 2, width)
+    c.write([6, 1, -1, 3, 2, 0, 6], None, rng)
+    c.write([4, 0, 7, 6, 1], np.array([0, 20, 25, 30, 31, 64], np.int32), rng, pad=(16, 0))
+
+
+def test_prompts_of_more_sequences_than_a_launch_takes():
+    """150 entries of host offsets, in launches of 64: empty ones, padding and repeats on both sides of their borders."""
+    say("write 150 ragged entries")
+    rng = np.random.default_rng(22)
+    lens = rng.integers(1, 40, 140)
+    t = R.scattered(rng, 140, lens.tolist(), 16)
+    c = Cache(t, rng, 2, 72)
+    seqs = rng.permutation(140)[:130].tolist() + [-1] * 20
+    seqs = np.array(seqs)[rng.permutation(150)]
+    seqs[63], seqs[64], seqs[65] = seqs[3], 140, seqs[64]
+    seqs[127], seqs[128], seqs[149] = seqs[70], -7, seqs[66]
+    rows = rng.integers(0, 12, 150)
+    rows[[0, 62, 64, 126, 129, 148]] = 0
+    rows[[63, 65, 127, 128, 149]] = 5
+    cu = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+    c.write(seqs, cu, rng)
+    rows[:64] = 0  # a first launch without rows
+    rows[64:] = 3
+    c.write(seqs, np.concatenate([[0], np.cumsum(rows)]).astype(np.int32), rng, pad=(8, 16))
+    c.write(seqs, np.concatenate([[0], np.cumsum(rng.integers(0, 60, 150))]).astype(np.int32), rng)
+
+
+def test_repeats_far_into_a_list():
+    """Sequences that entries past the 64th name, named again: the first has them, and their pages are given back once."""
+    say("repeats past the first 64 entries")
+    rng = np.random.default_rng(23)
+    t = R.scattered(rng, 400, rng.integers(1, 40, 400).tolist(), 16)
+    c = Cache(t, rng, 2, 8)
+    seqs = rng.permutation(400)[:300]
+    seqs[[130, 192, 260, 296, 297, 298, 299]] = seqs[[129, 64, 65, 64, 127, 128, 200]]
+    c.write(seqs, None, rng)
+    c.write(seqs, np.arange(301, dtype=np.int32) * 2, rng)
+    c.free(seqs)
+    assert (c.t.refs >= 0).all()
+    src = rng.permutation(np.flatnonzero(c.t.lens > 0))[:90]
+    dst = np.flatnonzero(c.t.lens == 0)[:90]
+    dst[[80, 89]] = dst[[64, 70]]
+    assert c.fork(src, dst) == 0
+    c.free(np.concatenate([seqs, dst, dst[::-1], src]))
+
+
+def test_two_tables_on_two_streams():
+    """Calls on different tables run at the same time."""
+    say("two tables on two streams")
+    rng = np.random.default_rng(24)
+    api, other = hip.api(), hip.Stream()
+    sides = []
+    for st, page in ((stream(), 16), (other, 48)):
+        c = Cache(R.scattered(rng, 40, rng.integers(1, 90, 20).tolist(), page, max_pages=9, spare=150), rng, 2, 128)
+        src, dst = rng.integers(0, 20, 20), np.arange(20, 40)
+        k, v = R.bf16(rng, 20, 128), R.bf16(rng, 20, 128)
+        sides.append((c, st, src, dst, k, v, [ints(src), ints(dst), dev(k), dev(v)], [ints([9]) for _ in range(3)]))
+    stream().sync()
+    for c, st, src, dst, k, v, (a, b, kb, vb), status in sides:
+        hip.check(api.cs1_kv_fork(c.d.ref, a.at(0), b.at(0), 20, c.ptrs, 2, 256, c.ws.at(0), status[0].at(0), st.handle), "fork")
+        hip.check(api.cs1_kv_reserve(c.d.ref, b.at(0), None, 20, status[1].at(0), st.handle), "reserve")
+        hip.check(api.cs1_kv_write(c.d.ref, b.at(0), None, 20, kb.at(0), 128, vb.at(0), 128, c.bufs[0].at(0), c.bufs[1].at(0), 1,
+                                   128, st.handle), "write")
+        hip.check(api.cs1_kv_free(c.d.ref, a.at(0), 20, st.handle), "free")
+        hip.check(api.cs1_kv_compact(c.d.ref, c.ptrs, 2, 256, c.ws.at(0), status[2].at(0), st.handle), "compact")
+    other.sync()
+    stream().sync()
+    for c, _, src, dst, k, v, _, status in sides:
+        want = [c.t.fork(src, dst, c.pools), c.t.reserve(dst)]
+        c.t.write(dst, None, k, v, c.pools[0], c.pools[1])
+        c.t.free(src)
+        want.append(c.t.compact(c.pools))
+        assert [int(get(s, np.int32, 1)[0]) for s in status] == want
+        c.check("both")
+    other.destroy()
+
+
 def test_pages_in_a_graph():
     """Free, fork, reserve, write, compact and copy recorded once and replayed for other lists, with eager calls between."""
     say("the page calls in a graph")
