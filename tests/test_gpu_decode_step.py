@@ -153,3 +153,129 @@ def test_prompt_fork_and_tokens_in_a_graph():
     d.check()
     assert (t.refs > 0).sum() == R.cdiv(prompt, PAGE)
     api.cs1_attention_paged_destroy(handle)
+
+
+def test_ragged_sequences_step_by_step():
+    """Sequences of five lengths in one batch, each row with the rotary rows of its own position.  The room for a step is
+    reserved before its graph is replayed and the status read, since a step without room must not run.  Every step is held
+    against float64 on what the device held before it, within float32's bounds."""
+    say("decode: ragged positions, reserve in front of the graph")
+    api, s = hip.api(), stream()
+    st = s.handle
+    rng = np.random.default_rng(1)
+    prompts, steps = {3: 75, 0: 1, 5: 16, 1: 130, 4: 33}, 6
+    rows = [4, -1, 0, 5, NSEQ, 3, 1]
+    B, scale = len(rows), DH ** -0.5
+    ald = 2 * HQ * DH + 2 * HK * DH
+    conv = (2 * GK + GH) * D
+    gld = conv + GH * D + 2 * GH
+    longest = max(prompts.values()) + steps
+    arow = {c: R.bf16(rng, n + steps, ald) for c, n in prompts.items()}
+    grow = {c: R.bf16(rng, n + steps, gld) for c, n in prompts.items()}
+    qw, kw = R.bf16(rng, DH, std=0.1), R.bf16(rng, DH, std=0.1)
+    ang = np.arange(longest)[:, None] / 1e7 ** (np.arange(HALF) / HALF)
+    cos, sin = (R.O.f32_to_bf16(f(ang).astype(np.float32)).reshape(longest, HALF) for f in (np.cos, np.sin))
+    cw, gw = R.bf16(rng, conv, 4, std=0.3), R.O.f32_to_bf16((1 + 0.1 * rng.standard_normal(D)).astype(np.float32))
+    al = R.O.f32_to_bf16(np.log(1 + 15 * rng.random(GH)).astype(np.float32))
+    dt = R.O.f32_to_bf16(rng.uniform(-6, -2, GH).astype(np.float32))
+    W = {k: dev(v) for k, v in dict(qw=qw, kw=kw, cw=cw, gw=gw, al=al, dt=dt).items()}
+    v_at = 2 * (2 * HQ * DH + HK * DH)
+
+    def prep_call(x, n, cb, sb, q, g, k):
+        hip.check(api.cs1_attn_prep(x.at(0), x.at(4 * HQ * DH), ald, W["qw"].at(0), W["kw"].at(0), cb.at(0), sb.at(0), q.at(0),
+                                    g.at(0), k.at(0), n, HQ, HK, DH, HALF, EPS, st), "prep")
+
+    t = Table(NSEQ, 12, 40, PAGE)
+    d = DeviceTable(t)
+    host = [np.full((t.npages, PAGE, HK * DH), 0x7fc0, np.uint16) for _ in range(2)]
+    pools = [dev(x) for x in host]
+    state, ring = np.full((NSEQ, GH, D, D), np.nan, np.float32), np.full((NSEQ, 4, conv), 0x7fc0, np.uint16)
+    states, rings = dev(state), dev(ring)
+    status = ints([9])
+    qs, gs, ks = {}, {}, {}
+
+    def reserved():
+        s.sync()
+        return int(get(status, np.int32, 1)[0])
+
+    # the prompts: their keys and values into pages, their states and last rows into slots
+    for c, n in prompts.items():
+        x, cb, sb = dev(arow[c]), dev(cos[:n + steps]), dev(sin[:n + steps])
+        m = n + steps
+        q, g, k = empty(m * HQ * DH * 2), empty(m * HQ * DH * 2), empty(m * HK * DH * 2)
+        prep_call(x, m, cb, sb, q, g, k)
+        qs[c], gs[c] = (get_bf16(b, m * HQ * DH).reshape(m, HQ, DH) for b in (q, g))
+        ks[c] = get_bf16(k, m * HK * DH).reshape(m, HK * DH)
+        one, cu = ints([c]), np.array([0, n], np.int32)
+        hip.check(api.cs1_kv_reserve(d.ref, one.at(0), cu.ctypes.data, 1, status.at(0), st), "reserve")
+        assert reserved() == t.reserve([c], cu) == 0
+        hip.check(api.cs1_kv_write(d.ref, one.at(0), cu.ctypes.data, 1, k.at(0), HK * DH, x.at(v_at), ald, pools[0].at(0),
+                                   pools[1].at(0), HK, DH, st), "write")
+        t.write([c], cu, ks[c][:n], arow[c][:n, v_at // 2:v_at // 2 + HK * DH], *host)
+        gx = dev(grow[c][:n])
+        gq, gk, gv, o = (empty(n * w * D * 2) for w in (GK, GK, GH, GH))
+        ws = empty(api.cs1_gdn_workspace_floats(n, GH) * 4)
+        zb = 2 * (conv + GH * D)
+        hip.check(api.cs1_gdn_conv(gx.at(0), gld, W["cw"].at(0), gq.at(0), gk.at(0), gv.at(0), n, GK * D, GH * D, st), "conv")
+        hip.check(api.cs1_gdn_prefill_gated_x(gq.at(0), gk.at(0), gv.at(0), gx.at(zb), gx.at(zb + 2 * GH), gld, W["al"].at(0),
+                                              W["dt"].at(0), o.at(0), ws.at(0), n, GH, GK, D ** -0.5, None,
+                                              states.at(c * GH * D * D * 4), st), "prefill")
+        for i in range(max(0, n - 4), n):  # on the device, from the projection's rows
+            hip.check(api.cs1_copy_dd(rings.at((c * 4 + i % 4) * conv * 2), gx.at(i * gld * 2), conv * 2, st), "ring")
+        s.sync()
+    d.check()
+
+    seqs, handle = ints(rows), api.cs1_attention_paged_create()
+    ax, gx = dev(np.zeros((B, ald), np.uint16)), dev(np.zeros((B, gld), np.uint16))
+    ac, asn = dev(np.zeros((B, HALF), np.uint16)), dev(np.zeros((B, HALF), np.uint16))
+    q, g, k = empty(B * HQ * DH * 2), empty(B * HQ * DH * 2), empty(B * HK * DH * 2)
+    out, gout = empty(B * HQ * DH * 2), empty(B * GH * D * 2)
+    lse = empty(HQ * B * 4)
+
+    def step():
+        prep_call(ax, B, ac, asn, q, g, k)
+        hip.check(api.cs1_kv_write(d.ref, seqs.at(0), None, B, k.at(0), HK * DH, ax.at(v_at), ald, pools[0].at(0),
+                                   pools[1].at(0), HK, DH, st), "write")
+        hip.check(api.cs1_attention_paged(handle, q.at(0), pools[0].at(0), pools[1].at(0), d.ref, seqs.at(0), g.at(0), out.at(0),
+                                          lse.at(0), B, HQ, HK, DH, scale, st), "attention")
+        zb = 2 * (conv + GH * D)
+        hip.check(api.cs1_gdn_decode(gx.at(0), gld, W["cw"].at(0), gx.at(2 * conv), gx.at(zb), gx.at(zb + 2 * GH), W["al"].at(0),
+                                     W["dt"].at(0), W["gw"].at(0), EPS, rings.at(0), states.at(0), seqs.at(0), d.lens.at(0), NSEQ,
+                                     gout.at(0), B, GH, GK, D ** -0.5, st), "gdn")
+
+    graph = hip.Graph(s, step)
+    for i in range(steps):
+        if i == 3:  # one ends, and its row is padding from here on
+            gone = ints([5])
+            hip.check(api.cs1_kv_free(d.ref, gone.at(0), 1, st), "free")
+            t.free([5])
+            rows[rows.index(5)] = -1
+            hip.upload(seqs, np.array(rows, np.int32), s)
+        live = [(r, c, prompts[c] + i) for r, c in enumerate(rows) if 0 <= c < NSEQ]  # row, sequence, position
+        a, x = np.full((B, ald), 0x7fc0, np.uint16), np.full((B, gld), 0x7fc0, np.uint16)
+        cs, sn = np.zeros((B, HALF), np.uint16), np.zeros((B, HALF), np.uint16)
+        for r, c, p in live:
+            a[r], x[r], cs[r], sn[r] = arow[c][p], grow[c][p], cos[p], sin[p]
+        for buf, arr in ((ax, a), (gx, x), (ac, cs), (asn, sn)):
+            hip.upload(buf, arr, s)
+        hip.check(api.cs1_kv_reserve(d.ref, seqs.at(0), None, B, status.at(0), st), "reserve")
+        assert reserved() == t.reserve(rows) == 0
+        state = get(states, np.float32, state.size).reshape(state.shape)
+        ring = get_bf16(rings, ring.size).reshape(ring.shape)
+        graph.launch(s)
+        qi, gi, ki = np.zeros((B, HQ, DH), np.uint16), np.zeros((B, HQ, DH), np.uint16), np.zeros((B, HK * DH), np.uint16)
+        for r, c, p in live:
+            assert int(t.lens[c]) == p + 1
+            qi[r], gi[r], ki[r] = qs[c][p], gs[c][p], ks[c][p]
+        t.write(rows, None, ki, a[:, v_at // 2:v_at // 2 + HK * DH], *host)
+        for buf, arr in zip(pools, host):
+            np.testing.assert_array_equal(R.read_pool(buf, arr), arr)
+        want, wl, tol, ltol = R.attention(t, rows, qi, *host, gi, HK, scale)
+        R.close(R.f64(get_bf16(out, B * HQ * DH).reshape(B, HQ, DH)), want, tol, f"step {i} attention")
+        R.close(get(lse, np.float32, HQ * B).reshape(HQ, B).astype(np.float64), wl, ltol, f"step {i} lse")
+        want, S, ring2, tol, stol = R.gdn_step(x, cw, al, dt, gw, ring, state, rows, t.lens, GH, GK, D ** -0.5, EPS)
+        R.close(R.f64(get_bf16(gout, B * GH * D).reshape(B, GH, D)), want, tol, f"step {i} delta rule")
+        R.close(get(states, np.float32, state.size).reshape(state.shape).astype(np.float64), S, stol, f"step {i} state")
+        np.testing.assert_array_equal(get_bf16(rings, ring.size).reshape(ring.shape), ring2)
+    d.check()
+    api.cs1_attention_paged_destroy(handle)
