@@ -261,9 +261,9 @@ int cs1_gdn_prefill_gated_varlen(const void* q, const void* k, const void* v, co
  * lens[s] tokens, token j in slot j % page of page table[s * max_pages + j / page]; refs[p] counts
  * the sequences that hold page p (0: free).  A program starts with table filled with -1 and
  * lens and refs with 0.  Limits: nseq <= 8192, npages <= 2^30, page a multiple of 16, max_pages *
- * page < 2^31. One layer's K pages and V pages are two buffers ("pools") of [npages, page, Hk, Dh], all layers
- * under the one table, on 16 bytes.  Only the calls below change the three arrays.  A page number
- * outside [0, npages) in a row of the table is never followed: its tokens are neither read nor
+ * page < 2^31.  One layer's K pages and V pages are two buffers ("pools") of [npages, page, Hk, Dh], all
+ * layers under the one table, on 16 bytes.  Only the calls below change the three arrays.  A page
+ * number outside [0, npages) in a row of the table is never followed: its tokens are neither read nor
  * written. */
 typedef struct Cs1PageTable {
     int32_t* table; /* [nseq, max_pages] */
@@ -286,6 +286,8 @@ int cs1_kv_reserve(const Cs1PageTable* pages, const int32_t* seqs, const int32_t
  * ldv), Hk * Dh values each, goes to the pages kp and vp.  cu_seqlens null: row i is the last
  * token (lens[s] - 1) of listed sequence i; else (HOST, cu_seqlens[n] <= 2^23) rows [cu_seqlens[i],
  * cu_seqlens[i + 1]) are its last tokens in order.  Rows of padding or before position 0 are left out.
+ * A row goes to its page whether or not forks hold that page too (cs1_kv_fork shares whole pages), and is then
+ * theirs as well: after a cs1_kv_reserve that found no room, a token's row would replace the last shared one.
  * Hk * Dh and both row lengths are multiples of 8, k and v on 16 bytes, n <= 8192; Hk * Dh <= 2^24. */
 int cs1_kv_write(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n, const void* k,
                  int ldk, const void* v, int ldv, void* kp, void* vp, int Hk, int Dh, void* stream);
@@ -321,7 +323,8 @@ int cs1_kv_compact(const Cs1PageTable* pages, void* const* pools, int npools, si
 int cs1_kv_copy(void* const* pools, int npools, size_t entry_bytes, int entries, const int32_t* src, const int32_t* dst,
                 int n, void* stream);
 
-/* Attention of one new token per row over the pages (after cs1_kv_write): q, gate (null: none) and
+/* Attention of one new token per row over the pages (after cs1_kv_write), which no other call reads: several new
+ * tokens of a sequence, behind its first prompt, go through it one after another.  q, gate (null: none) and
  * out [B, Hq, Dh], Dh 128 or 256; row r's q head h sees the lens[s] keys of sequence s = seqs[r] through kv
  * head h / (Hq / Hk).  lse [Hq, B] float32 (null: not written) as in cs1_attention_ex.  Unlike there the
  * output is rounded once, after the gate.  A padding row, or one of an empty sequence, gets zeros and an
@@ -343,7 +346,9 @@ int cs1_attention_paged(void* paged, const void* q, const void* kp, const void* 
  * ring bf16 [nseq, 4, (2 HK + H) * 128], the pre-conv row of position i in ring row i % 4; both are
  * updated in place.  At p = 0 the state and at p < 3 the rows before position 0 count as zero, whatever
  * is stored.  All in float32, rounded once in out [B, H, 128].  Padding rows (also lens[s] < 1) get
- * zeros.  lens is a page table's, or any device array of nseq lengths; B <= 8192, state on 16 bytes. */
+ * zeros.  lens is a page table's, or any device array of nseq lengths; B <= 8192, B * H <= 2^22, state on 16
+ * bytes.  After a prefill of n tokens, ring row i % 4 holds the projection's q | k | v of position i for
+ * n - 3 <= i < n: two cs1_copy2d at most. */
 int cs1_gdn_decode(const void* qkv, int ld, const void* w, const void* z, const void* b, const void* a,
                    const void* A_log, const void* dt_bias, const void* norm_w, float eps, void* ring, float* state,
                    const int32_t* seqs, const int32_t* lens, int nseq, void* out, int B, int H, int HK, float scale,

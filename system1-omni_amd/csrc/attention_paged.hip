@@ -643,12 +643,13 @@ extern "C" int cs1_attention_paged(void* paged, const void* q, const void* kp, c
     a.tiles = (a.G + ROWS - 1) / ROWS;
     a.halve = Dh == 128 && pairs >= p->blocks;  // the blocks, if the sequences are long
     a.blocks = a.halve ? p->blocks : p->cus;
-    // Where blocks have several sequences, the chunks are small and beginning one counts as much as 8 units of its
-    // keys (about 7 us): 43 sequences of up to 4096, 16/4 heads of 256, take 71 us so, 91 if it counts as nothing.
-    // A few alone are better cut into whole chunks of 4.  Short sequences are one chunk, which is not cut, and joined
-    // by no one; the fewer sequences, the longer they may be without the work being shared out badly: one of 300 keys
-    // (heads of 128) takes 8.4 us with 12 units and 9.8 with 8, 64 of 100 to 200 (256) 12.4 with 8 and 20.0 with 4, 40 of
-    // up to 1000 22.4 and 25.6 with 12, 300 of up to 400 66 with 4 and 80 with 8.
+    // A pair is a row with a kv head and tile.  From a pair to 16 blocks on the chunks are small, and beginning a pair
+    // counts as work: as much as 6 units of keys up to a pair a CU, as 8 beyond (about 7 us). 43 sequences of up to
+    // 4096, 16/4 heads of 256, take 71 us so, 91 if it counts as nothing.  Fewer pairs are better cut into whole chunks of 4.
+    // Short sequences are one chunk, which is not cut, and joined by no one; the fewer pairs, the longer they may
+    // be without the work being shared out badly: one of 300 keys (heads of 128) takes 8.4 us with 12 units and 9.8 with 8,
+    // 64 of 100 to 200 (256) 12.4 with 8 and 20.0 with 4, 40 of up to 1000 22.4 and 25.6 with 12, 300 of up to 400 66 with 4
+    // and 80 with 8.
     const bool several = pairs * 16 >= a.blocks, many = pairs > p->cus;
     a.unit = several ? 2 : 4;
     const int pad = many ? 4 : several ? 3 : 0, alone = many ? 4 : several ? 8 : 12;
