@@ -354,6 +354,61 @@ int cs1_gdn_decode(const void* qkv, int ld, const void* w, const void* z, const 
                    const int32_t* seqs, const int32_t* lens, int nseq, void* out, int B, int H, int HK, float scale,
                    void* stream);
 
+/* ---- additions: several new tokens of a sequence at once (no counterpart in the reference) ----
+ *
+ * The second turn of a chat, drafted tokens that are verified, a long prompt in parts, candidates behind a
+ * prompt of any length, and any mixture of them with single tokens.  The new tokens of listed
+ * sequence i are rows [cu_seqlens[i], cu_seqlens[i + 1]) of a packed batch, and the last tokens that the sequence
+ * holds; cu_seqlens is here a DEVICE array of n + 1 offsets that do not fall, from 0 on (n <= 8192), so that one
+ * captured graph serves other batches.  `rows` is the number of rows of the batch's buffers: those behind
+ * cu_seqlens[n] are no one's.  A step is cs1_kv_extend and cs1_kv_rows once, then per attention layer
+ * cs1_attn_prep_paged and cs1_attention_paged_varlen; cs1_token_logprobs reads its logits, and cs1_kv_trim
+ * takes tokens back that were not accepted. */
+
+/* cs1_kv_reserve for such a batch: sequence i grows by cu_seqlens[i + 1] - cu_seqlens[i] tokens (a negative number
+ * counts as 0).  Pages, status and what follows from it are as there. */
+int cs1_kv_extend(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n, int32_t* status,
+                  void* stream);
+
+/* Where each row is: pos[r] is its token's position in its sequence and slot[r] its place in the pools, page * pages->page
+ * + position % pages->page (int32 [rows] each).  Both are -1 for rows of padding entries (also those of a sequence that
+ * an earlier entry names), before position 0 or behind cu_seqlens[n]; slot also where the page's number is out of range.
+ * npages * page < 2^31. */
+int cs1_kv_rows(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n, int rows, int32_t* pos,
+                int32_t* slot, void* stream);
+
+/* Take the last drop[i] tokens (device, n <= 8192; less than 0 counts as 0, more than there are as all) off the listed
+ * sequences; whole pages behind the new end are released.  A sequence that would end inside a page which others hold
+ * too stays as it is (its next token would be written over theirs); *status receives the number of these. */
+int cs1_kv_trim(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* drop, int n, int32_t* status,
+                void* stream);
+
+/* Rotary positions.  The first `dims` dims of a head (a multiple of 16, 0: none) turn in pairs: (i, i + dims / 2), or
+ * with `interleaved` (2i, 2i + 1).  Pair i turns by freqs[i] (DEVICE float64 [dims / 2], on 8 bytes) radians a
+ * position, and grows by `magnitude`; angles are formed in float64, so that far positions lose nothing. */
+typedef struct Cs1Rotary {
+    const double* freqs;
+    int dims, interleaved;
+    float magnitude;
+} Cs1Rotary;
+
+/* freqs (HOST, dims / 2 values; dims even, > 0) for a rotary base, f_i = base^(-2i / dims), and a context `factor` (>= 1)
+ * times the `original` one: with r_i = original f_i / (2 pi) turns over it, f_i / factor up to r_i = slow,
+ * f_i from r_i = fast on, and in between ((1 - y) / factor + y) f_i with y = (r_i - slow) / (fast - slow) (Peng et al.,
+ * "YaRN", arXiv 2309.00071, section 3.2; slow = 1 and fast = 32 there, with magnitude 0.1 ln(factor) + 1).  fast =
+ * INFINITY slows all pairs alike (positions divided by the factor).  0 <= slow <= fast.  Needs no device. */
+int cs1_rotary_freqs(double* freqs, int dims, double base, double factor, double original, double slow, double fast);
+
+/* Attention inputs of T rows, straight into the pages: row t of qg is Hq heads of Dh (q) or with `gate` of 2 Dh (q | gate),
+ * row t of kr and v Hk heads of Dh, all in rows of ld.  q and k are normed (x rsqrt(mean x^2 + eps) (1 + w); qw, kw [Dh],
+ * null: not) and turned for position pos[t]; q and gate are written as [T, Hq, Dh], k and v to slot[t] of the pools
+ * kp and vp (pos and slot: cs1_kv_rows; of `pages` only npages and page are read).  In float32, each value rounded
+ * once.  Rows with pos[t] < 0 are left out, and k and v of rows whose slot is not in [0, npages * page).  Slots differ
+ * from row to row.  Dh 128 or 256; ld a multiple of 8, all tensors on 16 bytes; Hk * Dh <= 2^24. */
+int cs1_attn_prep_paged(const void* qg, const void* kr, const void* v, int ld, const void* qw, const void* kw, float eps,
+                        const Cs1Rotary* rotary, const Cs1PageTable* pages, const int32_t* pos, const int32_t* slot,
+                        void* q, void* gate, void* kp, void* vp, int T, int Hq, int Hk, int Dh, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -96,11 +96,12 @@ __device__ __forceinline__ int take_free(const int32_t* refs, int npages, int to
 }
 
 // PER: list entries a thread has at most. Lists of up to 1024 have one each, which leaves a third of the code: what
-// runs once takes its time to arrive (6.4 us with eight, 4.9 with one).
-template <int PER>
+// runs once takes its time to arrive (6.4 us with eight, 4.9 with one).  ROWS: the entries' tokens are the differences
+// of the device's offsets `rows`, and not of cu.
+template <int PER, bool ROWS>
 __global__ void __launch_bounds__(PLAN_THREADS)
-    kv_reserve_kernel(const Cs1PageTable t, const int32_t* __restrict__ seqs, const Offsets cu, int n,
-                      int32_t* status) {
+    kv_reserve_kernel(const Cs1PageTable t, const int32_t* __restrict__ seqs, const Offsets cu,
+                      const int32_t* __restrict__ rows, int n, int32_t* status) {
     __shared__ int work[MAX_LISTED];  // first entry that names a sequence, then the offsets off_i
     __shared__ int red[PLAN_WAVES];
     const int tid = threadIdx.x;
@@ -109,11 +110,16 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     const uint32_t bits = free_pages(t.refs, t.npages, 4 * tid);
     const int per = PER == 1 ? 1 : (n + PLAN_THREADS - 1) / PLAN_THREADS, i0 = tid * per;
     int seq[PER], len[PER];
+    int64_t add[PER];
 #pragma unroll
     for (int e = 0; e < PER; e++) {
-        seq[e] = e < per && i0 + e < n ? listed_seq(seqs, i0 + e, t.nseq) : -1;
+        const int i = i0 + e;
+        const bool in = e < per && i < n;
+        seq[e] = in ? listed_seq(seqs, i, t.nseq) : -1;
+        if (ROWS) add[e] = in ? max((int64_t)rows[i + 1] - rows[i], (int64_t)0) : 0;
         len[e] = seq[e] >= 0 ? max(t.lens[seq[e]], 0) : 0;
     }
+    auto grows = [&](int e) -> int64_t { return ROWS ? add[e] : cu.n ? cu.at[i0 + e + 1] - cu.at[i0 + e] : 1; };
     for (int s = tid; s < t.nseq; s += PLAN_THREADS) work[s] = n;
     __syncthreads();
 #pragma unroll
@@ -128,7 +134,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
         need[e] = 0;
         if (seq[e] >= 0 && work[seq[e]] != i) seq[e] = -1;
         if (seq[e] < 0) continue;
-        const int64_t to = (int64_t)len[e] + (cu.n ? cu.at[i + 1] - cu.at[i] : 1);
+        const int64_t to = (int64_t)len[e] + grows(e);
         if (to > (int64_t)t.max_pages * t.page)
             wide = true;
         else
@@ -164,9 +170,135 @@ __global__ void __launch_bounds__(PLAN_THREADS)
         __syncthreads();  // slot() has read the lengths
 #pragma unroll
         for (int e = 0; e < PER; e++)
-            if (seq[e] >= 0) t.lens[seq[e]] = len[e] + (cu.n ? cu.at[i0 + e + 1] - cu.at[i0 + e] : 1);
+            if (seq[e] >= 0) t.lens[seq[e]] = (int)(len[e] + grows(e));
     }
     if (tid == 0) *status = total - found;
+}
+
+// Where the rows of a packed batch are: a row a thread.  Every block makes the list's first entries for itself (n <= 8192
+// loads that a block has under way at once) and has the offsets in LDS, so that a row's chain is entry, length,
+// page, and the search between costs no memory.
+__global__ void __launch_bounds__(PLAN_THREADS)
+    kv_rows_kernel(const Cs1PageTable t, const int32_t* __restrict__ seqs, const int32_t* __restrict__ cu, int n,
+                   int rows, int32_t* __restrict__ pos, int32_t* __restrict__ slot) {
+    extern __shared__ int lists[];
+    int* const end = lists;          // [n] each entry's end
+    int* const first = lists + n;    // [nseq] the first entry that names a sequence
+    const int tid = threadIdx.x, r = blockIdx.x * PLAN_THREADS + tid;
+    asm volatile("" ::"s"(t.table), "s"(t.lens), "s"(t.nseq), "s"(t.max_pages), "s"(t.npages), "s"(t.page), "s"(seqs),
+                 "s"(cu), "s"(n), "s"(rows), "s"(pos), "s"(slot));
+    for (int s = tid; s < t.nseq; s += PLAN_THREADS) first[s] = n;
+    int seq[PER_MAX];
+#pragma unroll
+    for (int e = 0; e < PER_MAX; e++) {
+        const int i = tid + e * PLAN_THREADS;
+        seq[e] = -1;
+        if (i < n) {
+            seq[e] = listed_seq(seqs, i, t.nseq);
+            end[i] = cu[i + 1];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER_MAX; e++)
+        if (seq[e] >= 0) atomicMin(&first[seq[e]], tid + e * PLAN_THREADS);
+    __syncthreads();
+    if (r >= rows) return;
+    int lo = 0, hi = n;  // the entries that end at or before row r
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (end[mid] <= r)
+            lo = mid + 1;
+        else
+            hi = mid;
+    }
+    int p = -1, at = -1;
+    const int i = lo, s = i < n ? listed_seq(seqs, i, t.nseq) : -1;
+    // (offsets that do not rise may leave a row to an entry that begins behind it)
+    if (s >= 0 && first[s] == i && (i == 0 || end[i - 1] <= r)) {
+        const int64_t here = (int64_t)t.lens[s] - (end[i] - r);
+        if (here >= 0 && here < (int64_t)t.max_pages * t.page) {
+            p = (int)here;
+            const int pg = t.table[(size_t)s * t.max_pages + p / t.page];
+            if (pg >= 0 && pg < t.npages) at = pg * t.page + p % t.page;
+        }
+    }
+    pos[r] = p;
+    slot[r] = at;
+}
+
+// Tokens taken off the ends of sequences.  One block, since whether a page is shared is asked of all entries before any
+// count falls: the answer does not depend on which entry is first.
+template <int PER>
+__global__ void __launch_bounds__(PLAN_THREADS)
+    kv_trim_kernel(const Cs1PageTable t, const int32_t* __restrict__ seqs, const int32_t* __restrict__ drop, int n,
+                   int32_t* status) {
+    __shared__ int work[MAX_LISTED];  // first entry that names a sequence
+    __shared__ int red[PLAN_WAVES];
+    const int tid = threadIdx.x, lane = tid & 63;
+    asm volatile("" ::"s"(t.table), "s"(t.lens), "s"(t.refs), "s"(t.nseq), "s"(t.max_pages), "s"(t.npages), "s"(t.page),
+                 "s"(seqs), "s"(drop), "s"(n), "s"(status));
+    const int per = PER == 1 ? 1 : (n + PLAN_THREADS - 1) / PLAN_THREADS, i0 = tid * per;
+    int seq[PER], len[PER], to[PER];
+#pragma unroll
+    for (int e = 0; e < PER; e++) {
+        const bool in = e < per && i0 + e < n;
+        seq[e] = in ? listed_seq(seqs, i0 + e, t.nseq) : -1;
+        const int off = in ? max(drop[i0 + e], 0) : 0;
+        len[e] = seq[e] >= 0 ? max(t.lens[seq[e]], 0) : 0;
+        to[e] = max(len[e] - off, 0);
+    }
+    for (int s = tid; s < t.nseq; s += PLAN_THREADS) work[s] = n;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; e++)
+        if (seq[e] >= 0) atomicMin(&work[seq[e]], i0 + e);
+    __syncthreads();
+    int left = 0;
+#pragma unroll
+    for (int e = 0; e < PER; e++) {
+        if (seq[e] >= 0 && work[seq[e]] != i0 + e) seq[e] = -1;
+        if (seq[e] < 0 || to[e] == len[e]) {
+            seq[e] = -1;
+            continue;
+        }
+        const int last = to[e] / t.page;  // the page that is cut
+        if (to[e] % t.page == 0 || last >= t.max_pages) continue;
+        const int p = t.table[(size_t)seq[e] * t.max_pages + last];
+        if (p >= 0 && p < t.npages && t.refs[p] > 1) {
+            seq[e] = -1;
+            left++;
+        }
+    }
+    int all;
+    (void)block_scan(left, red, all);  // (its barriers stand between the counts' reads and their changes)
+    __syncthreads();
+    if (tid == 0) *status = all;
+#pragma unroll
+    for (int e = 0; e < PER; e++) {
+        int j = 0, held = 0;
+        int32_t* row = nullptr;
+        if (seq[e] >= 0) {
+            row = t.table + (size_t)seq[e] * t.max_pages;
+            j = pages_of(to[e], t.page);
+            held = min(pages_of(len[e], t.page), t.max_pages);
+            t.lens[seq[e]] = to[e];
+        }
+        auto release = [&](int32_t* entry) {
+            const int p = *entry;
+            *entry = -1;
+            if (p >= 0 && p < t.npages) atomicSub(&t.refs[p], 1);
+        };
+        // a few pages a thread, and where there are many a wave
+        if (held - j <= 4) {
+            for (; j < held; j++) release(row + j);
+        }
+        for (uint64_t many = __ballot(j < held); many; many &= many - 1) {
+            const int w = __ffsll((unsigned long long)many) - 1, to_page = __shfl(held, w, 64);
+            const int s = __shfl(seq[e], w, 64);
+            for (int k = __shfl(j, w, 64) + lane; k < to_page; k += 64) release(t.table + (size_t)s * t.max_pages + k);
+        }
+    }
 }
 
 // One wave a row.  The first of its keys and values are asked for before it is known where they go.
@@ -526,8 +658,37 @@ extern "C" int cs1_kv_reserve(const Cs1PageTable* pages, const int32_t* seqs, co
     cu.n = cu_seqlens ? n : 0;
     if (cu_seqlens)
         for (int i = 0; i <= n; i++) cu.at[i] = cu_seqlens[i];
-    const auto kernel = n <= PLAN_THREADS ? kv_reserve_kernel<1> : kv_reserve_kernel<PER_MAX>;
-    kernel<<<1, PLAN_THREADS, 0, static_cast<hipStream_t>(stream)>>>(*pages, seqs, cu, n, status);
+    const auto kernel = n <= PLAN_THREADS ? kv_reserve_kernel<1, false> : kv_reserve_kernel<PER_MAX, false>;
+    kernel<<<1, PLAN_THREADS, 0, static_cast<hipStream_t>(stream)>>>(*pages, seqs, cu, nullptr, n, status);
+    return hipGetLastError();
+}
+
+extern "C" int cs1_kv_extend(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n,
+                             int32_t* status, void* stream) {
+    if (!table_ok(pages) || n < 0 || n > MAX_LISTED || !status || (n > 0 && !cu_seqlens)) return hipErrorInvalidValue;
+    Offsets none;
+    none.n = 0;
+    const auto kernel = n <= PLAN_THREADS ? kv_reserve_kernel<1, true> : kv_reserve_kernel<PER_MAX, true>;
+    kernel<<<1, PLAN_THREADS, 0, static_cast<hipStream_t>(stream)>>>(*pages, seqs, none, cu_seqlens, n, status);
+    return hipGetLastError();
+}
+
+extern "C" int cs1_kv_rows(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n, int rows,
+                           int32_t* pos, int32_t* slot, void* stream) {
+    if (!table_ok(pages) || n < 0 || n > MAX_LISTED || rows < 0 || (int64_t)pages->npages * pages->page > INT32_MAX)
+        return hipErrorInvalidValue;
+    if (rows == 0) return hipSuccess;
+    if (!all_set({pos, slot}) || (n > 0 && !cu_seqlens)) return hipErrorInvalidValue;
+    kv_rows_kernel<<<cdiv(rows, PLAN_THREADS), PLAN_THREADS, 4 * ((size_t)n + pages->nseq),
+                     static_cast<hipStream_t>(stream)>>>(*pages, seqs, cu_seqlens, n, rows, pos, slot);
+    return hipGetLastError();
+}
+
+extern "C" int cs1_kv_trim(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* drop, int n, int32_t* status,
+                           void* stream) {
+    if (!table_ok(pages) || n < 0 || n > MAX_LISTED || !status || (n > 0 && !drop)) return hipErrorInvalidValue;
+    const auto kernel = n <= PLAN_THREADS ? kv_trim_kernel<1> : kv_trim_kernel<PER_MAX>;
+    kernel<<<1, PLAN_THREADS, 0, static_cast<hipStream_t>(stream)>>>(*pages, seqs, drop, n, status);
     return hipGetLastError();
 }
 

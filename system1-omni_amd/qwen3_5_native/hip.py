@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_float, c_int, c_size_t, c_uint32, c_void_p
+from ctypes import c_double, c_float, c_int, c_size_t, c_uint32, c_void_p
 
 import numpy as np
 
@@ -96,6 +96,11 @@ ADDITIONS = {
     "cs1_attention_paged_destroy": (None, [P]),
     "cs1_attention_paged": (_I, [P, P, P, P, P, P, P, P, P, _I, _I, _I, _I, c_float, P]),
     "cs1_gdn_decode": (_I, [P, _I, P, P, P, P, P, P, P, c_float, P, P, P, P, _I, P, _I, _I, _I, c_float, P]),
+    "cs1_kv_extend": (_I, [P, P, P, _I, P, P]),
+    "cs1_kv_rows": (_I, [P, P, P, _I, _I, P, P, P]),
+    "cs1_kv_trim": (_I, [P, P, P, _I, P, P]),
+    "cs1_rotary_freqs": (_I, [P, _I, c_double, c_double, c_double, c_double, c_double]),
+    "cs1_attn_prep_paged": (_I, [P, P, P, _I, P, P, c_float, P, P, P, P, P, P, P, P, _I, _I, _I, _I, P]),
 }
 # ... and test hooks outside the op ABI: one forces the GDN prep / scan kernel forms that the
 # bit-identity tests compare (-1: the shape-based choice), the others give the scan's form and the
@@ -118,6 +123,12 @@ class PageTable(ctypes.Structure):
 
     _fields_ = [("table", c_void_p), ("lens", c_void_p), ("refs", c_void_p), ("nseq", _I), ("max_pages", _I),
                 ("npages", _I), ("page", _I)]
+
+
+class Rotary(ctypes.Structure):
+    """Cs1Rotary: the device address of the float64 frequencies, turned dims, layout and magnitude."""
+
+    _fields_ = [("freqs", c_void_p), ("dims", _I), ("interleaved", _I), ("magnitude", c_float)]
 
 
 HIP_ERROR_INVALID_VALUE = 1
