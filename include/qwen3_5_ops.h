@@ -409,6 +409,18 @@ int cs1_attn_prep_paged(const void* qg, const void* kr, const void* v, int ld, c
                         const Cs1Rotary* rotary, const Cs1PageTable* pages, const int32_t* pos, const int32_t* slot,
                         void* q, void* gate, void* kp, void* vp, int T, int Hq, int Hk, int Dh, void* stream);
 
+/* Log-probabilities of given tokens, entropy and the best alternatives of `rows` rows of V logits (bfloat16, or
+ * float32 with is_float; rows of ld, on their own size): logprob[r] = log softmax(row)[targets[r]] (targets and logprob both or
+ * neither; 0 where the target is not in [0, V)), entropy[r] = -sum p log p in nats (null: not written), and the k <= 32 largest
+ * logits, the lowest index first among equals: top_ids and top_logprobs [rows, k], -1 and NaN behind the last of
+ * fewer.  In float32 throughout.  Logits of -inf have no weight; a row with a NaN or +inf, or of -inf only, has NaN for each
+ * value and -1 for each index.  V <= 2^28.  workspace: cs1_token_logprobs_workspace_bytes(rows, V, k) bytes on 16 (0:
+ * null will do), this call's own until it is done on the device. */
+size_t cs1_token_logprobs_workspace_bytes(int rows, int V, int k);
+int cs1_token_logprobs(const void* logits, int is_float, size_t ld, const int32_t* targets, int rows, int V, int k,
+                       float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs, void* workspace,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

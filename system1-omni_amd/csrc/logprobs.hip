@@ -1,0 +1,392 @@
+// Log-probabilities of given tokens, entropy and the best alternatives of rows of logits (cs1_token_logprobs).  With
+// m = max x, z = sum e^(x - m):
+//
+//   log p_t = (x_t - m) - log z,   H = -sum p log p = log z - sum e^(x - m) (x - m) / z,
+//
+// and the k largest logits, the lowest index first among equals.  No term of H is negative, so nothing cancels.
+//
+// Bound by the one pass over the logits.  A thread keeps a running base, sum and weighted sum of its own, and of its
+// values the largest with the load that it was in.  The alternatives need no more from that pass: the
+// k-th largest of the lanes' largest (64 lanes, each over the block's waves) is a value that k tokens reach at least, so
+// only what reaches it can be among the best, and only the threads whose largest does (about k of 512) look at
+// their loads again.  What they find, k tokens or a few more, is put in order by counting.
+//
+// A row is cut into parts where there are few rows; a second launch joins the parts in order.
+#include <math.h>
+
+#include <algorithm>
+#include <limits>
+
+#include "common.h"
+#include "paged.h"
+
+namespace q35 {
+namespace {
+
+constexpr int THREADS = 512, WAVES = THREADS / 64, LOADS = 4;
+constexpr int K_MAX = 32, PARTS_MAX = 64;
+constexpr int LIST = 1024;  // tokens that reach the threshold, kept in LDS
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// A logit with its index, larger for larger values and among equals for lower indices; 0 is below all.  (-0 is 0.)
+typedef unsigned long long Key;
+__device__ __forceinline__ Key key_of(float x, uint32_t index) {
+    const uint32_t b = __float_as_uint(x + 0.f), up = b & 0x80000000u ? ~b : b | 0x80000000u;
+    return (Key)up << 32 | (0xffffffffu - index);
+}
+__device__ __forceinline__ float value_of(Key k) {
+    const uint32_t up = (uint32_t)(k >> 32);
+    return __uint_as_float(up & 0x80000000u ? up & 0x7fffffffu : ~up);
+}
+__device__ __forceinline__ uint32_t index_of(Key k) { return 0xffffffffu - (uint32_t)k; }
+__device__ __forceinline__ Key shuffle_xor(Key k, int o) {
+    return (Key)__shfl_xor((uint32_t)(k >> 32), o, 64) << 32 | __shfl_xor((uint32_t)k, o, 64);
+}
+
+// The wave's keys in falling order, by compare and exchange in a bitonic net.
+__device__ __forceinline__ Key sorted(Key k) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int size = 2; size <= 64; size *= 2)
+#pragma unroll
+        for (int o = size / 2; o > 0; o /= 2) {
+            const Key other = shuffle_xor(k, o);
+            const bool first = (lane & o) == 0, falls = (lane & size) == 0 || size == 64;
+            k = (first == falls) == (k > other) ? k : other;
+        }
+    return k;
+}
+
+// Base m, sum of e^(x - m) and of that times x - m.  Differences and not logarithms of base 2 are kept, so that a large
+// base costs no bits.
+struct Sums {
+    float m, sum, dot, unused;
+};
+// By how much a base falls, as far as anything is left: -1e4 stands for all that leaves nothing, so that sums of values
+// near the type's lowest do not become infinities times zero.
+__device__ __forceinline__ float falls(float from, float to) { return fmaxf(from - to, -1e4f); }
+__device__ __forceinline__ Sums rebased(const Sums& a, float m) {
+    if (a.m == -INFINITY) return Sums{m, a.sum, a.dot, 0.f};  // no value yet, or none above -inf
+    const float by = falls(a.m, m), f = __builtin_amdgcn_exp2f(by * LOG2E);
+    return Sums{m, a.sum * f, (a.dot + a.sum * by) * f, 0.f};
+}
+__device__ __forceinline__ Sums merged(const Sums& a, const Sums& b) {
+    const float m = fmaxf(a.m, b.m);
+    const Sums x = rebased(a, m), y = rebased(b, m);
+    return Sums{m, x.sum + y.sum, x.dot + y.dot, 0.f};
+}
+__device__ __forceinline__ Sums wave_merged(Sums a) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        a = merged(a, Sums{__shfl_xor(a.m, o, 64), __shfl_xor(a.sum, o, 64), __shfl_xor(a.dot, o, 64), 0.f});
+    return a;
+}
+
+struct Args {
+    const void* logits;
+    const int32_t* targets;
+    float *logprob, *entropy, *top;
+    int32_t* ids;
+    Sums* sums;  // [rows, parts]
+    Key* keys;   // [rows, parts, k]
+    size_t ld;
+    int V, k, parts, each;  // each: logits a part, a multiple of 8
+};
+
+template <typename T>
+__device__ __forceinline__ float as_float(T x) {
+    if constexpr (sizeof(T) == 2)
+        return f32(x);
+    else
+        return x;
+}
+
+// A row whose sum is no positive number (a NaN or +inf among its logits, or all of them -inf) has no distribution.
+__device__ __forceinline__ bool proper(const Sums& s) { return s.sum > 0.f; }
+__device__ __forceinline__ float no_number() { return __uint_as_float(0x7fc00000); }
+
+template <typename T>
+__device__ __forceinline__ void store_row(const Args& a, int row, const Sums& s) {
+    const float log_z = log2f(s.sum) * LN2;
+    if (a.logprob) {
+        const int t = a.targets[row];
+        float lp = 0.f;
+        if (t >= 0 && t < a.V)
+            lp = proper(s) ? (as_float(static_cast<const T*>(a.logits)[(size_t)row * a.ld + t]) - s.m) - log_z
+                           : no_number();
+        a.logprob[row] = lp;
+    }
+    if (a.entropy) a.entropy[row] = proper(s) ? log_z - s.dot / s.sum : no_number();
+}
+__device__ __forceinline__ void store_top(const Args& a, int row, int i, Key k, const Sums& s) {
+    const bool ok = proper(s) && k != 0;
+    a.ids[(size_t)row * a.k + i] = ok ? (int)index_of(k) : -1;
+    a.top[(size_t)row * a.k + i] = ok ? (value_of(k) - s.m) - log2f(s.sum) * LN2 : no_number();
+}
+
+// A part of a row as loads of 16 bytes: number 0 has the logits in front of the first aligned one (fewer, or none), 1 ..
+// `whole` are full, and whole + 1 has what is left.  A thread has every THREADS-th, so its indices rise.
+template <typename T>
+struct Part {
+    static constexpr int N = 16 / sizeof(T);
+    const T* p;
+    int n, head, whole;
+
+    __device__ __forceinline__ Part(const T* p, int n) : p(p), n(n) {
+        const int off = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+        head = min(off ? N - off : 0, n);
+        whole = (n - head) / N;
+    }
+    __device__ __forceinline__ int index(int j) const { return j == 0 ? 0 : head + (j - 1) * N; }
+    __device__ __forceinline__ int count(int j) const {
+        return j == 0 ? head : j <= whole ? N : j == whole + 1 ? n - head - whole * N : 0;
+    }
+    __device__ __forceinline__ u32x4 full(int j) const {
+        return *reinterpret_cast<const u32x4*>(p + head + (size_t)(j - 1) * N);
+    }
+    static __device__ __forceinline__ float at(const u32x4& v, int e) {
+        if constexpr (sizeof(T) == 2)
+            return e & 1 ? hi_f32(v[e / 2]) : lo_f32(v[e / 2]);
+        else
+            return __uint_as_float(v[e]);
+    }
+    // f(key) for each logit of thread t's loads, shared out over a wave's lanes
+    template <typename F>
+    __device__ __forceinline__ void each_key(int t, int lane, uint32_t first, F f) const {
+        for (int j = t + lane * THREADS; j <= whole + 1; j += 64 * THREADS) {
+            if (j >= 1 && j <= whole) {
+                const u32x4 v = full(j);
+#pragma unroll
+                for (int e = 0; e < N; e++) f(key_of(at(v, e), first + index(j) + e));
+            } else {
+                for (int e = 0; e < count(j); e++) f(key_of(as_float(p[index(j) + e]), first + index(j) + e));
+            }
+        }
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS) logprobs_kernel(const Args a) {
+    constexpr int N = Part<T>::N;
+    __shared__ Sums wave_sums[WAVES];
+    __shared__ Key best_of[64], list[LIST], found;
+    __shared__ int listed, threads, who[THREADS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = blockIdx.x / (uint32_t)a.parts, part = blockIdx.x - row * a.parts;
+    const int first = part * a.each;
+    const Part<T> x(static_cast<const T*>(a.logits) + (size_t)row * a.ld + first, min(a.each, a.V - first));
+    if (tid < 64) best_of[tid] = 0;
+    if (tid == 0) listed = threads = 0;
+
+    float m = -INFINITY, sum = 0.f, dot = 0.f, best = -INFINITY;
+    int best_at = -1;  // the load that has the largest value first
+    auto rebase = [&](float top) {
+        if (top > m) {
+            const float by = falls(m, top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(by * LOG2E);
+            dot = m == -INFINITY ? 0.f : (dot + sum * by) * f;
+            sum *= f;
+            m = top;
+        }
+    };
+    auto add = [&](float v, float base) {
+        const float d = v - base, p = __builtin_amdgcn_exp2f(d * LOG2E);
+        sum += p;
+        dot += p * fmaxf(d, -1e4f);  // (what is -inf weighs nothing, and must not be multiplied by its zero)
+    };
+    auto single = [&](int j) {  // load 0 or the last one
+        for (int e = 0; e < x.count(j); e++) {
+            const float v = as_float(x.p[x.index(j) + e]);
+            rebase(v);
+            add(v, m == -INFINITY ? 0.f : m);
+            if (v > best || best_at < 0) {
+                best = fmaxf(v, -INFINITY);
+                best_at = j;
+            }
+        }
+    };
+    if (tid == 0) single(0);
+    for (int j0 = tid == 0 ? THREADS : tid; j0 <= x.whole; j0 += LOADS * THREADS) {
+        u32x4 v[LOADS];
+        constexpr uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;  // -inf
+#pragma unroll
+        for (int u = 0; u < LOADS; u++) {
+            v[u] = u32x4{none, none, none, none};
+            if (j0 + u * THREADS <= x.whole) v[u] = x.full(j0 + u * THREADS);
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < LOADS; u++) {
+            float most = x.at(v[u], 0);
+#pragma unroll
+            for (int e = 1; e < N; e++) most = fmaxf(most, x.at(v[u], e));
+            if (most > best || best_at < 0) {
+                best = fmaxf(most, -INFINITY);
+                best_at = j0 + u * THREADS;
+            }
+            top = fmaxf(top, most);
+        }
+        rebase(top);
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int u = 0; u < LOADS; u++)
+#pragma unroll
+            for (int e = 0; e < N; e++) add(x.at(v[u], e), base);
+    }
+    if (tid == (x.whole + 1) % THREADS) single(x.whole + 1);
+
+    Sums s = wave_merged(Sums{m, sum, dot, 0.f});
+    if (lane == 0) wave_sums[wave] = s;
+    __syncthreads();
+    s = wave_sums[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; w++) s = merged(s, wave_sums[w]);
+    if (tid == 0) {
+        if (a.parts == 1)
+            store_row<T>(a, row, s);
+        else
+            a.sums[blockIdx.x] = s;
+    }
+    if (a.k == 0) return;
+
+    // where the load has it is not known, so the value counts as its last logit here, and as its first below
+    if (best_at >= 0) atomicMax(&best_of[lane], key_of(best, first + x.index(best_at) + x.count(best_at) - 1));
+    __syncthreads();
+    const Key in_order = sorted(best_of[lane]);
+    const Key least = (Key)__shfl((uint32_t)(in_order >> 32), a.k - 1, 64) << 32 |
+                      (uint32_t)__shfl((uint32_t)in_order, a.k - 1, 64);
+    if (best_at >= 0 && key_of(best, first + x.index(best_at)) >= least) who[atomicAdd(&threads, 1)] = tid;
+    __syncthreads();
+    for (int i = wave; i < threads; i += WAVES)
+        x.each_key(who[i], lane, first, [&](Key k) {
+            if (k < least) return;
+            const int at = atomicAdd(&listed, 1);
+            if (at < LIST) list[at] = k;
+        });
+    __syncthreads();
+    auto store = [&](int i, Key k) {
+        if (a.parts == 1)
+            store_top(a, row, i, k, s);
+        else
+            a.keys[(size_t)blockIdx.x * a.k + i] = k;
+    };
+    if (listed <= LIST) {
+        for (int i = tid; i < max(listed, a.k); i += THREADS) {
+            if (i >= listed) {  // fewer logits than alternatives
+                store(i, 0);
+                continue;
+            }
+            const Key mine = list[i];
+            int rank = 0;
+            for (int j = 0; j < listed; j++) rank += list[j] > mine;
+            if (rank < a.k) store(rank, mine);
+        }
+        return;
+    }
+    // More than LIST reach it: a few lanes' loads have all large values.  The alternatives are looked for one by one.
+    Key before = ~(Key)0;
+    for (int i = 0; i < a.k; i++) {
+        if (tid == 0) found = 0;
+        __syncthreads();
+        Key mine = 0;
+        for (int t = wave; t < THREADS; t += WAVES)
+            x.each_key(t, lane, first, [&](Key k) {
+                if (k < before && k > mine) mine = k;
+            });
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const Key other = shuffle_xor(mine, o);
+            mine = mine > other ? mine : other;
+        }
+        if (lane == 0) atomicMax(&found, mine);
+        __syncthreads();
+        before = found;
+        if (tid == 0) store(i, before);
+        __syncthreads();
+    }
+}
+
+// A wave a row joins its parts: a lane has a part, whose alternatives are in order.
+template <typename T>
+__global__ void __launch_bounds__(64) logprobs_join_kernel(const Args a) {
+    __shared__ Key keys[PARTS_MAX * K_MAX];
+    const int row = blockIdx.x, lane = threadIdx.x;
+    Sums s = Sums{-INFINITY, 0.f, 0.f, 0.f};
+    if (lane < a.parts) s = a.sums[(size_t)row * a.parts + lane];
+    for (int i = lane; i < a.parts * a.k; i += 64) keys[i] = a.keys[(size_t)row * a.parts * a.k + i];
+    s = wave_merged(s);
+    if (lane == 0) store_row<T>(a, row, s);
+    __syncthreads();
+    Key mine = 0;  // the lane-th best
+    int next = 0;
+    for (int i = 0; i < a.k; i++) {
+        const Key head = lane < a.parts && next < a.k ? keys[lane * a.k + next] : 0;
+        Key most = head;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const Key other = shuffle_xor(most, o);
+            most = most > other ? most : other;
+        }
+        if (head == most) next++;  // (one lane's, or none is left)
+        if (lane == i) mine = most;
+    }
+    if (lane < a.k) store_top(a, row, lane, mine, s);
+}
+
+// Parts of a row: enough blocks for the chip, of at least a load a thread.
+struct Plan {
+    int parts, each;
+};
+Plan plan_of(int rows, int V) {
+    const int64_t wanted = (1024 + (int64_t)rows - 1) / rows, most = (V + 8 * THREADS - 1) / (8 * THREADS);
+    const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, most), PARTS_MAX));
+    const int each = (int)((((int64_t)V + parts - 1) / parts + 7) / 8 * 8);
+    return Plan{(int)(((int64_t)V + each - 1) / each), each};
+}
+
+constexpr int V_MAX = 1 << 28;
+
+}  // namespace
+}  // namespace q35
+
+using namespace q35;
+
+extern "C" size_t cs1_token_logprobs_workspace_bytes(int rows, int V, int k) {
+    if (rows <= 0 || V <= 0 || V > V_MAX || k < 0 || k > K_MAX) return 0;
+    const Plan p = plan_of(rows, V);
+    return p.parts == 1 ? 0 : (size_t)rows * p.parts * (sizeof(Sums) + sizeof(Key) * k);
+}
+
+extern "C" int cs1_token_logprobs(const void* logits, int is_float, size_t ld, const int32_t* targets, int rows, int V,
+                                  int k, float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs,
+                                  void* workspace, void* stream) {
+    if (rows < 0 || V <= 0 || V > V_MAX || ld < (size_t)V || k < 0 || k > K_MAX) return hipErrorInvalidValue;
+    if (rows == 0) return hipSuccess;
+    const Plan p = plan_of(rows, V);
+    if ((int64_t)rows * p.parts > INT32_MAX || !logits || (logprob != nullptr) != (targets != nullptr) ||
+        (k > 0 && !all_set({top_ids, top_logprobs})))
+        return hipErrorInvalidValue;
+    if ((reinterpret_cast<uintptr_t>(logits) & (is_float ? 3 : 1)) != 0) return hipErrorInvalidValue;
+    if (p.parts > 1 && (!workspace || !on16(workspace))) return hipErrorInvalidValue;
+    Args a;
+    a.logits = logits;
+    a.targets = targets;
+    a.logprob = logprob;
+    a.entropy = entropy;
+    a.top = top_logprobs;
+    a.ids = top_ids;
+    a.sums = static_cast<Sums*>(workspace);
+    a.keys = reinterpret_cast<Key*>(a.sums + (size_t)rows * p.parts);
+    a.ld = ld;
+    a.V = V;
+    a.k = k;
+    a.parts = p.parts;
+    a.each = p.each;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const auto kernel = is_float ? logprobs_kernel<float> : logprobs_kernel<bf16>;
+    kernel<<<rows * p.parts, THREADS, 0, st>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.parts == 1) return e;
+    const auto join = is_float ? logprobs_join_kernel<float> : logprobs_join_kernel<bf16>;
+    join<<<rows, 64, 0, st>>>(a);
+    return hipGetLastError();
+}

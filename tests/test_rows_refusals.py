@@ -101,3 +101,19 @@ def test_rotary_refusals(api):
         args = list(ok)
         args[i] = bad
         assert api.cs1_rotary_freqs(*args) == INVALID, (i, bad)
+
+
+def test_logprobs(api):
+    def call(x=A, f32=0, ld=1000, targets=A, rows=2, V=1000, k=5, lp=A, ent=A, ids=A, top=A, ws=A):
+        return api.cs1_token_logprobs(x, f32, ld, targets, rows, V, k, lp, ent, ids, top, ws, N)
+
+    assert call(rows=-1) == INVALID and call(V=0) == INVALID and call(V=(1 << 28) + 1, ld=1 << 29) == INVALID
+    assert call(ld=999) == INVALID and call(k=-1) == INVALID and call(k=33) == INVALID
+    assert call(x=N) == INVALID and call(x=A + 1) == INVALID and call(x=A + 2, f32=1) == INVALID
+    assert call(targets=N) == INVALID and call(lp=N) == INVALID  # both or neither
+    assert call(ids=N) == INVALID and call(top=N) == INVALID
+    assert call(V=100000, ld=100000, ws=N) == INVALID and call(V=100000, ld=100000, ws=A + 8) == INVALID
+    assert call(rows=0, x=N) == 0
+    size = api.cs1_token_logprobs_workspace_bytes
+    assert size(0, 1000, 5) == 0 and size(2, 0, 5) == 0 and size(2, 1000, 33) == 0 and size(2, 1000, 5) == 0
+    assert size(1, 248320, 20) > 0 and size(5000, 248320, 20) == 0
