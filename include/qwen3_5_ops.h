@@ -330,7 +330,7 @@ int cs1_kv_copy(void* const* pools, int npools, size_t entry_bytes, int entries,
  * output is rounded once, after the gate.  A padding row, or one of an empty sequence, gets zeros and an
  * lse of -inf.  q, kp, vp, gate and out on 16 bytes; Hk * Dh <= 2^24, B * Hq <= 2^22, npages * page < 2^31 and
  * B * Hk * ceil(Hq / Hk / 16) * (max_pages * page / 32 + 1) < 2^31.  The handle holds the partial
- * results of sequences that are split over the chip (16 MiB): it belongs to the device that is current
+ * results of sequences that are split over the chip (80 MiB): it belongs to the device that is current
  * when it is created (not during a capture; null if that fails) and, as a GEMM handle, serves one
  * thread and one stream at a time (graphs captured with one handle must not run at the same time). */
 void* cs1_attention_paged_create(void);
@@ -408,6 +408,18 @@ int cs1_rotary_freqs(double* freqs, int dims, double base, double factor, double
 int cs1_attn_prep_paged(const void* qg, const void* kr, const void* v, int ld, const void* qw, const void* kw, float eps,
                         const Cs1Rotary* rotary, const Cs1PageTable* pages, const int32_t* pos, const int32_t* slot,
                         void* q, void* gate, void* kp, void* vp, int T, int Hq, int Hk, int Dh, void* stream);
+
+/* Attention of such a batch's rows over the pages, which hold their keys and values already: q, gate (null: none) and
+ * out [rows, Hq, Dh]; the row at position p of its sequence sees keys 0 .. p.  max_new is the most rows that an entry has
+ * (those behind it are left out).  out and lse [Hq, rows] (float32, null: not written) as in cs1_attention_paged, but
+ * for the probabilities, which go to the second product as bfloat16.  Rows of padding entries and rows before position
+ * 0 get zeros and an lse of -inf; rows behind cu_seqlens[n] are left as they are.  A sequence may be named twice.  Keys of a page
+ * whose number is out of range are left out.  scale > 0 (1e-30 to 1e30), Hq / Hk <= 128, rows * Hq <= 2^24,
+ * Hk * Dh <= 2^24, npages * page < 2^31; q, kp, vp, gate and out on 16 bytes.  The handle is cs1_attention_paged's, with
+ * the same rules. */
+int cs1_attention_paged_varlen(void* paged, const void* q, const void* kp, const void* vp, const Cs1PageTable* pages,
+                               const int32_t* seqs, const int32_t* cu_seqlens, int n, int max_new, const void* gate,
+                               void* out, float* lse, int rows, int Hq, int Hk, int Dh, float scale, void* stream);
 
 /* Log-probabilities of given tokens, entropy and the best alternatives of `rows` rows of V logits (bfloat16, or
  * float32 with is_float; rows of ld, on their own size): logprob[r] = log softmax(row)[targets[r]] (targets and logprob both or

@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "tile32.h"
 
 namespace q35 {
 namespace {
@@ -545,19 +546,11 @@ struct Form {
 };
 // how far (log2 units) a row's maximum may exceed the exponent base before the base moves
 constexpr float RESCALE_SLACK = 8.f;
-
-// Chunk placement, conflict-free whether the LDS serves 128 or 256 bytes per cycle: 16-byte
-// chunk c of K row r sits at slot c ^ (r & 15) (8 or 16 consecutive rows read at one chunk hit
-// distinct slots); of V row r at slot c ^ f(r & 3), f = {0, 6, 12, 10}, which separates the
-// four rows of a transposing read both within 8 slots (two adjacent chunks per row, one lane
-// group) and within 16 (four chunks per row, two lane groups).
-__device__ __forceinline__ int k_slot(int r, int c) { return c ^ (r & 15); }
-__device__ __forceinline__ int v_slot(int r, int c) { return c ^ ((0xAC60 >> (4 * (r & 3))) & 15); }
-
-__device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
-                                                   0, 0);
-}
+using tile32::k_slot;
+using tile32::max_halves;
+using tile32::mfma32;
+using tile32::read_tr;
+using tile32::v_slot;
 
 // Buffer descriptor over rows [k0, min(T, k0 + BN)) of a row-major bf16 tensor (row stride
 // ld, rows of 128 elements); rows past T, and every row when !valid, read as zero.
@@ -581,18 +574,6 @@ __device__ __forceinline__ void dma(const u32x4& r, uint32_t dst, int ld, int r0
         const int row0 = r0 + 4 * n;
         dma16(r, dst + row0 * ROW, voff[is_k ? n : 0], row0 * ld * 2);
     }
-}
-
-// Maximum over the two lane halves (lanes l and l ^ 32): one v_permlane32_swap, no LDS trip.
-__device__ __forceinline__ float max_halves(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ u32x2 read_tr(const unsigned char* p) {
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                         (__attribute__((address_space(3))) s16x4*)(p)));
 }
 }  // namespace fa32
 

@@ -46,12 +46,6 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float LEAST = 0x1p-126f;  // bfloat16's smallest normal value
 constexpr float RISE = 6.f;  // in powers of two: P stays under 2^6, far from where float32 sums lose anything
 
-struct Paged {
-    int device, cus, blocks;
-    float* part;  // [2 blocks, ROWS, 256] partial sums, [2 blocks, ROWS, 2] maximum and sum
-    int* count;   // [2 blocks] parts of a group, [2 blocks] groups of a sequence that are done
-};
-
 struct Args {
     const bf16 *q, *kp, *vp, *gate;
     bf16* out;
@@ -572,7 +566,8 @@ using namespace q35;
 extern "C" void* cs1_attention_paged_create(void) {
     int device;
     const int cus = device_cus();
-    if (cus < 2 || hipGetDevice(&device) != hipSuccess || !configure<128>() || !configure<256>()) {
+    if (cus < 2 || hipGetDevice(&device) != hipSuccess || !configure<128>() || !configure<256>() ||
+        !chunk_configure()) {
         (void)hipGetLastError();
         return nullptr;
     }
@@ -582,11 +577,13 @@ extern "C" void* cs1_attention_paged_create(void) {
     p->cus = std::min(cus, GROUP * GROUP / 2);
     p->blocks = 2 * p->cus;
     const size_t floats = (size_t)2 * p->blocks * ROWS * (256 + 2), counts = (size_t)4 * p->blocks;
-    p->part = nullptr;
+    p->part = p->chunk = nullptr;
     if (hipMalloc(reinterpret_cast<void**>(&p->part), 4 * (floats + counts)) != hipSuccess ||
+        hipMalloc(reinterpret_cast<void**>(&p->chunk), chunk_bytes(p->cus)) != hipSuccess ||
         hipMemset(p->part + floats, 0, 4 * counts) != hipSuccess || hipStreamSynchronize(nullptr) != hipSuccess) {
         (void)hipGetLastError();
         if (p->part) (void)hipFree(p->part);
+        if (p->chunk) (void)hipFree(p->chunk);
         delete p;
         return nullptr;
     }
@@ -598,6 +595,7 @@ extern "C" void cs1_attention_paged_destroy(void* paged) {
     Paged* const p = static_cast<Paged*>(paged);
     if (!p) return;
     (void)hipFree(p->part);
+    (void)hipFree(p->chunk);
     delete p;
 }
 

@@ -9,6 +9,17 @@ constexpr int MAX_LISTED = 8192;  // sequences of a table, rows of a list (kv_pa
 // A scan's step past the last page is an int, and so is the last of compaction's entries (half as many again).
 constexpr int MAX_PAGES = 1 << 30;
 
+// What cs1_attention_paged_create makes: partial results of sequences that are split over the chip.
+struct Paged {
+    int device, cus, blocks;
+    float* part;   // single tokens: [2 blocks, 16, 256] partial sums, [2 blocks, 16, 2] maximum and sum
+    int* count;    // [2 blocks] parts of a group, [2 blocks] groups of a sequence that are done
+    float* chunk;  // several tokens: [2 cus, CHUNK_COLS, 256] and [2 cus, CHUNK_COLS, 2], then what a stretch cut
+};
+constexpr int CHUNK_COLS = 128;  // columns (row and q head) of an item of several tokens
+bool chunk_configure();
+size_t chunk_bytes(int cus);
+
 inline bool table_ok(const Cs1PageTable* t) {
     return t && all_set({t->table, t->lens, t->refs}) && t->nseq > 0 && t->nseq <= MAX_LISTED && t->max_pages > 0 &&
            t->npages > 0 && t->npages <= MAX_PAGES && t->page >= 16 && t->page % 16 == 0 &&

@@ -100,6 +100,7 @@ ADDITIONS = {
     "cs1_kv_rows": (_I, [P, P, P, _I, _I, P, P, P]),
     "cs1_kv_trim": (_I, [P, P, P, _I, P, P]),
     "cs1_rotary_freqs": (_I, [P, _I, c_double, c_double, c_double, c_double, c_double]),
+    "cs1_attention_paged_varlen": (_I, [P, P, P, P, P, P, P, _I, _I, P, P, P, _I, _I, _I, _I, c_float, P]),
     "cs1_token_logprobs_workspace_bytes": (_SZ, [_I, _I, _I]),
     "cs1_token_logprobs": (_I, [P, _I, _SZ, P, _I, _I, _I, P, P, P, P, P, P]),
     "cs1_attn_prep_paged": (_I, [P, P, P, _I, P, P, c_float, P, P, P, P, P, P, P, P, _I, _I, _I, _I, P]),

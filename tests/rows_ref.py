@@ -1,8 +1,8 @@
 """Plain implementations of the operations on several new tokens of a sequence, for their tests: room, positions and
-slots, tokens taken back, attention inputs with rotary positions.  Nothing here comes from the library."""
+slots, tokens taken back, attention inputs with rotary positions, attention of a batch's rows.  Nothing here comes from the library."""
 import numpy as np
 
-from decode_ref import E16, E32, cdiv
+from decode_ref import E16, E32, cdiv, f64
 
 
 def extend(t, seqs, cu):
@@ -73,3 +73,53 @@ def turned(x, w, eps, pos, freqs, dims, interleaved, magnitude):
         size = np.abs(ya) + np.abs(yb)
         tol[a] = tol[b] = size * (rel * magnitude + off + 4 * E32 * magnitude)
     return out, tol + E16 * (np.abs(out) + tol)
+
+
+def attention(t, seqs, cu, rows, max_new, q, kp, vp, gate, hk, scale):
+    """Float64 result, log-sum-exp, the bounds on the error of each, and which rows are someone's.
+
+    As decode_ref.attention, but for the probabilities, which are rounded to bfloat16 for the second product (E16 of each
+    weight there, and not in their sum)."""
+    _, hq, dh = q.shape
+    rep = hq // hk
+    out, lse = np.zeros((rows, hq, dh)), np.full((hq, rows), -np.inf)
+    tol, ltol = np.zeros((rows, hq, dh)), np.zeros((hq, rows))
+    ours = np.zeros(rows, bool)
+    for i, s in enumerate(seqs):
+        lo, hi = int(cu[i]), int(cu[i + 1])
+        L = min(hi - lo, max_new)
+        ours[lo:lo + L] = True
+        n = min(int(t.lens[s]), t.max_pages * t.page) if 0 <= s < t.nseq else 0
+        if L <= 0 or n == 0:
+            continue
+        j = np.arange(n)
+        pg = t.table[s, j // t.page]
+        there = (pg >= 0) & (pg < t.npages)
+        j = j[there]
+        if not len(j):
+            continue
+        K, V = f64(kp[pg[there], j % t.page]), f64(vp[pg[there], j % t.page])
+        sees = j[None, :] <= (n - (hi - lo) + np.arange(L))[:, None]
+        some = sees.any(1)
+        for h in range(hq):
+            k, v, x = K[:, h // rep], V[:, h // rep], f64(np.ascontiguousarray(q[lo:lo + L, h]))
+            sc = np.where(sees, (x @ k.T) * scale, -np.inf)
+            top = np.where(some, np.max(sc, 1, initial=-np.inf), 0.0)[:, None]
+            off = (dh + 2) * E32 * (np.abs(x) @ np.abs(k).T) * abs(scale) + 4 * E32 * np.abs(np.where(sees, sc, 0))
+            w = np.exp(sc - top)
+            z = w.sum(1, keepdims=True)
+            p = w / np.where(z > 0, z, 1)
+            o = p @ v
+            rel = 2 * (off + np.where(sees, off, 0).max(1, keepdims=True)) + 4 * E32 + 2 * n * E32
+            f = 1.0
+            if gate is not None:
+                f = 1 / (1 + np.exp(-f64(np.ascontiguousarray(gate[lo:lo + L, h]))))
+            mean = (p * rel).sum(1, keepdims=True)
+            err = (p * (rel + E16)) @ np.abs(v) + np.abs(o) * mean + 16 * E32 * np.abs(o)
+            out[lo:lo + L, h] = o * f
+            tol[lo:lo + L, h] = err * f + E16 * (np.abs(o * f) + err * f)
+            with np.errstate(divide="ignore"):
+                lse[h, lo:lo + L] = np.where(some, top[:, 0] + np.log(z[:, 0]), -np.inf)
+            size = np.where(some, np.abs(np.where(some, lse[h, lo:lo + L], 0)), 0)
+            ltol[h, lo:lo + L] = mean[:, 0] + 8 * E32 * (1 + size + np.log(max(n, 2)))
+    return out, lse, tol, ltol, ours

@@ -117,3 +117,21 @@ def test_logprobs(api):
     size = api.cs1_token_logprobs_workspace_bytes
     assert size(0, 1000, 5) == 0 and size(2, 0, 5) == 0 and size(2, 1000, 33) == 0 and size(2, 1000, 5) == 0
     assert size(1, 248320, 20) > 0 and size(5000, 248320, 20) == 0
+
+
+def test_attention(api):
+    def call(h=N, q=A, kp=A, vp=A, t=None, cu=A, n=1, most=4, gate=A, out=A, rows=4, hq=16, hk=4, dh=128, scale=0.1):
+        return api.cs1_attention_paged_varlen(h, q, kp, vp, t or table(), N, cu, n, most, gate, out, N, rows, hq, hk, dh, scale, N)
+
+    assert call() == INVALID  # no handle
+    # a handle is looked into last: for work that there is, on operands that are right
+    for bad in BAD_TABLES:
+        assert call(h=A, t=table(**bad)) == INVALID, bad
+    for kw in (dict(dh=64), dict(hk=0), dict(hq=0), dict(hq=15), dict(hq=516), dict(n=-1), dict(n=8193), dict(rows=-1), dict(most=-1),
+               dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(rows=(1 << 20) + 1),
+               dict(hq=1 << 18, hk=1 << 18, rows=1, dh=128), dict(t=table(npages=1 << 27))):
+        assert call(h=A, **kw) == INVALID, kw
+    for name in ("q", "kp", "vp", "out"):
+        assert call(h=A, **{name: N}) == INVALID and call(h=A, **{name: A + 8}) == INVALID, name
+    assert call(h=A, gate=A + 8) == INVALID and call(h=A, cu=N) == INVALID
+    assert call(h=A, rows=0, q=N) == 0 and call(h=A, n=0, cu=N) == 0 and call(h=A, most=0) == 0
