@@ -4,18 +4,21 @@
 //   S_i = scale q . k_i,  m = max S_i,  l = sum exp(S_i - m),  out = sigmoid(gate) (sum exp(S_i - m) v_i) / l,
 //   lse = m + log l.
 //
-// Work: an item is up to COLS columns, the q heads of one kv head at some of an entry's rows, with all keys that
+// Work: an item is up to 128 columns (heads of 256) or 256 (of 128), the q heads of one kv head at some of an entry's rows, with all keys that
 // they see: however many q heads share a kv head, they share its keys too.  All items of a launch form one line, measured in
 // keys, that is cut into equal stretches, one a block: a prompt's part on its own, drafts of a few tokens behind
 // long texts and single tokens share the chip alike, and only the device knows the lengths.  What a stretch has of an
 // item that others have parts of goes to memory, and a second launch joins the parts in order.
 //
-// A block has eight waves: four groups of 32 columns, two halves of the keys of each unit (64 keys with heads of 256, 128 with
-// heads of 128: 32 KiB of K and of V).  S^T = K Q^T and O^T += V^T P^T on the 32x32x16 MFMA: what the first leaves in a
-// lane is what the second wants, so probabilities stay in registers.  Units move from the pages into LDS without
-// registers, K two ahead and V one ahead; a wave's piece of a unit lies in one run of 16 tokens, which no page divides.
-// The halves' waves that share a SIMD take turns: one multiplies while the other has its exponentials (priority to the
-// first half).  At the end the halves are joined through LDS.
+// A block has eight waves: four groups of columns by two halves.  Of a unit of 64 keys a wave makes the scores of one half of
+// the keys, S^T = K Q^T, and then, with both halves' probabilities, one half of the dims of O^T += V^T P^T, on the
+// 32x32x16 MFMA: what the first product leaves in a lane is what the second wants, so a pair of waves exchanges only maxima
+// and the probabilities of its columns through LDS, every value is computed once, and a wave's sums are half as many
+// registers as they would be if the halves of the keys stayed apart.
+//
+// Step t: the scores of unit t beside the exponentials of unit t - 1, whose probabilities the waves then exchange; after a
+// barrier, O += P V of unit t - 1 beside the maxima of unit t.  Units move from the pages into LDS without registers; a
+// wave's piece of a unit lies in one run of 16 tokens, which no page divides.
 //
 // P is rounded to bfloat16 for the second product, as in the prefill: the matrix cores set the time here, and a second part of
 // P would cost half as much again.  Sums and maxima are float32; out is rounded once, after the gate.
@@ -37,7 +40,7 @@ using tile32::mfma32;
 using tile32::read_tr;
 using tile32::v_slot;
 
-constexpr int THREADS = 512, WAVES = 8, COLS = CHUNK_COLS;
+constexpr int THREADS = 512, WAVES = 8;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float SLACK = 8.f;  // how far (in powers of two) a maximum may pass the exponent's base before that moves
 
@@ -59,14 +62,19 @@ struct Args {
 
 template <int DH>
 struct Form {
-    static constexpr int UNIT = DH == 256 ? 64 : 128;  // keys
-    static constexpr int SUB = UNIT / 64;              // pieces of 32 keys of a wave's half
-    static constexpr int KS = DH / 16, DT = DH / 32;   // products along a head, and tiles of 32 of its dims
+    static constexpr int UNIT = 64;                    // keys
+    static constexpr int NC = 256 / DH;                // sets of 32 columns a wave
+    static constexpr int COLS = 128 * NC;
+    static constexpr int KS = DH / 16, DT = DH / 64;   // products along a head, and tiles of 32 dims of a half
     static constexpr int ROW = 2 * DH, TILE = UNIT * ROW;
-    static constexpr int KST = 3, VST = 2;             // LDS stages
-    static constexpr int BYTES = (KST + VST) * TILE;   // all of the LDS
-    static constexpr int XS = DT / 2 * 16 + 4;         // floats a lane of the exchange
-    static_assert(THREADS * XS * 4 <= BYTES && BYTES <= 160 * 1024, "the exchange fits in the stages");
+    static constexpr int AHEAD = DH == 256 ? 1 : 2;    // units that K is asked for before it is used, and V one less
+    static constexpr int STAGES = AHEAD + 1;           // of each
+    static constexpr int P_AT = 2 * STAGES * TILE, P_WAVE = 2048 * NC;
+    static constexpr int TOP_AT = P_AT + WAVES * P_WAVE;
+    static constexpr int FLAG_AT = TOP_AT + WAVES * 128 * NC;
+    static constexpr int OUT_ROW = 2 * DH + 16;        // bytes of a column's half of the sums at the end, padded
+    static constexpr int BYTES = FLAG_AT + 16 > WAVES * 32 * NC * OUT_ROW ? FLAG_AT + 16 : WAVES * 32 * NC * OUT_ROW;
+    static_assert(BYTES <= 160 * 1024, "fits in the LDS");
 };
 
 // An entry's sequence, first row, rows, and the position of the first one (less than 0: rows without keys).
@@ -114,16 +122,12 @@ __device__ __forceinline__ int64_t wave_scan(int64_t x) {
     return x;
 }
 
-// Of two bfloat16 values: is one no finite number; those that are; and 1 for each that is an infinity of this sign or a NaN.
+// Of two bfloat16 values: is one no finite number; those that are.
 __device__ __forceinline__ bool odd16(uint32_t x) {
     return ((x & 0x7f80u) == 0x7f80u) | ((x & 0x7f800000u) == 0x7f800000u);
 }
 __device__ __forceinline__ uint32_t common16(uint32_t x) {
     return ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu) | ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u);
-}
-__device__ __forceinline__ uint32_t ones16(uint32_t x, uint32_t sign) {
-    auto one = [&](uint32_t v) { return (v & 0x7f80u) == 0x7f80u && ((v & 0x7fu) != 0 || (v & 0x8000u) == sign); };
-    return (one(x & 0xffffu) ? 0x3f80u : 0u) | (one(x >> 16) ? 0x3f800000u : 0u);
 }
 
 // Four dims of an output from sums o over l (0: no key).
@@ -145,11 +149,11 @@ __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -
 template <int DH>
 __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args a) {
     using F = Form<DH>;
-    constexpr int UNIT = F::UNIT, SUB = F::SUB, KS = F::KS, DT = F::DT, ROW = F::ROW, TILE = F::TILE, KST = F::KST;
+    constexpr int UNIT = F::UNIT, NC = F::NC, COLS = F::COLS, KS = F::KS, DT = F::DT, ROW = F::ROW, TILE = F::TILE;
+    constexpr int AHEAD = F::AHEAD, STAGES = F::STAGES;
     extern __shared__ __align__(16) unsigned char smem[];
     const int wave = uniform(threadIdx.x >> 6);
-    const int cg = wave & 3, kg = wave >> 2;  // group of columns, half of the keys
-    if (kg == 0) __builtin_amdgcn_s_setprio(1);
+    const int cg = wave & 3, half = wave >> 2;  // group of columns; half of the keys, then of the dims
 
     // The line's length, from the sums of windows of 64 entries; lane i has windows 2 i and 2 i + 1.
     const int windows = (a.n + 63) / 64;
@@ -179,24 +183,22 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args 
     constexpr int MINE = UNIT / WAVES, PER = 1024 / ROW, NI = MINE / PER, CHUNKS = ROW / 16;  // rows of a wave's transfers
     const int token = 2 * a.Hk * DH;  // bytes
     const int r0 = wave * MINE;
-    const uint32_t lds0 = (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem) +
-                          r0 * ROW;
-    const int half_at = kg * (UNIT / 2) * ROW;
+    const uint32_t lds0 =
+        (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem) + r0 * ROW;
 
     // What is looked at once an item lies in memory in between: the loop over the keys needs the registers.
-    volatile int64_t kept[4];
+    volatile int64_t kept[3];
     kept[0] = w0;
     kept[1] = w1;
     kept[2] = upto;
     for (int64_t pos = begin; pos < end;) {
-        const int lane = lane_here(), c32 = lane & 31, hh = lane >> 5;
         // the item at `pos`
         const int64_t windows_upto = kept[2], window0 = kept[0], window1 = kept[1];
         const int l0 = __ffsll((unsigned long long)__ballot(windows_upto > pos)) - 1;
         const int64_t first0 = scalar64(window0, l0), before0 = scalar64(windows_upto, l0) - first0 - scalar64(window1, l0);
         const bool second = pos >= before0 + first0;
         const int64_t window_at = second ? before0 + first0 : before0;
-        const Entry mine = entry_of(a, (2 * l0 + second) * 64 + lane);
+        const Entry mine = entry_of(a, (2 * l0 + second) * 64 + lane_here());
         const int64_t entry_own = weight_of(mine), entry_upto = wave_scan(entry_own);
         const int el = __ffsll((unsigned long long)__ballot(window_at + entry_upto > pos)) - 1;
         const int seq = scalar(mine.s, el), erow = scalar(mine.row0, el), erows = scalar(mine.rows, el);
@@ -224,54 +226,68 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args 
         const bool whole = istart >= begin && iend <= end;
         pos = min(iend, end);
 
-        // this lane's column: a row and a q head of the kv head's
-        const int cols = ntok * a.G, col = cg * 32 + c32, tk = col / (uint32_t)a.G;
-        const bool used = col < cols;
-        const int head0 = head * a.G;
-        const size_t at_q = ((size_t)(row0 + (used ? tk : 0)) * a.Hq + head0 + (used ? col - tk * a.G : 0)) * DH;
-        const int last_key = used ? pos0 + tk : -1;
-        const bool active = cg * 32 < cols;
-        const int low_key = pos0 + cg * 32 / (uint32_t)a.G, high_key = pos0 + min(ntok - 1, (cg * 32 + 31) / (uint32_t)a.G);
-
-        u32x4 qf[KS];
+        // a column is a row and a q head of the kv head's
+        const int cols = ntok * a.G;
+        const bool active = cg * 32 * NC < cols;
+        const int low_key = pos0 + cg * 32 * NC / (uint32_t)a.G;  // that the wave's first column sees
+        struct Column {
+            int token, head;
+            size_t at;  // of q, gate and out
+        };
+        auto column = [&](int col) {
+            Column x;
+            x.token = col / (uint32_t)a.G;
+            x.head = head * a.G + col - x.token * a.G;
+            x.at = ((size_t)(row0 + x.token) * a.Hq + x.head) * DH;
+            return x;
+        };
+        u32x4 qf[NC][KS];
+        int last_key[NC];  // that this lane's columns see
+        auto load_q = [&]() __attribute__((always_inline)) {
+            const int lane = lane_here();
 #pragma unroll
-        for (int i = 0; i < KS; i++) {
-            qf[i] = u32x4{0, 0, 0, 0};
-            if (used) qf[i] = *reinterpret_cast<const u32x4*>(a.q + at_q + 16 * i + 8 * hh);
-        }
-
-        // The next 64 runs of 16 tokens: lane i has the pool's run of run number runs0 + i, -1 if its page is out of range
-        constexpr int RUNS = UNIT / 16, AHEAD = 64 / RUNS;
-        int where = 0, from_unit = -AHEAD;
-        uint64_t bad = 0;
-        auto look_up = [&](int unit) {
-            from_unit = unit;
-            const uint32_t run = unit * RUNS + lane, page = (uint32_t)a.page / 16;
-            where = -1;
-            const bool held = 16 * run < (uint32_t)keys;
-            if (held) {
-                uint32_t slot = __umulhi(run, a.page_inverse);
-                slot += (slot + 1) * page <= run;
-                const int pg = a.table[(size_t)seq * a.max_pages + slot];
-                if (pg >= 0 && pg < a.npages) where = pg * page + run - slot * page;
+            for (int n = 0; n < NC; n++) {
+                const int col = (cg * NC + n) * 32 + (lane & 31);
+                const Column x = column(min(col, cols - 1));
+                last_key[n] = col < cols ? pos0 + x.token : -1;
+#pragma unroll
+                for (int i = 0; i < KS; i++)
+                    qf[n][i] = *reinterpret_cast<const u32x4*>(a.q + x.at + 16 * i + 8 * (lane >> 5));
             }
-            bad = __ballot(held && where < 0);
         };
+        load_q();
+
+        // The next 64 runs of 16 tokens: lane i has the pool's run of run number i from here, -1 if its page is out of range
+        constexpr int RUNS = UNIT / 16, LOOK = 64 / RUNS;
+        int where = 0, from_unit = -LOOK;
+        uint64_t bad = 0;
         struct Piece {
-            int run, rows;      // of the pool; rows that are there, of the wave's
-            uint32_t bad;       // runs of the unit whose page is out of range
+            int run, rows;  // of the pool; rows that are there, of the wave's
+            uint32_t bad;   // runs of the unit whose page is out of range
         };
-        auto piece_of = [&](int unit) {
+        auto piece_of = [&](int unit) __attribute__((always_inline)) {
             Piece p{0, 0, 0};
             if (unit >= u1) return p;
-            if (unit >= from_unit + AHEAD) look_up(unit);
+            if (unit >= from_unit + LOOK) {
+                from_unit = unit;
+                const uint32_t run = unit * RUNS + lane_here(), page = (uint32_t)a.page / 16;
+                where = -1;
+                const bool held = 16 * run < (uint32_t)keys;
+                if (held) {
+                    uint32_t slot = __umulhi(run, a.page_inverse);
+                    slot += (slot + 1) * page <= run;
+                    const int pg = a.table[(size_t)seq * a.max_pages + slot];
+                    if (pg >= 0 && pg < a.npages) where = pg * page + run - slot * page;
+                }
+                bad = __ballot(held && where < 0);
+            }
             const int i = (unit - from_unit) * RUNS;
             p.run = scalar(where, i + r0 / 16);
             p.rows = p.run < 0 ? 0 : max(0, min(MINE, keys - unit * UNIT - r0));
             p.bad = (uint32_t)(bad >> i) & ((1u << RUNS) - 1);
             return p;
         };
-        auto move = [&](const bf16* pool, const Piece& p, uint32_t to, auto chunk) {
+        auto move = [&](const bf16* pool, const Piece& p, uint32_t to, auto chunk) __attribute__((always_inline)) {
             const uint64_t at = reinterpret_cast<uint64_t>(pool) +
                                 ((uint64_t)(uint32_t)max(p.run, 0) * 16 + r0 % 16) * (uint32_t)token + (uint32_t)(head * ROW);
             const u32x4 r = {(uint32_t)uniform((int)(uint32_t)at), (uint32_t)uniform((int)(uint32_t)(at >> 32)) & 0xffffu,
@@ -283,280 +299,368 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args 
                 dma16(r, (uint32_t)uniform((int)(to + i * 1024)), row * token + (chunk(i * PER + row, place) << 4),
                       uniform(i * PER * token));
         };
-        auto move_k = [&](const Piece& p, int stage) {
+        auto move_k = [&](const Piece& p, int stage) __attribute__((always_inline)) {
             move(a.kp, p, lds0 + stage * TILE, [&](int r, int c) { return k_slot(r0 + r, c); });
         };
-        auto move_v = [&](const Piece& p, int stage) {
-            move(a.vp, p, lds0 + (KST + stage) * TILE, [&](int r, int c) { return v_slot(r, c); });
+        auto move_v = [&](const Piece& p, int stage) __attribute__((always_inline)) {
+            move(a.vp, p, lds0 + (STAGES + stage) * TILE, [&](int r, int c) { return v_slot(r, c); });
         };
+        auto next_stage = [](int s) { return s == STAGES - 1 ? 0 : s + 1; };
+        // before unit t's V (the K of t + 1) is read, what was asked for behind it may be on its way
+        auto wait_all_but = [](auto n) { __builtin_amdgcn_s_waitcnt(0x0f70 | decltype(n)::value); };
+        using Behind = std::integral_constant<int, (2 * AHEAD - 1) * NI>;
 
-        f32x16 o[DT];
+        f32x16 o[NC][DT], s[NC], old[NC];  // scores of the last unit, and of the one before
 #pragma unroll
-        for (int t = 0; t < DT; t++)
+        for (int n = 0; n < NC; n++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) o[t][i] = 0.f;
-        float m = -INFINITY, l = 0.f;
+            for (int t = 0; t < DT; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[n][t][i] = 0.f;
+        float m[NC], l[NC], top[NC];
+#pragma unroll
+        for (int n = 0; n < NC; n++) m[n] = top[n] = -INFINITY, l[n] = 0.f;
 
-        Piece now = piece_of(u0), next = piece_of(u0 + 1);
-        if (u0 < u1) {
-            move_k(now, 0);
-            move_v(now, 0);
-            move_k(next, 1);
+        // queue[i]: the piece of unit t + i
+        Piece queue[AHEAD + 1];
+#pragma unroll
+        for (int i = 0; i <= AHEAD; i++) queue[i] = piece_of(u0 + i);
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            move_k(queue[i], i);
+            if (i + 1 < AHEAD) move_v(queue[i], i);
         }
 #pragma unroll
-        for (int i = 0; i < KS; i++) asm volatile("" ::"v"(qf[i]));
+        for (int n = 0; n < NC; n++)
+#pragma unroll
+            for (int i = 0; i < KS; i++) asm volatile("" ::"v"(qf[n][i]));
+        if (threadIdx.x == 0) *reinterpret_cast<int*>(smem + F::FLAG_AT) = 0;
         wait_vm_all();
         __syncthreads();
+        int stage = 0;  // of unit t's K, and of its V
 
-        int ks = 0, vs = 0;
-        for (int u = u0; u < u1; u++) {
-            const Piece after = piece_of(u + 2);
-            move_v(next, vs ^ 1);
-            move_k(after, ks == 0 ? 2 : ks - 1);
-            const int k0 = u * UNIT + kg * (UNIT / 2);  // this wave's first key
-            if (active && k0 <= high_key) {
-                const unsigned char *kb = smem + ks * TILE + half_at, *vb = smem + (KST + vs) * TILE + half_at;
-                f32x16 s[SUB];
+        // K as the first product wants it: row c32 of a half, chunk 2 i + hh
+        constexpr int K_READ = 3;
+        u32x4 kf[KS];
+        auto read_k = [&](const unsigned char* k, int i, int lane) __attribute__((always_inline)) {
+            const int c32 = lane & 31, hh = lane >> 5;
+            kf[i] = *reinterpret_cast<const u32x4*>(k + (32 * half + c32) * ROW + (k_slot(c32, 2 * i + hh) << 4));
+        };
+        // Of unit t: mask, then each column's largest score, for the other wave of the pair
+        auto maxima = [&](int t, uint32_t bad_runs) __attribute__((always_inline)) {
+            const int lane = lane_here(), hh = lane >> 5, k0 = t * UNIT + 32 * half;
+            const uint32_t lost = bad_runs >> (2 * half) & 3;
 #pragma unroll
-                for (int sub = 0; sub < SUB; sub++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) s[sub][i] = 0.f;
-                // K: row c32 of a piece, chunk 2 i + hh, K_AHEAD products ahead
-                constexpr int K_AHEAD = 3;
-                u32x4 kf[KS * SUB];
-                auto read_k = [&](int j) {
-                    const int sub = j / KS, i = j % KS;
-                    kf[j] = *reinterpret_cast<const u32x4*>(kb + (32 * sub + c32) * ROW + (k_slot(c32, 2 * i + hh) << 4));
-                };
-#pragma unroll
-                for (int j = 0; j < K_AHEAD; j++) read_k(j);
-#pragma unroll
-                for (int j = 0; j < KS * SUB; j++) {
-                    if (j + K_AHEAD < KS * SUB) read_k(j + K_AHEAD);
-                    s[j / KS] = mfma32(kf[j], qf[j % KS], s[j / KS]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                // s[sub][i] is key k0 + 32 sub + 8 (i / 4) + 4 hh + i % 4
-                const uint32_t lost = now.bad >> (kg * RUNS / 2) & ((1u << RUNS / 2) - 1);
-                const bool masked = k0 + UNIT / 2 - 1 > low_key || lost != 0;
-                if (masked) {
-#pragma unroll
-                    for (int sub = 0; sub < SUB; sub++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int key = 32 * sub + 8 * (i >> 2) + 4 * hh + (i & 3);
-                            if (k0 + key > last_key || (lost >> (2 * sub + (i >> 3)) & 1)) s[sub][i] = -INFINITY;
-                        }
-                }
-                float top = s[0][0];
-#pragma unroll
-                for (int i = 1; i < 16 * SUB; i++) top = fmaxf(top, s[i >> 4][i & 15]);
-                top = max_halves(top) * a.scale_log2;
-                if (!__all(top <= m + SLACK)) {
-                    const float to = fmaxf(m, top), by = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
-                    m = to;
-                    l *= by;
-#pragma unroll
-                    for (int t = 0; t < DT; t++) o[t] *= by;
-                }
-                const float base = m == -INFINITY ? 0.f : m;
-                // P^T of keys 16 j ..: what a lane has is what it holds of the operand, in the order of v_at's rows
-                u32x4 pf[2 * SUB];
-#pragma unroll
-                for (int sub = 0; sub < SUB; sub++) {
+            for (int n = 0; n < NC; n++) {
+                if (k0 + 31 > low_key || lost) {
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        s[sub][i] = __builtin_amdgcn_exp2f(fmaf(s[sub][i], a.scale_log2, -base));
-                        l += s[sub][i];
+                        const int key = 8 * (i >> 2) + 4 * hh + (i & 3);
+                        if (k0 + key > last_key[n] || (lost >> (i >> 3) & 1)) s[n][i] = -INFINITY;
                     }
-#pragma unroll
-                    for (int j = 0; j < 2; j++)
-                        pf[2 * sub + j] = u32x4{pack2(s[sub][8 * j], s[sub][8 * j + 1]), pack2(s[sub][8 * j + 2], s[sub][8 * j + 3]),
-                                                pack2(s[sub][8 * j + 4], s[sub][8 * j + 5]), pack2(s[sub][8 * j + 6], s[sub][8 * j + 7])};
                 }
-                // V^T as the transposing read hands it out: of tile t of the dims, keys 16 j ..
-                u32x4 v[DT][2 * SUB];
-                const int gi = lane & 15, gg = lane >> 4, vrow = 4 * (gg >> 1) + (gi >> 2), vdim = 16 * (gg & 1) + 4 * (gi & 3);
-                auto read_v = [&](int t) {
-                    const unsigned char* const at = vb + vrow * ROW + (v_slot(vrow, (32 * t + vdim) >> 3) << 4) + 2 * (vdim & 7);
+                float most = s[n][0];
 #pragma unroll
-                    for (int j = 0; j < 2 * SUB; j++) {
-                        const u32x2 lo = read_tr(at + 16 * j * ROW), hi = read_tr(at + (16 * j + 8) * ROW);
-                        v[t][j] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-                    }
-                };
-                bool odd = false;
-                if (masked) {
-                    // A value that some of the columns must not see may be an infinity or NaN, which a weight of zero does
-                    // not take away.
-                    u32x4 x[4];
-                    for (int i = 0; i < UNIT / 2 * ROW / 4096; i++) {
+                for (int i = 1; i < 16; i++) most = fmaxf(most, s[n][i]);
+                top[n] = max_halves(most) * a.scale_log2;
+                if (hh == 0)
+                    *reinterpret_cast<float*>(smem + F::TOP_AT + ((wave * NC + n) * 32 + lane) * 4) = top[n];
+            }
+        };
+        // The values of a unit from key k0 on that are no finite numbers, from the pages.
+        auto add_odd = [&](int k0) __attribute__((always_inline)) {
+            const int lane = lane_here();
+            for (int key = k0; key < min(k0 + UNIT, keys); key++) {
+                const int page = key / a.page, pg = a.table[(size_t)seq * a.max_pages + page];
+                if (pg < 0 || pg >= a.npages) continue;
+                const size_t slot = (size_t)pg * a.page + (key - page * a.page);
+                const bf16* const from = a.vp + (slot * a.Hk + head) * DH + half * (DH / 2) + 4 * (lane >> 5);
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            x[j] = *reinterpret_cast<const u32x4*>(vb + (4 * i + j) * 1024 + lane * 16);
+                for (int d = 0; d < DT; d++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) odd |= odd16(x[j][e]);
-                    }
-                    odd = __any(odd);
-                }
-                read_v(0);
-#pragma unroll
-                for (int t = 0; t < DT; t++) {
-                    if (t + 1 < DT) read_v(t + 1);
-                    if (odd) {  // such values leave the product
-#pragma unroll
-                        for (int j = 0; j < 2 * SUB; j++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) v[t][j][e] = common16(v[t][j][e]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 2 * SUB; j++) o[t] = mfma32(v[t][j], pf[j], o[t]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                if (odd) {
-                    // and the columns that see them are told so by products of whole numbers: how many +inf (and NaN) are there,
-                    // and how many -inf (and NaN)
-#pragma unroll
-                    for (int j = 0; j < 2 * SUB; j++)
+                    for (int g = 0; g < 4; g++) {
+                        const u32x2 x = *reinterpret_cast<const u32x2*>(from + 32 * d + 8 * g);
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const int key = 16 * j + 8 * (e >> 1) + 4 * hh + 2 * (e & 1);
-                            const bool gone = lost >> j & 1;
-                            pf[j][e] = (!gone && k0 + key <= last_key ? 0x3f80u : 0u) |
-                                       (!gone && k0 + key + 1 <= last_key ? 0x3f800000u : 0u);
+                            const float y = e & 1 ? hi_f32(x[e / 2]) : lo_f32(x[e / 2]);
+#pragma unroll
+                            for (int n = 0; n < NC; n++)
+                                o[n][d][4 * g + e] += key <= last_key[n] && !(fabsf(y) < INFINITY) ? y : 0.f;
                         }
-                    auto tell = [&](int t, uint32_t sign, float what) {
-                        f32x16 found;
-#pragma unroll
-                        for (int i = 0; i < 16; i++) found[i] = 0.f;
-                        read_v(t);
-#pragma unroll
-                        for (int j = 0; j < 2 * SUB; j++) {
-#pragma unroll
-                            for (int e = 0; e < 4; e++) v[t][j][e] = ones16(v[t][j][e], sign);
-                            found = mfma32(v[t][j], pf[j], found);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 16; i++) o[t][i] += found[i] > 0.f ? what : 0.f;
                         __builtin_amdgcn_sched_barrier(0);
-                    };
-#pragma unroll
-                    for (int t = 0; t < DT; t++) {
-                        tell(t, 0, INFINITY);
-                        tell(t, 0x8000u, -INFINITY);
                     }
+            }
+        };
+        // Step t: FIRST has no unit before it, LAST none of its own.
+        auto step = [&](int t, auto is_first, auto is_last) __attribute__((always_inline)) {
+            constexpr bool FIRST = decltype(is_first)::value, LAST = decltype(is_last)::value;
+            constexpr int NP = NC * 2;  // operands of probabilities of half a unit
+            u32x4 pf[NC][2];
+            if (!LAST) {
+                int to = stage;
+#pragma unroll
+                for (int i = 0; i < AHEAD; i++) to = next_stage(to);
+                move_k(queue[AHEAD], to);
+            }
+            if (active) {
+                const int lane = lane_here();
+                const unsigned char* const k = smem + stage * TILE;
+                if (!LAST) {
+#pragma unroll
+                    for (int i = 0; i < K_READ; i++) read_k(k, i, lane);
+                }
+                float base[NC];
+                if (!FIRST) {
+#pragma unroll
+                    for (int n = 0; n < NC; n++) {
+                        const float theirs = *reinterpret_cast<const float*>(
+                            smem + F::TOP_AT + (((wave ^ 4) * NC + n) * 32 + (lane & 31)) * 4);
+                        top[n] = fmaxf(top[n], theirs);
+                        old[n] = s[n];
+                    }
+                    bool rises = false;
+#pragma unroll
+                    for (int n = 0; n < NC; n++) rises |= !(top[n] <= m[n] + SLACK);
+                    if (__any(rises)) {
+#pragma unroll
+                        for (int n = 0; n < NC; n++) {
+                            const float to = fmaxf(m[n], top[n]);
+                            const float by = __builtin_amdgcn_exp2f(m[n] - (to == -INFINITY ? 0.f : to));
+                            m[n] = to;
+                            l[n] *= by;
+#pragma unroll
+                            for (int d = 0; d < DT; d++) o[n][d] *= by;
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NC; n++) base[n] = m[n] == -INFINITY ? 0.f : m[n];
+                }
+                if (!LAST) {
+#pragma unroll
+                    for (int n = 0; n < NC; n++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) s[n][i] = 0.f;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                // a product and the exponentials of one score beside it
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    if (!LAST) {
+                        const int i = j / NC, n = j % NC;
+                        if (n == 0 && i + K_READ < KS) read_k(k, i + K_READ, lane);
+                        s[n] = mfma32(kf[i], qf[n][i], s[n]);
+                    }
+                    if (!FIRST) {
+#pragma unroll
+                        for (int n = 0; n < NC; n++) {
+                            old[n][j] = __builtin_amdgcn_exp2f(fmaf(old[n][j], a.scale_log2, -base[n]));
+                            l[n] += old[n][j];
+                            if (j & 1) pf[n][j >> 3][j >> 1 & 3] = pack2(old[n][j - 1], old[n][j]);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (!FIRST) {
+                    // (a lane's probabilities are in the second product's order: keys 16 j + 4 hh .. + 3 and 8 behind these)
+#pragma unroll
+                    for (int n = 0; n < NC; n++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++)
+                            *reinterpret_cast<u32x4*>(smem + F::P_AT + ((wave * NC + n) * 2 + j) * 1024 + lane * 16) = pf[n][j];
                 }
             }
-            now = next;
-            next = after;
-            ks = ks == 2 ? 0 : ks + 1;
-            vs ^= 1;
-            __builtin_amdgcn_s_waitcnt(0x0f70 | NI);  // all but the K just asked for
+            LAST ? wait_vm_all() : wait_all_but(Behind{});
             __syncthreads();
+            int at = stage;  // of unit t - 1
+            if (STAGES == 2)
+                at ^= 1;
+            else
+                at = at == 0 ? STAGES - 1 : at - 1;
+            if (!LAST) {
+                int to = stage;
+#pragma unroll
+                for (int i = 0; i + 1 < AHEAD; i++) to = next_stage(to);
+                move_v(queue[AHEAD - 1], to);
+            }
+            // Where some rows must not see some of the keys, a value that is an infinity or NaN is not taken away by a weight of
+            // zero: it leaves the unit here, and is added below to the rows that see it.
+            const bool partly = !FIRST && t * UNIT - 1 > pos0;
+            int odd = 0;
+            if (partly) {
+                u32x4* const x = reinterpret_cast<u32x4*>(smem + (STAGES + at) * TILE) + wave * 64 * NI + lane_here();
+                bool here = false;
+                for (int i = 0; i < NI; i++) {
+                    u32x4 y = x[64 * i];
+                    bool any = false;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        any |= odd16(y[e]);
+                        y[e] = common16(y[e]);
+                    }
+                    if (any) x[64 * i] = y;
+                    here |= any;
+                }
+                int* const flag = reinterpret_cast<int*>(smem + F::FLAG_AT);
+                if (here) *flag = 1;
+                __syncthreads();
+                odd = uniform(*flag);
+            }
+            if (active) {
+                const int lane = lane_here();
+                if (!FIRST) {
+                    u32x4 both[NC][4];  // of all 64 keys
+                    const unsigned char* const p = smem + F::P_AT + (wave ^ 4) * F::P_WAVE + lane * 16;
+#pragma unroll
+                    for (int n = 0; n < NC; n++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            const u32x4 theirs = *reinterpret_cast<const u32x4*>(p + (n * 2 + j) * 1024);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                both[n][j][e] = half == 0 ? pf[n][j][e] : theirs[e];
+                                both[n][2 + j][e] = half == 0 ? theirs[e] : pf[n][j][e];
+                            }
+                        }
+                    // V^T as the transposing read hands it out: of a tile of this half's dims, keys 16 j ..
+                    const unsigned char* const v = smem + (STAGES + at) * TILE;
+                    const int gi = lane & 15, gg = lane >> 4, vrow = 4 * (gg >> 1) + (gi >> 2);
+                    const int vdim = half * (DH / 2) + 16 * (gg & 1) + 4 * (gi & 3);
+                    u32x4 vf[4 * DT];
+                    auto read_v = [&](int i) __attribute__((always_inline)) {
+                        const int d = i / 4, j = i % 4;
+                        const unsigned char* const from =
+                            v + (vrow + 16 * j) * ROW + (v_slot(vrow, (32 * d + vdim) >> 3) << 4) + 2 * (vdim & 7);
+                        const u32x2 lo = read_tr(from), hi = read_tr(from + 8 * ROW);
+                        vf[i] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                    };
+                    constexpr int V_READ = 3;
+#pragma unroll
+                    for (int i = 0; i < V_READ; i++) read_v(i);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < 4 * DT; i++) {
+                        if (i + V_READ < 4 * DT) read_v(i + V_READ);
+#pragma unroll
+                        for (int n = 0; n < NC; n++) o[n][i / 4] = mfma32(vf[i], both[n][i % 4], o[n][i / 4]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    if (odd) add_odd((t - 1) * UNIT);
+                }
+                if (!LAST) maxima(t, queue[0].bad);
+            }
+            if (!LAST) wait_all_but(Behind{});
+            __syncthreads();
+            if (partly && threadIdx.x == 0) *reinterpret_cast<int*>(smem + F::FLAG_AT) = 0;
+            if (!LAST) {
+#pragma unroll
+                for (int i = 0; i < AHEAD; i++) queue[i] = queue[i + 1];
+                queue[AHEAD] = piece_of(t + 1 + AHEAD);
+                stage = next_stage(stage);
+            }
+        };
+        if (u0 < u1) {
+            step(u0, std::true_type{}, std::false_type{});
+            for (int t = u0 + 1; t < u1; t++) step(t, std::false_type{}, std::false_type{});
+            step(u1, std::false_type{}, std::true_type{});
         }
         wait_vm_all();  // (transfers of nothing, behind the last unit)
-        __syncthreads();
 
-        // The halves of the keys: each wave hands over the sums of the dims that the other one ends, half of them, and puts
-        // its results where it found the other's.  (What follows is one loop's code and not one for each register: code that runs
-        // once comes from memory.)
-        constexpr int J = DT * 2;  // quads of dims that a lane ends
-        float* const mine_at = reinterpret_cast<float*>(smem) + (wave * 64 + lane) * F::XS;
-        f32x4* const from = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(smem) + ((wave ^ 4) * 64 + lane) * F::XS);
-        auto hand_over = [&](auto which) {
-            constexpr int K = decltype(which)::value;
-            f32x4* const to = reinterpret_cast<f32x4*>(mine_at);
+        // l: this wave's keys, both lane halves, and the other wave's
+        float sum[NC];
+        if (active) {
+            const int lane = lane_here();
 #pragma unroll
-            for (int j = 0; j < J; j++) {
-                const f32x16& x = o[(1 - K) * (DT / 2) + j / 4];
-                to[j] = f32x4{x[4 * (j % 4)], x[4 * (j % 4) + 1], x[4 * (j % 4) + 2], x[4 * (j % 4) + 3]};
+            for (int n = 0; n < NC; n++) {
+                sum[n] = l[n] + __shfl_xor(l[n], 32, 64);
+                if (lane < 32) *reinterpret_cast<float*>(smem + F::TOP_AT + ((wave * NC + n) * 32 + lane) * 4) = sum[n];
             }
-            to[J] = f32x4{m, l, 0.f, 0.f};
-        };
-        float top, sum;
-        auto join = [&](auto which) {
-            constexpr int K = decltype(which)::value;
-            const f32x4 theirs = from[J];
-            const float m0 = K == 0 ? m : theirs[0], m1 = K == 0 ? theirs[0] : m;
-            const float l0 = K == 0 ? l : theirs[1], l1 = K == 0 ? theirs[1] : l;
-            top = fmaxf(m0, m1);
-            const float base = top == -INFINITY ? 0.f : top;
-            const float f0 = __builtin_amdgcn_exp2f(m0 - base), f1 = __builtin_amdgcn_exp2f(m1 - base);
-            sum = l0 * f0 + l1 * f1;
-#pragma unroll
-            for (int j = 0; j < J; j++) {
-                f32x4 x = from[j];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float own = o[K * (DT / 2) + j / 4][4 * (j % 4) + e];
-                    x[e] = (K == 0 ? own : x[e]) * f0 + (K == 0 ? x[e] : own) * f1;
-                }
-                from[j] = x;
-            }
-        };
-        kg == 0 ? hand_over(std::integral_constant<int, 0>{}) : hand_over(std::integral_constant<int, 1>{});
+        }
         __syncthreads();
-        kg == 0 ? join(std::integral_constant<int, 0>{}) : join(std::integral_constant<int, 1>{});
-        sum += __shfl_xor(sum, 32, 64);
+        // The sums go through LDS, so that whole lines of a column are stored (and one loop's code does it, not one for
+        // each register: code that runs once comes from memory).
         const int slot = 2 * block + (istart >= begin);
         if (active) {
-            float* const part = a.part + (size_t)slot * (COLS * DH);
-            for (int j = 0; j < J; j++) {
-                if (!whole)
-                    *reinterpret_cast<f32x4*>(part + ((wave * J + j) * 64 + lane) * 4) = from[j];
-                else if (used)
-                    store_out(a, at_q + kg * (DH / 2) + 32 * (j / 4) + 8 * (j % 4) + 4 * hh, from[j], sum);
+            const int lane = lane_here();
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+                const float theirs =
+                    *reinterpret_cast<const float*>(smem + F::TOP_AT + (((wave ^ 4) * NC + n) * 32 + (lane & 31)) * 4);
+                l[n] = half == 0 ? sum[n] + theirs : theirs + sum[n];
             }
-            if (kg == 0 && hh == 0) {
-                if (!whole)
-                    *reinterpret_cast<f32x2*>(a.ml + ((size_t)slot * COLS + col) * 2) = f32x2{top, sum};
-                else if (used && a.lse)
-                    a.lse[(size_t)(at_q / DH % a.Hq) * a.rows + row0 + tk] = log_sum(top, sum);
+        }
+        __syncthreads();  // (what was read may lie where another wave writes now)
+        if (active) {
+            const int lane = lane_here(), c32 = lane & 31, hh = lane >> 5;
+            unsigned char* const mine_at = smem + wave * 32 * NC * F::OUT_ROW;
+#pragma unroll
+            for (int n = 0; n < NC; n++)
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int g = 0; g < 4; g++)
+                        *reinterpret_cast<f32x4*>(mine_at + (n * 32 + c32) * F::OUT_ROW + (32 * d + 8 * g + 4 * hh) * 4) =
+                            f32x4{o[n][d][4 * g], o[n][d][4 * g + 1], o[n][d][4 * g + 2], o[n][d][4 * g + 3]};
+            constexpr int QUADS = DH / 8, AT_ONCE = 64 / QUADS;  // quads of a column's half; columns at a time
+            for (int i = 0; i < 32 * NC / AT_ONCE; i++) {
+                const int here = i * AT_ONCE + lane / QUADS, d = lane % QUADS * 4, col = cg * 32 * NC + here;
+                const f32x4 x = *reinterpret_cast<const f32x4*>(mine_at + here * F::OUT_ROW + d * 4);
+                const float l0 = __shfl(l[0], here & 31, 64), l1 = __shfl(l[NC - 1], here & 31, 64);
+                if (col < cols && whole)
+                    store_out(a, column(col).at + half * (DH / 2) + d, x, here < 32 ? l0 : l1);
+                else if (col < cols)
+                    *reinterpret_cast<f32x4*>(a.part + ((size_t)slot * COLS + col) * DH + half * (DH / 2) + d) = x;
+            }
+            if (half == 0 && hh == 0) {
+#pragma unroll
+                for (int n = 0; n < NC; n++) {
+                    const int col = (cg * NC + n) * 32 + c32;
+                    if (col >= cols) continue;
+                    const Column x = column(col);
+                    if (!whole)
+                        *reinterpret_cast<f32x2*>(a.ml + ((size_t)slot * COLS + col) * 2) = f32x2{m[n], l[n]};
+                    else if (a.lse)
+                        a.lse[(size_t)x.head * a.rows + row0 + x.token] = log_sum(m[n], l[n]);
+                }
             }
         }
         if (!whole && iend <= end && threadIdx.x == 0) {
             const int first = (int)((uint64_t)istart / (uint64_t)each);
             a.cuts[block] = Cut{row0, ntok, head, first, block - first + 1};
         }
-        __syncthreads();  // the exchange is read
+        __syncthreads();  // the sums are read
     }
 }
 
-// Joins the parts of the item that stretch blockIdx.x ended, in the order of the stretches: block y has what wave y of each
-// part's block left.
+// Joins the parts of the item that stretch blockIdx.x ended, in the order of the stretches; block y has an eighth of the
+// columns.
+constexpr int JOIN_THREADS = 256, JOIN_SLICES = 8;
 template <int DH>
-__global__ void __launch_bounds__(256) attention_chunk_join_kernel(const Args a) {
-    constexpr int J = DH / 16, QUADS = J / 4;  // a wave's quads of dims a lane, and a thread's of them
+__global__ void __launch_bounds__(JOIN_THREADS) attention_chunk_join_kernel(const Args a) {
+    constexpr int COLS = Form<DH>::COLS, QUADS = DH / 4, MINE = COLS / JOIN_SLICES * QUADS / JOIN_THREADS;
+    static_assert(JOIN_THREADS % QUADS == 0, "a thread's quads are at one dim");
     const Cut cut = a.cuts[blockIdx.x];
-    const int wave = blockIdx.y, cg = wave & 3, kg = wave >> 2;
-    const int lane = threadIdx.x & 63, j0 = (threadIdx.x >> 6) * QUADS;
-    const int col = cg * 32 + (lane & 31), hh = lane >> 5;
-    if (cut.parts == 0 || cg * 32 >= cut.tokens * a.G) return;
-    auto slot_of = [&](int k) { return k == 0 ? 2 * cut.first + 1 : 2 * (cut.first + k); };
-    auto ml_of = [&](int k) { return *reinterpret_cast<const f32x2*>(a.ml + ((size_t)slot_of(k) * COLS + col) * 2); };
-    float top = -INFINITY, sum = 0.f;
-    for (int k = 0; k < cut.parts; k++) top = fmaxf(top, ml_of(k)[0]);
-    const float base = top == -INFINITY ? 0.f : top;
-    f32x4 o[QUADS];
+    const int cols = cut.tokens * a.G, col0 = blockIdx.y * (COLS / JOIN_SLICES) + threadIdx.x / QUADS;
+    const int d = threadIdx.x % QUADS * 4;
+    if (cut.parts == 0) return;
+    auto slot_of = [&](int k) { return (size_t)(k == 0 ? 2 * cut.first + 1 : 2 * (cut.first + k)) * COLS; };
 #pragma unroll
-    for (int j = 0; j < QUADS; j++) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < cut.parts; k++) {
-        const f32x2 ml = ml_of(k);
-        const float f = __builtin_amdgcn_exp2f(ml[0] - base);
-        const float* const part = a.part + (size_t)slot_of(k) * (COLS * DH);
-        sum += ml[1] * f;
-#pragma unroll
-        for (int j = 0; j < QUADS; j++)
-            o[j] += *reinterpret_cast<const f32x4*>(part + ((wave * J + j0 + j) * 64 + lane) * 4) * f;
+    for (int i = 0; i < MINE; i++) {
+        const int col = col0 + i * (JOIN_THREADS / QUADS);
+        if (col >= cols) return;
+        float top = -INFINITY, sum = 0.f;
+        for (int k = 0; k < cut.parts; k++) top = fmaxf(top, a.ml[(slot_of(k) + col) * 2]);
+        const float base = top == -INFINITY ? 0.f : top;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < cut.parts; k++) {
+            const f32x2 ml = *reinterpret_cast<const f32x2*>(a.ml + (slot_of(k) + col) * 2);
+            const float f = __builtin_amdgcn_exp2f(ml[0] - base);
+            sum += ml[1] * f;
+            o += *reinterpret_cast<const f32x4*>(a.part + (slot_of(k) + col) * DH + d) * f;
+        }
+        const int tk = col / (uint32_t)a.G, head = cut.head * a.G + col - tk * a.G, row = cut.row0 + tk;
+        store_out(a, ((size_t)row * a.Hq + head) * DH + d, o, sum);
+        if (a.lse && d == 0) a.lse[(size_t)head * a.rows + row] = log_sum(top, sum);
     }
-    if (col >= cut.tokens * a.G) return;
-    const int tk = col / (uint32_t)a.G, head = cut.head * a.G + col - tk * a.G, row = cut.row0 + tk;
-    const size_t at = ((size_t)row * a.Hq + head) * DH + kg * (DH / 2) + 4 * hh;
-#pragma unroll
-    for (int j = 0; j < QUADS; j++) store_out(a, at + 32 * ((j0 + j) / 4) + 8 * ((j0 + j) % 4), o[j], sum);
-    if (a.lse && wave < 4 && j0 == 0 && hh == 0) a.lse[(size_t)head * a.rows + row] = log_sum(top, sum);
 }
 
 template <int DH>
@@ -564,7 +668,7 @@ int launch(const Args& a, hipStream_t st) {
     attention_chunk_kernel<DH><<<a.blocks, THREADS, Form<DH>::BYTES, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    attention_chunk_join_kernel<DH><<<dim3(a.blocks, WAVES), 256, 0, st>>>(a);
+    attention_chunk_join_kernel<DH><<<dim3(a.blocks, JOIN_SLICES), JOIN_THREADS, 0, st>>>(a);
     return hipGetLastError();
 }
 
@@ -577,7 +681,10 @@ bool chunk_configure() {
     return set(reinterpret_cast<const void*>(attention_chunk_kernel<128>), Form<128>::BYTES) &&
            set(reinterpret_cast<const void*>(attention_chunk_kernel<256>), Form<256>::BYTES);
 }
-size_t chunk_bytes(int cus) { return (size_t)2 * cus * 4 * COLS * (256 + 2) + (size_t)cus * sizeof(Cut); }
+// [2 cus][a slot's columns] of sums, [2 cus][columns] of maxima and sums of weights, [cus] cuts
+constexpr size_t PART = Form<256>::COLS * 256, ML = Form<128>::COLS * 2;
+static_assert(Form<128>::COLS * 128 == PART, "the same room for both");
+size_t chunk_bytes(int cus) { return 4 * 2 * cus * (PART + ML) + cus * sizeof(Cut); }
 
 }  // namespace q35
 
@@ -588,7 +695,7 @@ extern "C" int cs1_attention_paged_varlen(void* paged, const void* q, const void
                                           int max_new, const void* gate, void* out, float* lse, int rows, int Hq, int Hk,
                                           int Dh, float scale, void* stream) {
     const Paged* const p = static_cast<const Paged*>(paged);
-    if (!p || !table_ok(pages) || (Dh != 128 && Dh != 256) || Hk <= 0 || Hq <= 0 || Hq % Hk != 0 || Hq / Hk > COLS)
+    if (!p || !table_ok(pages) || (Dh != 128 && Dh != 256) || Hk <= 0 || Hq <= 0 || Hq % Hk != 0 || Hq / Hk > Form<256>::COLS)
         return hipErrorInvalidValue;
     if (n < 0 || n > MAX_LISTED || rows < 0 || max_new < 0 || !(scale >= 1e-30f && scale <= 1e30f)) return hipErrorInvalidValue;
     constexpr int64_t LIMIT = int64_t{1} << 31;
@@ -607,8 +714,8 @@ extern "C" int cs1_attention_paged_varlen(void* paged, const void* q, const void
     a.out = static_cast<bf16*>(out);
     a.lse = lse;
     a.part = p->chunk;
-    a.ml = p->chunk + (size_t)2 * p->cus * COLS * 256;
-    a.cuts = reinterpret_cast<Cut*>(a.ml + (size_t)2 * p->cus * COLS * 2);
+    a.ml = p->chunk + 2 * p->cus * PART;
+    a.cuts = reinterpret_cast<Cut*>(a.ml + 2 * p->cus * ML);
     a.table = pages->table;
     a.lens = pages->lens;
     a.seqs = seqs;
@@ -623,7 +730,7 @@ extern "C" int cs1_attention_paged_varlen(void* paged, const void* q, const void
     a.Hq = Hq;
     a.Hk = Hk;
     a.G = Hq / Hk;
-    a.tokens = COLS / a.G;
+    a.tokens = (Dh == 128 ? Form<128>::COLS : Form<256>::COLS) / a.G;
     a.blocks = p->cus;
     a.pad = 128;
     a.least = 256;

@@ -14,9 +14,8 @@ struct Paged {
     int device, cus, blocks;
     float* part;   // single tokens: [2 blocks, 16, 256] partial sums, [2 blocks, 16, 2] maximum and sum
     int* count;    // [2 blocks] parts of a group, [2 blocks] groups of a sequence that are done
-    float* chunk;  // several tokens: [2 cus, CHUNK_COLS, 256] and [2 cus, CHUNK_COLS, 2], then what a stretch cut
+    float* chunk;  // several tokens: chunk_bytes
 };
-constexpr int CHUNK_COLS = 128;  // columns (row and q head) of an item of several tokens
 bool chunk_configure();
 size_t chunk_bytes(int cus);
 
