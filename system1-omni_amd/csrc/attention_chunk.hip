@@ -99,6 +99,9 @@ __device__ __forceinline__ int64_t line_of(const Args& a, int pos, int64_t c) {
     return c * (max(pos, 0) + a.pad) + a.tokens * (c * (c + 1) / 2);
 }
 __device__ __forceinline__ int items_of(const Args& a, int rows) { return (rows + a.tokens - 1) / (uint32_t)a.tokens; }
+__device__ __forceinline__ int64_t weight_of(const Args& a, const Entry& e) {
+    return line_of(a, e.pos, items_of(a, e.rows)) * a.Hk;
+}
 
 __device__ __forceinline__ int scalar(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -146,105 +149,123 @@ __device__ __forceinline__ void store_out(const Args& a, size_t at, const f32x4&
 }
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * LN2; }
 
+#define Q35_INLINE __attribute__((always_inline))
+
+// The arguments, read again where they are asked for: what only begins or ends an item is not to be held in scalar
+// registers over the loop over the keys.  (A kernel's arguments begin the segment that this points to.)
+__device__ __forceinline__ const Args& arguments() {
+    auto p = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const Args*)p;
+}
+
 template <int DH>
-__global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args) {
     using F = Form<DH>;
     constexpr int UNIT = F::UNIT, NC = F::NC, COLS = F::COLS, KS = F::KS, DT = F::DT, ROW = F::ROW, TILE = F::TILE;
     constexpr int AHEAD = F::AHEAD, STAGES = F::STAGES;
     extern __shared__ __align__(16) unsigned char smem[];
     const int wave = uniform(threadIdx.x >> 6);
     const int cg = wave & 3, half = wave >> 2;  // group of columns; half of the keys, then of the dims
-
-    // The line's length, from the sums of windows of 64 entries; lane i has windows 2 i and 2 i + 1.
-    const int windows = (a.n + 63) / 64;
-    auto weight_of = [&](const Entry& e) { return line_of(a, e.pos, items_of(a, e.rows)) * a.Hk; };
-    int64_t w0, w1, upto;
-    {
-        const int lane = lane_here();
-        int64_t* const sums = reinterpret_cast<int64_t*>(smem);
-        for (int w = wave; w < windows; w += WAVES) {
-            const int64_t all = wave_scan(weight_of(entry_of(a, w * 64 + lane)));
-            if (lane == 63) sums[w] = all;
-        }
-        __syncthreads();
-        w0 = 2 * lane < windows ? sums[2 * lane] : 0;
-        w1 = 2 * lane + 1 < windows ? sums[2 * lane + 1] : 0;
-        __syncthreads();
-        upto = wave_scan(w0 + w1);
-    }
-    const int64_t total = scalar64(upto, 63);
-    const int64_t each = max((total + a.blocks - 1) / a.blocks, (int64_t)a.least);
-    // neighbours of the line, which share keys, are on one XCD
-    const int block = a.blocks % 8 == 0 ? (blockIdx.x & 7) * (a.blocks / 8) + (blockIdx.x >> 3) : blockIdx.x;
-    const int64_t begin = block * each, end = min(total, begin + each);
-    if (threadIdx.x == 0) a.cuts[block].parts = 0;
-    if (begin >= end) return;
-
     constexpr int MINE = UNIT / WAVES, PER = 1024 / ROW, NI = MINE / PER, CHUNKS = ROW / 16;  // rows of a wave's transfers
-    const int token = 2 * a.Hk * DH;  // bytes
     const int r0 = wave * MINE;
-    const uint32_t lds0 =
-        (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem) + r0 * ROW;
 
     // What is looked at once an item lies in memory in between: the loop over the keys needs the registers.
     volatile int64_t kept[3];
-    kept[0] = w0;
-    kept[1] = w1;
-    kept[2] = upto;
-    for (int64_t pos = begin; pos < end;) {
-        // the item at `pos`
-        const int64_t windows_upto = kept[2], window0 = kept[0], window1 = kept[1];
-        const int l0 = __ffsll((unsigned long long)__ballot(windows_upto > pos)) - 1;
-        const int64_t first0 = scalar64(window0, l0), before0 = scalar64(windows_upto, l0) - first0 - scalar64(window1, l0);
-        const bool second = pos >= before0 + first0;
-        const int64_t window_at = second ? before0 + first0 : before0;
-        const Entry mine = entry_of(a, (2 * l0 + second) * 64 + lane_here());
-        const int64_t entry_own = weight_of(mine), entry_upto = wave_scan(entry_own);
-        const int el = __ffsll((unsigned long long)__ballot(window_at + entry_upto > pos)) - 1;
-        const int seq = scalar(mine.s, el), erow = scalar(mine.row0, el), erows = scalar(mine.rows, el);
-        const int epos = scalar(mine.pos, el), items = items_of(a, erows);
-        const int64_t own = line_of(a, epos, items);
-        const int64_t estart = window_at + scalar64(entry_upto - entry_own, el);
-        const int head = (int)((uint64_t)(pos - estart) / (uint64_t)own);
-        const int64_t hstart = estart + head * own;
-        int c = 0;  // the last item that begins at or before pos
-        for (int up = items - 1; c < up;) {
-            const int mid = (c + up + 1) >> 1;
-            if (hstart + line_of(a, epos, mid) <= pos)
-                c = mid;
-            else
-                up = mid - 1;
+    int64_t pos, end, each;
+    int block;
+    {
+        // The line's length, from the sums of windows of 64 entries; lane i has windows 2 i and 2 i + 1.
+        const Args a = arguments();
+        const int lane = lane_here(), windows = (a.n + 63) / 64;
+        int64_t* const sums = reinterpret_cast<int64_t*>(smem);
+        for (int w = wave; w < windows; w += WAVES) {
+            const int64_t all = wave_scan(weight_of(a, entry_of(a, w * 64 + lane)));
+            if (lane == 63) sums[w] = all;
         }
-        const int64_t istart = hstart + line_of(a, epos, c), iend = hstart + line_of(a, epos, c + 1);
-        const int tok0 = c * a.tokens, ntok = min(a.tokens, erows - tok0);
-        const int row0 = erow + tok0, pos0 = epos + tok0;  // of its first row
-        const int keys = max(pos0 + ntok, 0), units = (keys + UNIT - 1) / UNIT;
-        auto cut = [&](int64_t x) {
-            return x <= istart ? 0 : x >= iend ? units : (int)min((int64_t)units, max(x - istart - a.pad, (int64_t)0) / UNIT);
-        };
-        const int u0 = uniform(cut(begin)), u1 = uniform(cut(end));
-        const bool whole = istart >= begin && iend <= end;
-        pos = min(iend, end);
+        __syncthreads();
+        const int64_t w0 = 2 * lane < windows ? sums[2 * lane] : 0, w1 = 2 * lane + 1 < windows ? sums[2 * lane + 1] : 0;
+        __syncthreads();
+        const int64_t upto = wave_scan(w0 + w1), total = scalar64(upto, 63);
+        kept[0] = w0;
+        kept[1] = w1;
+        kept[2] = upto;
+        each = max((total + a.blocks - 1) / a.blocks, (int64_t)a.least);
+        // neighbours of the line, which share keys, are on one XCD
+        block = a.blocks % 8 == 0 ? (blockIdx.x & 7) * (a.blocks / 8) + (blockIdx.x >> 3) : blockIdx.x;
+        pos = block * each;
+        end = min(total, pos + each);
+        if (threadIdx.x == 0) a.cuts[block].parts = 0;
+    }
+    const int64_t begin = pos;
 
+    while (pos < end) {
+        int seq, row0, ntok, pos0, keys, head, u0, u1;
+        bool whole, began;  // all of the item is in this stretch; it begins there
+        int first_block = -1;  // of an item that ends here and began elsewhere
+        {
+            // the item at `pos`
+            const Args a = arguments();
+            const int64_t windows_upto = kept[2], window0 = kept[0], window1 = kept[1];
+            const int l0 = __ffsll((unsigned long long)__ballot(windows_upto > pos)) - 1;
+            const int64_t first0 = scalar64(window0, l0), before0 = scalar64(windows_upto, l0) - first0 - scalar64(window1, l0);
+            const bool second = pos >= before0 + first0;
+            const int64_t window_at = second ? before0 + first0 : before0;
+            const Entry mine = entry_of(a, (2 * l0 + second) * 64 + lane_here());
+            const int64_t entry_own = weight_of(a, mine), entry_upto = wave_scan(entry_own);
+            const int el = __ffsll((unsigned long long)__ballot(window_at + entry_upto > pos)) - 1;
+            const int erow = scalar(mine.row0, el), erows = scalar(mine.rows, el);
+            const int epos = scalar(mine.pos, el), items = items_of(a, erows);
+            const int64_t own = line_of(a, epos, items);
+            const int64_t estart = window_at + scalar64(entry_upto - entry_own, el);
+            seq = scalar(mine.s, el);
+            head = (int)((uint64_t)(pos - estart) / (uint64_t)own);
+            const int64_t hstart = estart + head * own;
+            int c = 0;  // the last item that begins at or before pos
+            for (int up = items - 1; c < up;) {
+                const int mid = (c + up + 1) >> 1;
+                if (hstart + line_of(a, epos, mid) <= pos)
+                    c = mid;
+                else
+                    up = mid - 1;
+            }
+            const int64_t istart = hstart + line_of(a, epos, c), iend = hstart + line_of(a, epos, c + 1);
+            const int tok0 = c * a.tokens;
+            ntok = min(a.tokens, erows - tok0);
+            row0 = erow + tok0;
+            pos0 = epos + tok0;  // of its first row
+            keys = max(pos0 + ntok, 0);
+            const int units = (keys + UNIT - 1) / UNIT;
+            auto cut = [&](int64_t x) {
+                return x <= istart ? 0 : x >= iend ? units : (int)min((int64_t)units, max(x - istart - a.pad, (int64_t)0) / UNIT);
+            };
+            u0 = uniform(cut(begin));
+            u1 = uniform(cut(end));
+            began = istart >= begin;
+            whole = began && iend <= end;
+            if (!began && iend <= end) first_block = (int)((uint64_t)istart / (uint64_t)each);
+            pos = min(iend, end);
+        }
         // a column is a row and a q head of the kv head's
-        const int cols = ntok * a.G;
+        const int G = uniform(arguments().G), Hq = uniform(arguments().Hq), cols = ntok * G;
         const bool active = cg * 32 * NC < cols;
-        const int low_key = pos0 + cg * 32 * NC / (uint32_t)a.G;  // that the wave's first column sees
+        const int low_key = pos0 + cg * 32 * NC / (uint32_t)G;  // that the wave's first column sees
         struct Column {
             int token, head;
             size_t at;  // of q, gate and out
         };
-        auto column = [&](int col) {
+        auto column = [&](int col) Q35_INLINE {
             Column x;
-            x.token = col / (uint32_t)a.G;
-            x.head = head * a.G + col - x.token * a.G;
-            x.at = ((size_t)(row0 + x.token) * a.Hq + x.head) * DH;
+            x.token = col / (uint32_t)G;
+            x.head = head * G + col - x.token * G;
+            x.at = ((size_t)(row0 + x.token) * Hq + x.head) * DH;
             return x;
         };
         u32x4 qf[NC][KS];
         int last_key[NC];  // that this lane's columns see
-        auto load_q = [&]() __attribute__((always_inline)) {
+        {
             const int lane = lane_here();
+            const bf16* const q = arguments().q;
 #pragma unroll
             for (int n = 0; n < NC; n++) {
                 const int col = (cg * NC + n) * 32 + (lane & 31);
@@ -252,63 +273,71 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args 
                 last_key[n] = col < cols ? pos0 + x.token : -1;
 #pragma unroll
                 for (int i = 0; i < KS; i++)
-                    qf[n][i] = *reinterpret_cast<const u32x4*>(a.q + x.at + 16 * i + 8 * (lane >> 5));
+                    qf[n][i] = *reinterpret_cast<const u32x4*>(q + x.at + 16 * i + 8 * (lane >> 5));
             }
-        };
-        load_q();
+        }
 
-        // The next 64 runs of 16 tokens: lane i has the pool's run of run number i from here, -1 if its page is out of range
+        // The next 64 runs of 16 tokens: lane i has the pool's run of run number i from here on, -1 if its page is out of range
         constexpr int RUNS = UNIT / 16, LOOK = 64 / RUNS;
-        int where = 0, from_unit = -LOOK;
+        int where = 0, from_unit = 0;
         uint64_t bad = 0;
-        struct Piece {
-            int run, rows;  // of the pool; rows that are there, of the wave's
-            uint32_t bad;   // runs of the unit whose page is out of range
-        };
-        auto piece_of = [&](int unit) __attribute__((always_inline)) {
-            Piece p{0, 0, 0};
-            if (unit >= u1) return p;
-            if (unit >= from_unit + LOOK) {
-                from_unit = unit;
-                const uint32_t run = unit * RUNS + lane_here(), page = (uint32_t)a.page / 16;
-                where = -1;
-                const bool held = 16 * run < (uint32_t)keys;
-                if (held) {
-                    uint32_t slot = __umulhi(run, a.page_inverse);
-                    slot += (slot + 1) * page <= run;
-                    const int pg = a.table[(size_t)seq * a.max_pages + slot];
-                    if (pg >= 0 && pg < a.npages) where = pg * page + run - slot * page;
-                }
-                bad = __ballot(held && where < 0);
+        auto look_up = [&](int unit) Q35_INLINE {
+            const auto& a = arguments();
+            from_unit = unit;
+            const uint32_t run = unit * RUNS + lane_here(), page = (uint32_t)a.page / 16;
+            where = -1;
+            const bool held = 16 * run < (uint32_t)keys;
+            if (held) {
+                uint32_t slot = __umulhi(run, a.page_inverse);
+                slot += (slot + 1) * page <= run;
+                const int pg = a.table[(size_t)seq * a.max_pages + slot];
+                if (pg >= 0 && pg < a.npages) where = pg * page + run - slot * page;
             }
+            bad = __ballot(held && where < 0);
+        };
+        look_up(u0);
+        const int keys_here = min(keys, u1 * UNIT);
+        const uint32_t token = 2 * (uint32_t)arguments().Hk * DH;  // bytes
+        const uint64_t k_pool = reinterpret_cast<uint64_t>(arguments().kp) + (uint32_t)(head * ROW) + r0 % 16 * token;
+        const uint64_t v_pool = reinterpret_cast<uint64_t>(arguments().vp) + (uint32_t)(head * ROW) + r0 % 16 * token;
+        // This wave's rows of a unit: where they lie in a pool, bytes up to the last one's end (0: none), and which of the unit's
+        // runs have no page
+        struct Piece {
+            uint64_t at;
+            uint32_t bytes, bad;
+        };
+        auto piece_of = [&](int unit) Q35_INLINE {
             const int i = (unit - from_unit) * RUNS;
-            p.run = scalar(where, i + r0 / 16);
-            p.rows = p.run < 0 ? 0 : max(0, min(MINE, keys - unit * UNIT - r0));
-            p.bad = (uint32_t)(bad >> i) & ((1u << RUNS) - 1);
-            return p;
+            const int run = scalar(where, (i + r0 / 16) & 63);
+            const int rows = run < 0 ? 0 : max(0, min(MINE, keys_here - unit * UNIT - r0));
+            return Piece{(uint64_t)((uint32_t)max(run, 0) * (uint64_t)(16 * token)),
+                         rows > 0 ? (rows - 1) * token + ROW : 0, (uint32_t)(bad >> (i & 63)) & ((1u << RUNS) - 1)};
         };
-        auto move = [&](const bf16* pool, const Piece& p, uint32_t to, auto chunk) __attribute__((always_inline)) {
-            const uint64_t at = reinterpret_cast<uint64_t>(pool) +
-                                ((uint64_t)(uint32_t)max(p.run, 0) * 16 + r0 % 16) * (uint32_t)token + (uint32_t)(head * ROW);
-            const u32x4 r = {(uint32_t)uniform((int)(uint32_t)at), (uint32_t)uniform((int)(uint32_t)(at >> 32)) & 0xffffu,
-                             (uint32_t)uniform(p.rows > 0 ? (p.rows - 1) * token + ROW : 0), 0x00020000u};
-            // lane l fills place l % CHUNKS of row l / CHUNKS with the chunk that belongs there
+        auto rows_at = [&](uint64_t pool, const Piece& p) Q35_INLINE {
+            const uint64_t at = pool + p.at;
+            return u32x4{(uint32_t)uniform((int)(uint32_t)at), (uint32_t)uniform((int)(uint32_t)(at >> 32)) & 0xffffu,
+                         (uint32_t)uniform(p.bytes), 0x00020000u};
+        };
+        // Lane l fills place l % CHUNKS of row l / CHUNKS of a transfer with the chunk that belongs there.  Other rows of a piece
+        // exchange other bits (k_slot, v_slot).
+        const uint32_t lds0 =
+            (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem) + r0 * ROW;
+        int k_lane, v_lane;
+        {
             const int lane = lane_here(), row = lane / CHUNKS, place = lane % CHUNKS;
-#pragma unroll
-            for (int i = 0; i < NI; i++)
-                dma16(r, (uint32_t)uniform((int)(to + i * 1024)), row * token + (chunk(i * PER + row, place) << 4),
-                      uniform(i * PER * token));
+            k_lane = row * token + (k_slot(r0 + row, place) << 4);
+            v_lane = row * token + (v_slot(row, place) << 4);
+        }
+        auto move_k = [&](const u32x4& r, int stage, int i) Q35_INLINE {
+            dma16(r, (uint32_t)uniform((int)(lds0 + stage * TILE + i * 1024)), k_lane ^ (i * PER) << 4, uniform(i * PER * token));
         };
-        auto move_k = [&](const Piece& p, int stage) __attribute__((always_inline)) {
-            move(a.kp, p, lds0 + stage * TILE, [&](int r, int c) { return k_slot(r0 + r, c); });
+        auto move_v = [&](const u32x4& r, int stage, int i) Q35_INLINE {
+            dma16(r, (uint32_t)uniform((int)(lds0 + (STAGES + stage) * TILE + i * 1024)), PER == 2 && i & 1 ? v_lane ^ 12 << 4 : v_lane,
+                  uniform(i * PER * token));
         };
-        auto move_v = [&](const Piece& p, int stage) __attribute__((always_inline)) {
-            move(a.vp, p, lds0 + (STAGES + stage) * TILE, [&](int r, int c) { return v_slot(r, c); });
-        };
-        auto next_stage = [](int s) { return s == STAGES - 1 ? 0 : s + 1; };
+        auto later = [](int s, int n) Q35_INLINE { return s + n >= STAGES ? s + n - STAGES : s + n; };
         // before unit t's V (the K of t + 1) is read, what was asked for behind it may be on its way
-        auto wait_all_but = [](auto n) { __builtin_amdgcn_s_waitcnt(0x0f70 | decltype(n)::value); };
-        using Behind = std::integral_constant<int, (2 * AHEAD - 1) * NI>;
+        constexpr int BEHIND = (2 * AHEAD - 1) * NI;
 
         f32x16 o[NC][DT], s[NC], old[NC];  // scores of the last unit, and of the one before
 #pragma unroll
@@ -321,54 +350,36 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args 
 #pragma unroll
         for (int n = 0; n < NC; n++) m[n] = top[n] = -INFINITY, l[n] = 0.f;
 
-        // queue[i]: the piece of unit t + i
-        Piece queue[AHEAD + 1];
+        Piece queue[AHEAD + 1];  // of units t + i
 #pragma unroll
         for (int i = 0; i <= AHEAD; i++) queue[i] = piece_of(u0 + i);
 #pragma unroll
-        for (int i = 0; i < AHEAD; i++) {
-            move_k(queue[i], i);
-            if (i + 1 < AHEAD) move_v(queue[i], i);
-        }
+        for (int i = 0; i < AHEAD; i++)
+#pragma unroll
+            for (int j = 0; j < NI; j++) {
+                move_k(rows_at(k_pool, queue[i]), i, j);
+                if (i + 1 < AHEAD) move_v(rows_at(v_pool, queue[i]), i, j);
+            }
 #pragma unroll
         for (int n = 0; n < NC; n++)
 #pragma unroll
             for (int i = 0; i < KS; i++) asm volatile("" ::"v"(qf[n][i]));
         if (threadIdx.x == 0) *reinterpret_cast<int*>(smem + F::FLAG_AT) = 0;
+        const float scale_log2 = arguments().scale_log2;
         wait_vm_all();
         __syncthreads();
         int stage = 0;  // of unit t's K, and of its V
 
-        // K as the first product wants it: row c32 of a half, chunk 2 i + hh
-        constexpr int K_READ = 3;
+        // K as the first product wants it: row c32 of a half, chunk 2 i + hh; in its place (k_slot) the chunk's low bits are
+        // exchanged by the row's, and 2 i is an exchange of bits too.
+        constexpr int K_READ = DH == 256 ? 6 : 3;  // products ahead
         u32x4 kf[KS];
-        auto read_k = [&](const unsigned char* k, int i, int lane) __attribute__((always_inline)) {
-            const int c32 = lane & 31, hh = lane >> 5;
-            kf[i] = *reinterpret_cast<const u32x4*>(k + (32 * half + c32) * ROW + (k_slot(c32, 2 * i + hh) << 4));
-        };
-        // Of unit t: mask, then each column's largest score, for the other wave of the pair
-        auto maxima = [&](int t, uint32_t bad_runs) __attribute__((always_inline)) {
-            const int lane = lane_here(), hh = lane >> 5, k0 = t * UNIT + 32 * half;
-            const uint32_t lost = bad_runs >> (2 * half) & 3;
-#pragma unroll
-            for (int n = 0; n < NC; n++) {
-                if (k0 + 31 > low_key || lost) {
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int key = 8 * (i >> 2) + 4 * hh + (i & 3);
-                        if (k0 + key > last_key[n] || (lost >> (i >> 3) & 1)) s[n][i] = -INFINITY;
-                    }
-                }
-                float most = s[n][0];
-#pragma unroll
-                for (int i = 1; i < 16; i++) most = fmaxf(most, s[n][i]);
-                top[n] = max_halves(most) * a.scale_log2;
-                if (hh == 0)
-                    *reinterpret_cast<float*>(smem + F::TOP_AT + ((wave * NC + n) * 32 + lane) * 4) = top[n];
-            }
+        auto read_k = [&](int from, int i) Q35_INLINE {
+            kf[i] = *reinterpret_cast<const u32x4*>(smem + ((from ^ (i & 7) << 5) + (i >> 3) * 256));
         };
         // The values of a unit from key k0 on that are no finite numbers, from the pages.
-        auto add_odd = [&](int k0) __attribute__((always_inline)) {
+        auto add_odd = [&](int k0) Q35_INLINE {
+            const auto& a = arguments();
             const int lane = lane_here();
             for (int key = k0; key < min(k0 + UNIT, keys); key++) {
                 const int page = key / a.page, pg = a.table[(size_t)seq * a.max_pages + page];
@@ -391,36 +402,52 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args 
                     }
             }
         };
+        const int top_at = F::TOP_AT + (wave * NC * 32) * 4, top_of = F::TOP_AT + ((wave ^ 4) * NC * 32) * 4;
         // Step t: FIRST has no unit before it, LAST none of its own.
-        auto step = [&](int t, auto is_first, auto is_last) __attribute__((always_inline)) {
+        auto step = [&](int t, auto is_first, auto is_last) Q35_INLINE {
             constexpr bool FIRST = decltype(is_first)::value, LAST = decltype(is_last)::value;
-            constexpr int NP = NC * 2;  // operands of probabilities of half a unit
             u32x4 pf[NC][2];
-            if (!LAST) {
-                int to = stage;
-#pragma unroll
-                for (int i = 0; i < AHEAD; i++) to = next_stage(to);
-                move_k(queue[AHEAD], to);
-            }
+            const int k_to = later(stage, AHEAD);
+            u32x4 rows = {};
+            if (!LAST) rows = rows_at(k_pool, queue[AHEAD]);
             if (active) {
-                const int lane = lane_here();
-                const unsigned char* const k = smem + stage * TILE;
-                if (!LAST) {
-#pragma unroll
-                    for (int i = 0; i < K_READ; i++) read_k(k, i, lane);
-                }
-                float base[NC];
+                const int lane = lane_here(), c32 = lane & 31;
+                float theirs[NC];
                 if (!FIRST) {
 #pragma unroll
                     for (int n = 0; n < NC; n++) {
-                        const float theirs = *reinterpret_cast<const float*>(
-                            smem + F::TOP_AT + (((wave ^ 4) * NC + n) * 32 + (lane & 31)) * 4);
-                        top[n] = fmaxf(top[n], theirs);
+                        theirs[n] = *reinterpret_cast<const float*>(smem + top_of + (n * 32 + c32) * 4);
                         old[n] = s[n];
                     }
+                }
+                const int k = stage * TILE + (32 * half + c32) * ROW + (k_slot(c32, lane >> 5) << 4);
+                if (!LAST) {
+#pragma unroll
+                    for (int i = 0; i < K_READ; i++) read_k(k, i);
+#pragma unroll
+                    for (int n = 0; n < NC; n++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) s[n][i] = 0.f;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                auto product = [&](int j) Q35_INLINE {
+                    const int i = j / NC, n = j % NC;
+                    if (n == 0 && i + K_READ < KS) read_k(k, i + K_READ);
+                    s[n] = mfma32(kf[i], qf[n][i], s[n]);
+                };
+                constexpr int LEAD = 3;  // products before the exponentials begin
+                if (!LAST) {
+#pragma unroll
+                    for (int j = 0; j < LEAD; j++) product(j);
+                }
+                float base[NC];
+                if (!FIRST) {
                     bool rises = false;
 #pragma unroll
-                    for (int n = 0; n < NC; n++) rises |= !(top[n] <= m[n] + SLACK);
+                    for (int n = 0; n < NC; n++) {
+                        top[n] = fmaxf(top[n], theirs[n]);
+                        rises |= !(top[n] <= m[n] + SLACK);
+                    }
                     if (__any(rises)) {
 #pragma unroll
                         for (int n = 0; n < NC; n++) {
@@ -435,28 +462,26 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args 
 #pragma unroll
                     for (int n = 0; n < NC; n++) base[n] = m[n] == -INFINITY ? 0.f : m[n];
                 }
-                if (!LAST) {
-#pragma unroll
-                    for (int n = 0; n < NC; n++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) s[n][i] = 0.f;
-                }
                 __builtin_amdgcn_sched_barrier(0);
-                // a product and the exponentials of one score beside it
+                // a product, the exponentials of scores and a transfer beside it
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
+                for (int j = LEAD; j < 16; j++) {
                     if (!LAST) {
-                        const int i = j / NC, n = j % NC;
-                        if (n == 0 && i + K_READ < KS) read_k(k, i + K_READ, lane);
-                        s[n] = mfma32(kf[i], qf[n][i], s[n]);
+                        product(j);
+#pragma unroll
+                        for (int i = 0; i < NI; i++)
+                            if (j == LEAD + 1 + i * (8 / NI)) move_k(rows, k_to, i);
                     }
                     if (!FIRST) {
+                        constexpr int N = 16 - LEAD;
 #pragma unroll
-                        for (int n = 0; n < NC; n++) {
-                            old[n][j] = __builtin_amdgcn_exp2f(fmaf(old[n][j], a.scale_log2, -base[n]));
-                            l[n] += old[n][j];
-                            if (j & 1) pf[n][j >> 3][j >> 1 & 3] = pack2(old[n][j - 1], old[n][j]);
-                        }
+                        for (int e = (j - LEAD) * 16 / N; e < (j - LEAD + 1) * 16 / N; e++)
+#pragma unroll
+                            for (int n = 0; n < NC; n++) {
+                                old[n][e] = __builtin_amdgcn_exp2f(fmaf(old[n][e], scale_log2, -base[n]));
+                                l[n] += old[n][e];
+                                if (e & 1) pf[n][e >> 3][e >> 1 & 3] = pack2(old[n][e - 1], old[n][e]);
+                            }
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -468,20 +493,14 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args 
                         for (int j = 0; j < 2; j++)
                             *reinterpret_cast<u32x4*>(smem + F::P_AT + ((wave * NC + n) * 2 + j) * 1024 + lane * 16) = pf[n][j];
                 }
-            }
-            LAST ? wait_vm_all() : wait_all_but(Behind{});
-            __syncthreads();
-            int at = stage;  // of unit t - 1
-            if (STAGES == 2)
-                at ^= 1;
-            else
-                at = at == 0 ? STAGES - 1 : at - 1;
-            if (!LAST) {
-                int to = stage;
+            } else if (!LAST) {
 #pragma unroll
-                for (int i = 0; i + 1 < AHEAD; i++) to = next_stage(to);
-                move_v(queue[AHEAD - 1], to);
+                for (int i = 0; i < NI; i++) move_k(rows, k_to, i);
             }
+            if (!LAST) rows = rows_at(v_pool, queue[AHEAD - 1]);
+            LAST ? wait_vm_all() : __builtin_amdgcn_s_waitcnt(0x0f70 | BEHIND);
+            __syncthreads();
+            const int at = later(stage, STAGES - 1), v_to = later(stage, AHEAD - 1);  // of unit t - 1, and for unit t + AHEAD - 1
             // Where some rows must not see some of the keys, a value that is an infinity or NaN is not taken away by a weight of
             // zero: it leaves the unit here, and is added below to the rows that see it.
             const bool partly = !FIRST && t * UNIT - 1 > pos0;
@@ -505,58 +524,89 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args 
                 __syncthreads();
                 odd = uniform(*flag);
             }
-            if (active) {
-                const int lane = lane_here();
-                if (!FIRST) {
-                    u32x4 both[NC][4];  // of all 64 keys
-                    const unsigned char* const p = smem + F::P_AT + (wave ^ 4) * F::P_WAVE + lane * 16;
-#pragma unroll
-                    for (int n = 0; n < NC; n++)
-#pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            const u32x4 theirs = *reinterpret_cast<const u32x4*>(p + (n * 2 + j) * 1024);
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                both[n][j][e] = half == 0 ? pf[n][j][e] : theirs[e];
-                                both[n][2 + j][e] = half == 0 ? theirs[e] : pf[n][j][e];
-                            }
-                        }
-                    // V^T as the transposing read hands it out: of a tile of this half's dims, keys 16 j ..
-                    const unsigned char* const v = smem + (STAGES + at) * TILE;
-                    const int gi = lane & 15, gg = lane >> 4, vrow = 4 * (gg >> 1) + (gi >> 2);
-                    const int vdim = half * (DH / 2) + 16 * (gg & 1) + 4 * (gi & 3);
-                    u32x4 vf[4 * DT];
-                    auto read_v = [&](int i) __attribute__((always_inline)) {
-                        const int d = i / 4, j = i % 4;
-                        const unsigned char* const from =
-                            v + (vrow + 16 * j) * ROW + (v_slot(vrow, (32 * d + vdim) >> 3) << 4) + 2 * (vdim & 7);
-                        const u32x2 lo = read_tr(from), hi = read_tr(from + 8 * ROW);
-                        vf[i] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-                    };
-                    constexpr int V_READ = 3;
-#pragma unroll
-                    for (int i = 0; i < V_READ; i++) read_v(i);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int i = 0; i < 4 * DT; i++) {
-                        if (i + V_READ < 4 * DT) read_v(i + V_READ);
-#pragma unroll
-                        for (int n = 0; n < NC; n++) o[n][i / 4] = mfma32(vf[i], both[n][i % 4], o[n][i / 4]);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                    if (odd) add_odd((t - 1) * UNIT);
-                }
-                if (!LAST) maxima(t, queue[0].bad);
-            }
-            if (!LAST) wait_all_but(Behind{});
-            __syncthreads();
-            if (partly && threadIdx.x == 0) *reinterpret_cast<int*>(smem + F::FLAG_AT) = 0;
+            const uint32_t lost = queue[0].bad >> (2 * half) & 3;  // of unit t's keys
             if (!LAST) {
 #pragma unroll
                 for (int i = 0; i < AHEAD; i++) queue[i] = queue[i + 1];
+                if (t + 1 + AHEAD >= from_unit + LOOK && t + 1 + AHEAD < u1) look_up(t + 1 + AHEAD);
                 queue[AHEAD] = piece_of(t + 1 + AHEAD);
-                stage = next_stage(stage);
             }
+            if (active) {
+                const int lane = lane_here(), hh = lane >> 5;
+                u32x4 theirs[NC][2], vf[4 * DT];
+                // V^T as the transposing read hands it out: of a tile of this half's dims, keys 16 j .. of this wave's half
+                // (j < 2) and of the other one.  (A tile is four chunks, which as in K are an exchange of bits.)
+                const int gi = lane & 15, gg = lane >> 4, vrow = 4 * (gg >> 1) + (gi >> 2);
+                const int vdim = half * (DH / 2) + 16 * (gg & 1) + 4 * (gi & 3);
+                const int v = (STAGES + at) * TILE + vrow * ROW + (v_slot(vrow, vdim >> 3) << 4) + 2 * (vdim & 7);
+                auto read_v = [&](int i) Q35_INLINE {
+                    const int d = i % DT, j = i / DT;
+                    const unsigned char* const from = smem + (v ^ d << 6) + (j < 2 ? half : 1 - half) * 32 * ROW + (j & 1) * 16 * ROW;
+                    const u32x2 lo = read_tr(from), hi = read_tr(from + 8 * ROW);
+                    vf[i] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                };
+                constexpr int V_READ = DH == 256 ? 6 : 3;
+                if (!FIRST) {
+#pragma unroll
+                    for (int i = 0; i < V_READ; i++) read_v(i);
+#pragma unroll
+                    for (int n = 0; n < NC; n++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++)
+                            theirs[n][j] = *reinterpret_cast<const u32x4*>(smem + F::P_AT + (wave ^ 4) * F::P_WAVE +
+                                                                           (n * 2 + j) * 1024 + lane * 16);
+                }
+                const int k0 = t * UNIT + 32 * half;
+                if (!LAST && (k0 + 31 > low_key || lost)) {
+#pragma unroll
+                    for (int n = 0; n < NC; n++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int key = 8 * (i >> 2) + 4 * hh + (i & 3);
+                            if (k0 + key > last_key[n] || (lost >> (i >> 3) & 1)) s[n][i] = -INFINITY;
+                        }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                // a product, the maxima of scores and a transfer beside it
+                float most[NC];
+#pragma unroll
+                for (int n = 0; n < NC; n++) most[n] = s[n][0];
+#pragma unroll
+                for (int i = 0; i < 4 * DT; i++) {
+                    if (!FIRST) {
+                        if (i + V_READ < 4 * DT) read_v(i + V_READ);
+#pragma unroll
+                        for (int n = 0; n < NC; n++)
+                            o[n][i % DT] = mfma32(vf[i], i < 2 * DT ? pf[n][i / DT] : theirs[n][i / DT - 2], o[n][i % DT]);
+                    }
+                    if (!LAST) {
+#pragma unroll
+                        for (int j = 0; j < NI; j++)
+                            if (i == 1 + j * (2 * DT / NI)) move_v(rows, v_to, j);
+                        constexpr int E = 16 / (2 * DT);  // scores each, in the first half
+                        if (i < 2 * DT)
+#pragma unroll
+                            for (int n = 0; n < NC; n++)
+#pragma unroll
+                                for (int e = i * E; e < (i + 1) * E; e++) most[n] = fmaxf(most[n], s[n][e]);
+                        if (i == 2 * DT)
+#pragma unroll
+                            for (int n = 0; n < NC; n++) top[n] = max_halves(most[n]) * scale_log2;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (!LAST && hh == 0)
+#pragma unroll
+                    for (int n = 0; n < NC; n++) *reinterpret_cast<float*>(smem + top_at + (n * 32 + lane) * 4) = top[n];
+                if (!FIRST && odd) add_odd((t - 1) * UNIT);
+            } else if (!LAST) {
+#pragma unroll
+                for (int i = 0; i < NI; i++) move_v(rows, v_to, i);
+            }
+            if (!LAST) __builtin_amdgcn_s_waitcnt(0x0f70 | BEHIND);
+            __syncthreads();
+            if (partly && threadIdx.x == 0) *reinterpret_cast<int*>(smem + F::FLAG_AT) = 0;
+            if (!LAST) stage = later(stage, 1);
         };
         if (u0 < u1) {
             step(u0, std::true_type{}, std::false_type{});
@@ -566,29 +616,28 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args 
         wait_vm_all();  // (transfers of nothing, behind the last unit)
 
         // l: this wave's keys, both lane halves, and the other wave's
-        float sum[NC];
         if (active) {
             const int lane = lane_here();
 #pragma unroll
             for (int n = 0; n < NC; n++) {
-                sum[n] = l[n] + __shfl_xor(l[n], 32, 64);
-                if (lane < 32) *reinterpret_cast<float*>(smem + F::TOP_AT + ((wave * NC + n) * 32 + lane) * 4) = sum[n];
+                l[n] += __shfl_xor(l[n], 32, 64);
+                if (lane < 32) *reinterpret_cast<float*>(smem + top_at + (n * 32 + lane) * 4) = l[n];
             }
         }
         __syncthreads();
-        // The sums go through LDS, so that whole lines of a column are stored (and one loop's code does it, not one for
-        // each register: code that runs once comes from memory).
-        const int slot = 2 * block + (istart >= begin);
         if (active) {
-            const int lane = lane_here();
+            const int c32 = lane_here() & 31;
 #pragma unroll
             for (int n = 0; n < NC; n++) {
-                const float theirs =
-                    *reinterpret_cast<const float*>(smem + F::TOP_AT + (((wave ^ 4) * NC + n) * 32 + (lane & 31)) * 4);
-                l[n] = half == 0 ? sum[n] + theirs : theirs + sum[n];
+                const float theirs = *reinterpret_cast<const float*>(smem + top_of + (n * 32 + c32) * 4);
+                l[n] = half == 0 ? l[n] + theirs : theirs + l[n];
             }
         }
         __syncthreads();  // (what was read may lie where another wave writes now)
+        // The sums go through LDS, so that whole lines of a column are stored (and one loop's code does it, not one for
+        // each register: code that runs once comes from memory).
+        const Args a = arguments();
+        const int slot = 2 * block + began;
         if (active) {
             const int lane = lane_here(), c32 = lane & 31, hh = lane >> 5;
             unsigned char* const mine_at = smem + wave * 32 * NC * F::OUT_ROW;
@@ -623,10 +672,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args 
                 }
             }
         }
-        if (!whole && iend <= end && threadIdx.x == 0) {
-            const int first = (int)((uint64_t)istart / (uint64_t)each);
-            a.cuts[block] = Cut{row0, ntok, head, first, block - first + 1};
-        }
+        if (first_block >= 0 && threadIdx.x == 0)
+            a.cuts[block] = Cut{row0, ntok, head, first_block, block - first_block + 1};
         __syncthreads();  // the sums are read
     }
 }
