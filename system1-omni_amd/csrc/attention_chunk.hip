@@ -37,7 +37,6 @@ namespace {
 using tile32::k_slot;
 using tile32::max_halves;
 using tile32::mfma32;
-using tile32::read_tr;
 using tile32::v_slot;
 
 constexpr int THREADS = 512, WAVES = 8;
@@ -67,8 +66,7 @@ struct Form {
     static constexpr int COLS = 128 * NC;
     static constexpr int KS = DH / 16, DT = DH / 64;   // products along a head, and tiles of 32 dims of a half
     static constexpr int ROW = 2 * DH, TILE = UNIT * ROW;
-    static constexpr int AHEAD = DH == 256 ? 1 : 2;    // units that K is asked for before it is used, and V one less
-    static constexpr int STAGES = AHEAD + 1;           // of each
+    static constexpr int STAGES = 2;                   // of K and of V
     static constexpr int P_AT = 2 * STAGES * TILE, P_WAVE = 2048 * NC;
     static constexpr int TOP_AT = P_AT + WAVES * P_WAVE;
     static constexpr int FLAG_AT = TOP_AT + WAVES * 128 * NC;
@@ -133,6 +131,12 @@ __device__ __forceinline__ uint32_t common16(uint32_t x) {
     return ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu) | ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u);
 }
 
+__device__ __forceinline__ u32x2 read_tr3(uint32_t at) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u32x2,
+                              __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
+}
+
 // Four dims of an output from sums o over l (0: no key).
 __device__ __forceinline__ void store_out(const Args& a, size_t at, const f32x4& o, float l) {
     const float inv = l != 0.f ? 1.f / l : 0.f;
@@ -150,6 +154,7 @@ __device__ __forceinline__ void store_out(const Args& a, size_t at, const f32x4&
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * LN2; }
 
 #define Q35_INLINE __attribute__((always_inline))
+#define Q35_RARELY(x) __builtin_expect(!!(x), 0)  // (what is rare is laid out behind the loop over the keys)
 
 // The arguments, read again where they are asked for: what only begins or ends an item is not to be held in scalar
 // registers over the loop over the keys.  (A kernel's arguments begin the segment that this points to.)
@@ -163,7 +168,7 @@ template <int DH>
 __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args) {
     using F = Form<DH>;
     constexpr int UNIT = F::UNIT, NC = F::NC, COLS = F::COLS, KS = F::KS, DT = F::DT, ROW = F::ROW, TILE = F::TILE;
-    constexpr int AHEAD = F::AHEAD, STAGES = F::STAGES;
+    constexpr int STAGES = F::STAGES;
     extern __shared__ __align__(16) unsigned char smem[];
     const int wave = uniform(threadIdx.x >> 6);
     const int cg = wave & 3, half = wave >> 2;  // group of columns; half of the keys, then of the dims
@@ -300,28 +305,28 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
         const uint32_t token = 2 * (uint32_t)arguments().Hk * DH;  // bytes
         const uint64_t k_pool = reinterpret_cast<uint64_t>(arguments().kp) + (uint32_t)(head * ROW) + r0 % 16 * token;
         const uint64_t v_pool = reinterpret_cast<uint64_t>(arguments().vp) + (uint32_t)(head * ROW) + r0 % 16 * token;
-        // This wave's rows of a unit: where they lie in a pool, bytes up to the last one's end (0: none), and which of the unit's
-        // runs have no page
+        // This wave's rows of a unit: where they lie in a pool, and bytes up to the last one's end (0: none)
         struct Piece {
             uint64_t at;
-            uint32_t bytes, bad;
+            uint32_t bytes;
         };
+        constexpr uint32_t NO_STRIDE = 0xffffu;
+        const uint32_t whole_bytes = (MINE - 1) * token + ROW;
+        auto run_of = [&](int unit) Q35_INLINE { return scalar(where, ((unit - from_unit) * RUNS + r0 / 16) & 63); };
         auto piece_of = [&](int unit) Q35_INLINE {
-            const int i = (unit - from_unit) * RUNS;
-            const int run = scalar(where, (i + r0 / 16) & 63);
-            const int rows = run < 0 ? 0 : max(0, min(MINE, keys_here - unit * UNIT - r0));
-            return Piece{(uint64_t)((uint32_t)max(run, 0) * (uint64_t)(16 * token)),
-                         rows > 0 ? (rows - 1) * token + ROW : 0, (uint32_t)(bad >> (i & 63)) & ((1u << RUNS) - 1)};
+            const int run = run_of(unit);
+            const int rows = max(0, min(MINE, min(keys_here - unit * UNIT - r0, run * MINE + MINE)));  // (none for run -1)
+            return Piece{(uint32_t)max(run, 0) * (uint64_t)(16 * token), rows > 0 ? (rows - 1) * token + ROW : 0};
         };
         auto rows_at = [&](uint64_t pool, const Piece& p) Q35_INLINE {
             const uint64_t at = pool + p.at;
-            return u32x4{(uint32_t)uniform((int)(uint32_t)at), (uint32_t)uniform((int)(uint32_t)(at >> 32)) & 0xffffu,
+            return u32x4{(uint32_t)uniform((int)(uint32_t)at), (uint32_t)uniform((int)(uint32_t)(at >> 32)) & NO_STRIDE,
                          (uint32_t)uniform(p.bytes), 0x00020000u};
         };
         // Lane l fills place l % CHUNKS of row l / CHUNKS of a transfer with the chunk that belongs there.  Other rows of a piece
         // exchange other bits (k_slot, v_slot).
-        const uint32_t lds0 =
-            (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem) + r0 * ROW;
+        const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+        const uint32_t lds0 = (uint32_t)uniform((int)lds) + r0 * ROW;
         int k_lane, v_lane;
         {
             const int lane = lane_here(), row = lane / CHUNKS, place = lane % CHUNKS;
@@ -335,9 +340,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
             dma16(r, (uint32_t)uniform((int)(lds0 + (STAGES + stage) * TILE + i * 1024)), PER == 2 && i & 1 ? v_lane ^ 12 << 4 : v_lane,
                   uniform(i * PER * token));
         };
-        auto later = [](int s, int n) Q35_INLINE { return s + n >= STAGES ? s + n - STAGES : s + n; };
-        // before unit t's V (the K of t + 1) is read, what was asked for behind it may be on its way
-        constexpr int BEHIND = (2 * AHEAD - 1) * NI;
 
         f32x16 o[NC][DT], s[NC], old[NC];  // scores of the last unit, and of the one before
 #pragma unroll
@@ -350,16 +352,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
 #pragma unroll
         for (int n = 0; n < NC; n++) m[n] = top[n] = -INFINITY, l[n] = 0.f;
 
-        Piece queue[AHEAD + 1];  // of units t + i
+        Piece now = piece_of(u0), next = piece_of(u0 + 1);  // of units t and t + 1
 #pragma unroll
-        for (int i = 0; i <= AHEAD; i++) queue[i] = piece_of(u0 + i);
-#pragma unroll
-        for (int i = 0; i < AHEAD; i++)
-#pragma unroll
-            for (int j = 0; j < NI; j++) {
-                move_k(rows_at(k_pool, queue[i]), i, j);
-                if (i + 1 < AHEAD) move_v(rows_at(v_pool, queue[i]), i, j);
-            }
+        for (int j = 0; j < NI; j++) move_k(rows_at(k_pool, now), 0, j);
 #pragma unroll
         for (int n = 0; n < NC; n++)
 #pragma unroll
@@ -370,12 +365,30 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
         __syncthreads();
         int stage = 0;  // of unit t's K, and of its V
 
-        // K as the first product wants it: row c32 of a half, chunk 2 i + hh; in its place (k_slot) the chunk's low bits are
-        // exchanged by the row's, and 2 i is an exchange of bits too.
-        constexpr int K_READ = DH == 256 ? 6 : 3;  // products ahead
-        u32x4 kf[KS];
-        auto read_k = [&](int from, int i) Q35_INLINE {
-            kf[i] = *reinterpret_cast<const u32x4*>(smem + ((from ^ (i & 7) << 5) + (i >> 3) * 256));
+        // Operands in LDS, by lane.  K: row c32 of a half, chunk 2 i + hh; in its place (k_slot) the chunk's low bits are
+        // exchanged by the row's, and 2 i is an exchange of bits too.  V^T as the transposing read hands it out: of a tile of this
+        // half's dims, keys 16 j .. of this wave's half (j < 2) and of the other one; a tile is four chunks, which are an
+        // exchange of bits again.
+        uint32_t k_base, v_base, p_base, top_base;
+        {
+            const int lane = lane_here(), c32 = lane & 31, gi = lane & 15, gg = lane >> 4, vrow = 4 * (gg >> 1) + (gi >> 2);
+            const int vdim = half * (DH / 2) + 16 * (gg & 1) + 4 * (gi & 3);
+            k_base = lds + (32 * half + c32) * ROW + (k_slot(c32, lane >> 5) << 4);
+            v_base = lds + STAGES * TILE + (half * 32 + vrow) * ROW + (v_slot(vrow, vdim >> 3) << 4) + 2 * (vdim & 7);
+            p_base = lds + F::P_AT + wave * F::P_WAVE + lane * 16;
+            top_base = lds + F::TOP_AT + (wave * NC * 32 + c32) * 4;
+        }
+        const int other = 4 - 8 * half;  // from this wave to the other one of its pair
+        auto lds_u4 = [](uint32_t at) Q35_INLINE { return (__attribute__((address_space(3))) u32x4*)at; };
+        auto lds_f = [](uint32_t at) Q35_INLINE { return (__attribute__((address_space(3))) float*)at; };
+        constexpr int K_READ = DH == 256 ? 6 : 3, V_READ = DH == 256 ? 6 : 3;  // operands read ahead
+        u32x4 kf[KS], vf[4 * DT];
+        auto read_k = [&](uint32_t k, int i) Q35_INLINE { kf[i] = *lds_u4((k ^ (i & 7) << 5) + (i >> 3) * 256); };
+        auto read_v = [&](uint32_t v, int i) Q35_INLINE {
+            const int d = i % DT, j = i / DT;
+            const uint32_t from = (v ^ d << 6) + (j < 2 ? 0 : (32 - 64 * half) * ROW) + (j & 1) * 16 * ROW;
+            const u32x2 lo = read_tr3(from), hi = read_tr3(from + 8 * ROW);
+            vf[i] = u32x4{lo[0], lo[1], hi[0], hi[1]};
         };
         // The values of a unit from key k0 on that are no finite numbers, from the pages.
         auto add_odd = [&](int k0) Q35_INLINE {
@@ -402,25 +415,23 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                     }
             }
         };
-        const int top_at = F::TOP_AT + (wave * NC * 32) * 4, top_of = F::TOP_AT + ((wave ^ 4) * NC * 32) * 4;
-        // Step t: FIRST has no unit before it, LAST none of its own.
-        auto step = [&](int t, auto is_first, auto is_last) Q35_INLINE {
+        // Step t.  FIRST: there is no unit before it; LAST: none of its own; PLAIN: both are whole, all rows see all of
+        // them, and so are the two behind.
+        auto step = [&](int t, auto is_first, auto is_last, auto is_plain) Q35_INLINE {
             constexpr bool FIRST = decltype(is_first)::value, LAST = decltype(is_last)::value;
-            u32x4 pf[NC][2];
-            const int k_to = later(stage, AHEAD);
-            u32x4 rows = {};
-            if (!LAST) rows = rows_at(k_pool, queue[AHEAD]);
-            if (active) {
-                const int lane = lane_here(), c32 = lane & 31;
+            constexpr bool PLAIN = decltype(is_plain)::value;
+            u32x4 pf[NC][2], rows = {};
+            if (!LAST) rows = rows_at(k_pool, next);
+            if (PLAIN || active) {
+                const uint32_t k = k_base + stage * TILE;
                 float theirs[NC];
                 if (!FIRST) {
 #pragma unroll
                     for (int n = 0; n < NC; n++) {
-                        theirs[n] = *reinterpret_cast<const float*>(smem + top_of + (n * 32 + c32) * 4);
+                        theirs[n] = *lds_f(top_base + (other * NC + n) * 128);
                         old[n] = s[n];
                     }
                 }
-                const int k = stage * TILE + (32 * half + c32) * ROW + (k_slot(c32, lane >> 5) << 4);
                 if (!LAST) {
 #pragma unroll
                     for (int i = 0; i < K_READ; i++) read_k(k, i);
@@ -448,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                         top[n] = fmaxf(top[n], theirs[n]);
                         rises |= !(top[n] <= m[n] + SLACK);
                     }
-                    if (__any(rises)) {
+                    if (Q35_RARELY(__any(rises))) {
 #pragma unroll
                         for (int n = 0; n < NC; n++) {
                             const float to = fmaxf(m[n], top[n]);
@@ -470,7 +481,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                         product(j);
 #pragma unroll
                         for (int i = 0; i < NI; i++)
-                            if (j == LEAD + 1 + i * (8 / NI)) move_k(rows, k_to, i);
+                            if (j == LEAD + 1 + i * (8 / NI)) move_k(rows, stage ^ 1, i);
                     }
                     if (!FIRST) {
                         constexpr int N = 16 - LEAD;
@@ -490,23 +501,21 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
 #pragma unroll
                     for (int n = 0; n < NC; n++)
 #pragma unroll
-                        for (int j = 0; j < 2; j++)
-                            *reinterpret_cast<u32x4*>(smem + F::P_AT + ((wave * NC + n) * 2 + j) * 1024 + lane * 16) = pf[n][j];
+                        for (int j = 0; j < 2; j++) *lds_u4(p_base + (n * 2 + j) * 1024) = pf[n][j];
                 }
             } else if (!LAST) {
 #pragma unroll
-                for (int i = 0; i < NI; i++) move_k(rows, k_to, i);
+                for (int i = 0; i < NI; i++) move_k(rows, stage ^ 1, i);
             }
-            if (!LAST) rows = rows_at(v_pool, queue[AHEAD - 1]);
-            LAST ? wait_vm_all() : __builtin_amdgcn_s_waitcnt(0x0f70 | BEHIND);
+            if (!LAST) rows = rows_at(v_pool, now);
+            LAST ? wait_vm_all() : __builtin_amdgcn_s_waitcnt(0x0f70 | NI);
             __syncthreads();
-            const int at = later(stage, STAGES - 1), v_to = later(stage, AHEAD - 1);  // of unit t - 1, and for unit t + AHEAD - 1
             // Where some rows must not see some of the keys, a value that is an infinity or NaN is not taken away by a weight of
             // zero: it leaves the unit here, and is added below to the rows that see it.
-            const bool partly = !FIRST && t * UNIT - 1 > pos0;
+            const bool partly = !PLAIN && !FIRST && t * UNIT - 1 > pos0;
             int odd = 0;
             if (partly) {
-                u32x4* const x = reinterpret_cast<u32x4*>(smem + (STAGES + at) * TILE) + wave * 64 * NI + lane_here();
+                u32x4* const x = reinterpret_cast<u32x4*>(smem + (STAGES + (stage ^ 1)) * TILE) + wave * 64 * NI + lane_here();
                 bool here = false;
                 for (int i = 0; i < NI; i++) {
                     u32x4 y = x[64 * i];
@@ -524,40 +533,32 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                 __syncthreads();
                 odd = uniform(*flag);
             }
-            const uint32_t lost = queue[0].bad >> (2 * half) & 3;  // of unit t's keys
+            uint32_t lost = 0;  // runs of unit t's keys that have no page
             if (!LAST) {
-#pragma unroll
-                for (int i = 0; i < AHEAD; i++) queue[i] = queue[i + 1];
-                if (t + 1 + AHEAD >= from_unit + LOOK && t + 1 + AHEAD < u1) look_up(t + 1 + AHEAD);
-                queue[AHEAD] = piece_of(t + 1 + AHEAD);
+                if (!PLAIN) {
+                    lost = (uint32_t)(bad >> ((t - from_unit) * RUNS + 2 * half & 63)) & 3;
+                    if (t + 2 >= from_unit + LOOK && t + 2 < u1) look_up(t + 1);
+                }
+                now = next;
+                if (PLAIN)
+                    next = Piece{(uint32_t)run_of(t + 2) * (uint64_t)(16 * token), whole_bytes};
+                else
+                    next = piece_of(t + 2);
             }
-            if (active) {
-                const int lane = lane_here(), hh = lane >> 5;
-                u32x4 theirs[NC][2], vf[4 * DT];
-                // V^T as the transposing read hands it out: of a tile of this half's dims, keys 16 j .. of this wave's half
-                // (j < 2) and of the other one.  (A tile is four chunks, which as in K are an exchange of bits.)
-                const int gi = lane & 15, gg = lane >> 4, vrow = 4 * (gg >> 1) + (gi >> 2);
-                const int vdim = half * (DH / 2) + 16 * (gg & 1) + 4 * (gi & 3);
-                const int v = (STAGES + at) * TILE + vrow * ROW + (v_slot(vrow, vdim >> 3) << 4) + 2 * (vdim & 7);
-                auto read_v = [&](int i) Q35_INLINE {
-                    const int d = i % DT, j = i / DT;
-                    const unsigned char* const from = smem + (v ^ d << 6) + (j < 2 ? half : 1 - half) * 32 * ROW + (j & 1) * 16 * ROW;
-                    const u32x2 lo = read_tr(from), hi = read_tr(from + 8 * ROW);
-                    vf[i] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-                };
-                constexpr int V_READ = DH == 256 ? 6 : 3;
+            if (PLAIN || active) {
+                const uint32_t v = v_base + (stage ^ 1) * TILE;
+                u32x4 theirs[NC][2];
                 if (!FIRST) {
 #pragma unroll
-                    for (int i = 0; i < V_READ; i++) read_v(i);
+                    for (int i = 0; i < V_READ; i++) read_v(v, i);
 #pragma unroll
                     for (int n = 0; n < NC; n++)
 #pragma unroll
-                        for (int j = 0; j < 2; j++)
-                            theirs[n][j] = *reinterpret_cast<const u32x4*>(smem + F::P_AT + (wave ^ 4) * F::P_WAVE +
-                                                                           (n * 2 + j) * 1024 + lane * 16);
+                        for (int j = 0; j < 2; j++) theirs[n][j] = *lds_u4(p_base + other * F::P_WAVE + (n * 2 + j) * 1024);
                 }
                 const int k0 = t * UNIT + 32 * half;
-                if (!LAST && (k0 + 31 > low_key || lost)) {
+                if (!PLAIN && !LAST && (k0 + 31 > low_key || lost)) {
+                    const int hh = lane_here() >> 5;
 #pragma unroll
                     for (int n = 0; n < NC; n++)
 #pragma unroll
@@ -574,7 +575,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
 #pragma unroll
                 for (int i = 0; i < 4 * DT; i++) {
                     if (!FIRST) {
-                        if (i + V_READ < 4 * DT) read_v(i + V_READ);
+                        if (i + V_READ < 4 * DT) read_v(v, i + V_READ);
 #pragma unroll
                         for (int n = 0; n < NC; n++)
                             o[n][i % DT] = mfma32(vf[i], i < 2 * DT ? pf[n][i / DT] : theirs[n][i / DT - 2], o[n][i % DT]);
@@ -582,7 +583,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                     if (!LAST) {
 #pragma unroll
                         for (int j = 0; j < NI; j++)
-                            if (i == 1 + j * (2 * DT / NI)) move_v(rows, v_to, j);
+                            if (i == 1 + j * (2 * DT / NI)) move_v(rows, stage, j);
                         constexpr int E = 16 / (2 * DT);  // scores each, in the first half
                         if (i < 2 * DT)
 #pragma unroll
@@ -595,41 +596,47 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                if (!LAST && hh == 0)
+                if (!LAST)  // (both lane halves have the same)
 #pragma unroll
-                    for (int n = 0; n < NC; n++) *reinterpret_cast<float*>(smem + top_at + (n * 32 + lane) * 4) = top[n];
-                if (!FIRST && odd) add_odd((t - 1) * UNIT);
+                    for (int n = 0; n < NC; n++) *lds_f(top_base + n * 128) = top[n];
+                if (!PLAIN && !FIRST && odd) add_odd((t - 1) * UNIT);
             } else if (!LAST) {
 #pragma unroll
-                for (int i = 0; i < NI; i++) move_v(rows, v_to, i);
+                for (int i = 0; i < NI; i++) move_v(rows, stage, i);
             }
-            if (!LAST) __builtin_amdgcn_s_waitcnt(0x0f70 | BEHIND);
+            if (!LAST) __builtin_amdgcn_s_waitcnt(0x0f70 | NI);
             __syncthreads();
             if (partly && threadIdx.x == 0) *reinterpret_cast<int*>(smem + F::FLAG_AT) = 0;
-            if (!LAST) stage = later(stage, 1);
+            if (!LAST) stage ^= 1;
         };
         if (u0 < u1) {
-            step(u0, std::true_type{}, std::false_type{});
-            for (int t = u0 + 1; t < u1; t++) step(t, std::false_type{}, std::false_type{});
-            step(u1, std::false_type{}, std::true_type{});
+            constexpr std::true_type yes;
+            constexpr std::false_type no;
+            step(u0, yes, no, no);
+            for (int t = u0 + 1; t < u1;) {
+                // units that all rows see, with whole units behind them whose pages are known and in range
+                int stop = min(min((pos0 + 1) / UNIT, keys_here / UNIT - 2), from_unit + LOOK - 2);
+                if (bad != 0 || !active) stop = t;
+                for (; t < stop; t++) step(t, no, no, yes);
+                if (t < u1) step(t++, no, no, no);
+            }
+            step(u1, no, yes, no);
         }
         wait_vm_all();  // (transfers of nothing, behind the last unit)
 
         // l: this wave's keys, both lane halves, and the other wave's
         if (active) {
-            const int lane = lane_here();
 #pragma unroll
             for (int n = 0; n < NC; n++) {
                 l[n] += __shfl_xor(l[n], 32, 64);
-                if (lane < 32) *reinterpret_cast<float*>(smem + top_at + (n * 32 + lane) * 4) = l[n];
+                *lds_f(top_base + n * 128) = l[n];
             }
         }
         __syncthreads();
         if (active) {
-            const int c32 = lane_here() & 31;
 #pragma unroll
             for (int n = 0; n < NC; n++) {
-                const float theirs = *reinterpret_cast<const float*>(smem + top_of + (n * 32 + c32) * 4);
+                const float theirs = *lds_f(top_base + (other * NC + n) * 128);
                 l[n] = half == 0 ? l[n] + theirs : theirs + l[n];
             }
         }
