@@ -56,7 +56,15 @@ struct Args {
     const int32_t *table, *lens, *seqs, *cu;
     int nseq, max_pages, npages, page, n, max_new, rows, Hq, Hk, G, tokens, blocks, pad, least;
     uint32_t page_inverse;  // 2^32 over page / 16, rounded down
+    uint32_t tokens_inverse, G_inverse;  // 2^32 over tokens and 2^16 over G, rounded up
+    double blocks_inverse;               // 1 / blocks
     float scale_log2;
+
+    // rows * Hq <= 2^24 and tokens <= 256; columns < 512 and G <= 128: exact
+    __device__ __forceinline__ int over_tokens(uint32_t x) const {
+        return tokens == 1 ? x : (int)__umulhi(x, tokens_inverse);
+    }
+    __device__ __forceinline__ int over_G(uint32_t col) const { return (int)(col * G_inverse >> 16); }
 };
 
 template <int DH>
@@ -96,7 +104,7 @@ __device__ __forceinline__ Entry entry_of(const Args& a, int i) {
 __device__ __forceinline__ int64_t line_of(const Args& a, int pos, int64_t c) {
     return c * (max(pos, 0) + a.pad) + a.tokens * (c * (c + 1) / 2);
 }
-__device__ __forceinline__ int items_of(const Args& a, int rows) { return (rows + a.tokens - 1) / (uint32_t)a.tokens; }
+__device__ __forceinline__ int items_of(const Args& a, int rows) { return a.over_tokens(rows + a.tokens - 1); }
 __device__ __forceinline__ int64_t weight_of(const Args& a, const Entry& e) {
     return line_of(a, e.pos, items_of(a, e.rows)) * a.Hk;
 }
@@ -175,57 +183,75 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
     constexpr int MINE = UNIT / WAVES, PER = 1024 / ROW, NI = MINE / PER, CHUNKS = ROW / 16;  // rows of a wave's transfers
     const int r0 = wave * MINE;
 
-    // What is looked at once an item lies in memory in between: the loop over the keys needs the registers.
-    volatile int64_t kept[3];
-    int64_t pos, end, each;
+    // Of the entries' part of the line in which `pos` is: 64 entries, a lane each, with their weights up to and with them, from
+    // the line's place window_at on.
+    Entry mine;
+    int64_t own_weight, upto, window_at = 0, pos, end, each;
+    volatile int64_t kept[3];  // (in memory: the loop over the keys needs the registers)
+    // more entries: lane i has the weights of windows 2 i and 2 i + 1 of 64 entries, and those up to them
+    auto find_window = [&](const Args& a) Q35_INLINE {
+        const int64_t all = kept[2], w0 = kept[0], w1 = kept[1];
+        const int lane = __ffsll((unsigned long long)__ballot(all > pos)) - 1;
+        const int64_t first = scalar64(w0, lane), before = scalar64(all, lane) - first - scalar64(w1, lane);
+        const bool second = pos >= before + first;
+        window_at = second ? before + first : before;
+        mine = entry_of(a, (2 * lane + second) * 64 + lane_here());
+        own_weight = weight_of(a, mine);
+        upto = wave_scan(own_weight);
+    };
     int block;
     {
-        // The line's length, from the sums of windows of 64 entries; lane i has windows 2 i and 2 i + 1.
-        const Args a = arguments();
+        const Args& a = arguments();
         const int lane = lane_here(), windows = (a.n + 63) / 64;
-        int64_t* const sums = reinterpret_cast<int64_t*>(smem);
-        for (int w = wave; w < windows; w += WAVES) {
-            const int64_t all = wave_scan(weight_of(a, entry_of(a, w * 64 + lane)));
-            if (lane == 63) sums[w] = all;
+        int64_t total;
+        if (windows == 1) {
+            mine = entry_of(a, lane);
+            own_weight = weight_of(a, mine);
+            upto = wave_scan(own_weight);
+            total = scalar64(upto, 63);
+        } else {
+            int64_t* const sums = reinterpret_cast<int64_t*>(smem);
+            for (int w = wave; w < windows; w += WAVES) {
+                const int64_t all = wave_scan(weight_of(a, entry_of(a, w * 64 + lane)));
+                if (lane == 63) sums[w] = all;
+            }
+            __syncthreads();
+            const int64_t w0 = 2 * lane < windows ? sums[2 * lane] : 0, w1 = 2 * lane + 1 < windows ? sums[2 * lane + 1] : 0;
+            __syncthreads();
+            const int64_t all = wave_scan(w0 + w1);
+            kept[0] = w0;
+            kept[1] = w1;
+            kept[2] = all;
+            total = scalar64(all, 63);
         }
-        __syncthreads();
-        const int64_t w0 = 2 * lane < windows ? sums[2 * lane] : 0, w1 = 2 * lane + 1 < windows ? sums[2 * lane + 1] : 0;
-        __syncthreads();
-        const int64_t upto = wave_scan(w0 + w1), total = scalar64(upto, 63);
-        kept[0] = w0;
-        kept[1] = w1;
-        kept[2] = upto;
-        each = max((total + a.blocks - 1) / a.blocks, (int64_t)a.least);
+        // (one more than need be; the line is far shorter than 2^50)
+        each = max((int64_t)((double)total * a.blocks_inverse) + 1, (int64_t)a.least);
+        each = (int64_t)(uint32_t)uniform((int)each) | (int64_t)uniform((int)(each >> 32)) << 32;
         // neighbours of the line, which share keys, are on one XCD
         block = a.blocks % 8 == 0 ? (blockIdx.x & 7) * (a.blocks / 8) + (blockIdx.x >> 3) : blockIdx.x;
         pos = block * each;
         end = min(total, pos + each);
         if (threadIdx.x == 0) a.cuts[block].parts = 0;
+        if (pos >= end) return;
+        if (windows > 1) find_window(a);
     }
     const int64_t begin = pos;
 
-    while (pos < end) {
-        int seq, row0, ntok, pos0, keys, head, u0, u1;
+    for (;;) {
+        int seq, row0, ntok, pos0, keys, head = 0, u0, u1;
         bool whole, began;  // all of the item is in this stretch; it begins there
-        int first_block = -1;  // of an item that ends here and began elsewhere
+        int parts = 0;      // of an item that ends here and began elsewhere
         {
             // the item at `pos`
-            const Args a = arguments();
-            const int64_t windows_upto = kept[2], window0 = kept[0], window1 = kept[1];
-            const int l0 = __ffsll((unsigned long long)__ballot(windows_upto > pos)) - 1;
-            const int64_t first0 = scalar64(window0, l0), before0 = scalar64(windows_upto, l0) - first0 - scalar64(window1, l0);
-            const bool second = pos >= before0 + first0;
-            const int64_t window_at = second ? before0 + first0 : before0;
-            const Entry mine = entry_of(a, (2 * l0 + second) * 64 + lane_here());
-            const int64_t entry_own = weight_of(a, mine), entry_upto = wave_scan(entry_own);
-            const int el = __ffsll((unsigned long long)__ballot(window_at + entry_upto > pos)) - 1;
+            const Args& a = arguments();
+            const int el = __ffsll((unsigned long long)__ballot(window_at + upto > pos)) - 1;
             const int erow = scalar(mine.row0, el), erows = scalar(mine.rows, el);
             const int epos = scalar(mine.pos, el), items = items_of(a, erows);
             const int64_t own = line_of(a, epos, items);
-            const int64_t estart = window_at + scalar64(entry_upto - entry_own, el);
+            int64_t hstart = window_at + scalar64(upto - own_weight, el);
             seq = scalar(mine.s, el);
-            head = (int)((uint64_t)(pos - estart) / (uint64_t)own);
-            const int64_t hstart = estart + head * own;
+#pragma unroll 1
+            for (; hstart + own <= pos; hstart += own) head++;
             int c = 0;  // the last item that begins at or before pos
             for (int up = items - 1; c < up;) {
                 const int mid = (c + up + 1) >> 1;
@@ -248,20 +274,23 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
             u1 = uniform(cut(end));
             began = istart >= begin;
             whole = began && iend <= end;
-            if (!began && iend <= end) first_block = (int)((uint64_t)istart / (uint64_t)each);
+            if (!began && iend <= end)
+#pragma unroll 1
+                for (int64_t x = begin + each; x > istart; x -= each) parts++;
             pos = min(iend, end);
         }
         // a column is a row and a q head of the kv head's
         const int G = uniform(arguments().G), Hq = uniform(arguments().Hq), cols = ntok * G;
+        const uint32_t G_inverse = uniform(arguments().G_inverse);
         const bool active = cg * 32 * NC < cols;
-        const int low_key = pos0 + cg * 32 * NC / (uint32_t)G;  // that the wave's first column sees
+        const int low_key = pos0 + (int)(cg * 32 * NC * G_inverse >> 16);  // that the wave's first column sees
         struct Column {
             int token, head;
             size_t at;  // of q, gate and out
         };
         auto column = [&](int col) Q35_INLINE {
             Column x;
-            x.token = col / (uint32_t)G;
+            x.token = (int)(col * G_inverse >> 16);
             x.head = head * G + col - x.token * G;
             x.at = ((size_t)(row0 + x.token) * Hq + x.head) * DH;
             return x;
@@ -415,108 +444,182 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                     }
             }
         };
-        // Step t.  FIRST: there is no unit before it; LAST: none of its own; PLAIN: both are whole, all rows see all of
-        // them, and so are the two behind.
-        auto step = [&](int t, auto is_first, auto is_last, auto is_plain) Q35_INLINE {
-            constexpr bool FIRST = decltype(is_first)::value, LAST = decltype(is_last)::value;
-            constexpr bool PLAIN = decltype(is_plain)::value;
-            u32x4 pf[NC][2], rows = {};
-            if (!LAST) rows = rows_at(k_pool, next);
-            if (PLAIN || active) {
-                const uint32_t k = k_base + stage * TILE;
-                float theirs[NC];
-                if (!FIRST) {
+        // Of a unit's scores in `x`: the exponentials, from a base that moves (seldom) with the maxima of both halves.
+        float base[NC];
+        auto move_base = [&](const float* theirs) Q35_INLINE {
+            bool rises = false;
 #pragma unroll
-                    for (int n = 0; n < NC; n++) {
-                        theirs[n] = *lds_f(top_base + (other * NC + n) * 128);
-                        old[n] = s[n];
-                    }
+            for (int n = 0; n < NC; n++) {
+                top[n] = fmaxf(top[n], theirs[n]);
+                rises |= !(top[n] <= m[n] + SLACK);
+            }
+            if (Q35_RARELY(__any(rises))) {
+#pragma unroll
+                for (int n = 0; n < NC; n++) {
+                    const float to = fmaxf(m[n], top[n]);
+                    const float by = __builtin_amdgcn_exp2f(m[n] - (to == -INFINITY ? 0.f : to));
+                    m[n] = to;
+                    l[n] *= by;
+#pragma unroll
+                    for (int d = 0; d < DT; d++) o[n][d] *= by;
                 }
-                if (!LAST) {
+            }
+#pragma unroll
+            for (int n = 0; n < NC; n++) base[n] = m[n] == -INFINITY ? 0.f : m[n];
+        };
+        u32x4 pf[NC][2];
+        auto exponential = [&](f32x16* x, int e) Q35_INLINE {
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+                x[n][e] = __builtin_amdgcn_exp2f(fmaf(x[n][e], scale_log2, -base[n]));
+                l[n] += x[n][e];
+                if (e & 1) pf[n][e >> 3][e >> 1 & 3] = pack2(x[n][e - 1], x[n][e]);
+            }
+        };
+        // (a lane's probabilities are in the second product's order: keys 16 j + 4 hh .. + 3 and 8 behind these)
+        auto hand_out = [&]() Q35_INLINE {
+#pragma unroll
+            for (int n = 0; n < NC; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) *lds_u4(p_base + (n * 2 + j) * 1024) = pf[n][j];
+        };
+        auto read_top = [&](float* theirs) Q35_INLINE {
+#pragma unroll
+            for (int n = 0; n < NC; n++) theirs[n] = *lds_f(top_base + (other * NC + n) * 128);
+        };
+        auto read_p = [&](u32x4 (*theirs)[2]) Q35_INLINE {
+#pragma unroll
+            for (int n = 0; n < NC; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) theirs[n][j] = *lds_u4(p_base + other * F::P_WAVE + (n * 2 + j) * 1024);
+        };
+        auto add_product = [&](const u32x4 (*theirs)[2], int i) Q35_INLINE {
+#pragma unroll
+            for (int n = 0; n < NC; n++)
+                o[n][i % DT] = mfma32(vf[i], i < 2 * DT ? pf[n][i / DT] : theirs[n][i / DT - 2], o[n][i % DT]);
+        };
+        auto write_top = [&]() Q35_INLINE {  // (both lane halves have the same)
+#pragma unroll
+            for (int n = 0; n < NC; n++) *lds_f(top_base + n * 128) = top[n];
+        };
+        auto end_half = [&]() Q35_INLINE {
+            __builtin_amdgcn_s_waitcnt(0x0f70 | NI);
+            __syncthreads();
+        };
+        // Step t where units t - 1 and t are whole, all rows see all of them, and so are the two behind.
+        auto plain_step = [&](int t) Q35_INLINE {
+            u32x4 rows = rows_at(k_pool, next);
+            const uint32_t k = k_base + stage * TILE, v = v_base + (stage ^ 1) * TILE;
+            float their_top[NC];
+            read_top(their_top);
+#pragma unroll
+            for (int n = 0; n < NC; n++) old[n] = s[n];
+#pragma unroll
+            for (int i = 0; i < K_READ; i++) read_k(k, i);
+#pragma unroll
+            for (int n = 0; n < NC; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[n][i] = 0.f;
+            __builtin_amdgcn_sched_barrier(0);
+            // a product, the exponentials of scores and a transfer beside it
+            constexpr int LEAD = 3, N = 16 - LEAD;  // products before the exponentials begin
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const int i = j / NC, n = j % NC;
+                if (j == LEAD) {
+                    move_base(their_top);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (n == 0 && i + K_READ < KS) read_k(k, i + K_READ);
+                s[n] = mfma32(kf[i], qf[n][i], s[n]);
+#pragma unroll
+                for (int x = 0; x < NI; x++)
+                    if (j == LEAD + 1 + x * (8 / NI)) move_k(rows, stage ^ 1, x);
+                if (j >= LEAD)
+#pragma unroll
+                    for (int e = (j - LEAD) * 16 / N; e < (j - LEAD + 1) * 16 / N; e++) exponential(old, e);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            hand_out();
+            rows = rows_at(v_pool, now);
+            end_half();
+            now = next;
+            next = Piece{(uint32_t)run_of(t + 2) * (uint64_t)(16 * token), whole_bytes};
+            u32x4 their_p[NC][2];
+#pragma unroll
+            for (int i = 0; i < V_READ; i++) read_v(v, i);
+            read_p(their_p);
+            __builtin_amdgcn_sched_barrier(0);
+            // a product, the maxima of scores and a transfer beside it
+            float most[NC];
+#pragma unroll
+            for (int n = 0; n < NC; n++) most[n] = s[n][0];
+#pragma unroll
+            for (int i = 0; i < 4 * DT; i++) {
+                if (i + V_READ < 4 * DT) read_v(v, i + V_READ);
+                add_product(their_p, i);
+#pragma unroll
+                for (int x = 0; x < NI; x++)
+                    if (i == 1 + x * (2 * DT / NI)) move_v(rows, stage, x);
+                constexpr int E = 16 / (2 * DT);  // scores each, in the first half
+#pragma unroll
+                for (int n = 0; n < NC; n++) {
+                    if (i < 2 * DT)
+#pragma unroll
+                        for (int e = i * E; e < (i + 1) * E; e++) most[n] = fmaxf(most[n], s[n][e]);
+                    if (i == 2 * DT) top[n] = max_halves(most[n]) * scale_log2;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            write_top();
+            end_half();
+            stage ^= 1;
+        };
+        // Any step: the first has no unit before it, the last none of its own.  (One copy of the code, part behind part: what a
+        // short item runs has to come from memory first.)
+        auto step = [&](int t) Q35_INLINE {
+            const bool first = t == u0, last = t == u1;
+            if (active && !first) {
+                float their_top[NC];
+                read_top(their_top);
+                move_base(their_top);
+#pragma unroll
+                for (int e = 0; e < 16; e++) exponential(s, e);
+                hand_out();
+            }
+            if (!last) {
+                const u32x4 rows = rows_at(k_pool, next);
+#pragma unroll
+                for (int i = 0; i < NI; i++) move_k(rows, stage ^ 1, i);
+                if (active) {
+                    const uint32_t k = k_base + stage * TILE;
 #pragma unroll
                     for (int i = 0; i < K_READ; i++) read_k(k, i);
 #pragma unroll
                     for (int n = 0; n < NC; n++)
 #pragma unroll
                         for (int i = 0; i < 16; i++) s[n][i] = 0.f;
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                auto product = [&](int j) Q35_INLINE {
-                    const int i = j / NC, n = j % NC;
-                    if (n == 0 && i + K_READ < KS) read_k(k, i + K_READ);
-                    s[n] = mfma32(kf[i], qf[n][i], s[n]);
-                };
-                constexpr int LEAD = 3;  // products before the exponentials begin
-                if (!LAST) {
 #pragma unroll
-                    for (int j = 0; j < LEAD; j++) product(j);
-                }
-                float base[NC];
-                if (!FIRST) {
-                    bool rises = false;
+                    for (int i = 0; i < KS; i++) {
+                        if (i + K_READ < KS) read_k(k, i + K_READ);
 #pragma unroll
-                    for (int n = 0; n < NC; n++) {
-                        top[n] = fmaxf(top[n], theirs[n]);
-                        rises |= !(top[n] <= m[n] + SLACK);
+                        for (int n = 0; n < NC; n++) s[n] = mfma32(kf[i], qf[n][i], s[n]);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                    if (Q35_RARELY(__any(rises))) {
-#pragma unroll
-                        for (int n = 0; n < NC; n++) {
-                            const float to = fmaxf(m[n], top[n]);
-                            const float by = __builtin_amdgcn_exp2f(m[n] - (to == -INFINITY ? 0.f : to));
-                            m[n] = to;
-                            l[n] *= by;
-#pragma unroll
-                            for (int d = 0; d < DT; d++) o[n][d] *= by;
-                        }
-                    }
-#pragma unroll
-                    for (int n = 0; n < NC; n++) base[n] = m[n] == -INFINITY ? 0.f : m[n];
                 }
-                __builtin_amdgcn_sched_barrier(0);
-                // a product, the exponentials of scores and a transfer beside it
-#pragma unroll
-                for (int j = LEAD; j < 16; j++) {
-                    if (!LAST) {
-                        product(j);
-#pragma unroll
-                        for (int i = 0; i < NI; i++)
-                            if (j == LEAD + 1 + i * (8 / NI)) move_k(rows, stage ^ 1, i);
-                    }
-                    if (!FIRST) {
-                        constexpr int N = 16 - LEAD;
-#pragma unroll
-                        for (int e = (j - LEAD) * 16 / N; e < (j - LEAD + 1) * 16 / N; e++)
-#pragma unroll
-                            for (int n = 0; n < NC; n++) {
-                                old[n][e] = __builtin_amdgcn_exp2f(fmaf(old[n][e], scale_log2, -base[n]));
-                                l[n] += old[n][e];
-                                if (e & 1) pf[n][e >> 3][e >> 1 & 3] = pack2(old[n][e - 1], old[n][e]);
-                            }
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                if (!FIRST) {
-                    // (a lane's probabilities are in the second product's order: keys 16 j + 4 hh .. + 3 and 8 behind these)
-#pragma unroll
-                    for (int n = 0; n < NC; n++)
-#pragma unroll
-                        for (int j = 0; j < 2; j++) *lds_u4(p_base + (n * 2 + j) * 1024) = pf[n][j];
-                }
-            } else if (!LAST) {
-#pragma unroll
-                for (int i = 0; i < NI; i++) move_k(rows, stage ^ 1, i);
+                __builtin_amdgcn_s_waitcnt(0x0f70 | NI);
+            } else {
+                wait_vm_all();
             }
-            if (!LAST) rows = rows_at(v_pool, now);
-            LAST ? wait_vm_all() : __builtin_amdgcn_s_waitcnt(0x0f70 | NI);
             __syncthreads();
             // Where some rows must not see some of the keys, a value that is an infinity or NaN is not taken away by a weight of
             // zero: it leaves the unit here, and is added below to the rows that see it.
-            const bool partly = !PLAIN && !FIRST && t * UNIT - 1 > pos0;
+            const bool partly = !first && t * UNIT - 1 > pos0;
             int odd = 0;
             if (partly) {
                 u32x4* const x = reinterpret_cast<u32x4*>(smem + (STAGES + (stage ^ 1)) * TILE) + wave * 64 * NI + lane_here();
                 bool here = false;
+#pragma unroll 1
                 for (int i = 0; i < NI; i++) {
                     u32x4 y = x[64 * i];
                     bool any = false;
@@ -533,95 +636,63 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                 __syncthreads();
                 odd = uniform(*flag);
             }
-            uint32_t lost = 0;  // runs of unit t's keys that have no page
-            if (!LAST) {
-                if (!PLAIN) {
-                    lost = (uint32_t)(bad >> ((t - from_unit) * RUNS + 2 * half & 63)) & 3;
-                    if (t + 2 >= from_unit + LOOK && t + 2 < u1) look_up(t + 1);
-                }
-                now = next;
-                if (PLAIN)
-                    next = Piece{(uint32_t)run_of(t + 2) * (uint64_t)(16 * token), whole_bytes};
-                else
-                    next = piece_of(t + 2);
-            }
-            if (PLAIN || active) {
-                const uint32_t v = v_base + (stage ^ 1) * TILE;
-                u32x4 theirs[NC][2];
-                if (!FIRST) {
-#pragma unroll
-                    for (int i = 0; i < V_READ; i++) read_v(v, i);
-#pragma unroll
-                    for (int n = 0; n < NC; n++)
-#pragma unroll
-                        for (int j = 0; j < 2; j++) theirs[n][j] = *lds_u4(p_base + other * F::P_WAVE + (n * 2 + j) * 1024);
-                }
-                const int k0 = t * UNIT + 32 * half;
-                if (!PLAIN && !LAST && (k0 + 31 > low_key || lost)) {
-                    const int hh = lane_here() >> 5;
-#pragma unroll
-                    for (int n = 0; n < NC; n++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int key = 8 * (i >> 2) + 4 * hh + (i & 3);
-                            if (k0 + key > last_key[n] || (lost >> (i >> 3) & 1)) s[n][i] = -INFINITY;
-                        }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                // a product, the maxima of scores and a transfer beside it
-                float most[NC];
-#pragma unroll
-                for (int n = 0; n < NC; n++) most[n] = s[n][0];
-#pragma unroll
-                for (int i = 0; i < 4 * DT; i++) {
-                    if (!FIRST) {
-                        if (i + V_READ < 4 * DT) read_v(v, i + V_READ);
-#pragma unroll
-                        for (int n = 0; n < NC; n++)
-                            o[n][i % DT] = mfma32(vf[i], i < 2 * DT ? pf[n][i / DT] : theirs[n][i / DT - 2], o[n][i % DT]);
-                    }
-                    if (!LAST) {
-#pragma unroll
-                        for (int j = 0; j < NI; j++)
-                            if (i == 1 + j * (2 * DT / NI)) move_v(rows, stage, j);
-                        constexpr int E = 16 / (2 * DT);  // scores each, in the first half
-                        if (i < 2 * DT)
-#pragma unroll
-                            for (int n = 0; n < NC; n++)
-#pragma unroll
-                                for (int e = i * E; e < (i + 1) * E; e++) most[n] = fmaxf(most[n], s[n][e]);
-                        if (i == 2 * DT)
-#pragma unroll
-                            for (int n = 0; n < NC; n++) top[n] = max_halves(most[n]) * scale_log2;
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                if (!LAST)  // (both lane halves have the same)
-#pragma unroll
-                    for (int n = 0; n < NC; n++) *lds_f(top_base + n * 128) = top[n];
-                if (!PLAIN && !FIRST && odd) add_odd((t - 1) * UNIT);
-            } else if (!LAST) {
+            if (!last) {
+                const u32x4 rows = rows_at(v_pool, now);
 #pragma unroll
                 for (int i = 0; i < NI; i++) move_v(rows, stage, i);
+                const uint32_t lost = (uint32_t)(bad >> ((t - from_unit) * RUNS + 2 * half & 63)) & 3;  // runs without a page
+                if (t + 2 >= from_unit + LOOK && t + 2 < u1) look_up(t + 1);
+                now = next;
+                next = piece_of(t + 2);
+                if (active) {
+                    const int k0 = t * UNIT + 32 * half;
+                    if (k0 + 31 > low_key || lost) {
+                        const int hh = lane_here() >> 5;
+#pragma unroll
+                        for (int n = 0; n < NC; n++)
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                const int key = 8 * (i >> 2) + 4 * hh + (i & 3);
+                                if (k0 + key > last_key[n] || (lost >> (i >> 3) & 1)) s[n][i] = -INFINITY;
+                            }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NC; n++) {
+                        float most = s[n][0];
+#pragma unroll
+                        for (int e = 1; e < 16; e++) most = fmaxf(most, s[n][e]);
+                        top[n] = max_halves(most) * scale_log2;
+                    }
+                    write_top();
+                }
             }
-            if (!LAST) __builtin_amdgcn_s_waitcnt(0x0f70 | NI);
+            if (active && !first) {
+                const uint32_t v = v_base + (stage ^ 1) * TILE;
+                u32x4 their_p[NC][2];
+#pragma unroll
+                for (int i = 0; i < V_READ; i++) read_v(v, i);
+                read_p(their_p);
+#pragma unroll
+                for (int i = 0; i < 4 * DT; i++) {
+                    if (i + V_READ < 4 * DT) read_v(v, i + V_READ);
+                    add_product(their_p, i);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (odd) add_odd((t - 1) * UNIT);
+            }
+            if (!last) __builtin_amdgcn_s_waitcnt(0x0f70 | NI);
             __syncthreads();
             if (partly && threadIdx.x == 0) *reinterpret_cast<int*>(smem + F::FLAG_AT) = 0;
-            if (!LAST) stage ^= 1;
+            if (!last) stage ^= 1;
         };
-        if (u0 < u1) {
-            constexpr std::true_type yes;
-            constexpr std::false_type no;
-            step(u0, yes, no, no);
-            for (int t = u0 + 1; t < u1;) {
+        if (u0 < u1)
+            for (int t = u0; t <= u1;) {
                 // units that all rows see, with whole units behind them whose pages are known and in range
                 int stop = min(min((pos0 + 1) / UNIT, keys_here / UNIT - 2), from_unit + LOOK - 2);
-                if (bad != 0 || !active) stop = t;
-                for (; t < stop; t++) step(t, no, no, yes);
-                if (t < u1) step(t++, no, no, no);
+                if (bad != 0 || !active || t == u0) stop = t;
+                for (; t < stop; t++) plain_step(t);
+                step(t++);
             }
-            step(u1, no, yes, no);
-        }
         wait_vm_all();  // (transfers of nothing, behind the last unit)
 
         // l: this wave's keys, both lane halves, and the other wave's
@@ -643,7 +714,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
         __syncthreads();  // (what was read may lie where another wave writes now)
         // The sums go through LDS, so that whole lines of a column are stored (and one loop's code does it, not one for
         // each register: code that runs once comes from memory).
-        const Args a = arguments();
+        const Args& a = arguments();
         const int slot = 2 * block + began;
         if (active) {
             const int lane = lane_here(), c32 = lane & 31, hh = lane >> 5;
@@ -657,6 +728,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                         *reinterpret_cast<f32x4*>(mine_at + (n * 32 + c32) * F::OUT_ROW + (32 * d + 8 * g + 4 * hh) * 4) =
                             f32x4{o[n][d][4 * g], o[n][d][4 * g + 1], o[n][d][4 * g + 2], o[n][d][4 * g + 3]};
             constexpr int QUADS = DH / 8, AT_ONCE = 64 / QUADS;  // quads of a column's half; columns at a time
+#pragma unroll 1
             for (int i = 0; i < 32 * NC / AT_ONCE; i++) {
                 const int here = i * AT_ONCE + lane / QUADS, d = lane % QUADS * 4, col = cg * 32 * NC + here;
                 const f32x4 x = *reinterpret_cast<const f32x4*>(mine_at + here * F::OUT_ROW + d * 4);
@@ -679,9 +751,16 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                 }
             }
         }
-        if (first_block >= 0 && threadIdx.x == 0)
-            a.cuts[block] = Cut{row0, ntok, head, first_block, block - first_block + 1};
+        if (parts > 0 && threadIdx.x == 0) a.cuts[block] = Cut{row0, ntok, head, block - parts + 1, parts};
+        if (pos >= end) return;
         __syncthreads();  // the sums are read
+        if (a.n <= 64) {
+            mine = entry_of(a, lane_here());
+            own_weight = weight_of(a, mine);
+            upto = wave_scan(own_weight);
+        } else {
+            find_window(a);
+        }
     }
 }
 
@@ -788,6 +867,9 @@ extern "C" int cs1_attention_paged_varlen(void* paged, const void* q, const void
     a.blocks = p->cus;
     a.pad = 128;
     a.least = 256;
+    a.tokens_inverse = (uint32_t)(((uint64_t{1} << 32) + a.tokens - 1) / a.tokens);
+    a.G_inverse = (65536 + a.G - 1) / a.G;
+    a.blocks_inverse = 1.0 / a.blocks;
     a.page_inverse = (uint32_t)std::min<uint64_t>(0xffffffffu, (uint64_t{1} << 32) / (a.page / 16));
     a.scale_log2 = scale * LOG2E;
     const hipStream_t st = static_cast<hipStream_t>(stream);
