@@ -40,6 +40,7 @@ using tile32::mfma32;
 using tile32::v_slot;
 
 constexpr int THREADS = 512, WAVES = 8;
+constexpr int FEW = 16;       // columns that are few
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float SLACK = 8.f;  // how far (in powers of two) a maximum may pass the exponent's base before that moves
 
@@ -55,6 +56,7 @@ struct Args {
     Cut* cuts;
     const int32_t *table, *lens, *seqs, *cu;
     int nseq, max_pages, npages, page, n, max_new, rows, Hq, Hk, G, tokens, blocks, pad, least;
+    int others;  // entries of up to so many rows are another kernel's
     uint32_t page_inverse;  // 2^32 over page / 16, rounded down
     uint32_t tokens_inverse, G_inverse;  // 2^32 over tokens and 2^16 over G, rounded up
     double blocks_inverse;               // 1 / blocks
@@ -92,9 +94,11 @@ __device__ __forceinline__ Entry entry_of(const Args& a, int i) {
     if (i >= a.n) return e;
     const int lo = a.cu[i], hi = a.cu[i + 1];
     if (lo < 0 || hi <= lo || lo >= a.rows) return e;
+    const int rows = min(min(hi, a.rows) - lo, a.max_new);
+    if (rows <= a.others) return e;
     e.s = listed_seq(a.seqs, i, a.nseq);
     e.row0 = lo;
-    e.rows = min(min(hi, a.rows) - lo, a.max_new);
+    e.rows = rows;
     const int64_t held = e.s < 0 ? 0 : min((int64_t)max(a.lens[e.s], 0), (int64_t)a.max_pages * a.page);
     e.pos = (int)(held - (hi - lo));
     return e;
@@ -131,31 +135,23 @@ __device__ __forceinline__ int64_t wave_scan(int64_t x) {
     return x;
 }
 
-// Of two bfloat16 values: is one no finite number; those that are.
-__device__ __forceinline__ bool odd16(uint32_t x) {
-    return ((x & 0x7f80u) == 0x7f80u) | ((x & 0x7f800000u) == 0x7f800000u);
-}
-__device__ __forceinline__ uint32_t common16(uint32_t x) {
-    return ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu) | ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u);
-}
-
 __device__ __forceinline__ u32x2 read_tr3(uint32_t at) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     return __builtin_bit_cast(u32x2,
                               __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
 }
 
-// Four dims of an output from sums o over l (0: no key).
-__device__ __forceinline__ void store_out(const Args& a, size_t at, const f32x4& o, float l) {
+// Four dims of an output from sums o over l (zero: no key); g: their gates, if there are any.
+__device__ __forceinline__ u32x2 load_gate(const Args& a, size_t at) {
+    return a.gate ? *reinterpret_cast<const u32x2*>(a.gate + at) : u32x2{0, 0};
+}
+__device__ __forceinline__ void store_out(const Args& a, size_t at, const f32x4& o, float l, const u32x2& g) {
     const float inv = l != 0.f ? 1.f / l : 0.f;
     float y[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) y[e] = l != 0.f ? o[e] * inv : 0.f;
-    if (a.gate) {
-        const u32x2 g = *reinterpret_cast<const u32x2*>(a.gate + at);
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (l != 0.f) y[e] *= sigmoid(e & 1 ? hi_f32(g[e / 2]) : lo_f32(g[e / 2]));
+    for (int e = 0; e < 4; e++) {
+        y[e] = l != 0.f ? o[e] * inv : 0.f;
+        if (a.gate && l != 0.f) y[e] *= sigmoid(e & 1 ? hi_f32(g[e / 2]) : lo_f32(g[e / 2]));
     }
     *reinterpret_cast<u32x2*>(a.out + at) = u32x2{pack2(y[0], y[1]), pack2(y[2], y[3])};
 }
@@ -728,15 +724,34 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                         *reinterpret_cast<f32x4*>(mine_at + (n * 32 + c32) * F::OUT_ROW + (32 * d + 8 * g + 4 * hh) * 4) =
                             f32x4{o[n][d][4 * g], o[n][d][4 * g + 1], o[n][d][4 * g + 2], o[n][d][4 * g + 3]};
             constexpr int QUADS = DH / 8, AT_ONCE = 64 / QUADS;  // quads of a column's half; columns at a time
+            if (!whole) {
+#pragma unroll 2
+                for (int i = 0; i < 32 * NC / AT_ONCE; i++) {
+                    const int here = i * AT_ONCE + lane / QUADS, d = lane % QUADS * 4, col = cg * 32 * NC + here;
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(mine_at + here * F::OUT_ROW + d * 4);
+                    if (col < cols)
+                        *reinterpret_cast<f32x4*>(a.part + ((size_t)slot * COLS + col) * DH + half * (DH / 2) + d) = x;
+                }
+            } else {
+                // (a column's gates are on their way while the one before is stored)
+                auto at_of = [&](int i) Q35_INLINE {
+                    const int here = i * AT_ONCE + lane / QUADS, d = lane % QUADS * 4, col = cg * 32 * NC + here;
+                    return column(min(col, cols - 1)).at + half * (DH / 2) + d;
+                };
+                constexpr int AHEAD = 4;
+                u32x2 gates[AHEAD];
 #pragma unroll 1
-            for (int i = 0; i < 32 * NC / AT_ONCE; i++) {
-                const int here = i * AT_ONCE + lane / QUADS, d = lane % QUADS * 4, col = cg * 32 * NC + here;
-                const f32x4 x = *reinterpret_cast<const f32x4*>(mine_at + here * F::OUT_ROW + d * 4);
-                const float l0 = __shfl(l[0], here & 31, 64), l1 = __shfl(l[NC - 1], here & 31, 64);
-                if (col < cols && whole)
-                    store_out(a, column(col).at + half * (DH / 2) + d, x, here < 32 ? l0 : l1);
-                else if (col < cols)
-                    *reinterpret_cast<f32x4*>(a.part + ((size_t)slot * COLS + col) * DH + half * (DH / 2) + d) = x;
+                for (int i0 = 0; i0 < 32 * NC / AT_ONCE; i0 += AHEAD) {
+#pragma unroll
+                    for (int i = 0; i < AHEAD; i++) gates[i] = load_gate(a, at_of(i0 + i));
+#pragma unroll
+                    for (int i = 0; i < AHEAD; i++) {
+                        const int here = (i0 + i) * AT_ONCE + lane / QUADS, d = lane % QUADS * 4, col = cg * 32 * NC + here;
+                        const f32x4 x = *reinterpret_cast<const f32x4*>(mine_at + here * F::OUT_ROW + d * 4);
+                        const float l0 = __shfl(l[0], here & 31, 64), l1 = __shfl(l[NC - 1], here & 31, 64);
+                        if (col < cols) store_out(a, at_of(i0 + i), x, here < 32 ? l0 : l1, gates[i]);
+                    }
+                }
             }
             if (half == 0 && hh == 0) {
 #pragma unroll
@@ -764,35 +779,66 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
     }
 }
 
-// Joins the parts of the item that stretch blockIdx.x ended, in the order of the stretches; block y has an eighth of the
-// columns.
-constexpr int JOIN_THREADS = 256, JOIN_SLICES = 8;
+// Joins the parts of the items that are cut, in the order of the stretches: a thread has four dims of a column, a block a
+// few columns, one piece after another of all the pieces there are. The time is that of getting at the parts, so
+// BATCH of them are asked for at once.
+constexpr int JOIN_THREADS = 256, JOIN_A_CU = 8, BATCH = 4;
 template <int DH>
-__global__ void __launch_bounds__(JOIN_THREADS) attention_chunk_join_kernel(const Args a) {
-    constexpr int COLS = Form<DH>::COLS, QUADS = DH / 4, MINE = COLS / JOIN_SLICES * QUADS / JOIN_THREADS;
-    static_assert(JOIN_THREADS % QUADS == 0, "a thread's quads are at one dim");
-    const Cut cut = a.cuts[blockIdx.x];
-    const int cols = cut.tokens * a.G, col0 = blockIdx.y * (COLS / JOIN_SLICES) + threadIdx.x / QUADS;
-    const int d = threadIdx.x % QUADS * 4;
-    if (cut.parts == 0) return;
-    auto slot_of = [&](int k) { return (size_t)(k == 0 ? 2 * cut.first + 1 : 2 * (cut.first + k)) * COLS; };
-#pragma unroll
-    for (int i = 0; i < MINE; i++) {
-        const int col = col0 + i * (JOIN_THREADS / QUADS);
-        if (col >= cols) return;
-        float top = -INFINITY, sum = 0.f;
-        for (int k = 0; k < cut.parts; k++) top = fmaxf(top, a.ml[(slot_of(k) + col) * 2]);
-        const float base = top == -INFINITY ? 0.f : top;
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < cut.parts; k++) {
-            const f32x2 ml = *reinterpret_cast<const f32x2*>(a.ml + (slot_of(k) + col) * 2);
-            const float f = __builtin_amdgcn_exp2f(ml[0] - base);
-            sum += ml[1] * f;
-            o += *reinterpret_cast<const f32x4*>(a.part + (slot_of(k) + col) * DH + d) * f;
+__global__ void __launch_bounds__(JOIN_THREADS, JOIN_A_CU) attention_chunk_join_kernel(const Args a) {
+    constexpr int COLS = Form<DH>::COLS, QUADS = DH / 4, MINE = JOIN_THREADS / QUADS, PIECES = COLS / MINE;
+    __shared__ int list[JOIN_THREADS], counts[JOIN_THREADS / 64];
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const int d = tid % QUADS * 4;
+    for (int block0 = 0; block0 < a.blocks; block0 += JOIN_THREADS) {
+        const bool cut_here = block0 + tid < a.blocks && a.cuts[block0 + tid].parts > 0;
+        const uint64_t hits = __ballot(cut_here);
+        if ((tid & 63) == 0) counts[wave] = __popcll(hits);
+        __syncthreads();
+        int at = __popcll(hits & ((uint64_t{1} << (tid & 63)) - 1)), all = 0;
+        for (int w = 0; w < JOIN_THREADS / 64; w++) {
+            if (w < wave) at += counts[w];
+            all += counts[w];
         }
-        const int tk = col / (uint32_t)a.G, head = cut.head * a.G + col - tk * a.G, row = cut.row0 + tk;
-        store_out(a, ((size_t)row * a.Hq + head) * DH + d, o, sum);
-        if (a.lse && d == 0) a.lse[(size_t)head * a.rows + row] = log_sum(top, sum);
+        if (cut_here) list[at] = block0 + tid;
+        __syncthreads();
+        for (int i = blockIdx.x; i < all * PIECES; i += gridDim.x) {
+            const Cut cut = a.cuts[list[i / PIECES]];
+            const int col = i % PIECES * MINE + tid / QUADS;
+            if (col >= cut.tokens * a.G) continue;
+            const int tk = a.over_G(col), head = cut.head * a.G + col - tk * a.G, row = cut.row0 + tk;
+            const size_t to = ((size_t)row * a.Hq + head) * DH + d;
+            const u32x2 gate = load_gate(a, to);
+            float top = -INFINITY, sum = 0.f;
+            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+            for (int k0 = 0; k0 < cut.parts; k0 += BATCH) {
+                f32x4 v[BATCH];
+                f32x2 ml[BATCH];
+#pragma unroll
+                for (int j = 0; j < BATCH; j++) {
+                    const int k = min(k0 + j, cut.parts - 1);
+                    const size_t slot = (size_t)(k == 0 ? 2 * cut.first + 1 : 2 * (cut.first + k)) * COLS + col;
+                    ml[j] = *reinterpret_cast<const f32x2*>(a.ml + slot * 2);
+                    v[j] = *reinterpret_cast<const f32x4*>(a.part + slot * DH + d);
+                }
+                float most = top;
+#pragma unroll
+                for (int j = 0; j < BATCH; j++) most = fmaxf(most, ml[j][0]);
+                const float base = most == -INFINITY ? 0.f : most, keep = __builtin_amdgcn_exp2f(top - base);
+                sum *= keep;
+                o *= keep;
+#pragma unroll
+                for (int j = 0; j < BATCH; j++) {
+                    if (k0 + j >= cut.parts) break;
+                    const float f = __builtin_amdgcn_exp2f(ml[j][0] - base);
+                    sum += ml[j][1] * f;
+                    o += v[j] * f;
+                }
+                top = most;
+            }
+            store_out(a, to, o, sum, gate);
+            if (a.lse && d == 0) a.lse[(size_t)head * a.rows + row] = log_sum(top, sum);
+        }
+        __syncthreads();
     }
 }
 
@@ -801,7 +847,7 @@ int launch(const Args& a, hipStream_t st) {
     attention_chunk_kernel<DH><<<a.blocks, THREADS, Form<DH>::BYTES, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    attention_chunk_join_kernel<DH><<<dim3(a.blocks, JOIN_SLICES), JOIN_THREADS, 0, st>>>(a);
+    attention_chunk_join_kernel<DH><<<a.blocks * JOIN_A_CU, JOIN_THREADS, 0, st>>>(a);
     return hipGetLastError();
 }
 
@@ -839,7 +885,21 @@ extern "C" int cs1_attention_paged_varlen(void* paged, const void* q, const void
         return hipErrorInvalidValue;
     int device;
     if (hipGetDevice(&device) != hipSuccess || device != p->device) return hipErrorInvalidDevice;
+    // Entries of up to 16 columns are each one tile of the kernel for single tokens, where others may be, in a launch before
+    // theirs: 43 entries of 1 to 4 tokens behind up to 4096 (16/4 heads of 256) take 90 us so and 107 in the tiles here,
+    // one of 4 behind 700 (heads of 128) 14.4 and 32; 29 of a token beside a prompt's 1021 132 and 144. One entry that may
+    // be longer is taken for longer.
+    const int64_t pairs = (int64_t)n * Hk;
+    const bool all_few = max_new <= FEW / (Hq / Hk);
     Args a;
+    a.others = 0;
+    if ((all_few || (n > 1 && Hq / Hk <= FEW)) && pairs <= 1 << 22 &&
+        pairs * ((int64_t)pages->max_pages * pages->page / 32 + 1) < LIMIT) {
+        const Call c{q, kp, vp, pages, seqs, gate, out, lse, n, Hq, Hk, Dh, scale};
+        const int e = paged_rows(p, c, cu_seqlens, max_new, rows, stream);
+        if (e != hipSuccess || all_few) return e;
+        a.others = FEW / (Hq / Hk);
+    }
     a.q = static_cast<const bf16*>(q);
     a.kp = static_cast<const bf16*>(kp);
     a.vp = static_cast<const bf16*>(vp);

@@ -55,6 +55,10 @@ struct Args {
     int nseq, max_pages, npages, page, B, Hq, Hk, G, tiles, blocks, halve, unit, pad_alone;
     uint32_t page_inverse, blocks_inverse;  // 2^32 over page / 16, rounded down, and over blocks, rounded up
     float scale_log2;
+    // several tokens a row: the offsets of their rows, at most how many, the buffers' rows, 2^16 over G rounded up
+    const int32_t* cu;
+    int max_new, all_rows;
+    uint32_t G_inverse;
 
     __device__ __forceinline__ int pad() const { return pad_alone & 255; }
     __device__ __forceinline__ int alone() const { return pad_alone >> 8; }
@@ -64,13 +68,36 @@ struct Args {
 // zero must stay one: LEAST times a value of bfloat16's largest size is 4.)
 __device__ __forceinline__ float rest(float p, float part) { return __builtin_amdgcn_fmed3f(p - part, p, LEAST); }
 
-// Row r's sequence (of its keys: none for padding).
+// Row r's sequence (of its keys: none for padding).  SEVERAL: row r is a list entry, whose tokens are `tokens` rows from
+// row0 on; n is the number of keys that the last of them sees.
 struct Row {
     int s, n;
 };
-__device__ __forceinline__ Row row_of(const Args& a, int r) {
-    const int s = r < a.B ? listed_seq(a.seqs, r, a.nseq) : -1;
-    return s < 0 ? Row{0, 0} : Row{s, (int)min((int64_t)max(a.lens[s], 0), (int64_t)a.max_pages * a.page)};
+struct Rows16 : Row {
+    int row0, tokens;
+};
+__device__ __forceinline__ int held_by(const Args& a, int s) {
+    return (int)min((int64_t)max(a.lens[s], 0), (int64_t)a.max_pages * a.page);
+}
+template <bool SEVERAL>
+__device__ __forceinline__ auto row_of(const Args& a, int r) {
+    if constexpr (SEVERAL) {
+        Rows16 x{{0, 0}, 0, 0};
+        if (r >= a.B) return x;
+        const int lo = a.cu[r], hi = a.cu[r + 1];
+        if (lo < 0 || hi <= lo || lo >= a.all_rows) return x;
+        const int s = listed_seq(a.seqs, r, a.nseq);
+        x.row0 = lo;
+        x.tokens = min(min(hi, a.all_rows) - lo, a.max_new);
+        if (x.tokens > ROWS || x.tokens * a.G > ROWS) return Rows16{{0, 0}, 0, 0};  // (another kernel's)
+        if (s < 0) return x;
+        x.s = s;
+        x.n = (int)max((int64_t)held_by(a, s) - (hi - lo) + x.tokens, (int64_t)0);
+        return x;
+    } else {
+        const int s = r < a.B ? listed_seq(a.seqs, r, a.nseq) : -1;
+        return s < 0 ? Row{0, 0} : Row{s, held_by(a, s)};
+    }
 }
 
 __device__ __forceinline__ int units_of(int n) { return n / UNIT + (n % UNIT != 0); }
@@ -117,8 +144,9 @@ __device__ __forceinline__ float over_groups(float x, F f) {
 }
 
 // Rows in the work's order, a wave's 64 at a time: only the device knows the lengths.
+template <typename R>
 struct Rows {
-    Row row;           // one row,
+    R row;             // one row,
     int chunks, upto;  // its chunks, and those of the wave's rows up to it
 };
 
@@ -127,6 +155,7 @@ struct Segment {
     int from, to, next;         // units of it (none: the stretch ends before its keys), and the chunk behind them
     int first, parts, part;     // the first block that has some of it, how many have, and which of them this is
     int slot0;                  // where the first one's results go; the others' go to 2 x their block
+    int row0, tokens;           // several tokens: as in Rows16
 
     __device__ __forceinline__ int slot(int k) const { return k == 0 ? slot0 : 2 * (first + k); }
 };
@@ -134,7 +163,8 @@ struct Segment {
 // Looks for the segment that begins at chunk `pos` of this block's stretch, which ends at `end`, among 64 rows from
 // r0 on, which begin at chunk `before`; stretches are `each` chunks long. (What runs once a launch is kept short: its
 // instructions come from memory, and divisions are long.)
-__device__ __forceinline__ bool segment_at(const Args& a, const Rows& rows, int r0, int before, int pos, int end,
+template <typename R>
+__device__ __forceinline__ bool segment_at(const Args& a, const Rows<R>& rows, int r0, int before, int pos, int end,
                                            int each, Segment& s) {
     const int heads = a.Hk * a.tiles;
     const uint64_t hit = __ballot(pos < before + rows.upto * heads);
@@ -145,6 +175,10 @@ __device__ __forceinline__ bool segment_at(const Args& a, const Rows& rows, int 
     s.row = r0 + w;
     s.s = scalar(rows.row.s, w);
     s.n = scalar(rows.row.n, w);
+    if constexpr (!std::is_same_v<R, Row>) {
+        s.row0 = scalar(rows.row.row0, w);
+        s.tokens = scalar(rows.row.tokens, w);
+    }
     for (; whole + chunks <= pos; whole += chunks)
         if (++s.tile == a.tiles) {
             s.tile = 0;
@@ -206,21 +240,26 @@ struct Shared {
     }
 };
 
-template <int DH>
+// SEVERAL: a row of the work is a list entry with up to 16 columns, its tokens' q heads of a kv head; otherwise it is a
+// token with the q heads alone.
+template <int DH, bool SEVERAL>
 __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args a) {
+    using R = std::conditional_t<SEVERAL, Rows16, Row>;
     constexpr int C = DH / 32, H = DH / 128, PITCH = DH + 8;
     // Q as operands, [C][64 lanes] x 16 bytes; then the waves' results, [WAVES][rows][PITCH]; then what joins parts
     extern __shared__ __attribute__((aligned(16))) float lds[];
     __shared__ float wm[WAVES][ROWS], wl[WAVES][ROWS];
     const int wave = scalar(threadIdx.x >> 6, 0);
     // THREADS rows at a time, a thread each, in LDS; of more than that, those last looked at
-    __shared__ Rows table[THREADS];
+    __shared__ Rows<R> table[THREADS];
     __shared__ int sums[WAVES];
     auto look_at = [&](int r0) {
         const int i = wave * 64 + lane_here(), r = r0 + i;
-        Rows x;
-        x.row = row_of(a, r);
+        Rows<R> x;
+        x.row = row_of<SEVERAL>(a, r);
         x.chunks = r < a.B ? chunks_of(a, x.row.n) : 0;
+        if constexpr (SEVERAL)
+            if (x.row.tokens == 0) x.chunks = 0;
         x.upto = wave_scan(x.chunks);
         __syncthreads();
         table[i] = x;
@@ -232,6 +271,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
     int total = look_at(0);
     for (int r0 = THREADS; r0 < a.B; r0 += THREADS) total += look_at(r0);
     total = __builtin_amdgcn_readfirstlane(total * heads);
+    if (SEVERAL && total == 0) return;
     // With heads of 128 two blocks fit on a CU (and are launched for many sequences): where these are short, on
     // average under 10 chunks (384 keys), a block's time is that of beginning and ending each, and two at once hide it.
     // 200 sequences of 260 to 384 keys take 35.3 us so and 39.0 with one, of 200 to 800 53.4 and 48.5 (16/4 heads).
@@ -251,8 +291,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
         const int lane = lane_here(), col = lane & 15, grp = lane >> 4;
         pos = sh.next;
         if (sh.parts == 0) break;
-        const int rows = min(ROWS, a.G - sh.tile * ROWS), head0 = sh.head * a.G + sh.tile * ROWS;
-        const size_t out0 = ((size_t)sh.row * a.Hq + head0) * DH;  // of q, gate and out
+        const int rows = SEVERAL ? sh.tokens * a.G : min(ROWS, a.G - sh.tile * ROWS);
+        const int head0 = sh.head * a.G + sh.tile * ROWS;
+        // of q, gate and out, the row and head that a row of the tile has
+        auto at_row = [&](int row) {
+            if constexpr (SEVERAL) {
+                const int token = (int)(row * a.G_inverse >> 16);
+                return ((size_t)(sh.row0 + token) * a.Hq + head0 + row - token * a.G) * DH;
+            } else {
+                return ((size_t)sh.row * a.Hq + head0) * DH + row * DH;
+            }
+        };
         const int u_end = sh.to;
         int u = sh.from + wave;
 
@@ -264,7 +313,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
         for (int i = 0; i < C / WAVES; i++) {
             qs[i] = u32x4{0, 0, 0, 0};
             if (col < rows)
-                qs[i] = *reinterpret_cast<const u32x4*>(a.q + out0 + col * DH + (wave + i * WAVES) * 32 + grp * 8);
+                qs[i] = *reinterpret_cast<const u32x4*>(a.q + at_row(col) + (wave + i * WAVES) * 32 + grp * 8);
         }
         f32x4 acc[H][8];
 #pragma unroll
@@ -350,6 +399,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
         __syncthreads();
         for (; u < u_end; u += WAVES) {
             const int valid[2] = {have[0], have[1]};
+            const size_t v_at[2] = {at[0], at[1]};
             f32x4 st[2][2] = {};  // two sums a half: a product does not wait for the one before
 #pragma unroll
             for (int c = 0; c < C; c++) {
@@ -367,6 +417,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
 #pragma unroll
                 for (int i = 0; i < 8; i++)
                     if (grp * 4 + (i & 3) >= valid[i >> 2]) sc[i] = -INFINITY;
+            // the last keys are tokens that those before them do not see
+            bool partly = false;
+            if constexpr (SEVERAL) {
+                partly = (u + 1) * UNIT > sh.n - (sh.tokens - 1);
+                if (partly) {
+                    const int sees = sh.n - (sh.tokens - 1) + (int)(col * a.G_inverse >> 16) - u * UNIT - grp * 4;
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        if ((i >> 2) * 16 + (i & 3) >= sees) sc[i] = -INFINITY;
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 8; i++) top = fmaxf(top, sc[i]);
             if (__any(top > m + RISE)) {
@@ -391,6 +452,27 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
                 pm[i] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302);
                 pl[i] = pack2(rest(r0, lo_f32(pm[i])), rest(r1, hi_f32(pm[i])));
             }
+            // a value there that is an infinity or NaN leaves the product, and is added to the columns that see it
+            bool odd = false;
+            if constexpr (SEVERAL) {
+                if (partly) {
+#pragma unroll
+                    for (int h = 0; h < H; h++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) odd |= odd16(vf[h][i][e]);
+                    odd = __any(odd);
+                    if (odd) {
+#pragma unroll
+                        for (int h = 0; h < H; h++)
+#pragma unroll
+                            for (int i = 0; i < 8; i++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) vf[h][i][e] = common16(vf[h][i][e]);
+                    }
+                }
+            }
 #pragma unroll
             for (int h = 0; h < H; h++) {
                 u32x4 vt[8];
@@ -406,6 +488,29 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
                 for (int j = 0; j < 8; j++) acc[h][j] = mfma16(vt[j], pm, acc[h][j]);
 #pragma unroll
                 for (int j = 0; j < 8; j++) acc[h][j] = mfma16(vt[j], pl, acc[h][j]);
+            }
+            if constexpr (SEVERAL) {
+                if (odd) {
+                    // (a lane has dims 8 (4 grp + r) + j of its column)
+                    const int sees = sh.n - (sh.tokens - 1) + (int)(col * a.G_inverse >> 16) - u * UNIT;
+#pragma unroll 1
+                    for (int key = 0; key < UNIT; key++) {
+                        const int t = key >> 4, row = key & 15;
+                        if (row >= (t ? valid[1] : valid[0])) continue;
+                        const bf16* const from = a.vp + (t ? v_at[1] : v_at[0]) + row * token + grp * 32;
+#pragma unroll
+                        for (int h = 0; h < H; h++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                const u32x4 x = *reinterpret_cast<const u32x4*>(from + h * 128 + r * 8);
+#pragma unroll
+                                for (int j = 0; j < 8; j++) {
+                                    const float y = j & 1 ? hi_f32(x[j / 2]) : lo_f32(x[j / 2]);
+                                    acc[h][j][r] += key < sees && !(fabsf(y) < INFINITY) ? y : 0.f;
+                                }
+                            }
+                    }
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
             load_v();
@@ -437,8 +542,14 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
         auto store = [&](int slot, int e, float top, float sum, const f32x4& o, const u32x2& g, bool out) {
             const int row = e / QUADS, d = e % QUADS * 4;
             if (out) {
-                store_out(a, out0 + row * DH + d, o, sum, g);
-                if (a.lse && d == 0) a.lse[(size_t)(head0 + row) * a.B + sh.row] = log_sum(top, sum);
+                store_out(a, at_row(row) + d, o, sum, g);
+                if constexpr (SEVERAL) {
+                    const int token = (int)(row * a.G_inverse >> 16);
+                    if (a.lse && d == 0)
+                        a.lse[(size_t)(head0 + row - token * a.G) * a.all_rows + sh.row0 + token] = log_sum(top, sum);
+                } else if (a.lse && d == 0) {
+                    a.lse[(size_t)(head0 + row) * a.B + sh.row] = log_sum(top, sum);
+                }
                 return;
             }
             const int at = slot * ROWS + row;
@@ -485,7 +596,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
                 u32x2 g = {0, 0};
                 f32x4 o = {0.f, 0.f, 0.f, 0.f};
                 float top, sum = 0.f;
-                if (out) g = load_gate(a, out0 + row * DH + d);
+                if (out) g = load_gate(a, at_row(row) + d);
                 if (stage == 0) {
                     top = fmaxf(fmaxf(wm[0][row], wm[1][row]), fmaxf(wm[2][row], wm[3][row]));
 #pragma unroll
@@ -548,17 +659,74 @@ size_t lds_bytes(int rows) {
 
 template <int DH>
 bool configure() {
-    return hipFuncSetAttribute(reinterpret_cast<const void*>(attention_paged_kernel<DH>),
-                               hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes<DH>(ROWS)) == hipSuccess;
+    for (const void* kernel : {reinterpret_cast<const void*>(attention_paged_kernel<DH, false>),
+                               reinterpret_cast<const void*>(attention_paged_kernel<DH, true>)})
+        if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes<DH>(ROWS)) != hipSuccess)
+            return false;
+    return true;
 }
 
 template <int DH>
 int launch(const Args& a, hipStream_t st) {
-    attention_paged_kernel<DH><<<a.blocks, THREADS, lds_bytes<DH>(a.G < ROWS ? a.G : ROWS), st>>>(a);
+    if (a.cu)
+        attention_paged_kernel<DH, true><<<a.blocks, THREADS, lds_bytes<DH>(a.max_new < ROWS ? std::min(a.max_new * a.G, ROWS) : ROWS), st>>>(a);
+    else
+        attention_paged_kernel<DH, false><<<a.blocks, THREADS, lds_bytes<DH>(a.G < ROWS ? a.G : ROWS), st>>>(a);
     return hipGetLastError();
 }
 
 }  // namespace
+
+// A call's operands as they come: n rows, or with cu (device) n list entries of up to max_new tokens each.
+int paged_rows(const Paged* p, const Call& c, const int32_t* cu, int max_new, int all_rows, void* stream) {
+    Args a;
+    a.q = static_cast<const bf16*>(c.q);
+    a.kp = static_cast<const bf16*>(c.kp);
+    a.vp = static_cast<const bf16*>(c.vp);
+    a.gate = static_cast<const bf16*>(c.gate);
+    a.out = static_cast<bf16*>(c.out);
+    a.lse = c.lse;
+    a.part = p->part;
+    a.ml = p->part + (size_t)2 * p->blocks * ROWS * 256;
+    a.count = p->count;
+    a.count2 = p->count + 2 * p->blocks;
+    a.table = c.pages->table;
+    a.lens = c.pages->lens;
+    a.seqs = c.seqs;
+    a.nseq = c.pages->nseq;
+    a.max_pages = c.pages->max_pages;
+    a.npages = c.pages->npages;
+    a.page = c.pages->page;
+    a.B = c.n;
+    a.Hq = c.Hq;
+    a.Hk = c.Hk;
+    a.G = c.Hq / c.Hk;
+    a.tiles = cu ? 1 : (a.G + ROWS - 1) / ROWS;
+    a.cu = cu;
+    a.max_new = max_new;
+    a.all_rows = all_rows;
+    a.G_inverse = (65536 + a.G - 1) / a.G;  // (exact for up to 16 columns)
+    const int64_t pairs = (int64_t)c.n * c.Hk * a.tiles;
+    a.halve = c.Dh == 128 && pairs >= p->blocks;  // the blocks, if the sequences are long
+    a.blocks = a.halve ? p->blocks : p->cus;
+    // A pair is a row with a kv head and tile.  From a pair to 16 blocks on the chunks are small, and beginning a pair
+    // counts as work: as much as 6 units of keys up to a pair a CU, as 8 beyond (about 7 us). 43 sequences of up to
+    // 4096, 16/4 heads of 256, take 71 us so, 91 if it counts as nothing.  Fewer pairs are better cut into whole chunks of 4.
+    // Short sequences are one chunk, which is not cut, and joined by no one; the fewer pairs, the longer they may
+    // be without the work being shared out badly: one of 300 keys (heads of 128) takes 8.4 us with 12 units and 9.8 with 8,
+    // 64 of 100 to 200 (256) 12.4 with 8 and 20.0 with 4, 40 of up to 1000 22.4 and 25.6 with 12, 300 of up to 400 66 with 4
+    // and 80 with 8.
+    const bool several = pairs * 16 >= a.blocks, many = pairs > p->cus;
+    a.unit = several ? 2 : 4;
+    const int pad = many ? 4 : several ? 3 : 0, alone = many ? 4 : several ? 8 : 12;
+    a.pad_alone = alone << 8 | pad;
+    a.page_inverse = (uint32_t)std::min<uint64_t>(0xffffffffu, (uint64_t{1} << 32) / (a.page / 16));
+    a.blocks_inverse = (uint32_t)(((uint64_t{1} << 32) + a.blocks - 1) / a.blocks);
+    a.scale_log2 = c.scale * LOG2E;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    return c.Dh == 128 ? launch<128>(a, st) : launch<256>(a, st);
+}
+
 }  // namespace q35
 
 using namespace q35;
@@ -616,45 +784,6 @@ extern "C" int cs1_attention_paged(void* paged, const void* q, const void* kp, c
         return hipErrorInvalidValue;
     int device;
     if (hipGetDevice(&device) != hipSuccess || device != p->device) return hipErrorInvalidDevice;
-    Args a;
-    a.q = static_cast<const bf16*>(q);
-    a.kp = static_cast<const bf16*>(kp);
-    a.vp = static_cast<const bf16*>(vp);
-    a.gate = static_cast<const bf16*>(gate);
-    a.out = static_cast<bf16*>(out);
-    a.lse = lse;
-    a.part = p->part;
-    a.ml = p->part + (size_t)2 * p->blocks * ROWS * 256;
-    a.count = p->count;
-    a.count2 = p->count + 2 * p->blocks;
-    a.table = pages->table;
-    a.lens = pages->lens;
-    a.seqs = seqs;
-    a.nseq = pages->nseq;
-    a.max_pages = pages->max_pages;
-    a.npages = pages->npages;
-    a.page = pages->page;
-    a.B = B;
-    a.Hq = Hq;
-    a.Hk = Hk;
-    a.G = Hq / Hk;
-    a.tiles = (a.G + ROWS - 1) / ROWS;
-    a.halve = Dh == 128 && pairs >= p->blocks;  // the blocks, if the sequences are long
-    a.blocks = a.halve ? p->blocks : p->cus;
-    // A pair is a row with a kv head and tile.  From a pair to 16 blocks on the chunks are small, and beginning a pair
-    // counts as work: as much as 6 units of keys up to a pair a CU, as 8 beyond (about 7 us). 43 sequences of up to
-    // 4096, 16/4 heads of 256, take 71 us so, 91 if it counts as nothing.  Fewer pairs are better cut into whole chunks of 4.
-    // Short sequences are one chunk, which is not cut, and joined by no one; the fewer pairs, the longer they may
-    // be without the work being shared out badly: one of 300 keys (heads of 128) takes 8.4 us with 12 units and 9.8 with 8,
-    // 64 of 100 to 200 (256) 12.4 with 8 and 20.0 with 4, 40 of up to 1000 22.4 and 25.6 with 12, 300 of up to 400 66 with 4
-    // and 80 with 8.
-    const bool several = pairs * 16 >= a.blocks, many = pairs > p->cus;
-    a.unit = several ? 2 : 4;
-    const int pad = many ? 4 : several ? 3 : 0, alone = many ? 4 : several ? 8 : 12;
-    a.pad_alone = alone << 8 | pad;
-    a.page_inverse = (uint32_t)std::min<uint64_t>(0xffffffffu, (uint64_t{1} << 32) / (a.page / 16));
-    a.blocks_inverse = (uint32_t)(((uint64_t{1} << 32) + a.blocks - 1) / a.blocks);
-    a.scale_log2 = scale * LOG2E;
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    return Dh == 128 ? launch<128>(a, st) : launch<256>(a, st);
+    const Call c{q, kp, vp, pages, seqs, gate, out, lse, B, Hq, Hk, Dh, scale};
+    return paged_rows(p, c, nullptr, 0, 0, stream);
 }

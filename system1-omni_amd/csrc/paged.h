@@ -16,6 +16,17 @@ struct Paged {
     int* count;    // [2 blocks] parts of a group, [2 blocks] groups of a sequence that are done
     float* chunk;  // several tokens: chunk_bytes
 };
+struct Call {
+    const void *q, *kp, *vp;
+    const Cs1PageTable* pages;
+    const int32_t* seqs;
+    const void* gate;
+    void* out;
+    float* lse;
+    int n, Hq, Hk, Dh;
+    float scale;
+};
+int paged_rows(const Paged* p, const Call& c, const int32_t* cu, int max_new, int all_rows, void* stream);
 bool chunk_configure();
 size_t chunk_bytes(int cus);
 
@@ -26,6 +37,14 @@ inline bool table_ok(const Cs1PageTable* t) {
 }
 
 inline bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Of two bfloat16 values: is one no finite number; those that are.
+__device__ __forceinline__ bool odd16(uint32_t x) {
+    return ((x & 0x7f80u) == 0x7f80u) | ((x & 0x7f800000u) == 0x7f800000u);
+}
+__device__ __forceinline__ uint32_t common16(uint32_t x) {
+    return ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu) | ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u);
+}
 
 // The sequence of list entry i, or -1 for a padding row.
 __device__ __forceinline__ int listed_seq(const int32_t* __restrict__ seqs, int i, int nseq) {
