@@ -5,7 +5,7 @@
 // pages that a list of sequences receives are the lowest-numbered free ones in the list's order.
 // With need_i new pages for entry i and off_i the sum of the needs before it, the free page with k
 // free pages below it goes to the entry with off_i <= k < off_i + need_i.  One block of 1024 threads does
-// that: a scan over the needs, then scans over 4096 counts at a time until enough pages are found.
+// that: a scan over the needs, then scans over 4096 counts, and then 16384 at a time, until enough pages are found.
 // What moves keys and values is a kernel of its own that fills the chip: a page's filled rows are one run of bytes in
 // each pool.
 #include "common.h"
@@ -67,31 +67,87 @@ __device__ __forceinline__ int entry_of(const int* off, int n, int k) {
     return lo;
 }
 
-// Whether pages p .. p + 3 are free, as four bits.
-__device__ __forceinline__ uint32_t free_pages(const int32_t* __restrict__ refs, int npages, int p) {
-    int count[4];
+// Counts of pages from `base` on: a wave has 64 N of them in a row, a lane every 64th.
+constexpr int NEAR = 4, FAR = 16;
+template <int N>
+struct Counts {
+    int of[N];
+};
+template <int N>
+__device__ __forceinline__ Counts<N> page_counts(const int32_t* __restrict__ refs, int npages, int base) {
+    Counts<N> c;
+    const uint32_t p = (uint32_t)base + (threadIdx.x >> 6) * (64 * N) + (threadIdx.x & 63);
 #pragma unroll
-    for (int e = 0; e < 4; e++) count[e] = refs[min(p + e, npages - 1)];
-    uint32_t bits = 0;
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-        bits |= (uint32_t)((p + e < npages) & (count[e] == 0)) << e;
-    return bits;
+    for (int j = 0; j < N; j++) c.of[j] = refs[min(p + j * 64, (uint32_t)npages - 1)];
+    return c;
 }
 
-// Calls take(k, page) for the `total` lowest free pages, k = 0 .., or for all there are; returns their number. bits: of
-// pages 4 threadIdx.x .. + 3, asked for early by the caller.
-template <typename Take>
-__device__ __forceinline__ int take_free(const int32_t* refs, int npages, int total, uint32_t bits, int* red,
-                                         Take take) {
-    int found = 0;
-    for (int base = 0; base < npages && found < total; base += 4 * PLAN_THREADS) {
-        const int p = base + 4 * threadIdx.x;
-        if (base > 0) bits = free_pages(refs, npages, p);
-        int all, k = found + block_scan(__popc(bits), red, all);
-        for (; bits && k < total; bits &= bits - 1, k++) take(k, p + __ffs(bits) - 1);
-        found = min(total, found + all);
+// Free pages, by their number k among all free ones, as far as they are found.  They are collected in LDS and taken all
+// at once, a thread each: taking one is a search and two loads, one after the other, and where few pages are free among
+// many every scan would wait for its own (200 sequences of 39 new tokens, 800 free pages among 52000: 30 us with
+// scans of 4096 that took what they found, 16 with a thread for each found, 14 so).
+struct Free {
+    int page[4096], wave[PLAN_WAVES];  // numbers from `taken` on
+};
+template <int N, typename Take>
+__device__ __forceinline__ void find_among(const Counts<N>& counts, int npages, int base, int total, int& taken, int& found,
+                                           Free& f, Take take) {
+    constexpr int ROOM = sizeof(f.page) / sizeof(int);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int at = base + wave * (64 * N);
+    uint64_t free[N];
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        free[j] = __ballot(at + j * 64 + lane < npages && counts.of[j] == 0);
+        mine += __popcll(free[j]);
     }
+    __syncthreads();
+    if (lane == 0) f.wave[wave] = mine;
+    __syncthreads();
+    int first = found, all = 0;
+#pragma unroll
+    for (int w = 0; w < PLAN_WAVES; w++) {
+        const int r = f.wave[w];
+        if (w < wave) first += r;
+        all += r;
+    }
+    found = min(total, found + all);
+    for (;;) {
+        int k0 = first;
+        if (mine > 0)
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const int k = k0 + __popcll(free[j] & ((uint64_t{1} << lane) - 1));
+                if ((free[j] >> lane & 1) && k >= taken && k < min(found, taken + ROOM)) f.page[k - taken] = at + j * 64 + lane;
+                k0 += __popcll(free[j]);
+            }
+        if (found - taken < ROOM) break;
+        __syncthreads();
+        for (int k = threadIdx.x; k < ROOM; k += PLAN_THREADS) take(taken + k, f.page[k]);
+        __syncthreads();
+        taken += ROOM;
+    }
+}
+
+// Calls take(k, page) for the `total` lowest free pages, k = 0 .., or for all there are; returns their number.  near: the
+// counts of the first pages, asked for early by the caller.
+template <typename Take>
+__device__ __forceinline__ int take_free(const int32_t* refs, int npages, int total, const Counts<NEAR>& near, Free& f,
+                                         Take take) {
+    int found = 0, taken = 0, base = NEAR * PLAN_THREADS;
+    if (total <= 0) return 0;
+    find_among(near, npages, 0, total, taken, found, f, take);
+    if (found < total && base < npages) {
+        auto counts = page_counts<FAR>(refs, npages, base);
+        for (; base < npages && found < total; base += FAR * PLAN_THREADS) {
+            const auto next = page_counts<FAR>(refs, npages, base + FAR * PLAN_THREADS);  // (on its way meanwhile)
+            find_among(counts, npages, base, total, taken, found, f, take);
+            counts = next;
+        }
+    }
+    __syncthreads();
+    for (int k = taken + (int)threadIdx.x; k < found; k += PLAN_THREADS) take(k, f.page[k - taken]);
     return found;
 }
 
@@ -104,10 +160,11 @@ __global__ void __launch_bounds__(PLAN_THREADS)
                       const int32_t* __restrict__ rows, int n, int32_t* status) {
     __shared__ int work[MAX_LISTED];  // first entry that names a sequence, then the offsets off_i
     __shared__ int red[PLAN_WAVES];
+    __shared__ Free free;
     const int tid = threadIdx.x;
     asm volatile("" ::"s"(t.table), "s"(t.lens), "s"(t.refs), "s"(t.nseq), "s"(t.max_pages), "s"(t.npages), "s"(t.page),
                  "s"(seqs), "s"(cu.n), "s"(n), "s"(status));
-    const uint32_t bits = free_pages(t.refs, t.npages, 4 * tid);
+    const Counts<NEAR> near = page_counts<NEAR>(t.refs, t.npages, 0);
     const int per = PER == 1 ? 1 : (n + PLAN_THREADS - 1) / PLAN_THREADS, i0 = tid * per;
     int seq[PER], len[PER];
     int64_t add[PER];
@@ -155,7 +212,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
         const int i = entry_of(work, n, k), s = listed_seq(seqs, i, t.nseq);
         return t.table + (size_t)s * t.max_pages + pages_of(max(t.lens[s], 0), t.page) + (k - work[i]);
     };
-    const int found = take_free(t.refs, t.npages, total, bits, red, [&](int k, int p) {
+    const int found = take_free(t.refs, t.npages, total, near, free, [&](int k, int p) {
         *slot(k) = p;
         t.refs[p] = 1;
     });
@@ -284,19 +341,32 @@ __global__ void __launch_bounds__(PLAN_THREADS)
             held = min(pages_of(len[e], t.page), t.max_pages);
             t.lens[seq[e]] = to[e];
         }
-        auto release = [&](int32_t* entry) {
-            const int p = *entry;
-            *entry = -1;
+        auto release = [&](int p) {
             if (p >= 0 && p < t.npages) atomicSub(&t.refs[p], 1);
         };
         // a few pages a thread, and where there are many a wave
-        if (held - j <= 4) {
-            for (; j < held; j++) release(row + j);
+        constexpr int FEW = 4;
+        if (held - j <= 2 * FEW) {
+            for (; j < held; j += FEW) {
+                int p[FEW];
+#pragma unroll
+                for (int u = 0; u < FEW; u++) p[u] = j + u < held ? row[j + u] : -1;
+#pragma unroll
+                for (int u = 0; u < FEW; u++) {
+                    if (j + u < held) row[j + u] = -1;
+                    release(p[u]);
+                }
+            }
         }
         for (uint64_t many = __ballot(j < held); many; many &= many - 1) {
             const int w = __ffsll((unsigned long long)many) - 1, to_page = __shfl(held, w, 64);
             const int s = __shfl(seq[e], w, 64);
-            for (int k = __shfl(j, w, 64) + lane; k < to_page; k += 64) release(t.table + (size_t)s * t.max_pages + k);
+            for (int k = __shfl(j, w, 64) + lane; k < to_page; k += 64) {
+                int32_t* const entry = t.table + (size_t)s * t.max_pages + k;
+                const int p = *entry;
+                *entry = -1;
+                release(p);
+            }
         }
     }
 }
@@ -366,10 +436,11 @@ __global__ void __launch_bounds__(PLAN_THREADS)
                         Pair* __restrict__ plan, int32_t* status) {
     __shared__ int work[MAX_LISTED];
     __shared__ int red[PLAN_WAVES];
+    __shared__ Free free;
     const int tid = threadIdx.x;
     asm volatile("" ::"s"(t.table), "s"(t.lens), "s"(t.refs), "s"(t.nseq), "s"(t.max_pages), "s"(t.npages), "s"(t.page),
                  "s"(src), "s"(dst), "s"(n), "s"(plan), "s"(status));
-    const uint32_t bits = free_pages(t.refs, t.npages, 4 * tid);
+    const Counts<NEAR> near = page_counts<NEAR>(t.refs, t.npages, 0);
     const int per = PER == 1 ? 1 : (n + PLAN_THREADS - 1) / PLAN_THREADS, i0 = tid * per;
     int from[PER], to[PER];
     Pair mine[PER];
@@ -409,7 +480,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
         off += mine[e].rows > 0;
     }
     __syncthreads();
-    const int found = take_free(t.refs, t.npages, total, bits, red, [&](int k, int p) {
+    const int found = take_free(t.refs, t.npages, total, near, free, [&](int k, int p) {
         plan[entry_of(work, n, k)].to = p;
         t.refs[p] = 1;
     });

@@ -39,22 +39,44 @@ __device__ __forceinline__ float value_of(Key k) {
     return __uint_as_float(up & 0x80000000u ? up & 0x7fffffffu : ~up);
 }
 __device__ __forceinline__ uint32_t index_of(Key k) { return 0xffffffffu - (uint32_t)k; }
-__device__ __forceinline__ Key shuffle_xor(Key k, int o) {
-    return (Key)__shfl_xor((uint32_t)(k >> 32), o, 64) << 32 | __shfl_xor((uint32_t)k, o, 64);
-}
 
-// The wave's keys in falling order, by compare and exchange in a bitonic net.
-__device__ __forceinline__ Key sorted(Key k) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int size = 2; size <= 64; size *= 2)
-#pragma unroll
-        for (int o = size / 2; o > 0; o /= 2) {
-            const Key other = shuffle_xor(k, o);
-            const bool first = (lane & o) == 0, falls = (lane & size) == 0 || size == 64;
-            k = (first == falls) == (k > other) ? k : other;
-        }
-    return k;
+// Over a wave's lanes, the same in each: within rows of 16, then each row's last lane to the next row, then lane 31 to
+// the upper half.  (Shuffles go through LDS and take many times as long: a row's alternatives from 38 parts took 11 us by
+// them, and take 6 so.)
+template <typename T, typename F>
+__device__ __forceinline__ T over_wave(T x, T none, F f) {
+#define Q35_STEP(ctrl, rows)                                                                                            \
+    x = f(x, __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, x), \
+                                                               ctrl, rows, 0xf, false)))
+    Q35_STEP(0x111, 0xf);
+    Q35_STEP(0x112, 0xf);
+    Q35_STEP(0x114, 0xf);
+    Q35_STEP(0x118, 0xf);
+    Q35_STEP(0x142, 0xa);
+    Q35_STEP(0x143, 0xc);
+#undef Q35_STEP
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+    return over_wave(x, 0u, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+__device__ __forceinline__ float wave_max(float x) {
+    return over_wave(x, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float wave_sum(float x) {
+    return over_wave(x, 0.f, [](float a, float b) { return a + b; });
+}
+// The lane that has the largest key of the wave (the first of several), and the key.
+__device__ __forceinline__ int wave_best(Key mine, Key& best) {
+    const uint32_t hi = (uint32_t)(mine >> 32), lo = (uint32_t)mine, most = wave_max(hi);
+    uint64_t have = __ballot(hi == most);
+    if (have & (have - 1)) {
+        const uint32_t of = hi == most ? lo : 0u, first = wave_max(of);
+        have = __ballot(hi == most && of == first);
+    }
+    const int lane = __ffsll((unsigned long long)have) - 1;
+    best = (Key)most << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, lane);
+    return lane;
 }
 
 // Base m, sum of e^(x - m) and of that times x - m.  Differences and not logarithms of base 2 are kept, so that a large
@@ -76,10 +98,8 @@ __device__ __forceinline__ Sums merged(const Sums& a, const Sums& b) {
     return Sums{m, x.sum + y.sum, x.dot + y.dot, 0.f};
 }
 __device__ __forceinline__ Sums wave_merged(Sums a) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        a = merged(a, Sums{__shfl_xor(a.m, o, 64), __shfl_xor(a.sum, o, 64), __shfl_xor(a.dot, o, 64), 0.f});
-    return a;
+    a = rebased(a, wave_max(a.m));
+    return Sums{a.m, wave_sum(a.sum), wave_sum(a.dot), 0.f};
 }
 
 struct Args {
@@ -150,17 +170,15 @@ struct Part {
         else
             return __uint_as_float(v[e]);
     }
-    // f(key) for each logit of thread t's loads, shared out over a wave's lanes
+    // f(key) for each logit of load j
     template <typename F>
-    __device__ __forceinline__ void each_key(int t, int lane, uint32_t first, F f) const {
-        for (int j = t + lane * THREADS; j <= whole + 1; j += 64 * THREADS) {
-            if (j >= 1 && j <= whole) {
-                const u32x4 v = full(j);
+    __device__ __forceinline__ void each_key(int j, uint32_t first, F f) const {
+        if (j >= 1 && j <= whole) {
+            const u32x4 v = full(j);
 #pragma unroll
-                for (int e = 0; e < N; e++) f(key_of(at(v, e), first + index(j) + e));
-            } else {
-                for (int e = 0; e < count(j); e++) f(key_of(as_float(p[index(j) + e]), first + index(j) + e));
-            }
+            for (int e = 0; e < N; e++) f(key_of(at(v, e), first + index(j) + e));
+        } else {
+            for (int e = 0; e < count(j); e++) f(key_of(as_float(p[index(j) + e]), first + index(j) + e));
         }
     }
 };
@@ -169,13 +187,16 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS) logprobs_kernel(const Args a) {
     constexpr int N = Part<T>::N;
     __shared__ Sums wave_sums[WAVES];
-    __shared__ Key best_of[64], list[LIST], found;
-    __shared__ int listed, threads, who[THREADS];
+    __shared__ Key best_of[64], list[LIST + WAVES], found;
+    __shared__ int listed, threads, who[THREADS], above[64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row = blockIdx.x / (uint32_t)a.parts, part = blockIdx.x - row * a.parts;
     const int first = part * a.each;
     const Part<T> x(static_cast<const T*>(a.logits) + (size_t)row * a.ld + first, min(a.each, a.V - first));
-    if (tid < 64) best_of[tid] = 0;
+    if (tid < 64) {
+        best_of[tid] = 63 - tid;  // below all, and none like another
+        above[tid] = 0;
+    }
     if (tid == 0) listed = threads = 0;
 
     float m = -INFINITY, sum = 0.f, dot = 0.f, best = -INFINITY;
@@ -251,13 +272,20 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const Args a) {
     // where the load has it is not known, so the value counts as its last logit here, and as its first below
     if (best_at >= 0) atomicMax(&best_of[lane], key_of(best, first + x.index(best_at) + x.count(best_at) - 1));
     __syncthreads();
-    const Key in_order = sorted(best_of[lane]);
-    const Key least = (Key)__shfl((uint32_t)(in_order >> 32), a.k - 1, 64) << 32 |
-                      (uint32_t)__shfl((uint32_t)in_order, a.k - 1, 64);
+    const Key its = best_of[lane];
+    int larger = 0;
+#pragma unroll
+    for (int j = 0; j < 64 / WAVES; j++) larger += best_of[wave * (64 / WAVES) + j] > its;
+    atomicAdd(&above[lane], larger);
+    __syncthreads();
+    const int kth = __ffsll((unsigned long long)__ballot(above[lane] == a.k - 1)) - 1;
+    const Key least = (Key)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(its >> 32), kth) << 32 |
+                      (uint32_t)__builtin_amdgcn_readlane((uint32_t)its, kth);
     if (best_at >= 0 && key_of(best, first + x.index(best_at)) >= least) who[atomicAdd(&threads, 1)] = tid;
     __syncthreads();
-    for (int i = wave; i < threads; i += WAVES)
-        x.each_key(who[i], lane, first, [&](Key k) {
+    const int loads = (x.whole + 1) / THREADS + 1;  // of a thread, at most
+    for (int i = tid; i < threads * loads; i += THREADS)
+        x.each_key(who[i / (uint32_t)loads] + i % (uint32_t)loads * THREADS, first, [&](Key k) {
             if (k < least) return;
             const int at = atomicAdd(&listed, 1);
             if (at < LIST) list[at] = k;
@@ -277,7 +305,9 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const Args a) {
             }
             const Key mine = list[i];
             int rank = 0;
-            for (int j = 0; j < listed; j++) rank += list[j] > mine;
+            for (int j = 0; j < listed; j += WAVES)  // (some on their way at once)
+#pragma unroll
+                for (int u = 0; u < WAVES; u++) rank += j + u < listed && list[j + u] > mine;
             if (rank < a.k) store(rank, mine);
         }
         return;
@@ -288,15 +318,11 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const Args a) {
         if (tid == 0) found = 0;
         __syncthreads();
         Key mine = 0;
-        for (int t = wave; t < THREADS; t += WAVES)
-            x.each_key(t, lane, first, [&](Key k) {
+        for (int j = tid; j <= x.whole + 1; j += THREADS)
+            x.each_key(j, first, [&](Key k) {
                 if (k < before && k > mine) mine = k;
             });
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const Key other = shuffle_xor(mine, o);
-            mine = mine > other ? mine : other;
-        }
+        (void)wave_best(mine, mine);
         if (lane == 0) atomicMax(&found, mine);
         __syncthreads();
         before = found;
@@ -305,29 +331,39 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const Args a) {
     }
 }
 
-// A wave a row joins its parts: a lane has a part, whose alternatives are in order.
+// Joins a row's parts: wave 0 the alternatives, a lane for a part, whose own are in order; wave 1 the sums.
+constexpr int JOIN_THREADS = 256;
 template <typename T>
-__global__ void __launch_bounds__(64) logprobs_join_kernel(const Args a) {
+__global__ void __launch_bounds__(JOIN_THREADS) logprobs_join_kernel(const Args a) {
+    constexpr int MINE = PARTS_MAX * K_MAX / JOIN_THREADS;
     __shared__ Key keys[PARTS_MAX * K_MAX];
-    const int row = blockIdx.x, lane = threadIdx.x;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, all = a.parts * a.k;
+    Key v[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; i++)
+        if (tid + i * JOIN_THREADS < all) v[i] = a.keys[(size_t)row * all + tid + i * JOIN_THREADS];
     Sums s = Sums{-INFINITY, 0.f, 0.f, 0.f};
     if (lane < a.parts) s = a.sums[(size_t)row * a.parts + lane];
-    for (int i = lane; i < a.parts * a.k; i += 64) keys[i] = a.keys[(size_t)row * a.parts * a.k + i];
-    s = wave_merged(s);
-    if (lane == 0) store_row<T>(a, row, s);
+#pragma unroll
+    for (int i = 0; i < MINE; i++)
+        if (tid + i * JOIN_THREADS < all) keys[tid + i * JOIN_THREADS] = v[i];
     __syncthreads();
+    if (tid >= 128) return;
+    s = wave_merged(s);
+    if (tid == 64) store_row<T>(a, row, s);
+    if (tid >= 64) return;
     Key mine = 0;  // the lane-th best
     int next = 0;
+    auto at = [&](int i) { return lane < a.parts && i < a.k ? keys[lane * a.k + i] : (Key)0; };
+    Key head = at(0), after = at(1);  // (what follows is on its way while the best is looked for)
     for (int i = 0; i < a.k; i++) {
-        const Key head = lane < a.parts && next < a.k ? keys[lane * a.k + next] : 0;
-        Key most = head;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const Key other = shuffle_xor(most, o);
-            most = most > other ? most : other;
+        Key best;
+        const int from = wave_best(head, best);
+        if (lane == i) mine = best;
+        if (lane == from) {
+            head = after;
+            after = at(++next + 1);
         }
-        if (head == most) next++;  // (one lane's, or none is left)
-        if (lane == i) mine = most;
     }
     if (lane < a.k) store_top(a, row, lane, mine, s);
 }
@@ -387,6 +423,6 @@ extern "C" int cs1_token_logprobs(const void* logits, int is_float, size_t ld, c
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.parts == 1) return e;
     const auto join = is_float ? logprobs_join_kernel<float> : logprobs_join_kernel<bf16>;
-    join<<<rows, 64, 0, st>>>(a);
+    join<<<rows, JOIN_THREADS, 0, st>>>(a);
     return hipGetLastError();
 }
