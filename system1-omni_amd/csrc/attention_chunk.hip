@@ -125,13 +125,19 @@ __device__ __forceinline__ int lane_here() {
     asm volatile("" : "+v"(lane));
     return lane;
 }
-// Sum over this lane and those below.
+// Sum over this lane and those below: within rows of 16 lanes, then each row's last lane to the next row (into rows
+// 1 and 3), then lane 31 to the upper half.
 __device__ __forceinline__ int64_t wave_scan(int64_t x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int lo = __shfl_up((int)x, o, 64), hi = __shfl_up((int)(x >> 32), o, 64);
-        if ((int)(threadIdx.x & 63) >= o) x += (int64_t)(uint32_t)lo | (int64_t)hi << 32;
-    }
+#define Q35_ADD(ctrl, rows)                                                                                \
+    x += (int64_t)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false) |               \
+         (int64_t)__builtin_amdgcn_update_dpp(0, (int)(x >> 32), ctrl, rows, 0xf, false) << 32
+    Q35_ADD(0x111, 0xf);
+    Q35_ADD(0x112, 0xf);
+    Q35_ADD(0x114, 0xf);
+    Q35_ADD(0x118, 0xf);
+    Q35_ADD(0x142, 0xa);
+    Q35_ADD(0x143, 0xc);
+#undef Q35_ADD
     return x;
 }
 
@@ -235,11 +241,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
 
     for (;;) {
         int seq, row0, ntok, pos0, keys, head = 0, u0, u1;
-        bool whole, began;  // all of the item is in this stretch; it begins there
+        bool whole, began;  // all of the item's keys are in this stretch; they begin there
         int parts = 0;      // of an item that ends here and began elsewhere
-        {
-            // the item at `pos`
-            const Args& a = arguments();
+        // The item at `pos`.  What a stretch has of the pad alone is no part of the item: a stretch without keys of it goes on.
+        // (Item of no keys: its zeros are written where it begins.)
+        for (const Args& a = arguments();;) {
+            head = 0;
             const int el = __ffsll((unsigned long long)__ballot(window_at + upto > pos)) - 1;
             const int erow = scalar(mine.row0, el), erows = scalar(mine.rows, el);
             const int epos = scalar(mine.pos, el), items = items_of(a, erows);
@@ -248,13 +255,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
             seq = scalar(mine.s, el);
 #pragma unroll 1
             for (; hstart + own <= pos; hstart += own) head++;
-            int c = 0;  // the last item that begins at or before pos
-            for (int up = items - 1; c < up;) {
-                const int mid = (c + up + 1) >> 1;
-                if (hstart + line_of(a, epos, mid) <= pos)
-                    c = mid;
-                else
-                    up = mid - 1;
+            int c = -1;  // the last item that begins at or before pos
+            for (int c0 = 0; c0 < items; c0 += 64) {
+                const int it = c0 + lane_here();
+                const int n = __popcll(__ballot(it < items && hstart + line_of(a, epos, it) <= pos));
+                c += n;
+                if (n < 64) break;
             }
             const int64_t istart = hstart + line_of(a, epos, c), iend = hstart + line_of(a, epos, c + 1);
             const int tok0 = c * a.tokens;
@@ -268,12 +274,18 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
             };
             u0 = uniform(cut(begin));
             u1 = uniform(cut(end));
-            began = istart >= begin;
-            whole = began && iend <= end;
-            if (!began && iend <= end)
-#pragma unroll 1
-                for (int64_t x = begin + each; x > istart; x -= each) parts++;
+            began = u0 == 0;
+            whole = began && u1 == units;
             pos = min(iend, end);
+            if (u0 < u1 || (units == 0 && istart >= begin)) {
+                if (began || u1 < units) break;
+                parts = 2;
+#pragma unroll 1
+                for (int64_t x = begin - each; cut(x) > 0; x -= each) parts++;
+                break;
+            }
+            if (pos >= end) return;
+            if (a.n > 64) find_window(a);
         }
         // a column is a row and a q head of the kv head's
         const int G = uniform(arguments().G), Hq = uniform(arguments().Hq), cols = ntok * G;
@@ -291,20 +303,23 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
             x.at = ((size_t)(row0 + x.token) * Hq + x.head) * DH;
             return x;
         };
-        u32x4 qf[NC][KS];
-        int last_key[NC];  // that this lane's columns see
+        // Q, a pair's columns by halves: whole lines here, and as operands by way of LDS (operands from memory, 16 bytes a
+        // column at a time, took 2 us more)
+        constexpr int QN = 16 * NC * CHUNKS / 64;
+        u32x4 qs[QN];
         {
-            const int lane = lane_here();
             const bf16* const q = arguments().q;
 #pragma unroll
-            for (int n = 0; n < NC; n++) {
-                const int col = (cg * NC + n) * 32 + (lane & 31);
-                const Column x = column(min(col, cols - 1));
-                last_key[n] = col < cols ? pos0 + x.token : -1;
-#pragma unroll
-                for (int i = 0; i < KS; i++)
-                    qf[n][i] = *reinterpret_cast<const u32x4*>(q + x.at + 16 * i + 8 * (lane >> 5));
+            for (int i = 0; i < QN; i++) {
+                const int at = i * 64 + lane_here(), col = cg * 32 * NC + half * 16 * NC + at / CHUNKS;
+                qs[i] = *reinterpret_cast<const u32x4*>(q + column(min(col, cols - 1)).at + at % CHUNKS * 8);
             }
+        }
+        int last_key[NC];  // that this lane's columns see
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            const int col = (cg * NC + n) * 32 + (lane_here() & 31);
+            last_key[n] = col < cols ? pos0 + column(col).token : -1;
         }
 
         // The next 64 runs of 16 tokens: lane i has the pool's run of run number i from here on, -1 if its page is out of range
@@ -380,10 +395,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
         Piece now = piece_of(u0), next = piece_of(u0 + 1);  // of units t and t + 1
 #pragma unroll
         for (int j = 0; j < NI; j++) move_k(rows_at(k_pool, now), 0, j);
+        constexpr int Q_AT = STAGES * TILE;  // (where no value is before the first step's barrier)
 #pragma unroll
-        for (int n = 0; n < NC; n++)
-#pragma unroll
-            for (int i = 0; i < KS; i++) asm volatile("" ::"v"(qf[n][i]));
+        for (int i = 0; i < QN; i++) {
+            const int at = i * 64 + lane_here(), col = half * 16 * NC + at / CHUNKS;
+            *reinterpret_cast<u32x4*>(smem + Q_AT + (cg * 32 * NC + col) * ROW + (k_slot(col, at % CHUNKS) << 4)) = qs[i];
+        }
         if (threadIdx.x == 0) *reinterpret_cast<int*>(smem + F::FLAG_AT) = 0;
         const float scale_log2 = arguments().scale_log2;
         wait_vm_all();
@@ -406,6 +423,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
         const int other = 4 - 8 * half;  // from this wave to the other one of its pair
         auto lds_u4 = [](uint32_t at) Q35_INLINE { return (__attribute__((address_space(3))) u32x4*)at; };
         auto lds_f = [](uint32_t at) Q35_INLINE { return (__attribute__((address_space(3))) float*)at; };
+        u32x4 qf[NC][KS];
+        {
+            const int lane = lane_here(), c32 = lane & 31;
+            const uint32_t q = lds + Q_AT + (cg * 32 * NC + c32) * ROW + (k_slot(c32, lane >> 5) << 4);
+#pragma unroll
+            for (int n = 0; n < NC; n++)
+#pragma unroll
+                for (int i = 0; i < KS; i++) qf[n][i] = *lds_u4((q + n * 32 * ROW ^ (i & 7) << 5) + (i >> 3) * 256);
+        }
         constexpr int K_READ = DH == 256 ? 6 : 3, V_READ = DH == 256 ? 6 : 3;  // operands read ahead
         u32x4 kf[KS], vf[4 * DT];
         auto read_k = [&](uint32_t k, int i) Q35_INLINE { kf[i] = *lds_u4((k ^ (i & 7) << 5) + (i >> 3) * 256); };
@@ -925,8 +951,8 @@ extern "C" int cs1_attention_paged_varlen(void* paged, const void* q, const void
     a.G = Hq / Hk;
     a.tokens = (Dh == 128 ? Form<128>::COLS : Form<256>::COLS) / a.G;
     a.blocks = p->cus;
-    a.pad = 128;
-    a.least = 256;
+    a.pad = 256;
+    a.least = 192;
     a.tokens_inverse = (uint32_t)(((uint64_t{1} << 32) + a.tokens - 1) / a.tokens);
     a.G_inverse = (65536 + a.G - 1) / a.G;
     a.blocks_inverse = 1.0 / a.blocks;
