@@ -412,7 +412,8 @@ int cs1_attn_prep_paged(const void* qg, const void* kr, const void* v, int ld, c
 /* Attention of such a batch's rows over the pages, which hold their keys and values already: q, gate (null: none) and
  * out [rows, Hq, Dh]; the row at position p of its sequence sees keys 0 .. p.  max_new is the most rows that an entry has
  * (those behind it are left out).  out and lse [Hq, rows] (float32, null: not written) as in cs1_attention_paged, but
- * for the probabilities, which go to the second product as bfloat16.  Rows of padding entries and rows before position
+ * for the probabilities, which go to the second product as bfloat16 (entries of up to 16 / (Hq / Hk) rows: as there, if
+ * max_new is no more or n > 1).  Rows of padding entries and rows before position
  * 0 get zeros and an lse of -inf; rows behind cu_seqlens[n] are left as they are.  A sequence may be named twice.  Keys of a page
  * whose number is out of range are left out.  scale > 0 (1e-30 to 1e30), Hq / Hk <= 128, rows * Hq <= 2^24,
  * Hk * Dh <= 2^24, npages * page < 2^31; q, kp, vp, gate and out on 16 bytes.  The handle is cs1_attention_paged's, with
