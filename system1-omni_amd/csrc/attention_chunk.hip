@@ -163,6 +163,17 @@ __device__ __forceinline__ void store_out(const Args& a, size_t at, const f32x4&
 }
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * LN2; }
 
+// Two transfers of 1024 bytes (dma16) in a row of LDS: the offset in the instruction counts in LDS and in memory, so the
+// second scalar offset is less by 1024.
+__device__ __forceinline__ void dma16x2(const u32x4& rsrc, uint32_t lds, int voff0, int voff1, int soff, int step) {
+    const int soff1 = __builtin_amdgcn_readfirstlane(soff + step - 1024);
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 3\n\t"
+        "buffer_load_dwordx4 %1, %3, %4 offen lds\n\tbuffer_load_dwordx4 %2, %3, %5 offen offset:1024 lds" ::"s"(lds),
+        "v"(voff0), "v"(voff1), "s"(rsrc), "s"(soff), "s"(soff1)
+        : "memory");
+}
+
 #define Q35_INLINE __attribute__((always_inline))
 #define Q35_RARELY(x) __builtin_expect(!!(x), 0)  // (what is rare is laid out behind the loop over the keys)
 
@@ -239,6 +250,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
     }
     const int64_t begin = pos;
 
+    // The end of an item that began elsewhere comes last of a stretch, so that at any time those blocks that have as much
+    // of a line (the q heads of a kv head at different rows, all with nearly the same keys) are at the same key: whole items and
+    // beginnings go on from key 0 at once, and what is left of the first item is as far from its end as the stretch is.  (Where
+    // a stretch is shorter than its item there is less of that than a second search takes.)
+    // A unit that is read by the 32 blocks of an XCD comes from its L2 then (2048 rows behind 30720, 24/4 heads of
+    // 256: 1680 us in the line's order, 1530 so).
+    enum { STRAIGHT, FIRST_IS_LEFT, AT_FIRST } order = STRAIGHT;
     for (;;) {
         int seq, row0, ntok, pos0, keys, head = 0, u0, u1;
         bool whole, began;  // all of the item's keys are in this stretch; they begin there
@@ -277,14 +295,21 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
             began = u0 == 0;
             whole = began && u1 == units;
             pos = min(iend, end);
-            if (u0 < u1 || (units == 0 && istart >= begin)) {
+            const bool some = u0 < u1 || (units == 0 && istart >= begin);
+            if (some && order == STRAIGHT && !began && pos < end && iend - istart <= each) {
+                order = FIRST_IS_LEFT;
+            } else if (some) {
                 if (began || u1 < units) break;
                 parts = 2;
 #pragma unroll 1
                 for (int64_t x = begin - each; cut(x) > 0; x -= each) parts++;
                 break;
             }
-            if (pos >= end) return;
+            if (pos >= end) {
+                if (order != FIRST_IS_LEFT) return;
+                order = AT_FIRST;
+                pos = begin;
+            }
             if (a.n > 64) find_window(a);
         }
         // a column is a row and a q head of the kv head's
@@ -373,12 +398,23 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
             k_lane = row * token + (k_slot(r0 + row, place) << 4);
             v_lane = row * token + (v_slot(row, place) << 4);
         }
-        auto move_k = [&](const u32x4& r, int stage, int i) Q35_INLINE {
-            dma16(r, (uint32_t)uniform((int)(lds0 + stage * TILE + i * 1024)), k_lane ^ (i * PER) << 4, uniform(i * PER * token));
+        // A wave's transfers of a unit go one by one between the products; where there are only two, together, which saves a
+        // few instructions (1000 rows behind 8000, 32/8 heads of 128: 172 us apart, 166 so; of four, two or all together are
+        // slower: 2048 behind 30720, 24/4 heads of 256, 1680 us apart, 1690 in twos, 1735 at once).
+        constexpr int SET = NI == 2 ? 2 : 1, SETS = NI / SET;
+        auto move = [&](const u32x4& r, int at, int set, auto lane_of) Q35_INLINE {
+            const uint32_t to = (uint32_t)uniform((int)(lds0 + at + set * SET * 1024));
+            const int from = uniform(set * SET * PER * token);
+            if constexpr (SET == 2)
+                dma16x2(r, to, lane_of(0), lane_of(1), from, PER * token);
+            else
+                dma16(r, to, lane_of(set), from);
         };
-        auto move_v = [&](const u32x4& r, int stage, int i) Q35_INLINE {
-            dma16(r, (uint32_t)uniform((int)(lds0 + (STAGES + stage) * TILE + i * 1024)), PER == 2 && i & 1 ? v_lane ^ 12 << 4 : v_lane,
-                  uniform(i * PER * token));
+        auto move_k = [&](const u32x4& r, int stage, int set) Q35_INLINE {
+            move(r, stage * TILE, set, [&](int i) Q35_INLINE { return k_lane ^ (i * PER) << 4; });
+        };
+        auto move_v = [&](const u32x4& r, int stage, int set) Q35_INLINE {
+            move(r, (STAGES + stage) * TILE, set, [&](int i) Q35_INLINE { return PER == 2 && i & 1 ? v_lane ^ 12 << 4 : v_lane; });
         };
 
         f32x16 o[NC][DT], s[NC], old[NC];  // scores of the last unit, and of the one before
@@ -394,7 +430,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
 
         Piece now = piece_of(u0), next = piece_of(u0 + 1);  // of units t and t + 1
 #pragma unroll
-        for (int j = 0; j < NI; j++) move_k(rows_at(k_pool, now), 0, j);
+        for (int j = 0; j < SETS; j++) move_k(rows_at(k_pool, now), 0, j);
         constexpr int Q_AT = STAGES * TILE;  // (where no value is before the first step's barrier)
 #pragma unroll
         for (int i = 0; i < QN; i++) {
@@ -555,8 +591,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                 if (n == 0 && i + K_READ < KS) read_k(k, i + K_READ);
                 s[n] = mfma32(kf[i], qf[n][i], s[n]);
 #pragma unroll
-                for (int x = 0; x < NI; x++)
-                    if (j == LEAD + 1 + x * (8 / NI)) move_k(rows, stage ^ 1, x);
+                for (int x = 0; x < SETS; x++)
+                    if (j == LEAD + 1 + x * (8 / SETS)) move_k(rows, stage ^ 1, x);
                 if (j >= LEAD)
 #pragma unroll
                     for (int e = (j - LEAD) * 16 / N; e < (j - LEAD + 1) * 16 / N; e++) exponential(old, e);
@@ -581,8 +617,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                 if (i + V_READ < 4 * DT) read_v(v, i + V_READ);
                 add_product(their_p, i);
 #pragma unroll
-                for (int x = 0; x < NI; x++)
-                    if (i == 1 + x * (2 * DT / NI)) move_v(rows, stage, x);
+                for (int x = 0; x < SETS; x++)
+                    if (i == 1 + x * (2 * DT / SETS)) move_v(rows, stage, x);
                 constexpr int E = 16 / (2 * DT);  // scores each, in the first half
 #pragma unroll
                 for (int n = 0; n < NC; n++) {
@@ -612,7 +648,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
             if (!last) {
                 const u32x4 rows = rows_at(k_pool, next);
 #pragma unroll
-                for (int i = 0; i < NI; i++) move_k(rows, stage ^ 1, i);
+                for (int i = 0; i < SETS; i++) move_k(rows, stage ^ 1, i);
                 if (active) {
                     const uint32_t k = k_base + stage * TILE;
 #pragma unroll
@@ -661,7 +697,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
             if (!last) {
                 const u32x4 rows = rows_at(v_pool, now);
 #pragma unroll
-                for (int i = 0; i < NI; i++) move_v(rows, stage, i);
+                for (int i = 0; i < SETS; i++) move_v(rows, stage, i);
                 const uint32_t lost = (uint32_t)(bad >> ((t - from_unit) * RUNS + 2 * half & 63)) & 3;  // runs without a page
                 if (t + 2 >= from_unit + LOOK && t + 2 < u1) look_up(t + 1);
                 now = next;
@@ -793,7 +829,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
             }
         }
         if (parts > 0 && threadIdx.x == 0) a.cuts[block] = Cut{row0, ntok, head, block - parts + 1, parts};
-        if (pos >= end) return;
+        if (order == AT_FIRST) return;
+        if (pos >= end) {
+            if (order == STRAIGHT) return;
+            order = AT_FIRST;
+            pos = begin;
+        }
         __syncthreads();  // the sums are read
         if (a.n <= 64) {
             mine = entry_of(a, lane_here());
