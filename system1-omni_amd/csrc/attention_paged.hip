@@ -241,9 +241,10 @@ struct Shared {
 };
 
 // SEVERAL: a row of the work is a list entry with up to 16 columns, its tokens' q heads of a kv head; otherwise it is a
-// token with the q heads alone.
+// token with the q heads alone.  (Heads of 128 then have more code that wants registers, and the compiler has to be told that
+// two blocks share a CU: 200 entries behind up to 400 take 35 us so, 54 with one.)
 template <int DH, bool SEVERAL>
-__global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, SEVERAL && DH == 128 ? 2 : 1) attention_paged_kernel(const Args a) {
     using R = std::conditional_t<SEVERAL, Rows16, Row>;
     constexpr int C = DH / 32, H = DH / 128, PITCH = DH + 8;
     // Q as operands, [C][64 lanes] x 16 bytes; then the waves' results, [WAVES][rows][PITCH]; then what joins parts
@@ -588,6 +589,49 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
             const bool out = stage == 0 ? sh.parts == 1 : stage == 2 || groups == 1;
             const int k0 = stage == 1 ? g0 : 0, step = stage == 2 ? group : 1, n = stage == 1 ? members : groups;
             const int ways = stage == 0 ? 1 : max(1, THREADS / QUADS >> rows_log);
+            auto find_weights = [&]() {
+                if constexpr (SEVERAL) {  // 16 lanes a row, all rows at once (4 rows behind 700: 14.5 us a wave a row, 13.0 so)
+                    const int me = wave * 64 + lane_here(), r = me / 16, c = me % 16;
+                    f32x2 m[GROUP / 16];
+                    float most = -INFINITY, all = 0.f;
+#pragma unroll
+                    for (int j = 0; j < GROUP / 16; j++) {
+                        const int k = c + 16 * j;
+                        m[j] = shared.get_ml(k < n && r < rows ? (sh.slot(k0 + k * step) * ROWS + r) * 8 : -1);
+                        if (k >= n) m[j][0] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int j = 0; j < GROUP / 16; j++) most = fmaxf(most, m[j][0]);
+                    most = lane_max<16>(most);
+#pragma unroll
+                    for (int j = 0; j < GROUP / 16; j++) {
+                        const int k = c + 16 * j;
+                        const float f = k >= n ? 0.f : m[j][0] == most ? 1.f : __builtin_amdgcn_exp2f(m[j][0] - most);
+                        weight[k * ROWS + r] = f;
+                        if (k < n) all += m[j][1] * f;
+                    }
+                    all = lane_sum<16>(all);
+                    if (c == 0 && r < rows) {
+                        wm[0][r] = most;
+                        wl[0][r] = all;
+                    }
+                    __syncthreads();
+                    return;
+                }
+                const int k = tid & 63;
+                for (int r = wave; r < rows; r += WAVES) {
+                    const f32x2 m = shared.get_ml((sh.slot(k0 + min(k, n - 1) * step) * ROWS + r) * 8);
+                    const float most = lane_max<64>(m[0]);
+                    const float f = k >= n ? 0.f : m[0] == most ? 1.f : __builtin_amdgcn_exp2f(m[0] - most);
+                    weight[k * ROWS + r] = f;
+                    const float all = lane_sum<64>(k < n ? m[1] * f : 0.f);
+                    if (k == 0) {
+                        wm[0][r] = most;
+                        wl[0][r] = all;
+                    }
+                }
+                __syncthreads();
+            };
             for (int e0 = 0; e0 < items; e0 += THREADS) {
                 const int way = ways > 1 ? tid / QUADS >> rows_log : 0;
                 const int e = e0 + (ways > 1 ? tid & ((QUADS << rows_log) - 1) : tid);
@@ -613,21 +657,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_paged_kernel(const Args 
                             const int k = k1 + i * ways;
                             v[i] = shared.get(k < n ? ((sh.slot(k0 + k * step) * ROWS + row) * DH + d) * 4 : -1);
                         }
-                        if (e0 == 0 && k1 == way) {
-                            const int k = tid & 63;
-                            for (int r = wave; r < rows; r += WAVES) {
-                                const f32x2 m = shared.get_ml((sh.slot(k0 + min(k, n - 1) * step) * ROWS + r) * 8);
-                                const float most = lane_max<64>(m[0]);
-                                const float f = k >= n ? 0.f : m[0] == most ? 1.f : __builtin_amdgcn_exp2f(m[0] - most);
-                                weight[k * ROWS + r] = f;
-                                const float all = lane_sum<64>(k < n ? m[1] * f : 0.f);
-                                if (k == 0) {
-                                    wm[0][r] = most;
-                                    wl[0][r] = all;
-                                }
-                            }
-                            __syncthreads();
-                        }
+                        if (e0 == 0 && k1 == way) find_weights();
 #pragma unroll
                         for (int i = 0; i < BATCH; i++) o += v[i] * weight[min(k1 + i * ways, GROUP - 1) * ROWS + row];
                     }
