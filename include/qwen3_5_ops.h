@@ -323,8 +323,8 @@ int cs1_kv_compact(const Cs1PageTable* pages, void* const* pools, int npools, si
 int cs1_kv_copy(void* const* pools, int npools, size_t entry_bytes, int entries, const int32_t* src, const int32_t* dst,
                 int n, void* stream);
 
-/* Attention of one new token per row over the pages (after cs1_kv_write), which no other call reads: several new
- * tokens of a sequence, behind its first prompt, go through it one after another.  q, gate (null: none) and
+/* Attention of one new token per row over the pages (after cs1_kv_write); of several of a sequence at once:
+ * cs1_attention_paged_varlen.  q, gate (null: none) and
  * out [B, Hq, Dh], Dh 128 or 256; row r's q head h sees the lens[s] keys of sequence s = seqs[r] through kv
  * head h / (Hq / Hk).  lse [Hq, B] float32 (null: not written) as in cs1_attention_ex.  Unlike there the
  * output is rounded once, after the gate.  A padding row, or one of an empty sequence, gets zeros and an

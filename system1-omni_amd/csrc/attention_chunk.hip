@@ -4,10 +4,10 @@
 //   S_i = scale q . k_i,  m = max S_i,  l = sum exp(S_i - m),  out = sigmoid(gate) (sum exp(S_i - m) v_i) / l,
 //   lse = m + log l.
 //
-// Work: an item is up to 128 columns (heads of 256) or 256 (of 128), the q heads of one kv head at some of an entry's rows, with all keys that
-// they see: however many q heads share a kv head, they share its keys too.  All items of a launch form one line, measured in
-// keys, that is cut into equal stretches, one a block: a prompt's part on its own, drafts of a few tokens behind
-// long texts and single tokens share the chip alike, and only the device knows the lengths.  What a stretch has of an
+// Work: an item is up to 128 columns (heads of 256) or 256 (of 128), the q heads of one kv head at some of an entry's rows, with
+// all keys that they see: however many q heads share a kv head, they share its keys too.  All items of a launch form one
+// line, measured in keys, that is cut into equal stretches, one a block: a prompt's part on its own and drafts
+// behind long texts share the chip alike, and only the device knows the lengths.  What a stretch has of an
 // item that others have parts of goes to memory, and a second launch joins the parts in order.
 //
 // A block has eight waves: four groups of columns by two halves.  Of a unit of 64 keys a wave makes the scores of one half of
@@ -22,6 +22,10 @@
 //
 // P is rounded to bfloat16 for the second product, as in the prefill: the matrix cores set the time here, and a second part of
 // P would cost half as much again.  Sums and maxima are float32; out is rounded once, after the gate.
+//
+// 2048 rows behind 30720 (24/4 heads of 256) take 1531 us, 1044 TFLOP/s where a large product reaches 1436: 3640 clocks a unit
+// of which the matrix cores are busy 2048.  333 behind 936 (16/4 heads) take 36: of about 45 thousand clocks a block 20 are its
+// four units, 8 finding them, 6 Q and the first K, 5 the sums' way out, and then the join.
 #include <math.h>
 
 #include <algorithm>
@@ -992,6 +996,9 @@ extern "C" int cs1_attention_paged_varlen(void* paged, const void* q, const void
     a.G = Hq / Hk;
     a.tokens = (Dh == 128 ? Form<128>::COLS : Form<256>::COLS) / a.G;
     a.blocks = p->cus;
+    // What an item takes around its steps counts as 256 keys (four units), and no stretch is shorter than three units: 512 rows
+    // alone (24/4 heads of 256) take 42.6 us so, 58 with 192 keys and 42.9 with 320; 20 behind 300 (16/4) 21.5, and 24.3
+    // and 27.1 with stretches of at least 256 and 384.
     a.pad = 256;
     a.least = 192;
     a.tokens_inverse = (uint32_t)(((uint64_t{1} << 32) + a.tokens - 1) / a.tokens);
