@@ -96,11 +96,11 @@ struct Entry {
 __device__ __forceinline__ Entry entry_of(const Args& a, int i) {
     Entry e{-1, 0, 0, 0};
     if (i >= a.n) return e;
-    const int lo = a.cu[i], hi = a.cu[i + 1];
+    const int lo = a.cu[i], hi = a.cu[i + 1], s = listed_seq(a.seqs, i, a.nseq);  // (asked for together)
     if (lo < 0 || hi <= lo || lo >= a.rows) return e;
     const int rows = min(min(hi, a.rows) - lo, a.max_new);
     if (rows <= a.others) return e;
-    e.s = listed_seq(a.seqs, i, a.nseq);
+    e.s = s;
     e.row0 = lo;
     e.rows = rows;
     const int64_t held = e.s < 0 ? 0 : min((int64_t)max(a.lens[e.s], 0), (int64_t)a.max_pages * a.page);

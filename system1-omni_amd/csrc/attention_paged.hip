@@ -84,9 +84,8 @@ __device__ __forceinline__ auto row_of(const Args& a, int r) {
     if constexpr (SEVERAL) {
         Rows16 x{{0, 0}, 0, 0};
         if (r >= a.B) return x;
-        const int lo = a.cu[r], hi = a.cu[r + 1];
+        const int lo = a.cu[r], hi = a.cu[r + 1], s = listed_seq(a.seqs, r, a.nseq);  // (asked for together)
         if (lo < 0 || hi <= lo || lo >= a.all_rows) return x;
-        const int s = listed_seq(a.seqs, r, a.nseq);
         x.row0 = lo;
         x.tokens = min(min(hi, a.all_rows) - lo, a.max_new);
         if (x.tokens > ROWS || x.tokens * a.G > ROWS) return Rows16{{0, 0}, 0, 0};  // (another kernel's)
