@@ -151,23 +151,13 @@ __device__ __forceinline__ u32x2 read_tr3(uint32_t at) {
                               __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
 }
 
-// Four dims of an output from sums o over l (zero: no key); g: their gates, if there are any.
-__device__ __forceinline__ u32x2 load_gate(const Args& a, size_t at) {
-    return a.gate ? *reinterpret_cast<const u32x2*>(a.gate + at) : u32x2{0, 0};
-}
-__device__ __forceinline__ void store_out(const Args& a, size_t at, const f32x4& o, float l, const u32x2& g) {
-    // (the hardware's reciprocal, within a float32 step as the gate's, and no branches: with divisions and the gate behind a
-    // branch a whole item's way out took 14 us of 5)
-    const float inv = __builtin_amdgcn_rcpf(l);
-    float y[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) y[e] = o[e] * inv;
-    if (a.gate)
-#pragma unroll
-        for (int e = 0; e < 4; e++) y[e] *= gate_sigmoid(e & 1 ? hi_f32(g[e / 2]) : lo_f32(g[e / 2]));
-#pragma unroll
-    for (int e = 0; e < 4; e++) y[e] = l != 0.f ? y[e] : 0.f;
-    *reinterpret_cast<u32x2*>(a.out + at) = u32x2{pack2(y[0], y[1]), pack2(y[2], y[3])};
+// Dims of an output from their sums over l (zero: no key); the words of g have their gates, if there are any.
+__device__ __forceinline__ uint32_t out_of(bool gated, float o0, float o1, float l, float inv, uint32_t g) {
+    if (gated) {
+        o0 *= gate_sigmoid(lo_f32(g));
+        o1 *= gate_sigmoid(hi_f32(g));
+    }
+    return pack2(l != 0.f ? o0 * inv : 0.f, l != 0.f ? o1 * inv : 0.f);
 }
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * LN2; }
 
@@ -793,8 +783,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                     for (int g = 0; g < 4; g++)
                         *reinterpret_cast<f32x4*>(mine_at + (n * 32 + c32) * F::OUT_ROW + (32 * d + 8 * g + 4 * hh) * 4) =
                             f32x4{o[n][d][4 * g], o[n][d][4 * g + 1], o[n][d][4 * g + 2], o[n][d][4 * g + 3]};
-            constexpr int QUADS = DH / 8, AT_ONCE = 64 / QUADS;  // quads of a column's half; columns at a time
             if (!whole) {
+                constexpr int QUADS = DH / 8, AT_ONCE = 64 / QUADS;  // quads of a column's half; columns at a time
 #pragma unroll 2
                 for (int i = 0; i < 32 * NC / AT_ONCE; i++) {
                     const int here = i * AT_ONCE + lane / QUADS, d = lane % QUADS * 4, col = cg * 32 * NC + here;
@@ -803,24 +793,30 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
                         *reinterpret_cast<f32x4*>(a.part + ((size_t)slot * COLS + col) * DH + half * (DH / 2) + d) = x;
                 }
             } else {
-                // (a column's gates are on their way while the one before is stored)
-                auto at_of = [&](int i) Q35_INLINE {
-                    const int here = i * AT_ONCE + lane / QUADS, d = lane % QUADS * 4, col = cg * 32 * NC + here;
-                    return column(min(col, cols - 1)).at + half * (DH / 2) + d;
-                };
-                constexpr int AHEAD = 4;
-                u32x2 gates[AHEAD];
-#pragma unroll 1
-                for (int i0 = 0; i0 < 32 * NC / AT_ONCE; i0 += AHEAD) {
+                // a lane has eight dims of every AT_ONCE-th column, whose gates are asked for together
+                constexpr int LANES = DH / 16, AT_ONCE = 64 / LANES, EACH = 32 * NC / AT_ONCE;
+                const int first = lane / LANES, d = lane % LANES * 8;
+                u32x4 gates[EACH];
+                size_t to[EACH];
 #pragma unroll
-                    for (int i = 0; i < AHEAD; i++) gates[i] = load_gate(a, at_of(i0 + i));
+                for (int i = 0; i < EACH; i++) {
+                    to[i] = column(min(cg * 32 * NC + i * AT_ONCE + first, cols - 1)).at + half * (DH / 2) + d;
+                    gates[i] = u32x4{0, 0, 0, 0};
+                    if (a.gate) gates[i] = *reinterpret_cast<const u32x4*>(a.gate + to[i]);
+                }
+                float inv[NC];  // (the hardware's reciprocal, within a float32 step as the gate's)
 #pragma unroll
-                    for (int i = 0; i < AHEAD; i++) {
-                        const int here = (i0 + i) * AT_ONCE + lane / QUADS, d = lane % QUADS * 4, col = cg * 32 * NC + here;
-                        const f32x4 x = *reinterpret_cast<const f32x4*>(mine_at + here * F::OUT_ROW + d * 4);
-                        const float l0 = __shfl(l[0], here & 31, 64), l1 = __shfl(l[NC - 1], here & 31, 64);
-                        if (col < cols) store_out(a, at_of(i0 + i), x, here < 32 ? l0 : l1, gates[i]);
-                    }
+                for (int n = 0; n < NC; n++) inv[n] = __builtin_amdgcn_rcpf(l[n]);
+#pragma unroll
+                for (int i = 0; i < EACH; i++) {
+                    const int here = i * AT_ONCE + first, n = i * AT_ONCE / 32;
+                    const f32x4* const x = reinterpret_cast<const f32x4*>(mine_at + here * F::OUT_ROW + d * 4);
+                    const f32x4 x0 = x[0], x1 = x[1];
+                    const float sum = __shfl(l[n], here & 31, 64), r = __shfl(inv[n], here & 31, 64);
+                    const bool gated = a.gate != nullptr;
+                    const u32x4 y = {out_of(gated, x0[0], x0[1], sum, r, gates[i][0]), out_of(gated, x0[2], x0[3], sum, r, gates[i][1]),
+                                     out_of(gated, x1[0], x1[1], sum, r, gates[i][2]), out_of(gated, x1[2], x1[3], sum, r, gates[i][3])};
+                    if (cg * 32 * NC + here < cols) *reinterpret_cast<u32x4*>(a.out + to[i]) = y;
                 }
             }
             if (half == 0 && hh == 0) {
@@ -882,7 +878,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, JOIN_A_CU) attention_chunk_join_
             if (col >= cut.tokens * a.G) continue;
             const int tk = a.over_G(col), head = cut.head * a.G + col - tk * a.G, row = cut.row0 + tk;
             const size_t to = ((size_t)row * a.Hq + head) * DH + d;
-            const u32x2 gate = load_gate(a, to);
+            const u32x2 gate = a.gate ? *reinterpret_cast<const u32x2*>(a.gate + to) : u32x2{0, 0};
             float top = -INFINITY, sum = 0.f;
             f32x4 o = {0.f, 0.f, 0.f, 0.f};
             for (int k0 = 0; k0 < cut.parts; k0 += BATCH) {
@@ -910,7 +906,9 @@ __global__ void __launch_bounds__(JOIN_THREADS, JOIN_A_CU) attention_chunk_join_
                 }
                 top = most;
             }
-            store_out(a, to, o, sum, gate);
+            const float inv = __builtin_amdgcn_rcpf(sum);
+            *reinterpret_cast<u32x2*>(a.out + to) = u32x2{out_of(a.gate != nullptr, o[0], o[1], sum, inv, gate[0]),
+                                                          out_of(a.gate != nullptr, o[2], o[3], sum, inv, gate[1])};
             if (a.lse && d == 0) a.lse[(size_t)head * a.rows + row] = log_sum(top, sum);
         }
         __syncthreads();
