@@ -199,9 +199,22 @@ __device__ __forceinline__ bool segment_at(const Args& a, const Rows<R>& rows, i
 __device__ __forceinline__ u32x2 load_gate(const Args& a, size_t at) {
     return a.gate ? *reinterpret_cast<const u32x2*>(a.gate + at) : u32x2{0, 0};
 }
+template <bool SEVERAL>
 __device__ __forceinline__ void store_out(const Args& a, size_t at, const f32x4& o, float l, const u32x2& g) {
-    const float inv = l != 0.f ? 1.f / l : 0.f;
     float y[4];
+    if constexpr (SEVERAL) {  // a thread has some: the hardware's reciprocal, within a float32 step, and no branches
+        const float inv = __builtin_amdgcn_rcpf(l);
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = o[e] * inv;
+        if (a.gate)
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] *= gate_sigmoid(e & 1 ? hi_f32(g[e / 2]) : lo_f32(g[e / 2]));
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = l != 0.f ? y[e] : 0.f;
+        *reinterpret_cast<u32x2*>(a.out + at) = u32x2{pack2(y[0], y[1]), pack2(y[2], y[3])};
+        return;
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         y[e] = l != 0.f ? o[e] * inv : 0.f;
@@ -542,7 +555,7 @@ __global__ void __launch_bounds__(THREADS, SEVERAL && DH == 128 ? 2 : 1) attenti
         auto store = [&](int slot, int e, float top, float sum, const f32x4& o, const u32x2& g, bool out) {
             const int row = e / QUADS, d = e % QUADS * 4;
             if (out) {
-                store_out(a, at_row(row) + d, o, sum, g);
+                store_out<SEVERAL>(a, at_row(row) + d, o, sum, g);
                 if constexpr (SEVERAL) {
                     const int token = (int)(row * a.G_inverse >> 16);
                     if (a.lse && d == 0)
