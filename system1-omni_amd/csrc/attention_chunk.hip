@@ -85,7 +85,8 @@ struct Form {
     static constexpr int TOP_AT = P_AT + WAVES * P_WAVE;
     static constexpr int FLAG_AT = TOP_AT + WAVES * 128 * NC;
     static constexpr int OUT_ROW = 2 * DH + 16;        // bytes of a column's half of the sums at the end, padded
-    static constexpr int BYTES = FLAG_AT + 16 > WAVES * 32 * NC * OUT_ROW ? FLAG_AT + 16 : WAVES * 32 * NC * OUT_ROW;
+    static constexpr int KEPT_AT = FLAG_AT + 16 > WAVES * 32 * NC * OUT_ROW ? FLAG_AT + 16 : WAVES * 32 * NC * OUT_ROW;
+    static constexpr int BYTES = KEPT_AT + 3 * 64 * 8;  // (what a wave has for the search of many entries, see find_window)
     static_assert(BYTES <= 160 * 1024, "fits in the LDS");
 };
 
@@ -198,10 +199,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
     // the line's place window_at on.
     Entry mine;
     int64_t own_weight, upto, window_at = 0, pos, end, each;
-    volatile int64_t kept[3];  // (in memory: the loop over the keys needs the registers)
-    // more entries: lane i has the weights of windows 2 i and 2 i + 1 of 64 entries, and those up to them
+    // more entries: lane i has the weights of windows 2 i and 2 i + 1 of 64 entries, and those up to them (in LDS: the loop over
+    // the keys needs the registers)
+    int64_t* const kept = reinterpret_cast<int64_t*>(smem + F::KEPT_AT);
     auto find_window = [&](const Args& a) Q35_INLINE {
-        const int64_t all = kept[2], w0 = kept[0], w1 = kept[1];
+        const int at = lane_here();
+        const int64_t all = kept[128 + at], w0 = kept[at], w1 = kept[64 + at];
         const int lane = __ffsll((unsigned long long)__ballot(all > pos)) - 1;
         const int64_t first = scalar64(w0, lane), before = scalar64(all, lane) - first - scalar64(w1, lane);
         const bool second = pos >= before + first;
@@ -228,11 +231,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
             }
             __syncthreads();
             const int64_t w0 = 2 * lane < windows ? sums[2 * lane] : 0, w1 = 2 * lane + 1 < windows ? sums[2 * lane + 1] : 0;
-            __syncthreads();
             const int64_t all = wave_scan(w0 + w1);
-            kept[0] = w0;
-            kept[1] = w1;
-            kept[2] = all;
+            if (wave == 0) {
+                kept[lane] = w0;
+                kept[64 + lane] = w1;
+                kept[128 + lane] = all;
+            }
+            __syncthreads();
             total = scalar64(all, 63);
         }
         // (one more than need be; the line is far shorter than 2^50)
