@@ -270,20 +270,23 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
             head = 0;
             const int el = __ffsll((unsigned long long)__ballot(window_at + upto > pos)) - 1;
             const int erow = scalar(mine.row0, el), erows = scalar(mine.rows, el);
-            const int epos = scalar(mine.pos, el), items = items_of(a, erows);
-            const int64_t own = line_of(a, epos, items);
+            const int own_items = items_of(a, mine.rows), epos = scalar(mine.pos, el), items = scalar(own_items, el);
+            const int64_t own = scalar64(line_of(a, mine.pos, own_items), el);
             int64_t hstart = window_at + scalar64(upto - own_weight, el);
             seq = scalar(mine.s, el);
 #pragma unroll 1
             for (; hstart + own <= pos; hstart += own) head++;
-            int c = -1;  // the last item that begins at or before pos
+            int c = 0;  // the last item that begins at or before pos, and where it does
+            int64_t istart = hstart;
             for (int c0 = 0; c0 < items; c0 += 64) {
                 const int it = c0 + lane_here();
-                const int n = __popcll(__ballot(it < items && hstart + line_of(a, epos, it) <= pos));
-                c += n;
-                if (n < 64) break;
+                const int64_t at = hstart + line_of(a, epos, it);
+                const int n = __popcll(__ballot(it < items && at <= pos));
+                if (n == 0) break;
+                c = c0 + n - 1;
+                istart = scalar64(at, n - 1);
             }
-            const int64_t istart = hstart + line_of(a, epos, c), iend = hstart + line_of(a, epos, c + 1);
+            const int64_t iend = istart + max(epos, 0) + a.pad + (int64_t)a.tokens * (c + 1);
             const int tok0 = c * a.tokens;
             ntok = min(a.tokens, erows - tok0);
             row0 = erow + tok0;
