@@ -23,9 +23,9 @@
 // P is rounded to bfloat16 for the second product, as in the prefill: the matrix cores set the time here, and a second part of
 // P would cost half as much again.  Sums and maxima are float32; out is rounded once, after the gate.
 //
-// 2048 rows behind 30720 (24/4 heads of 256) take 1531 us, 1044 TFLOP/s where a large product reaches 1436: 3640 clocks a unit
-// of which the matrix cores are busy 2048.  333 behind 936 (16/4 heads) take 36: of about 45 thousand clocks a block 20 are its
-// four units, 8 finding them, 6 Q and the first K, 5 the sums' way out, and then the join.
+// 2048 rows behind 30720 (24/4 heads of 256) take 1529 us, 1045 TFLOP/s where a large product reaches 1436: 3640 clocks a unit
+// of which the matrix cores are busy 2048.  333 behind 936 (16/4 heads) take 34.5: of about 40 thousand clocks a block 20 are
+// its four units, 8 finding them, 6 Q and the first K, 5 the sums' way out, and then the join.
 #include <math.h>
 
 #include <algorithm>
@@ -967,8 +967,8 @@ extern "C" int cs1_attention_paged_varlen(void* paged, const void* q, const void
     int device;
     if (hipGetDevice(&device) != hipSuccess || device != p->device) return hipErrorInvalidDevice;
     // Entries of up to 16 columns are each one tile of the kernel for single tokens, where others may be, in a launch before
-    // theirs: 43 entries of 1 to 4 tokens behind up to 4096 (16/4 heads of 256) take 91 us so and 107 in the tiles here,
-    // one of 4 behind 700 (heads of 128) 13.0 and 32; 29 of a token beside a prompt's 1021 12 less. One entry that may
+    // theirs: 43 entries of 1 to 4 tokens behind up to 4096 (16/4 heads of 256) take 88 us so and 107 in the tiles here,
+    // one of 4 behind 700 (heads of 128) 12.3 and 32; 29 of a token beside a prompt's 1021 12 less. One entry that may
     // be longer is taken for longer.
     const int64_t pairs = (int64_t)n * Hk;
     const bool all_few = max_new <= FEW / (Hq / Hk);
