@@ -8,13 +8,13 @@
 // Bound by the one pass over the logits.  A thread keeps a running base, sum and weighted sum of its own, and of its
 // values the largest with the load that it was in.  The alternatives need no more from that pass: the
 // k-th largest of the lanes' largest (64 lanes, each over the block's waves) is a value that k tokens reach at least, so
-// only what reaches it can be among the best, and only the threads whose largest does (about k of 512) look at
+// only what reaches it can be among the best, and only the threads whose largest does (about k of them) look at
 // their loads again.  What they find, k tokens or a few more, is put in order by counting.
 //
 // A row is cut into parts where there are few rows; a second launch joins the parts in order.
 //
-// 1217 rows of 248320 bfloat16 logits with 5 alternatives take 118 us (5.1 TB/s), one row of 151936 with 20 in 38 parts 8.2
-// and 5.8 us: in the first launch the load, the sums' and the alternatives' exchanges, in the second the alternatives one by one.
+// 1217 rows of 248320 bfloat16 logits with 5 alternatives take 118 us (5.1 TB/s), one row of 151936 with 20 in 64 parts 12.8
+// in two launches: in the first the load, the sums' and the alternatives' exchanges, in the second the alternatives one by one.
 #include <math.h>
 
 #include <algorithm>
@@ -26,7 +26,7 @@
 namespace q35 {
 namespace {
 
-constexpr int THREADS = 512, WAVES = THREADS / 64, LOADS = 4;
+constexpr int LOADS = 4;  // of 16 bytes a thread has under way
 constexpr int K_MAX = 32, PARTS_MAX = 64;
 constexpr int LIST = 1024;  // tokens that reach the threshold, kept in LDS
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -148,7 +148,7 @@ __device__ __forceinline__ void store_top(const Args& a, int row, int i, Key k, 
 }
 
 // A part of a row as loads of 16 bytes: number 0 has the logits in front of the first aligned one (fewer, or none), 1 ..
-// `whole` are full, and whole + 1 has what is left.  A thread has every THREADS-th, so its indices rise.
+// `whole` are full, and whole + 1 has what is left.  A thread has every so many-th, so its indices rise.
 template <typename T>
 struct Part {
     static constexpr int N = 16 / sizeof(T);
@@ -186,9 +186,9 @@ struct Part {
     }
 };
 
-template <typename T>
+template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) logprobs_kernel(const Args a) {
-    constexpr int N = Part<T>::N;
+    constexpr int N = Part<T>::N, WAVES = THREADS / 64;
     __shared__ Sums wave_sums[WAVES];
     __shared__ Key best_of[64], list[LIST + WAVES], found;
     __shared__ int listed, threads, who[THREADS], above[64];
@@ -371,15 +371,18 @@ __global__ void __launch_bounds__(JOIN_THREADS) logprobs_join_kernel(const Args 
     if (lane < a.k) store_top(a, row, lane, mine, s);
 }
 
-// Parts of a row: enough blocks for the chip, of at least a load a thread.
+// Parts of a row: enough blocks for the chip, of at least a load a thread.  A block has 256 threads, which begin and end
+// sooner, or 512, which read on more evenly, from 2^26 logits on: 300 rows of 151936 take 25.0 and 29.7 us, 2000 of 1400 9.9 and
+// 14.4, one of 151936 with 20 alternatives 12.7 and 13.8; 1217 of 248320 119.6 and 117.5, 500 of 151936 in float32 58 and 56.
 struct Plan {
-    int parts, each;
+    int parts, each, threads;
 };
 Plan plan_of(int rows, int V) {
-    const int64_t wanted = (1024 + (int64_t)rows - 1) / rows, most = (V + 8 * THREADS - 1) / (8 * THREADS);
+    const int threads = (int64_t)rows * V < 1 << 26 ? 256 : 512;
+    const int64_t wanted = (1024 + (int64_t)rows - 1) / rows, most = (V + 8 * threads - 1) / (8 * threads);
     const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, most), PARTS_MAX));
     const int each = (int)((((int64_t)V + parts - 1) / parts + 7) / 8 * 8);
-    return Plan{(int)(((int64_t)V + each - 1) / each), each};
+    return Plan{(int)(((int64_t)V + each - 1) / each), each, threads};
 }
 
 constexpr int V_MAX = 1 << 28;
@@ -421,8 +424,9 @@ extern "C" int cs1_token_logprobs(const void* logits, int is_float, size_t ld, c
     a.parts = p.parts;
     a.each = p.each;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const auto kernel = is_float ? logprobs_kernel<float> : logprobs_kernel<bf16>;
-    kernel<<<rows * p.parts, THREADS, 0, st>>>(a);
+    const auto kernel = p.threads == 256 ? (is_float ? logprobs_kernel<float, 256> : logprobs_kernel<bf16, 256>)
+                                         : (is_float ? logprobs_kernel<float, 512> : logprobs_kernel<bf16, 512>);
+    kernel<<<rows * p.parts, p.threads, 0, st>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.parts == 1) return e;
     const auto join = is_float ? logprobs_join_kernel<float> : logprobs_join_kernel<bf16>;
