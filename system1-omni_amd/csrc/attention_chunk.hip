@@ -967,7 +967,7 @@ extern "C" int cs1_attention_paged_varlen(void* paged, const void* q, const void
     int device;
     if (hipGetDevice(&device) != hipSuccess || device != p->device) return hipErrorInvalidDevice;
     // Entries of up to 16 columns are each one tile of the kernel for single tokens, where others may be, in a launch before
-    // theirs: 43 entries of 1 to 4 tokens behind up to 4096 (16/4 heads of 256) take 88 us so and 107 in the tiles here,
+    // theirs: 43 entries of 1 to 4 tokens behind up to 4096 (16/4 heads of 256) take 80 us so and 107 in the tiles here,
     // one of 4 behind 700 (heads of 128) 12.3 and 32; 29 of a token beside a prompt's 1021 12 less. One entry that may
     // be longer is taken for longer.
     const int64_t pairs = (int64_t)n * Hk;

@@ -286,9 +286,9 @@ __global__ void __launch_bounds__(THREADS, SEVERAL && DH == 128 ? 2 : 1) attenti
     total = __builtin_amdgcn_readfirstlane(total * heads);
     if (SEVERAL && total == 0) return;
     // With heads of 128 two blocks fit on a CU (and are launched for many sequences): where these are short, on
-    // average under 10 chunks (384 keys), a block's time is that of beginning and ending each, and two at once hide it.
+    // average under 10 chunks (384 keys; 11 where beginning counts for one more), a block's time is that of beginning and ending each, and two at once hide it.
     // 200 sequences of 260 to 384 keys take 35.3 us so and 39.0 with one, of 200 to 800 53.4 and 48.5 (16/4 heads).
-    const uint32_t inverse = a.halve && total >= 10 * a.B * heads ? 2 * a.blocks_inverse : a.blocks_inverse;
+    const uint32_t inverse = a.halve && total >= (SEVERAL ? 11 : 10) * a.B * heads ? 2 * a.blocks_inverse : a.blocks_inverse;
     const int each = __umulhi(total - 1, inverse) + 1;  // (one more than need be where the inverse's rounding shows)
     const int begin = (int)blockIdx.x * each, end = min(total, begin + each);
     // (the rows go on from one segment to the next: r0 the 64 that are searched, which begin at chunk `before`)
@@ -754,13 +754,15 @@ int paged_rows(const Paged* p, const Call& c, const int32_t* cu, int max_new, in
     // A pair is a row with a kv head and tile.  From a pair to 16 blocks on the chunks are small, and beginning a pair
     // counts as work: as much as 6 units of keys up to a pair a CU, as 8 beyond (about 7 us). 43 sequences of up to
     // 4096, 16/4 heads of 256, take 71 us so, 91 if it counts as nothing.  Fewer pairs are better cut into whole chunks of 4.
+    // With several tokens, whose joins have more rows, it counts as 10: 43 entries behind up to 4096 80 us so, 88 with 6; 150
+    // behind up to 2000 (32/8 heads of 128) 127, and 136 with 8; 48 of up to 16 rows of one column 27 and 35 with 6.
     // Short sequences are one chunk, which is not cut, and joined by no one; the fewer pairs, the longer they may
     // be without the work being shared out badly: one of 300 keys (heads of 128) takes 8.4 us with 12 units and 9.8 with 8,
     // 64 of 100 to 200 (256) 12.4 with 8 and 20.0 with 4, 40 of up to 1000 22.4 and 25.6 with 12, 300 of up to 400 66 with 4
     // and 80 with 8.
     const bool several = pairs * 16 >= a.blocks, many = pairs > p->cus;
     a.unit = several ? 2 : 4;
-    const int pad = many ? 4 : several ? 3 : 0, alone = many ? 4 : several ? 8 : 12;
+    const int pad = cu && several ? 5 : many ? 4 : several ? 3 : 0, alone = many ? 4 : several ? 8 : 12;
     a.pad_alone = alone << 8 | pad;
     a.page_inverse = (uint32_t)std::min<uint64_t>(0xffffffffu, (uint64_t{1} << 32) / (a.page / 16));
     a.blocks_inverse = (uint32_t)(((uint64_t{1} << 32) + a.blocks - 1) / a.blocks);
