@@ -364,7 +364,7 @@ def _plain_logprobs(s, c):
     R, V = c["rows"], c["vocab"]
     index = torch.arange(V, device="cuda", dtype=torch.int32)[None, :]
     for a in range(0, R, 256):  # what 256 rows take in 32 bits fits the card several times over
-        x = s["logits"][a:a + 256, :V].float()
+        x = s["logits"][a:a + 256, :V].to(F32, copy=True)  # (the alternatives are taken out of it below)
         m = x.amax(-1, keepdim=True)
         e = torch.exp(x - m)
         z = e.sum(-1, keepdim=True)
