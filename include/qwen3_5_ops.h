@@ -428,7 +428,9 @@ int cs1_attention_paged_varlen(void* paged, const void* q, const void* kp, const
  * logits, the lowest index first among equals: top_ids and top_logprobs [rows, k], -1 and NaN behind the last of
  * fewer.  In float32 throughout.  Logits of -inf have no weight; a row with a NaN or +inf, or of -inf only, has NaN for each
  * value and -1 for each index.  V <= 2^28.  workspace: cs1_token_logprobs_workspace_bytes(rows, V, k) bytes on 16 (0:
- * null will do), this call's own until it is done on the device. */
+ * null will do), this call's own until it is done on the device.  What it says for rows, V and k is enough for fewer of
+ * each as well (under 560 KB), but for 1024 rows and more, which need none: a program whose batches may be
+ * smaller than its largest asks for the smaller of that and 1023 rows. */
 size_t cs1_token_logprobs_workspace_bytes(int rows, int V, int k);
 int cs1_token_logprobs(const void* logits, int is_float, size_t ld, const int32_t* targets, int rows, int V, int k,
                        float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs, void* workspace,

@@ -374,12 +374,13 @@ __global__ void __launch_bounds__(JOIN_THREADS) logprobs_join_kernel(const Args 
 // Parts of a row: enough blocks for the chip, of at least a load a thread.  A block has 256 threads, which begin and end
 // sooner, or 512, which read on more evenly, from 2^26 logits on: 300 rows of 151936 take 25.0 and 29.7 us, 2000 of 1400 9.9 and
 // 14.4, one of 151936 with 20 alternatives 12.7 and 13.8; 1217 of 248320 119.6 and 117.5, 500 of 151936 in float32 58 and 56.
+constexpr int ONE_PART = 1024;  // blocks that are enough: so many rows and more are not cut
 struct Plan {
     int parts, each, threads;
 };
 Plan plan_of(int rows, int V) {
     const int threads = (int64_t)rows * V < 1 << 26 ? 256 : 512;
-    const int64_t wanted = (1024 + (int64_t)rows - 1) / rows, most = (V + 8 * threads - 1) / (8 * threads);
+    const int64_t wanted = (ONE_PART + (int64_t)rows - 1) / rows, most = (V + 8 * threads - 1) / (8 * threads);
     const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, most), PARTS_MAX));
     const int each = (int)((((int64_t)V + parts - 1) / parts + 7) / 8 * 8);
     return Plan{(int)(((int64_t)V + each - 1) / each), each, threads};
@@ -394,8 +395,12 @@ using namespace q35;
 
 extern "C" size_t cs1_token_logprobs_workspace_bytes(int rows, int V, int k) {
     if (rows <= 0 || V <= 0 || V > V_MAX || k < 0 || k > K_MAX) return 0;
-    const Plan p = plan_of(rows, V);
-    return p.parts == 1 ? 0 : (size_t)rows * p.parts * (sizeof(Sums) + sizeof(Key) * k);
+    // The plan's own number of parts goes up and down with the rows and tokens; this bound on it only up, so that a
+    // program can keep one workspace: up to 64 parts of a row, none shorter than 2048 logits, ceil(1024 / rows) at most.
+    constexpr int LEAST = 8 * 256;
+    if (rows >= ONE_PART || V <= LEAST) return 0;
+    const int most = std::min((V + LEAST - 1) / LEAST, PARTS_MAX);
+    return (size_t)std::min(rows * most, rows + ONE_PART - 1) * (sizeof(Sums) + sizeof(Key) * k);
 }
 
 extern "C" int cs1_token_logprobs(const void* logits, int is_float, size_t ld, const int32_t* targets, int rows, int V,
