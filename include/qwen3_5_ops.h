@@ -363,7 +363,10 @@ int cs1_gdn_decode(const void* qkv, int ld, const void* w, const void* z, const 
  * captured graph serves other batches.  `rows` is the number of rows of the batch's buffers: those behind
  * cu_seqlens[n] are no one's.  A step is cs1_kv_extend and cs1_kv_rows once, then per attention layer
  * cs1_attn_prep_paged and cs1_attention_paged_varlen; cs1_token_logprobs reads its logits, and cs1_kv_trim
- * takes tokens back that were not accepted. */
+ * takes tokens back that were not accepted.  A step without room must not run: its rows would be the
+ * sequences' last tokens, whose keys and values prep would write over, also in pages that forks share, and cs1_kv_trim would
+ * take tokens of earlier steps.  So cs1_kv_extend's status is read before the rest is queued, or the rest goes by it
+ * on the device: cs1_kv_rows_if_room in place of cs1_kv_rows, and a drop of 0 for cs1_kv_trim. */
 
 /* cs1_kv_reserve for such a batch: sequence i grows by cu_seqlens[i + 1] - cu_seqlens[i] tokens (a negative number
  * counts as 0).  Pages, status and what follows from it are as there. */
@@ -376,6 +379,12 @@ int cs1_kv_extend(const Cs1PageTable* pages, const int32_t* seqs, const int32_t*
  * npages * page < 2^31. */
 int cs1_kv_rows(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n, int rows, int32_t* pos,
                 int32_t* slot, void* stream);
+
+/* cs1_kv_rows behind a cs1_kv_extend in one graph: where *status (device, that call's answer) is not 0, all of pos and slot
+ * are -1, so that cs1_attn_prep_paged leaves q, gate and the pages as they are.  (What attention then makes of such
+ * a step has no meaning.) */
+int cs1_kv_rows_if_room(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n, int rows,
+                        const int32_t* status, int32_t* pos, int32_t* slot, void* stream);
 
 /* Take the last drop[i] tokens (device, n <= 8192; less than 0 counts as 0, more than there are as all) off the listed
  * sequences; whole pages behind the new end are released.  A sequence that would end inside a page which others hold

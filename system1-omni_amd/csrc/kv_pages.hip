@@ -234,16 +234,19 @@ __global__ void __launch_bounds__(PLAN_THREADS)
 
 // Where the rows of a packed batch are: a row a thread.  Every block makes the list's first entries for itself (n <= 8192
 // loads that a block has under way at once) and has the offsets in LDS, so that a row's chain is entry, length,
-// page, and the search between costs no memory.  (7800 rows of 200 entries: 4.0 us.)
+// page, and the search between costs no memory.  (7800 rows of 200 entries: 4.0 us.)  status: no row is anywhere if it is
+// not 0 (null: not looked at).
 __global__ void __launch_bounds__(PLAN_THREADS)
     kv_rows_kernel(const Cs1PageTable t, const int32_t* __restrict__ seqs, const int32_t* __restrict__ cu, int n,
-                   int rows, int32_t* __restrict__ pos, int32_t* __restrict__ slot) {
+                   int rows, const int32_t* __restrict__ status, int32_t* __restrict__ pos,
+                   int32_t* __restrict__ slot) {
     extern __shared__ int lists[];
     int* const end = lists;          // [n] each entry's end
     int* const first = lists + n;    // [nseq] the first entry that names a sequence
     const int tid = threadIdx.x, r = blockIdx.x * PLAN_THREADS + tid;
     asm volatile("" ::"s"(t.table), "s"(t.lens), "s"(t.nseq), "s"(t.max_pages), "s"(t.npages), "s"(t.page), "s"(seqs),
-                 "s"(cu), "s"(n), "s"(rows), "s"(pos), "s"(slot));
+                 "s"(cu), "s"(n), "s"(rows), "s"(status), "s"(pos), "s"(slot));
+    const bool room = !status || *status == 0;
     for (int s = tid; s < t.nseq; s += PLAN_THREADS) first[s] = n;
     int seq[PER_MAX];
 #pragma unroll
@@ -272,7 +275,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     int p = -1, at = -1;
     const int i = lo, s = i < n ? listed_seq(seqs, i, t.nseq) : -1;
     // (offsets that do not rise may leave a row to an entry that begins behind it)
-    if (s >= 0 && first[s] == i && (i == 0 || end[i - 1] <= r)) {
+    if (room && s >= 0 && first[s] == i && (i == 0 || end[i - 1] <= r)) {
         const int64_t here = (int64_t)t.lens[s] - (end[i] - r);
         if (here >= 0 && here < (int64_t)t.max_pages * t.page) {
             p = (int)here;
@@ -744,15 +747,26 @@ extern "C" int cs1_kv_extend(const Cs1PageTable* pages, const int32_t* seqs, con
     return hipGetLastError();
 }
 
-extern "C" int cs1_kv_rows(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n, int rows,
-                           int32_t* pos, int32_t* slot, void* stream) {
+static int kv_rows(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n, int rows,
+                   const int32_t* status, int32_t* pos, int32_t* slot, void* stream) {
     if (!table_ok(pages) || n < 0 || n > MAX_LISTED || rows < 0 || (int64_t)pages->npages * pages->page > INT32_MAX)
         return hipErrorInvalidValue;
     if (rows == 0) return hipSuccess;
     if (!all_set({pos, slot}) || (n > 0 && !cu_seqlens)) return hipErrorInvalidValue;
     kv_rows_kernel<<<cdiv(rows, PLAN_THREADS), PLAN_THREADS, 4 * ((size_t)n + pages->nseq),
-                     static_cast<hipStream_t>(stream)>>>(*pages, seqs, cu_seqlens, n, rows, pos, slot);
+                     static_cast<hipStream_t>(stream)>>>(*pages, seqs, cu_seqlens, n, rows, status, pos, slot);
     return hipGetLastError();
+}
+
+extern "C" int cs1_kv_rows(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n, int rows,
+                           int32_t* pos, int32_t* slot, void* stream) {
+    return kv_rows(pages, seqs, cu_seqlens, n, rows, nullptr, pos, slot, stream);
+}
+
+extern "C" int cs1_kv_rows_if_room(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n,
+                                   int rows, const int32_t* status, int32_t* pos, int32_t* slot, void* stream) {
+    if (!status) return hipErrorInvalidValue;
+    return kv_rows(pages, seqs, cu_seqlens, n, rows, status, pos, slot, stream);
 }
 
 extern "C" int cs1_kv_trim(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* drop, int n, int32_t* status,

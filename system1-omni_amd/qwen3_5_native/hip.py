@@ -98,6 +98,7 @@ ADDITIONS = {
     "cs1_gdn_decode": (_I, [P, _I, P, P, P, P, P, P, P, c_float, P, P, P, P, _I, P, _I, _I, _I, c_float, P]),
     "cs1_kv_extend": (_I, [P, P, P, _I, P, P]),
     "cs1_kv_rows": (_I, [P, P, P, _I, _I, P, P, P]),
+    "cs1_kv_rows_if_room": (_I, [P, P, P, _I, _I, P, P, P, P]),
     "cs1_kv_trim": (_I, [P, P, P, _I, P, P]),
     "cs1_rotary_freqs": (_I, [P, _I, c_double, c_double, c_double, c_double, c_double]),
     "cs1_attention_paged_varlen": (_I, [P, P, P, P, P, P, P, _I, _I, P, P, P, _I, _I, _I, _I, c_float, P]),
