@@ -369,7 +369,7 @@ int cs1_gdn_decode(const void* qkv, int ld, const void* w, const void* z, const 
  * on the device: cs1_kv_rows_if_room in place of cs1_kv_rows, and a drop of 0 for cs1_kv_trim. */
 
 /* cs1_kv_reserve for such a batch: sequence i grows by cu_seqlens[i + 1] - cu_seqlens[i] tokens (a negative number
- * counts as 0).  Pages, status and what follows from it are as there. */
+ * counts as 0).  Pages, status and what follows from it are as there.  max_pages times the lesser of n and nseq < 2^31. */
 int cs1_kv_extend(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n, int32_t* status,
                   void* stream);
 

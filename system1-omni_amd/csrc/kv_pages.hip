@@ -8,6 +8,8 @@
 // that: a scan over the needs, then scans over 4096 counts, and then 16384 at a time, until enough pages are found.
 // What moves keys and values is a kernel of its own that fills the chip: a page's filled rows are one run of bytes in
 // each pool.
+#include <algorithm>
+
 #include "common.h"
 #include "paged.h"
 
@@ -740,6 +742,8 @@ extern "C" int cs1_kv_reserve(const Cs1PageTable* pages, const int32_t* seqs, co
 extern "C" int cs1_kv_extend(const Cs1PageTable* pages, const int32_t* seqs, const int32_t* cu_seqlens, int n,
                              int32_t* status, void* stream) {
     if (!table_ok(pages) || n < 0 || n > MAX_LISTED || !status || (n > 0 && !cu_seqlens)) return hipErrorInvalidValue;
+    // new pages are counted in 32 bits; offsets on the device that fall and rise again can ask for any number of them
+    if ((int64_t)std::min(n, pages->nseq) * pages->max_pages > INT32_MAX) return hipErrorInvalidValue;
     Offsets none;
     none.n = 0;
     const auto kernel = n <= PLAN_THREADS ? kv_reserve_kernel<1, true> : kv_reserve_kernel<PER_MAX, true>;
