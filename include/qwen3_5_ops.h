@@ -413,7 +413,7 @@ int cs1_rotary_freqs(double* freqs, int dims, double base, double factor, double
  * null: not) and turned for position pos[t]; q and gate are written as [T, Hq, Dh], k and v to slot[t] of the pools
  * kp and vp (pos and slot: cs1_kv_rows; of `pages` only npages and page are read).  In float32, each value rounded
  * once.  Rows with pos[t] < 0 are left out, and k and v of rows whose slot is not in [0, npages * page).  Slots differ
- * from row to row.  Dh 128 or 256; ld a multiple of 8, all tensors on 16 bytes; Hk * Dh <= 2^24. */
+ * from row to row.  Dh 128 or 256; ld a multiple of 8, all tensors on 16 bytes; Hk * Dh <= 2^24, T < 2^24. */
 int cs1_attn_prep_paged(const void* qg, const void* kr, const void* v, int ld, const void* qw, const void* kw, float eps,
                         const Cs1Rotary* rotary, const Cs1PageTable* pages, const int32_t* pos, const int32_t* slot,
                         void* q, void* gate, void* kp, void* vp, int T, int Hq, int Hk, int Dh, void* stream);
@@ -436,7 +436,7 @@ int cs1_attention_paged_varlen(void* paged, const void* q, const void* kp, const
  * neither; 0 where the target is not in [0, V)), entropy[r] = -sum p log p in nats (null: not written), and the k <= 32 largest
  * logits, the lowest index first among equals: top_ids and top_logprobs [rows, k], -1 and NaN behind the last of
  * fewer.  In float32 throughout.  Logits of -inf have no weight; a row with a NaN or +inf, or of -inf only, has NaN for each
- * value and -1 for each index.  V <= 2^28.  workspace: cs1_token_logprobs_workspace_bytes(rows, V, k) bytes on 16 (0:
+ * value and -1 for each index.  V <= 2^28, rows < 2^23.  workspace: cs1_token_logprobs_workspace_bytes(rows, V, k) bytes on 16 (0:
  * null will do), this call's own until it is done on the device.  What it says for rows, V and k is enough for fewer of
  * each as well (under 560 KB), but for 1024 rows and more, which need none: a program whose batches may be
  * smaller than its largest asks for the smaller of that and 1023 rows. */

@@ -386,7 +386,7 @@ Plan plan_of(int rows, int V) {
     return Plan{(int)(((int64_t)V + each - 1) / each), each, threads};
 }
 
-constexpr int V_MAX = 1 << 28;
+constexpr int V_MAX = 1 << 28, ROWS_MAX = (1 << 23) - 1;  // (a launch has under 2^32 threads, 512 for a row)
 
 }  // namespace
 }  // namespace q35
@@ -406,10 +406,10 @@ extern "C" size_t cs1_token_logprobs_workspace_bytes(int rows, int V, int k) {
 extern "C" int cs1_token_logprobs(const void* logits, int is_float, size_t ld, const int32_t* targets, int rows, int V,
                                   int k, float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs,
                                   void* workspace, void* stream) {
-    if (rows < 0 || V <= 0 || V > V_MAX || ld < (size_t)V || k < 0 || k > K_MAX) return hipErrorInvalidValue;
+    if (rows < 0 || rows > ROWS_MAX || V <= 0 || V > V_MAX || ld < (size_t)V || k < 0 || k > K_MAX) return hipErrorInvalidValue;
     if (rows == 0) return hipSuccess;
     const Plan p = plan_of(rows, V);
-    if ((int64_t)rows * p.parts > INT32_MAX || !logits || (logprob != nullptr) != (targets != nullptr) ||
+    if (!logits || (logprob != nullptr) != (targets != nullptr) ||
         (k > 0 && !all_set({top_ids, top_logprobs})))
         return hipErrorInvalidValue;
     if ((reinterpret_cast<uintptr_t>(logits) & (is_float ? 3 : 1)) != 0) return hipErrorInvalidValue;

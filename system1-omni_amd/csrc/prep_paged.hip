@@ -140,6 +140,7 @@ extern "C" int cs1_attn_prep_paged(const void* qg, const void* kr, const void* v
                                    const int32_t* pos, const int32_t* slot, void* q, void* gate, void* kp, void* vp,
                                    int T, int Hq, int Hk, int Dh, void* stream) {
     if (T < 0 || Hq <= 0 || Hk <= 0 || (Dh != 128 && Dh != 256) || !rotary || !pages) return hipErrorInvalidValue;
+    if ((int64_t)T * THREADS > UINT32_MAX) return hipErrorInvalidValue;  // (a launch has under 2^32 threads)
     const int64_t wide = (int64_t)Hq * Dh * (gate ? 2 : 1), slots = (int64_t)pages->npages * pages->page;
     if (ld % 8 != 0 || ld < wide || ld < (int64_t)Hk * Dh || (int64_t)Hk * Dh > (1 << 24) || pages->npages <= 0 ||
         pages->page <= 0 || slots > INT32_MAX)
