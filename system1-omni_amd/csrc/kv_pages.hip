@@ -71,6 +71,7 @@ __device__ __forceinline__ int entry_of(const int* off, int n, int k) {
 
 // Counts of pages from `base` on: a wave has 64 N of them in a row, a lane every 64th.
 constexpr int NEAR = 4, FAR = 16;
+constexpr int DIRECT = 64;  // pages that are few
 template <int N>
 struct Counts {
     int of[N];
@@ -87,7 +88,9 @@ __device__ __forceinline__ Counts<N> page_counts(const int32_t* __restrict__ ref
 // Free pages, by their number k among all free ones, as far as they are found.  They are collected in LDS and taken all
 // at once, a thread each: taking one is a search and two loads, one after the other, and where few pages are free among
 // many every scan would wait for its own (200 sequences of 39 new tokens, 800 free pages among 52000: 30 us with
-// scans of 4096 that took what they found, 16 with a thread for each found, 14 so).
+// scans of 4096 that took what they found, 16 with a thread for each found, 14 so).  Up to DIRECT pages that the first scan
+// finds all are taken by the waves that have them, a lane each, without that way through LDS: one token of 1, 32 and 64
+// sequences that need a page each 4.3, 5.0 and 5.0 us so, 4.9, 5.6 and 5.6 by LDS.
 struct Free {
     int page[4096], wave[PLAN_WAVES];  // numbers from `taken` on
 };
@@ -115,6 +118,32 @@ __device__ __forceinline__ void find_among(const Counts<N>& counts, int npages, 
         all += r;
     }
     found = min(total, found + all);
+    if (N == NEAR && total <= DIRECT && found == total) {
+        // lane i has the wave's i-th: the 64 pages that it is in, then by halves
+        uint64_t among = free[0];
+        int i = lane, p = at;
+#pragma unroll
+        for (int j = 0; j < N - 1; j++) {
+            const int n = __popcll(free[j]);
+            if (p == at + j * 64 && i >= n) {
+                i -= n;
+                p += 64;
+                among = free[j + 1];
+            }
+        }
+#pragma unroll
+        for (int half = 32; half > 0; half >>= 1) {
+            const int n = __popcll(among & ((uint64_t{1} << half) - 1));
+            if (i >= n) {
+                i -= n;
+                p += half;
+                among >>= half;
+            }
+        }
+        if (lane < mine && first + lane < total) take(first + lane, p);
+        taken = total;
+        return;
+    }
     for (;;) {
         int k0 = first;
         if (mine > 0)
@@ -140,6 +169,7 @@ __device__ __forceinline__ int take_free(const int32_t* refs, int npages, int to
     int found = 0, taken = 0, base = NEAR * PLAN_THREADS;
     if (total <= 0) return 0;
     find_among(near, npages, 0, total, taken, found, f, take);
+    if (taken == total) return total;
     if (found < total && base < npages) {
         auto counts = page_counts<FAR>(refs, npages, base);
         for (; base < npages && found < total; base += FAR * PLAN_THREADS) {
