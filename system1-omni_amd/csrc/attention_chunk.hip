@@ -23,9 +23,9 @@
 // P is rounded to bfloat16 for the second product, as in the prefill: the matrix cores set the time here, and a second part of
 // P would cost half as much again.  Sums and maxima are float32; out is rounded once, after the gate.
 //
-// 2048 rows behind 30720 (24/4 heads of 256) take 1529 us, 1045 TFLOP/s where a large product reaches 1436: 3640 clocks a unit
-// of which the matrix cores are busy 2048.  333 behind 936 (16/4 heads) take 34.5: of about 40 thousand clocks a block 20 are
-// its four units, 8 finding them, 6 Q and the first K, 5 the sums' way out, and then the join.
+// 2048 rows behind 30720 (24/4 heads of 256) take 1430 to 1480 us, 1080 to 1120 TFLOP/s where a large product reaches 1436: 4020
+// clocks a unit over the launch, of which the matrix cores are busy 2040.  333 behind 936 (16/4 heads) take 34.5: of about 40
+// thousand clocks a block 20 are its four units, 8 finding them, 6 Q and the first K, 5 the sums' way out, and then the join.
 #include <math.h>
 
 #include <algorithm>
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
     // beginnings go on from key 0 at once, and what is left of the first item is as far from its end as the stretch is.  (Where
     // a stretch is shorter than its item there is less of that than a second search takes.)
     // A unit that is read by the 32 blocks of an XCD comes from its L2 then (2048 rows behind 30720, 24/4 heads of
-    // 256: 1680 us in the line's order, 1530 so).
+    // 256: 1617 us in the line's order, 1460 so).
     enum { STRAIGHT, FIRST_IS_LEFT, AT_FIRST } order = STRAIGHT;
     for (;;) {
         int seq, row0, ntok, pos0, keys, head = 0, u0, u1;
@@ -405,8 +405,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_chunk_kernel(const Args)
             v_lane = row * token + (v_slot(row, place) << 4);
         }
         // A wave's transfers of a unit go one by one between the products; where there are only two, together, which saves a
-        // few instructions (1000 rows behind 8000, 32/8 heads of 128: 172 us apart, 166 so; of four, two or all together are
-        // slower: 2048 behind 30720, 24/4 heads of 256, 1680 us apart, 1690 in twos, 1735 at once).
+        // few instructions (1000 rows behind 8000, 32/8 heads of 128: 160 us apart, 157 so; of four, twos are slower: 2048
+        // behind 30720, 24/4 heads of 256, 1460 us apart, 1471 in twos).
         constexpr int SET = NI == 2 ? 2 : 1, SETS = NI / SET;
         auto move = [&](const u32x4& r, int at, int set, auto lane_of) Q35_INLINE {
             const uint32_t to = (uint32_t)uniform((int)(lds0 + at + set * SET * 1024));
@@ -967,8 +967,8 @@ extern "C" int cs1_attention_paged_varlen(void* paged, const void* q, const void
     int device;
     if (hipGetDevice(&device) != hipSuccess || device != p->device) return hipErrorInvalidDevice;
     // Entries of up to 16 columns are each one tile of the kernel for single tokens, where others may be, in a launch before
-    // theirs: 43 entries of 1 to 4 tokens behind up to 4096 (16/4 heads of 256) take 80 us so and 107 in the tiles here,
-    // one of 4 behind 700 (heads of 128) 12.3 and 32; 29 of a token beside a prompt's 1021 12 less. One entry that may
+    // theirs: 43 entries of 1 to 4 tokens behind up to 4096 (16/4 heads of 256) take 80 us so and 82 in the tiles here,
+    // one of 4 behind 700 (heads of 128) 12.3 and 19.8, 29 of a token beside a prompt's 1021 94 and 99. One entry that may
     // be longer is taken for longer.
     const int64_t pairs = (int64_t)n * Hk;
     const bool all_few = max_new <= FEW / (Hq / Hk);
@@ -1006,9 +1006,9 @@ extern "C" int cs1_attention_paged_varlen(void* paged, const void* q, const void
     a.G = Hq / Hk;
     a.tokens = (Dh == 128 ? Form<128>::COLS : Form<256>::COLS) / a.G;
     a.blocks = p->cus;
-    // What an item takes around its steps counts as 256 keys (four units), and no stretch is shorter than three units: 512 rows
-    // alone (24/4 heads of 256) take 42.6 us so, 58 with 192 keys and 42.9 with 320; 20 behind 300 (16/4) 21.5, and 24.3
-    // and 27.1 with stretches of at least 256 and 384.
+    // What an item takes around its steps counts as 256 keys (four units), and no stretch is shorter than three units: a prompt's
+    // 1021 rows beside 29 tokens (16/4 heads of 128) take 94.2 us so, 96.8, 95.2 and 94.6 with 128, 192 and 320 keys, 333 behind
+    // 936 (256) 35.2, and 36.3, 35.9 and 37.1; 20 behind 300 20.3, and 22.8 and 24.3 with stretches of at least 256 and 384.
     a.pad = 256;
     a.least = 192;
     a.tokens_inverse = (uint32_t)(((uint64_t{1} << 32) + a.tokens - 1) / a.tokens);

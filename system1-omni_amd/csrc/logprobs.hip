@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) logprobs_join_kernel(const Args 
 }
 
 // Parts of a row: enough blocks for the chip, of at least a load a thread.  A block has 256 threads, which begin and end
-// sooner, or 512, which read on more evenly, from 2^26 logits on: 300 rows of 151936 take 25.0 and 29.7 us, 2000 of 1400 9.9 and
+// sooner, or 512, which read on more evenly, from 2^26 logits on: 300 rows of 151936 take 25.6 and 29.7 us, 2000 of 1400 9.9 and
 // 14.4, one of 151936 with 20 alternatives 12.7 and 13.8; 1217 of 248320 119.6 and 117.5, 500 of 151936 in float32 58 and 56.
 constexpr int ONE_PART = 1024;  // blocks that are enough: so many rows and more are not cut
 struct Plan {
